@@ -60,6 +60,11 @@ extern "C" {
 #define MOE_ACT_GEGLU 1       /* tanh-GELU(g) * u (Gemma-4) */
 #define MOE_ACT_GPTOSS 2      /* g = min(g,7), u = clip(u,-7,7), g * sigmoid(1.702 g) * (u + 1) */
 
+/* activations of moe_linear_run */
+#define MOE_LIN_NONE 0
+#define MOE_LIN_SILU 1        /* z * sigmoid(z) */
+#define MOE_LIN_GELU 2        /* tanh-GELU(z) */
+
 /* expert-path selection for moe_experts_run */
 #define MOE_PATH_AUTO 0       /* T == 1 -> per-slot GEMV (two launches); T > 1 -> grouped expert tiles */
 #define MOE_PATH_SLOTS 1      /* per-slot GEMV over all T*k slots, no grouping, two launches (the stock-style
@@ -307,6 +312,97 @@ size_t moe_experts_shared_workspace_bytes(const moe_experts_t* w, int S, int T, 
  */
 #define MOE_PROBE_SINK 1024
 int moe_probe_read(const void* src, size_t nbytes, uint32_t* sink, void* stream);
+
+/*
+ * Products grouped by expert, 16-bit weights (the reference multiplies quantised experts only; its unquantised form is the
+ * per-expert loop of moelab/variants/cuda/torch_loop.py:11-17). Slots p = 0 .. M - 1 are sorted by group: group e holds
+ * offsets[e] <= p < offsets[e + 1] (offsets [E + 1] int32 on the device, offsets[0] = 0; values outside [0, M] are
+ * clamped). offsets NULL: one group of all M slots (E = 1).
+ *   moe_grouped_mm:    y[p][n]     = sum_k x[r(p)][k] w[e][n][k] (+ bias[e][n]),  r(p) = rows[p], or p when rows is NULL
+ *   moe_grouped_mm_dx: dx[p][k]    = sum_n dy[r(p)][n] w[e][n][k]
+ *   moe_grouped_mm_dw: dw[e][n][k] = sum_p dy[dy_idx[p]][n] x[x_idx[p]][k],  dbias[e][n] = sum_p dy[dy_idx[p]][n]
+ *                      (groups without a slot: zeros; a NULL index list: the slot itself)
+ * Operands and bias are of one type, MOE_DTYPE_BF16 or MOE_DTYPE_F16; the result is of that type, rounded once from fp32
+ * sums in a fixed order, or MOE_DTYPE_F32 (dbias: the operands' type). x [x_rows, K] with ldx elements from row to row
+ * (dy alike); w [E, N, K], results and bias contiguous. Slots behind the last group are left as they were, or set to zero
+ * with fill = 1. An index outside its matrix reads as a row of zeros.
+ * Requirements: N % 8 == 0, K % 8 == 0, strides % 8 == 0, N, K <= 2^20, strides <= 2^21; pointers 16-byte aligned; a matrix
+ * read through an index list (for dw: either, then both) at most 0xB0000000 bytes.
+ */
+int moe_grouped_mm(const void* x, const void* w, const void* bias, const int32_t* offsets, const int32_t* rows, int64_t M,
+                   int64_t x_rows, int64_t ldx, int E, int N, int K, int dtype, void* y, int y_dtype, int fill,
+                   void* stream);
+int moe_grouped_mm_dx(const void* dy, const void* w, const int32_t* offsets, const int32_t* rows, int64_t M,
+                      int64_t dy_rows, int64_t lddy, int E, int N, int K, int dtype, void* dx, int dx_dtype, int fill,
+                      void* stream);
+int moe_grouped_mm_dw(const void* dy, const void* x, const int32_t* offsets, const int32_t* dy_idx, const int32_t* x_idx,
+                      int64_t M, int64_t dy_rows, int64_t lddy, int64_t x_rows, int64_t ldx, int E, int N, int K, int dtype,
+                      void* dw, int dw_dtype, void* dbias, void* stream);
+
+/*
+ * One product with its epilogue: y = act(x w^T + bias) + residual, x [T, K] (ldx elements from row to row), w [N, K],
+ * bias [N], residual and y [T, N]; types, alignment and sizes as moe_grouped_mm; act: MOE_LIN_*. The sums, bias, activation
+ * and residual are fp32, rounded once. z [T, N] (or NULL): the sums with bias before the activation, in the operands' type,
+ * what moe_linear_act_bwd takes. Gradients: dz = dy act'(z) by moe_linear_act_bwd (dz = dy without an activation), then
+ * moe_grouped_mm_dx / _dw of dz with E = 1 and no offsets. residual may be y.
+ * workspace: moe_linear_workspace_bytes(T, N, K) bytes, any contents (0: NULL will do).
+ */
+size_t moe_linear_workspace_bytes(int64_t T, int N, int K);
+int moe_linear(const void* x, const void* w, const void* bias, const void* residual, int act, int64_t T, int64_t ldx, int N,
+               int K, int dtype, void* y, int y_dtype, void* z, void* workspace, size_t workspace_bytes, void* stream);
+/* z [T, N] in 16 bits, or NULL and its 8-bit form codes, scales (moe_act8_pack). */
+int moe_linear_act_bwd(const void* dy, int64_t lddy, const void* z, const void* codes, const void* scales, int act, int64_t T,
+                       int N, int dtype, void* dz, void* stream);
+
+/*
+ * Activations kept in 8 bits for a backward pass. Rows of C values (C % 32 == 0) as int8 codes [M, C] and one exponent byte
+ * per 32 neighbours, scales [M, C / 32]: value = code * 2^(scale - 133), |code| <= 127, a rounding of at most half a step.
+ * scale = biased exponent of the block's largest magnitude, one more if that would round to 128 (254 at most: there the
+ * code stays 127); 255: the block holds an infinity or NaN and reads as NaN.
+ *   moe_act8_pack, _unpack: 16-bit values to that form, and back (to bf16, fp16 or fp32; into the type they came from it is
+ *                           exact).
+ *   moe_glu_fwd: gu [M, 2 F] (gate columns, then up; ldgu elements from row to row) -> h [M, F] = act(gate, up) and, codes not
+ *                NULL, gu's 8-bit form (codes [M, 2 F], scales [M, 2 F / 32]). act: MOE_ACT_*; F % 32 == 0.
+ *   moe_glu_bwd: from that form (or gu itself with codes NULL), dh [M, F] (16-bit or MOE_DTYPE_F32) and row weights wts [M]
+ *                (NULL: 1): dgu [M, 2 F] = wts dh act'(gate, up), hw [M, F] = wts h (or NULL), dwts [M] = sum_f dh h (or
+ *                NULL). Where an act-2 clamp holds, the gradient is 0.
+ */
+int moe_act8_pack(const void* x, int64_t ldx, int64_t M, int C, int dtype, void* codes, void* scales, void* stream);
+int moe_act8_unpack(const void* codes, const void* scales, int64_t M, int C, void* out, int dtype, void* stream);
+int moe_glu_fwd(const void* gu, int64_t ldgu, int64_t M, int F, int act, int dtype, void* h, void* codes, void* scales,
+                void* stream);
+int moe_glu_bwd(const void* codes, const void* scales, const void* gu, int64_t ldgu, const void* dh, int dh_dtype,
+                const float* wts, int64_t M, int F, int act, int dtype, void* dgu, void* hw, float* dwts, void* stream);
+
+/*
+ * The expert layer on 16-bit weights, forward and backward (the unquantised form of moe_experts_run; reference
+ * moelab/variants/cuda/torch_loop.py:11-17, which has no backward pass):
+ *   y[t] = residual[t] + sum_j wts[t][j] w_down[e] . act(w_gate_up[e] . x[t]),  e = idx[t][j]
+ * w_gate_up [E, 2 F, d] (gate rows, then up), w_down [E, d, F]; x, residual [T, d] and the weights of m->dtype, y too or
+ * MOE_DTYPE_F32; idx [T, k] int32 (a slot with an id outside [0, E) adds nothing), wts [T, k] fp32.
+ * The gate/up rows, h and the slots' outputs are rounded to the 16-bit type between the launches.
+ *   keep [moe_mlp_keep_bytes]: the slots' grouping, which the backward pass reads; written in every case.
+ *   gu [T k, 2 F], or codes [T k, 2 F] and scales [T k, F / 16]: what the backward pass needs of the gate/up rows, in 16 or in
+ *   8 bits (forward: each may be NULL; backward: one of the two forms).
+ *   moe_mlp_bwd: dx [T, d], dwts [T, k] fp32, dw_gate_up, dw_down (as the weights), each may be NULL. dwts of slots with an id
+ *   outside [0, E) is left as it was. From the kept 8-bit values, gradients are those of the function at these values.
+ * Requirements: d % 8 == 0, F % 32 == 0, T d at most 0x58000000, T k < 2^31; pointers 16-byte aligned. workspace: any contents;
+ * forward and backward sizes from their queries. moe_mlp_bwd takes T > 0.
+ */
+typedef struct {
+    int32_t E, d, F, act, dtype;
+    const void* w_gate_up;
+    const void* w_down;
+} moe_mlp_t;
+size_t moe_mlp_keep_bytes(const moe_mlp_t* m, int T, int k);
+size_t moe_mlp_fwd_workspace_bytes(const moe_mlp_t* m, int T, int k);
+size_t moe_mlp_bwd_workspace_bytes(const moe_mlp_t* m, int T, int k);
+int moe_mlp_fwd(const moe_mlp_t* m, const void* x, const int32_t* idx, const float* wts, int T, int k, const void* residual,
+                void* y, int y_dtype, void* keep, void* gu, void* codes, void* scales, void* workspace, size_t workspace_bytes,
+                void* stream);
+int moe_mlp_bwd(const moe_mlp_t* m, const void* x, const float* wts, const void* dy, int T, int k, const void* keep, const void* gu,
+                const void* codes, const void* scales, void* dx, float* dwts, void* dw_gate_up, void* dw_down, void* workspace,
+                size_t workspace_bytes, void* stream);
 
 /* Library version and build target, for logs. */
 const char* moe_version(void);

@@ -25,7 +25,10 @@ EXPORTS = ("moe_router", "moe_router_counter_count", "moe_topk", "moe_group", "m
            "moe_tiles_pack", "moe_shared_experts_run", "moe_shared_experts_workspace_bytes", "moe_version",
            "moe_experts_run_static", "moe_layer_run", "moe_layer_workspace_bytes", "moe_experts_run_shared",
            "moe_experts_shared_workspace_bytes", "moe_router_group", "moe_layer_run_shared",
-           "moe_layer_shared_workspace_bytes", "moe_probe_read")
+           "moe_layer_shared_workspace_bytes", "moe_probe_read", "moe_grouped_mm", "moe_grouped_mm_dx", "moe_grouped_mm_dw",
+           "moe_linear", "moe_linear_workspace_bytes", "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack",
+           "moe_glu_fwd", "moe_glu_bwd", "moe_mlp_fwd", "moe_mlp_bwd", "moe_mlp_keep_bytes",
+           "moe_mlp_fwd_workspace_bytes", "moe_mlp_bwd_workspace_bytes")
 PROBE_SINK = 1024   # MOE_PROBE_SINK
 STATIC_SCRATCH_BYTES = 32 << 20   # MOE_STATIC_SCRATCH_BYTES: the workspace array of moe_experts_run_static
 STAGE_GATE_UP, STAGE_DOWN, STAGE_ALL = 1, 2, 3
@@ -54,6 +57,11 @@ class Experts(ctypes.Structure):
                 ("gate", Proj), ("up", Proj), ("down", Proj)]
 
 
+class Mlp(ctypes.Structure):
+    _fields_ = [("E", ctypes.c_int32), ("d", ctypes.c_int32), ("F", ctypes.c_int32), ("act", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("w_gate_up", ctypes.c_void_p), ("w_down", ctypes.c_void_p)]
+
+
 _lib = None
 
 
@@ -63,7 +71,7 @@ def lib():
         if not os.path.exists(LIB_PATH):
             raise RuntimeError(f"HIP library not built: {LIB_PATH} (run __graft_entry__.build())")
         L = ctypes.CDLL(LIB_PATH)
-        vp, i, f, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+        vp, i, i64, f, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
         L.moe_router.argtypes = [vp, vp, vp, i, i, i, i, i, f, vp, vp, vp, vp, vp]
         L.moe_router_counter_count.argtypes = [i]
         L.moe_topk.argtypes = [vp, i, i, i, i, i, f, vp, vp, vp]
@@ -85,6 +93,23 @@ def lib():
         L.moe_layer_workspace_bytes.restype = sz
         L.moe_version.restype = ctypes.c_char_p
         L.moe_probe_read.argtypes = [vp, sz, vp, vp]
+        L.moe_grouped_mm.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i, i, i, i, vp, i, i, vp]
+        L.moe_grouped_mm_dx.argtypes = [vp, vp, vp, vp, i64, i64, i64, i, i, i, i, vp, i, i, vp]
+        L.moe_grouped_mm_dw.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i, i, i, i, vp, i, vp, vp]
+        L.moe_linear.argtypes = [vp, vp, vp, vp, i, i64, i64, i, i, i, vp, i, vp, vp, sz, vp]
+        L.moe_linear_workspace_bytes.argtypes = [i64, i, i]
+        L.moe_linear_act_bwd.argtypes = [vp, i64, vp, vp, vp, i, i64, i, i, vp, vp]
+        L.moe_act8_pack.argtypes = [vp, i64, i64, i, i, vp, vp, vp]
+        L.moe_act8_unpack.argtypes = [vp, vp, i64, i, vp, i, vp]
+        L.moe_glu_fwd.argtypes = [vp, i64, i64, i, i, i, vp, vp, vp, vp]
+        L.moe_glu_bwd.argtypes = [vp, vp, vp, i64, vp, i, vp, i64, i, i, i, vp, vp, vp, vp]
+        mlp = ctypes.POINTER(Mlp)
+        L.moe_mlp_fwd.argtypes = [mlp, vp, vp, vp, i, i, vp, vp, i, vp, vp, vp, vp, vp, sz, vp]
+        L.moe_mlp_bwd.argtypes = [mlp, vp, vp, vp, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+        for n in ("moe_mlp_keep_bytes", "moe_mlp_fwd_workspace_bytes", "moe_mlp_bwd_workspace_bytes"):
+            getattr(L, n).argtypes = [mlp, i, i]
+            getattr(L, n).restype = sz
+        L.moe_linear_workspace_bytes.restype = sz
         L.moe_row_bytes.argtypes = [i, i]
         L.moe_row_bytes.restype = sz
         L.moe_tile_bytes.argtypes = [i, i, i]
@@ -100,7 +125,9 @@ def lib():
         for n in ("moe_router", "moe_router_counter_count", "moe_topk", "moe_group", "moe_experts_run",
                   "moe_experts_run_stages", "moe_tiles_pack", "moe_shared_experts_run", "moe_experts_run_static",
                   "moe_layer_run", "moe_experts_run_shared", "moe_router_group", "moe_layer_run_shared",
-                  "moe_probe_read"):
+                  "moe_probe_read", "moe_grouped_mm", "moe_grouped_mm_dx", "moe_grouped_mm_dw", "moe_linear",
+                  "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack", "moe_glu_fwd", "moe_glu_bwd", "moe_mlp_fwd",
+                  "moe_mlp_bwd"):
             getattr(L, n).restype = ctypes.c_int
         _lib = L
     return _lib
@@ -168,3 +195,69 @@ def workspace(device, nbytes):
         return buf
     return grow(_WS, device.index, max(int(nbytes), 256),
                 lambda n: torch.empty(n, dtype=torch.uint8, device=device), "the expert workspace")
+
+
+def call(name, device, *args):
+    """One library call on the current stream of `device` (the last C argument); another current device than the tensors' is
+    changed for the launch."""
+    fn = getattr(lib(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream_of(device))
+    if rc != MOE_OK:
+        raise MoeError(name, rc)
+
+
+def half_matrix(t, name, cols=None, device=None, dtype=None):
+    """t [rows, columns] as the 16-bit entry points take it: bf16 or fp16 (dtype if given), rows of neighbouring values, 16
+    bytes aligned with a stride of whole 16 bytes; any other layout is copied. Wrong types and shapes raise."""
+    require_device(t, name)
+    if t.dtype not in (torch.bfloat16, torch.float16) or (dtype is not None and t.dtype != dtype):
+        raise TypeError(f"{name} is {t.dtype}: " + ("bf16 or fp16 expected" if dtype is None else f"{dtype} expected, as the other operands"))
+    if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}: [rows, {'columns' if cols is None else cols}] expected")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < t.shape[1] or t.stride(0) > 1 << 21 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def plain(t, name, shape, device, dtype):
+    """t of exactly this shape, type and device, contiguous and 16-byte aligned (copied where it is not); None stays None."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{name} is {t.dtype}: {dtype} expected")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}: {tuple(shape)} expected")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+    if not t.is_contiguous() or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def result(out, shape, dtype, out_dtype, device):
+    """The call's output: out (checked), or a new tensor of out_dtype (the operands' type, or fp32)."""
+    if out is None:
+        out_dtype = dtype if out_dtype is None else out_dtype
+        if out_dtype not in (dtype, torch.float32):
+            raise TypeError(f"out_dtype {out_dtype}: the operands' type {dtype} or fp32 expected")
+        return torch.empty(shape, dtype=out_dtype, device=device)
+    if out.dtype not in (dtype, torch.float32) or (out_dtype is not None and out.dtype != out_dtype):
+        raise TypeError(f"out is {out.dtype}: the operands' type {dtype} or fp32 expected")
+    if tuple(out.shape) != tuple(shape) or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out: a contiguous, 16-byte aligned tensor of shape {tuple(shape)} on {device} expected")
+    return out
+
+
+def wants_grad(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def multiple_of(n, m, what):
+    if n < m or n % m:
+        raise ValueError(f"{what} = {n}: a multiple of {m} expected")
