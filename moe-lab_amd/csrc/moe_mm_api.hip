@@ -11,6 +11,7 @@ bool bad_ld(int64_t ld, int64_t cols) { return ld < cols || ld % 8 || ld > (1 <<
 bool too_far(int64_t rows, int64_t ld) { return rows * ld * 2 > 0xB0000000ll; }
 bool two_byte(int dtype) { return dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16; }
 bool bad_act8(int64_t M, int64_t C) { return M < 0 || M > 0x7fffffff || C < 32 || C % 32 || C > (1 << 20); }
+bool bad_rows(const int32_t* idx, int64_t rows, int64_t M) { return rows > 0x7fffffff || rows < (idx ? 1 : M); }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Parts of the expert layer's buffers, in bytes from their start.
@@ -48,7 +49,7 @@ struct MlpLayout {
     }
 };
 int check_mlp(const moe_mlp_t* m, int T, int k) {
-    if (!m || T < 0 || k < 1 || m->E < 1 || m->E > 8192 || (int64_t)T * k > 0x7fffffff) return MOE_ERR_ARG;
+    if (!m || T < 0 || k < 1 || m->E < 1 || m->E > MM_MAX_E || (int64_t)T * k > 0x7fffffff) return MOE_ERR_ARG;
     if (!two_byte(m->dtype)) return MOE_ERR_DTYPE;
     if (m->act < 0 || m->act > MOE_ACT_GPTOSS || bad_dim(m->d) || bad_act8(0, m->F) || bad_dim(2 * (int64_t)m->F)) return MOE_ERR_ARG;
     if (!m->w_gate_up || !m->w_down) return MOE_ERR_ARG;
@@ -65,9 +66,9 @@ int moe_grouped_mm(const void* x, const void* w, const void* bias, const int32_t
                    void* stream) {
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return MOE_ERR_DTYPE;
     if (y_dtype != dtype && y_dtype != MOE_DTYPE_F32) return MOE_ERR_DTYPE;
-    if (E < 1 || (!offsets && E != 1) || M < 0 || M > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(ldx, K)) return MOE_ERR_ARG;
+    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(ldx, K)) return MOE_ERR_ARG;
     if (M == 0) return MOE_OK;
-    if (!x || !w || !y || (!rows && x_rows < M) || (rows && x_rows < 1)) return MOE_ERR_ARG;
+    if (!x || !w || !y || bad_rows(rows, x_rows, M)) return MOE_ERR_ARG;
     if (misaligned(x) || misaligned(w) || misaligned(y) || misaligned(bias)) return MOE_ERR_ALIGN;
     if (rows && too_far(x_rows, ldx)) return MOE_ERR_ARG;
     moe::MmArgs a{};
@@ -76,9 +77,9 @@ int moe_grouped_mm(const void* x, const void* w, const void* bias, const int32_t
     a.offsets = offsets;
     a.arows = rows;
     a.y = y;
-    a.M = M;
-    a.a_n = x_rows;
-    a.lda = ldx;
+    a.M = (int)M;
+    a.a_n = (int)x_rows;
+    a.lda = (int)ldx;
     a.ldb = K;
     a.E = E;
     a.I = 0;
@@ -96,9 +97,9 @@ int moe_grouped_mm_dx(const void* dy, const void* w, const int32_t* offsets, con
                       void* stream) {
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return MOE_ERR_DTYPE;
     if (dx_dtype != dtype && dx_dtype != MOE_DTYPE_F32) return MOE_ERR_DTYPE;
-    if (E < 1 || (!offsets && E != 1) || M < 0 || M > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
+    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
     if (M == 0) return MOE_OK;
-    if (!dy || !w || !dx || (!rows && dy_rows < M) || (rows && dy_rows < 1)) return MOE_ERR_ARG;
+    if (!dy || !w || !dx || bad_rows(rows, dy_rows, M)) return MOE_ERR_ARG;
     if (misaligned(dy) || misaligned(w) || misaligned(dx)) return MOE_ERR_ALIGN;
     if (rows && too_far(dy_rows, lddy)) return MOE_ERR_ARG;
     moe::MmArgs a{};
@@ -107,9 +108,9 @@ int moe_grouped_mm_dx(const void* dy, const void* w, const int32_t* offsets, con
     a.offsets = offsets;
     a.arows = rows;
     a.y = dx;
-    a.M = M;
-    a.a_n = dy_rows;
-    a.lda = lddy;
+    a.M = (int)M;
+    a.a_n = (int)dy_rows;
+    a.lda = (int)lddy;
     a.ldb = K;
     a.E = E;
     a.J = K;
@@ -125,11 +126,11 @@ int moe_grouped_mm_dw(const void* dy, const void* x, const int32_t* offsets, con
                       void* dw, int dw_dtype, void* dbias, void* stream) {
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return MOE_ERR_DTYPE;
     if (dw_dtype != dtype && dw_dtype != MOE_DTYPE_F32) return MOE_ERR_DTYPE;
-    if (E < 1 || (!offsets && E != 1) || M < 0 || M > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N) ||
+    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N) ||
         bad_ld(ldx, K))
         return MOE_ERR_ARG;
     if (!dw || (M > 0 && (!dy || !x))) return MOE_ERR_ARG;
-    if (M > 0 && ((dy_idx ? dy_rows < 1 : dy_rows < M) || (x_idx ? x_rows < 1 : x_rows < M))) return MOE_ERR_ARG;
+    if (M > 0 && (bad_rows(dy_idx, dy_rows, M) || bad_rows(x_idx, x_rows, M))) return MOE_ERR_ARG;
     if (misaligned(dy) || misaligned(x) || misaligned(dw)) return MOE_ERR_ALIGN;
     // with a list for either operand both are addressed from their start
     if ((dy_idx || x_idx) && (too_far(dy_rows, lddy) || too_far(x_rows, ldx))) return MOE_ERR_ARG;
@@ -141,11 +142,11 @@ int moe_grouped_mm_dw(const void* dy, const void* x, const int32_t* offsets, con
     a.brows = x_idx;
     a.y = dw;
     a.dbias = dbias;
-    a.M = M;
-    a.a_n = dy_rows;
-    a.b_n = x_rows;
-    a.lda = lddy;
-    a.ldb = ldx;
+    a.M = (int)M;
+    a.a_n = (int)dy_rows;
+    a.b_n = (int)x_rows;
+    a.lda = (int)lddy;
+    a.ldb = (int)ldx;
     a.E = E;
     a.I = N;
     a.J = K;
@@ -174,9 +175,9 @@ int moe_linear(const void* x, const void* w, const void* bias, const void* resid
     a.a = x;
     a.b = w;
     a.y = y;
-    a.M = T;
-    a.a_n = T;
-    a.lda = ldx;
+    a.M = (int)T;
+    a.a_n = (int)T;
+    a.lda = (int)ldx;
     a.ldb = K;
     a.E = 1;
     a.J = N;
@@ -279,8 +280,8 @@ int moe_mlp_fwd(const moe_mlp_t* m, const void* x, const int32_t* idx, const flo
     a.offsets = offsets;
     a.arows = rows;
     a.y = g;
-    a.M = n;
-    a.a_n = T;
+    a.M = (int)n;
+    a.a_n = (int)T;
     a.lda = m->d;
     a.ldb = m->d;
     a.E = m->E;
@@ -297,7 +298,7 @@ int moe_mlp_fwd(const moe_mlp_t* m, const void* x, const int32_t* idx, const flo
     a.b = m->w_down;
     a.arows = nullptr;
     a.y = ws + L.ys;
-    a.a_n = n;
+    a.a_n = (int)n;
     a.lda = m->F;
     a.ldb = m->F;
     a.J = m->d;
@@ -335,8 +336,8 @@ int moe_mlp_bwd(const moe_mlp_t* m, const void* x, const float* wts, const void*
     a.offsets = offsets;
     a.arows = rows;
     a.y = ws + L.dh;
-    a.M = n;
-    a.a_n = T;
+    a.M = (int)n;
+    a.a_n = (int)T;
     a.lda = m->d;
     a.ldb = m->F;
     a.E = m->E;
@@ -356,8 +357,8 @@ int moe_mlp_bwd(const moe_mlp_t* m, const void* x, const float* wts, const void*
         a.b = m->w_gate_up;
         a.arows = nullptr;
         a.y = ws + L.dxs;
-        a.a_n = n;
-        a.lda = 2 * (int64_t)m->F;
+        a.a_n = (int)n;
+        a.lda = 2 * m->F;
         a.ldb = m->d;
         a.J = m->d;
         a.R = 2 * m->F;
@@ -369,7 +370,7 @@ int moe_mlp_bwd(const moe_mlp_t* m, const void* x, const float* wts, const void*
     }
     moe::MmArgs w{};
     w.offsets = offsets;
-    w.M = n;
+    w.M = (int)n;
     w.E = m->E;
     w.f16 = f16;
     w.ydt = m->dtype;
@@ -378,9 +379,9 @@ int moe_mlp_bwd(const moe_mlp_t* m, const void* x, const float* wts, const void*
         w.b = x;
         w.brows = rows;
         w.y = dw_gate_up;
-        w.a_n = n;
+        w.a_n = (int)n;
         w.b_n = T;
-        w.lda = 2 * (int64_t)m->F;
+        w.lda = 2 * m->F;
         w.ldb = m->d;
         w.I = 2 * m->F;
         w.J = m->d;
@@ -394,7 +395,7 @@ int moe_mlp_bwd(const moe_mlp_t* m, const void* x, const float* wts, const void*
         w.brows = nullptr;
         w.y = dw_down;
         w.a_n = T;
-        w.b_n = n;
+        w.b_n = (int)n;
         w.lda = m->d;
         w.ldb = m->F;
         w.I = m->d;

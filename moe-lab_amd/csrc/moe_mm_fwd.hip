@@ -2,17 +2,23 @@
 
 namespace moe {
 
-int launch_mm_fwd(const MmArgs& a, hipStream_t st) {
+template <bool F16>
+static int launch(const MmArgs& a, hipStream_t st) {
     const int force = env_int("MM_CFG", -1);
     const int64_t live = a.offsets ? (a.E < a.M ? a.E : a.M) : 1;   // groups that can hold a slot
     const int64_t avg = a.M / live;
-    auto tiles = [&](int b) { return (live + a.M / b) * ((a.J + b - 1) / b); };
-    int c = avg <= 4 ? 3 : avg > 64 && tiles(256) >= 192 ? 0 : avg > 32 && tiles(128) >= 192 ? 1 : 2;
+    auto tiles = [&](int bi, int bj) { return (live + a.M / bi) * ((a.J + bj - 1) / bj); };
+    int c = avg <= 4 ? 3 : avg > 64 && tiles(256, 256) >= 192 ? 0 : avg > 32 && tiles(128, 128) >= 192 ? 1 : 2;
     if (force >= 0) c = force;
-    if (c == 3) return launch_mm_rows(a, st);
-    if (c == 0) return a.f16 ? launch_mm_cfg<MM_FWD, true, 8, 8, 2, 1>(a, st) : launch_mm_cfg<MM_FWD, false, 8, 8, 2, 1>(a, st);
-    if (c == 1) return a.f16 ? launch_mm_cfg<MM_FWD, true, 4, 4, 2, 2>(a, st) : launch_mm_cfg<MM_FWD, false, 4, 4, 2, 2>(a, st);
-    return a.f16 ? launch_mm_cfg<MM_FWD, true, 2, 2, 4, 2>(a, st) : launch_mm_cfg<MM_FWD, false, 2, 2, 4, 2>(a, st);
+    switch (c) {
+        case 0: return launch_mm_cfg<MM_FWD, F16, 8, 8, 2, 2, 1>(a, st);
+        case 5: return launch_mm_cfg<MM_FWD, F16, 8, 4, 4, 2, 1>(a, st);
+        case 1: return launch_mm_cfg<MM_FWD, F16, 4, 4, 2, 2, 2>(a, st);
+        case 2: return launch_mm_cfg<MM_FWD, F16, 2, 2, 2, 4, 2>(a, st);
+        case 4: return launch_mm_cfg<MM_FWD, F16, 4, 8, 2, 3, 1>(a, st);
+        default: return launch_mm_rows(a, st);
+    }
 }
+int launch_mm_fwd(const MmArgs& a, hipStream_t st) { return a.f16 ? launch<true>(a, st) : launch<false>(a, st); }
 
 }  // namespace moe

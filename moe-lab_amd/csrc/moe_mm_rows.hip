@@ -15,14 +15,13 @@ template <bool F16, int R, int MR>
 __global__ void __launch_bounds__(256) k_mm_rows(const MmArgs g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n0 = (blockIdx.x * 4 + wave) * R;
-    const int64_t p = blockIdx.y;
-    int e = 0;
-    int64_t lo = 0, hi = g.M;
+    const int p = blockIdx.y;
+    int e = 0, lo = 0, hi = g.M;
     if (g.offsets) {
         // the group whose first slot is p (none: p lies inside a group, or behind the last)
         e = -1;
         for (int base = 0; base < g.E && e < 0; base += 64) {
-            int64_t l = -1, h = -1;
+            int l = -1, h = -1;
             if (base + lane < g.E) group_of(g, base + lane, l, h);
             const uint64_t hit = __ballot(l == p && h > l);
             if (hit) {
@@ -33,27 +32,27 @@ __global__ void __launch_bounds__(256) k_mm_rows(const MmArgs g) {
         }
         if (e < 0) {
             if (!g.fill) return;
-            int64_t l, h;
+            int l, h;
             group_of(g, g.E - 1, l, h);
             if (p < h) return;
             if (lane < R && n0 + lane < g.J) {
-                if (g.ydt == MOE_DTYPE_F32) ((float*)g.y)[p * g.J + n0 + lane] = 0.f;
-                else ((uint16_t*)g.y)[p * g.J + n0 + lane] = 0;
+                if (g.ydt == MOE_DTYPE_F32) ((float*)g.y)[(int64_t)p * g.J + n0 + lane] = 0.f;
+                else ((uint16_t*)g.y)[(int64_t)p * g.J + n0 + lane] = 0;
             }
             return;
         }
     }
     if (n0 >= g.J) return;
     const uint16_t* w = (const uint16_t*)g.b + ((int64_t)e * g.J + n0) * g.ldb;
-    for (int64_t m0 = lo; m0 < hi; m0 += MR) {
+    for (int m0 = lo; m0 < hi; m0 += MR) {
         const uint16_t* x[MR];
         bool live[MR];
 #pragma unroll
         for (int m = 0; m < MR; ++m) {
-            int64_t s = m0 + m < hi ? m0 + m : lo;
+            int s = m0 + m < hi ? m0 + m : lo;
             if (g.arows) s = g.arows[s];
             live[m] = s >= 0 && s < g.a_n;
-            x[m] = (const uint16_t*)g.a + (live[m] ? s : 0) * g.lda;
+            x[m] = (const uint16_t*)g.a + (int64_t)(live[m] ? s : 0) * g.lda;
         }
         float acc[R][MR] = {};
         auto chunk = [&](int c) {
@@ -88,7 +87,7 @@ __global__ void __launch_bounds__(256) k_mm_rows(const MmArgs g) {
             const int n = n0 + lane;
             if (lane < R && n < g.J) {
                 if (!live[m]) v = 0.f;
-                const int64_t at = (m0 + m) * g.J + n;
+                const int64_t at = (int64_t)(m0 + m) * g.J + n;
                 if (g.epi.bias) v += un16<F16>(((const uint16_t*)g.epi.bias)[(int64_t)e * g.J + n]);
                 if (g.epi.z) ((uint16_t*)g.epi.z)[at] = (uint16_t)pack16<F16>(v, 0.f);
                 v = lin_act(g.epi.act, v);

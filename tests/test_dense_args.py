@@ -35,7 +35,7 @@ def lin(**k):
     return _lib.lib().moe_linear(*a.values(), None)
 
 
-COMMON = [(dict(dt=2), DT), (dict(dt=7), DT), (dict(E=0), ARG), (dict(off=None), ARG), (dict(M=-1), ARG), (dict(M=2 ** 31), ARG),
+COMMON = [(dict(dt=2), DT), (dict(dt=7), DT), (dict(E=0), ARG), (dict(E=1025), ARG), (dict(off=None), ARG), (dict(M=-1), ARG), (dict(M=2 ** 31), ARG),
           (dict(N=60), ARG), (dict(K=4), ARG), (dict(N=0), ARG), (dict(K=2 ** 21), ARG), (dict(w=BAD), AL), (dict(w=None), ARG)]
 
 
@@ -107,7 +107,7 @@ def _mlp(**k):
 
 @pytest.mark.parametrize("m,case,rc", [
     (dict(dtype=2), {}, DT), (dict(act=4), {}, ARG), (dict(d=60), {}, ARG), (dict(F=40), {}, ARG), (dict(E=0), {}, ARG),
-    (dict(E=10000), {}, ARG), (dict(w_down=None), {}, ARG), (dict(w_gate_up=BAD), {}, AL), ({}, dict(T=-1), ARG), ({}, dict(k=0), ARG),
+    (dict(E=1025), {}, ARG), (dict(w_down=None), {}, ARG), (dict(w_gate_up=BAD), {}, AL), ({}, dict(T=-1), ARG), ({}, dict(k=0), ARG),
     ({}, dict(T=FAR), ARG), ({}, dict(T=2 ** 30, k=4), ARG), ({}, dict(ydt=1), DT), ({}, dict(x=None), ARG), ({}, dict(keep=None), ARG),
     ({}, dict(codes=P), ARG), ({}, dict(ws=None), WS), ({}, dict(wsb=100), WS), ({}, dict(y=BAD), AL), ({}, dict(T=0, x=None), 0)])
 def test_mlp_fwd(m, case, rc):
