@@ -380,13 +380,13 @@ int moe_glu_bwd(const void* codes, const void* scales, const void* gu, int64_t l
  *   y[t] = residual[t] + sum_j wts[t][j] w_down[e] . act(w_gate_up[e] . x[t]),  e = idx[t][j]
  * w_gate_up [E, 2 F, d] (gate rows, then up), w_down [E, d, F]; x, residual [T, d] and the weights of m->dtype, y too or
  * MOE_DTYPE_F32; idx [T, k] int32 (a slot with an id outside [0, E) adds nothing), wts [T, k] fp32.
- * The gate/up rows, h and the slots' outputs are rounded to the 16-bit type between the launches.
+ * h and the slots' outputs are rounded to the 16-bit type between the launches; the GLU takes the gate/up sums in fp32.
  *   keep [moe_mlp_keep_bytes]: the slots' grouping, which the backward pass reads; written in every case.
  *   gu [T k, 2 F], or codes [T k, 2 F] and scales [T k, F / 16]: what the backward pass needs of the gate/up rows, in 16 or in
  *   8 bits (forward: each may be NULL; backward: one of the two forms).
  *   moe_mlp_bwd: dx [T, d], dwts [T, k] fp32, dw_gate_up, dw_down (as the weights), each may be NULL. dwts of slots with an id
  *   outside [0, E) is left as it was. From the kept 8-bit values, gradients are those of the function at these values.
- * Requirements: E <= 1024, d % 8 == 0, F % 32 == 0, T d at most 0x58000000, T k < 2^31; pointers 16-byte aligned. workspace: any contents;
+ * Requirements: E <= 1024, d % 8 == 0, F % 32 == 0, T d and 2 F d at most 0x58000000, T k < 2^31; pointers 16-byte aligned. workspace: any contents;
  * forward and backward sizes from their queries. moe_mlp_bwd takes T > 0.
  */
 typedef struct {

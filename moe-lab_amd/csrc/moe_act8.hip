@@ -6,12 +6,6 @@
 
 namespace moe {
 
-// ---------------------------------------------------------------------------------------------- 8-bit values
-// Blocks of 32 neighbours share one exponent byte s: value = q 2^(s - 133), q in [-127, 127]. s is the biased exponent of
-// the block's largest magnitude (so that one keeps 7 bits, 64 <= |q| <= 127), one more where it would round to 128; 0 for a
-// block below 2^-126 (whose 16-bit values stay exact), 255 marks a block that holds an infinity or NaN and reads as NaN.
-// With a power of two the scaling is exact, so an element is off by its rounding alone, at most half a step 2^(s - 133):
-// 1/128 to 1/256 of the block's largest.
 __device__ __forceinline__ uint32_t max_block(uint32_t v) {   // over the 4 lanes of 8 values that make a block of 32
     v = dpp_umax<0xB1>(v);
     return dpp_umax<0x4E>(v);
@@ -36,52 +30,17 @@ __device__ __forceinline__ u32x2 quantise8(const float (&v)[8], uint32_t& s) {
         const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
         b = a > b ? a : b;
     }
-    b = max_block(b);
-    s = b >> 23;
-    if (s > 0 && s < 254 && (b & 0x7fffffu) >= 0x7f0000u) ++s;   // 127.5 and up
+    s = exponent8(max_block(b));
     u32x2 q = {0, 0};
     if (s < 255) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float r = fminf(fmaxf(rintf(ldexpf(v[i], 133 - (int)s)), -127.f), 127.f);
-            q[i >> 2] |= ((uint32_t)(int)r & 255u) << (8 * (i & 3));
-        }
+        for (int i = 0; i < 8; ++i) q[i >> 2] |= code8(v[i], s) << (8 * (i & 3));
     }
     return q;
 }
 __device__ __forceinline__ void values8(u32x2 q, uint32_t s, float (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float f = (float)(int8_t)(q[i >> 2] >> (8 * (i & 3)));
-        v[i] = s == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(f, (int)s - 133);
-    }
-}
-
-// ---------------------------------------------------------------------------------------------- GLU and gradients
-// h = f(g) * m(u), with df/dg and dm/du. act 2 clamps g <= 7, |u| <= 7: no gradient where the clamp holds.
-__device__ __forceinline__ void glu_parts(int act, float g, float u, float& f, float& m, float& df, float& dm) {
-    m = u;
-    dm = 1.f;
-    if (act == MOE_ACT_GEGLU) {
-        const float z = 1.5957691216057308f * (g + 0.044715f * g * g * g), s = sigmoid_fast(z);
-        f = g * s;
-        // far out sigmoid' is 0 and the polynomial overflows: their product is 0
-        const float ds = s * (1.f - s);
-        df = s + (ds == 0.f ? 0.f : g * ds * 1.5957691216057308f * (1.f + 0.134145f * g * g));
-        return;
-    }
-    float a = 1.f, on = 1.f;
-    if (act == MOE_ACT_GPTOSS) {
-        a = 1.702f;
-        // comparisons that a NaN fails leave it in place
-        on = g > 7.f ? 0.f : 1.f;
-        dm = u > 7.f || u < -7.f ? 0.f : 1.f;
-        g = g > 7.f ? 7.f : g;
-        m = (u > 7.f ? 7.f : u < -7.f ? -7.f : u) + 1.f;
-    }
-    const float s = sigmoid_fast(a * g), ds = s * (1.f - s);
-    f = g * s;
-    df = on * (s + (ds == 0.f ? 0.f : a * g * ds));
+    for (int i = 0; i < 8; ++i) v[i] = value8(q[i >> 2] >> (8 * (i & 3)), s);
 }
 
 // gu [M, 2 F] -> h [M, F], and (codes not null) the 8-bit form of gu. One item: 8 columns of gate and up.

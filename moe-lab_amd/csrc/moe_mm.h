@@ -6,6 +6,7 @@
 // (x and w in the forward pass, dy in dx) or with its own index contiguous (w in dx, both operands in dw).
 #pragma once
 #include "moe_common.h"
+#include "moe_glu8.h"
 #include "moe_internal.h"
 
 namespace moe {
@@ -137,11 +138,21 @@ struct Operand {
     }
 };
 
+// What the forward product's epilogue does with a tile's sums.
+enum MmEpiKind {
+    EPI_PLAIN = 0,
+    EPI_LIN = 1,    // bias, activation, residual, z (moe_linear; bias alone: moe_grouped_mm)
+    EPI_GLU = 2     // w is [E, 2 F, K], gate rows then up: y = act(gate, up) [M, F], and optionally the gate/up rows themselves
+                    // in 16 bits or in 8 (moe_glu8.h)
+};
 struct MmEpi {
     const void* bias;        // [E, J] of the operands' type, or null
     const void* residual;    // [M, J] of the operands' type, or null
     void* z;                 // [M, J] of the operands' type: the sums with bias, before the activation; or null
-    int act;                 // MOE_LIN_*
+    int act;                 // MOE_LIN_*; EPI_GLU: MOE_ACT_*
+    void* gu;                // EPI_GLU: [M, 2 F] of the operands' type, or null
+    uint8_t* codes;          // EPI_GLU: [M, 2 F] and scales [M, F / 16], or null
+    uint8_t* scales;
 };
 
 struct MmArgs {
@@ -155,7 +166,8 @@ struct MmArgs {
     int M;                   // slots
     int a_n, b_n;            // rows of a and (dw) b
     int lda, ldb;            // elements between rows; ldb of forward and dx: K
-    int E, I, J, R;          // dw: I = N, J = K; forward: J = N, R = K; dx: J = K, R = N
+    int E, I, J, R;          // dw: I = N, J = K; forward: J = N (EPI_GLU: F), R = K; dx: J = K, R = N
+    int kind;                // forward: MmEpiKind
     int f16, ydt, fill;      // ydt: MOE_DTYPE_*; fill: rows behind the last group are set to zero
     MmEpi epi;
 };
@@ -274,12 +286,14 @@ __device__ __forceinline__ f32x4 load4(const void* p, int64_t i) {
 // A workgroup goes through its tiles with two streams: loads run ST steps ahead of the products and pass from one tile into the
 // next, so a tile's first stages arrive during the last one's products and stores. Every step loads the same number of pieces
 // (past the last tile from empty descriptors: zeros, no traffic), so the waits are constants.
-// FULL: the epilogue with bias, activation, residual and z.
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, bool GATHER, bool FULL>
+// EPI_GLU: the tile's columns are BJ / 2 of gate and the same of up, half by half for each wave, so that a lane holds both.
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, bool GATHER, int EPI>
 struct MmKernel {
+    static constexpr bool GLU = EPI == EPI_GLU;
     static constexpr bool ACC = FA * FB * 4 >= 256;   // the sums fill the accumulation registers
     static constexpr bool AX = MODE == MM_DW, BX = MODE != MM_FWD;   // operand with its own index contiguous
     static constexpr int NW = 2 * NWJ, BI = 32 * FA, BJ = 16 * NWJ * FB;
+    static constexpr int TJ = GLU ? BJ / 2 : BJ;   // output columns of a tile
     using A = Operand<AX, BI, NW>;
     using B = Operand<BX, BJ, NW>;
     static constexpr int PA = A::PIECES, PB = B::PIECES;
@@ -314,7 +328,7 @@ struct MmKernel {
             for (int h = 0; h < FB; h += 2) {
                 f32x4 v[2] = {acc[f][h], acc[f][h + 1]};
                 uint32_t zz[2][2];
-                if constexpr (FULL) {
+                if constexpr (EPI == EPI_LIN) {
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const int j = jw + 16 * (h + u) + 4 * q;
@@ -332,14 +346,10 @@ struct MmKernel {
                         }
                     }
                 }
-                // 16-bit rows: two column blocks change halves between neighbouring rows of lanes, so that a lane holds
-                // eight neighbours and stores 16 bytes
                 const int jj = jw + 16 * (h + (q & 1)) + 4 * (q & 2);
                 const uint32_t to = jj < g.J ? (row + jj) * 2 : MM_OOB;
                 auto put = [&](__amdgpu_buffer_rsrc_t out, uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
-                    const auto s0 = __builtin_amdgcn_permlane16_swap(a0, b0, false, false);
-                    const auto s1 = __builtin_amdgcn_permlane16_swap(a1, b1, false, false);
-                    __builtin_amdgcn_raw_buffer_store_b128((u32x4){s0[0], s1[0], s0[1], s1[1]}, out, to, 0, 0);
+                    __builtin_amdgcn_raw_buffer_store_b128(eight(a0, a1, b0, b1), out, to, 0, 0);
                 };
                 if (f32) {
 #pragma unroll
@@ -351,8 +361,103 @@ struct MmKernel {
                     put(yb, pack16<F16>(v[0][0], v[0][1]), pack16<F16>(v[0][2], v[0][3]), pack16<F16>(v[1][0], v[1][1]),
                         pack16<F16>(v[1][2], v[1][3]));
                 }
-                if constexpr (FULL) put(zb, zz[0][0], zz[0][1], zz[1][0], zz[1][1]);
+                if constexpr (EPI == EPI_LIN) put(zb, zz[0][0], zz[0][1], zz[1][0], zz[1][1]);
                 __builtin_amdgcn_sched_barrier(0);   // not all pairs' loads and packed sums at once: they would spill
+            }
+        }
+    }
+
+    // Column pairs (h, h + 1) of 16-bit halves x, y of a lane's row: two column blocks change halves between neighbouring rows of
+    // lanes, so that a lane holds eight neighbours.
+    static __device__ __forceinline__ u32x4 eight(uint32_t a0, uint32_t a1, uint32_t b0, uint32_t b1) {
+        const auto s0 = __builtin_amdgcn_permlane16_swap(a0, b0, false, false);
+        const auto s1 = __builtin_amdgcn_permlane16_swap(a1, b1, false, false);
+        return (u32x4){s0[0], s1[0], s0[1], s1[1]};
+    }
+    static __device__ __forceinline__ uint32_t max_rows(uint32_t v) {   // over the four lanes of one output row
+        const auto s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = s[0] > s[1] ? s[0] : s[1];
+        const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return p[0] > p[1] ? p[0] : p[1];
+    }
+    // EPI_GLU. Two column blocks (32 columns: one block of the 8-bit form) at a time: h = act(gate, up) from the fp32 sums; the kept
+    // rows from the sums rounded to 16 bits, as a pass over 16-bit rows would find them.
+    static __device__ __forceinline__ void store_glu(const MmArgs& g, const MmTile& t, f32x4 (&acc)[FA][FB], int lane, int wi, int wj) {
+        constexpr int H = FB / 2;
+        static_assert(!GLU || H % 2 == 0, "a block of 32 columns per wave");
+        const int l = lane & 15, q = lane >> 4, jw = t.j0 + wj * H * 16, F = g.J;
+        const auto rsrc = [&](const void* p, int64_t row_bytes) {
+            return __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<void*>(p) + t.lo * row_bytes, 0,
+                                                     p ? (uint32_t)t.rows * (uint32_t)row_bytes : 0u, 0x00027000);
+        };
+        const auto hb = rsrc(g.y, (int64_t)F * 2), gb = rsrc(g.epi.gu, (int64_t)F * 4), cb = rsrc(g.epi.codes, (int64_t)F * 2),
+                   sb = rsrc(g.epi.scales, F / 16);
+#pragma unroll
+        for (int f = 0; f < FA; ++f) {
+            if (32 * f >= t.rows) break;
+            if constexpr (ACC) {
+#pragma unroll
+                for (int h = 0; h < FB; ++h) asm volatile("" : "+a"(acc[f][h]));
+            }
+            const int i = 16 * (2 * f + wi) + l;
+            const bool in = i < t.rows;
+#pragma unroll
+            for (int h = 0; h < H; h += 2) {
+                const int jj = jw + 16 * (h + (q & 1)) + 4 * (q & 2);   // the eight columns this lane stores
+                const bool ok = in && jj < F;
+                uint32_t w[2][2][2], o[2][2];   // [gate or up][column block][pair], and h
+                uint32_t top[2] = {0, 0};
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const f32x4 a = acc[f][h + u], b = acc[f][H + h + u];
+                    float r[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float x, m, dx, dm;
+                        glu_parts(g.epi.act, a[c], b[c], x, m, dx, dm);
+                        r[c] = x * m;
+                    }
+                    o[u][0] = pack16<F16>(r[0], r[1]);
+                    o[u][1] = pack16<F16>(r[2], r[3]);
+                    w[0][u][0] = pack16<F16>(a[0], a[1]);
+                    w[0][u][1] = pack16<F16>(a[2], a[3]);
+                    w[1][u][0] = pack16<F16>(b[0], b[1]);
+                    w[1][u][1] = pack16<F16>(b[2], b[3]);
+                }
+                __builtin_amdgcn_raw_buffer_store_b128(eight(o[0][0], o[0][1], o[1][0], o[1][1]), hb,
+                                                       ok ? ((uint32_t)i * F + jj) * 2 : MM_OOB, 0, 0);
+                if (g.epi.gu) {
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+                        __builtin_amdgcn_raw_buffer_store_b128(eight(w[s][0][0], w[s][0][1], w[s][1][0], w[s][1][1]), gb,
+                                                               ok ? ((uint32_t)i * 2 * F + s * F + jj) * 2 : MM_OOB, 0, 0);
+                }
+                if (g.epi.codes) {
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        float v[2][4];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                v[u][c] = un16<F16>(w[s][u][c >> 1] >> (16 * (c & 1)));
+                                const uint32_t m = __float_as_uint(v[u][c]) & 0x7fffffffu;
+                                top[s] = m > top[s] ? m : top[s];
+                            }
+                        const uint32_t e = exponent8(max_rows(top[s]));
+                        uint32_t k[2] = {0, 0};
+                        if (e < 255)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) k[u] |= code8(v[u][c], e) << (8 * c);
+                        const auto p = __builtin_amdgcn_permlane16_swap(k[0], k[1], false, false);
+                        __builtin_amdgcn_raw_buffer_store_b64((u32x2){p[0], p[1]}, cb, ok ? (uint32_t)i * 2 * F + s * F + jj : MM_OOB, 0, 0);
+                        if (q == 0)
+                            __builtin_amdgcn_raw_buffer_store_b8((uint8_t)e, sb, ok ? (uint32_t)i * (F / 16) + (s * F + jw + 16 * h) / 32 : MM_OOB, 0, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
@@ -365,7 +470,7 @@ struct MmKernel {
         const int lda2 = g.lda * 2, ldb2 = g.ldb * 2;
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)sm;
 
-        const int nj = (g.J + BJ - 1) / BJ;
+        const int nj = (g.J + TJ - 1) / TJ;
         int tiles;
         if constexpr (MODE == MM_DW) {
             tiles = g.E * ((g.I + BI - 1) / BI) * nj;
@@ -376,8 +481,8 @@ struct MmKernel {
         }
         const MmRun run = xcd_run(tiles);
         auto tile = [&](int id, MmTile& t) {
-            if constexpr (MODE == MM_DW) tile_at_dw<BI, BJ>(g, id, t);
-            else tile_at<BI, BJ>(g, pre, id, t);
+            if constexpr (MODE == MM_DW) tile_at_dw<BI, TJ>(g, id, t);
+            else tile_at<BI, TJ>(g, pre, id, t);
         };
         auto steps_of = [&](const MmTile& t) -> int { return MODE == MM_DW ? (t.cnt + 63) / 64 : (g.R + 63) / 64; };
 
@@ -428,11 +533,16 @@ struct MmKernel {
             }
 #pragma unroll
             for (int i = 0; i < PB; ++i) {
-                const int c = B::col_of(colb, i);
-                offb[i] = (uint32_t)((rowb + B::ROWS * i) * ldb2 + c * 2);
+                const int c = B::col_of(colb, i), r = rowb + B::ROWS * i;
+                offb[i] = (uint32_t)(r * ldb2 + c * 2);
                 if (BX && lt.j0 + c >= g.J) offb[i] = MM_OOB;
+                if constexpr (GLU) {
+                    constexpr int W = 16 * FB, H = W / 2;   // a wave's columns, and its gate ones
+                    const int j = lt.j0 + r / W * H + r % H;
+                    offb[i] = j < g.J ? (uint32_t)((r % W < H ? j : g.J + j) * ldb2 + c * 2) : MM_OOB;
+                }
             }
-            if constexpr (MODE == MM_FWD) pb += ((int64_t)lt.e * g.J + lt.j0) * ldb2;
+            if constexpr (MODE == MM_FWD) pb += GLU ? (int64_t)lt.e * 2 * g.J * ldb2 : ((int64_t)lt.e * g.J + lt.j0) * ldb2;
             if constexpr (MODE == MM_DX) pb += (int64_t)lt.e * g.R * ldb2 + (int64_t)lt.j0 * 2;
             if constexpr (MODE == MM_DW) pb += (gath_b ? 0 : (int64_t)lt.lo * ldb2) + (int64_t)lt.j0 * 2;
             fetch_rows();
@@ -446,7 +556,7 @@ struct MmKernel {
         };
         auto bytes_b = [&]() -> uint32_t {
             if (!lrows) return 0;
-            if constexpr (!BX) return (uint32_t)(min(BJ, g.J - lt.j0) - 1) * (uint32_t)ldb2 + (uint32_t)(g.R - 64 * ls) * 2;
+            if constexpr (!BX) return (uint32_t)((GLU ? 2 * g.J : min(BJ, g.J - lt.j0)) - 1) * (uint32_t)ldb2 + (uint32_t)(g.R - 64 * ls) * 2;
             const int rows = MODE == MM_DX ? min(64, g.R - 64 * ls) : gath_b ? g.b_n : min(64, lt.cnt - 64 * ls);
             return (uint32_t)(rows - 1) * (uint32_t)ldb2 + (uint32_t)(g.J - lt.j0) * 2;
         };
@@ -605,7 +715,8 @@ struct MmKernel {
 #pragma unroll
                     for (int h = 0; h < FB; ++h) asm volatile("" : "+a"(acc[f][h]));
             }
-            store(g, t, acc, lane, wi, wj);
+            if constexpr (GLU) store_glu(g, t, acc, lane, wi, wj);
+            else store(g, t, acc, lane, wi, wj);
             if constexpr (DB) {
                 if (bias && wj == 0) {
 #pragma unroll
@@ -622,9 +733,9 @@ struct MmKernel {
     }
 };
 
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, bool GATHER, bool FULL>
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, bool GATHER, int EPI>
 __global__ void __launch_bounds__(128 * NWJ, OCC * NWJ / 2) k_mm(const MmArgs g) {
-    using K = MmKernel<MODE, F16, FA, FB, NWJ, ST, GATHER, FULL>;
+    using K = MmKernel<MODE, F16, FA, FB, NWJ, ST, GATHER, EPI>;
     __shared__ __attribute__((aligned(1024))) char sm[ST * K::STAGE];
     __shared__ int pre[MODE == MM_DW ? 1 : MM_MAX_E + 1];
     K::block(g, sm, pre);
@@ -645,21 +756,30 @@ inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
 template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC>
 int launch_mm_cfg(const MmArgs& a, hipStream_t st) {
-    const int64_t nj = (a.J + 16 * NWJ * FB - 1) / (16 * NWJ * FB);
+    const bool glu = MODE == MM_FWD && a.kind == EPI_GLU, gather = a.arows || (MODE == MM_DW && a.brows);
+    const int bj = 16 * NWJ * FB / (glu ? 2 : 1);
+    const int64_t nj = (a.J + bj - 1) / bj;
     const int64_t ni = MODE == MM_DW ? (int64_t)a.E * ((a.I + 32 * FA - 1) / (32 * FA)) : mm_row_tiles(a, 32 * FA);
     if (ni * nj == 0) return MOE_OK;
-    const int64_t most = 256 * OCC, grid = round8(ni * nj) < most ? round8(ni * nj) : most;   // 256 CUs
     if (ni * nj > 0x7fffffff) return MOE_ERR_ARG;
-    const bool gather = a.arows || (MODE == MM_DW && a.brows);
+    const int64_t most = 256 * OCC, grid = round8(ni * nj) < most ? round8(ni * nj) : most;   // 256 CUs
+    auto go = [&](auto epi) {
+        constexpr int EPI = decltype(epi)::value;
+        if (gather) k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, true, EPI><<<(unsigned)grid, 128 * NWJ, 0, st>>>(a);
+        else k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, false, EPI><<<(unsigned)grid, 128 * NWJ, 0, st>>>(a);
+    };
     if constexpr (MODE == MM_FWD) {
-        if (a.epi.bias || a.epi.residual || a.epi.z || a.epi.act != MOE_LIN_NONE) {
-            if (gather) k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, true, true><<<(unsigned)grid, 128 * NWJ, 0, st>>>(a);
-            else k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, false, true><<<(unsigned)grid, 128 * NWJ, 0, st>>>(a);
-            return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;
+        if (glu) {
+            if constexpr (FB % 4 == 0) go(std::integral_constant<int, EPI_GLU>{});
+            else return MOE_ERR_ARG;
+        } else if (a.kind == EPI_LIN) {
+            go(std::integral_constant<int, EPI_LIN>{});
+        } else {
+            go(std::integral_constant<int, EPI_PLAIN>{});
         }
+    } else {
+        go(std::integral_constant<int, EPI_PLAIN>{});
     }
-    if (gather) k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, true, false><<<(unsigned)grid, 128 * NWJ, 0, st>>>(a);
-    else k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, false, false><<<(unsigned)grid, 128 * NWJ, 0, st>>>(a);
     return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;
 }
 

@@ -17,7 +17,7 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 // Parts of the expert layer's buffers, in bytes from their start.
 struct MlpLayout {
     size_t offsets, sorted, rows, pos, keep;                 // kept for the backward pass
-    size_t counts, active, meta, chunks, gu, h, ys, fwd;     // forward workspace
+    size_t counts, active, meta, chunks, h, ys, fwd;     // forward workspace
     size_t dh, dgu, hw, dxs, bwd;                            // backward workspace
     MlpLayout(const moe_mlp_t& m, int64_t n) {
         size_t at = 0;
@@ -36,7 +36,6 @@ struct MlpLayout {
         active = take((size_t)m.E * 4);
         meta = take(16);
         chunks = take((size_t)256 * m.E * 4);
-        gu = take((size_t)n * 2 * m.F * 2);
         h = take((size_t)n * m.F * 2);
         ys = take((size_t)n * m.d * 2);
         fwd = at;
@@ -54,7 +53,7 @@ int check_mlp(const moe_mlp_t* m, int T, int k) {
     if (m->act < 0 || m->act > MOE_ACT_GPTOSS || bad_dim(m->d) || bad_act8(0, m->F) || bad_dim(2 * (int64_t)m->F)) return MOE_ERR_ARG;
     if (!m->w_gate_up || !m->w_down) return MOE_ERR_ARG;
     if (misaligned(m->w_gate_up) || misaligned(m->w_down)) return MOE_ERR_ALIGN;
-    if (too_far(T, m->d)) return MOE_ERR_ARG;
+    if (too_far(T, m->d) || too_far(2 * (int64_t)m->F, m->d)) return MOE_ERR_ARG;
     return MOE_OK;
 }
 }  // namespace
@@ -89,6 +88,7 @@ int moe_grouped_mm(const void* x, const void* w, const void* bias, const int32_t
     a.ydt = y_dtype;
     a.fill = fill;
     a.epi.bias = bias;
+    a.kind = bias ? moe::EPI_LIN : moe::EPI_PLAIN;
     return moe::launch_mm_fwd(a, (hipStream_t)stream);
 }
 
@@ -184,7 +184,8 @@ int moe_linear(const void* x, const void* w, const void* bias, const void* resid
     a.R = K;
     a.f16 = dtype == MOE_DTYPE_F16;
     a.ydt = y_dtype;
-    a.epi = moe::MmEpi{bias, residual, z, act};
+    a.epi = moe::MmEpi{bias, residual, z, act, nullptr, nullptr, nullptr};
+    a.kind = bias || residual || z || act != MOE_LIN_NONE ? moe::EPI_LIN : moe::EPI_PLAIN;
     return moe::launch_mm_fwd(a, (hipStream_t)stream);
 }
 
@@ -273,26 +274,27 @@ int moe_mlp_fwd(const moe_mlp_t* m, const void* x, const int32_t* idx, const flo
     if (rc) return rc;
     rc = moe::launch_slots(idx, sorted, offsets, (int)n, k, m->E, rows, pos, st);
     if (rc) return rc;
-    void* g = gu ? gu : ws + L.gu;
     moe::MmArgs a{};
     a.a = x;
     a.b = m->w_gate_up;
     a.offsets = offsets;
     a.arows = rows;
-    a.y = g;
+    a.y = ws + L.h;
     a.M = (int)n;
-    a.a_n = (int)T;
+    a.a_n = T;
     a.lda = m->d;
     a.ldb = m->d;
     a.E = m->E;
-    a.J = 2 * m->F;
+    a.J = m->F;
     a.R = m->d;
     a.f16 = f16;
     a.ydt = m->dtype;
-    a.fill = 1;
+    a.kind = moe::EPI_GLU;
+    a.epi.act = m->act;
+    a.epi.gu = gu;
+    a.epi.codes = (uint8_t*)codes;
+    a.epi.scales = (uint8_t*)scales;
     rc = moe::launch_mm_fwd(a, st);
-    if (rc) return rc;
-    rc = moe::launch_glu_fwd(g, 2 * (int64_t)m->F, n, m->F, m->act, f16, ws + L.h, (uint8_t*)codes, (uint8_t*)scales, st);
     if (rc) return rc;
     a.a = ws + L.h;
     a.b = m->w_down;
@@ -303,7 +305,8 @@ int moe_mlp_fwd(const moe_mlp_t* m, const void* x, const int32_t* idx, const flo
     a.ldb = m->F;
     a.J = m->d;
     a.R = m->F;
-    a.fill = 0;
+    a.kind = moe::EPI_PLAIN;
+    a.epi = moe::MmEpi{};
     rc = moe::launch_mm_fwd(a, st);
     if (rc) return rc;
     return moe::launch_slot_sum(ws + L.ys, pos, wts, residual, n, T, k, m->d, f16, y, y_dtype, st);

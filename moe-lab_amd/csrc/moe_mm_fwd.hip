@@ -8,13 +8,17 @@ static int launch(const MmArgs& a, hipStream_t st) {
     const int64_t live = a.offsets ? (a.E < a.M ? a.E : a.M) : 1;   // groups that can hold a slot
     const int64_t avg = a.M / live;
     auto tiles = [&](int bi, int bj) { return (live + a.M / bi) * ((a.J + bj - 1) / bj); };
-    int c = avg <= 4 ? 3 : avg > 64 && tiles(256, 256) >= 192 ? 0 : avg > 32 && tiles(128, 128) >= 192 ? 1 : 2;
+    // with kept rows the dot products are not used: they have no block of 32 columns
+    const bool few = avg <= 4 && !(a.kind == EPI_GLU && (a.epi.gu || a.epi.codes));
+    int c = few ? 3 : avg > 64 && tiles(256, 256) >= 192 ? 0 : avg > 32 && tiles(128, 128) >= 192 ? 1 : 2;
     if (force >= 0) c = force;
     switch (c) {
         case 0: return launch_mm_cfg<MM_FWD, F16, 8, 8, 2, 2, 1>(a, st);
         case 5: return launch_mm_cfg<MM_FWD, F16, 8, 4, 4, 2, 1>(a, st);
         case 1: return launch_mm_cfg<MM_FWD, F16, 4, 4, 2, 2, 2>(a, st);
-        case 2: return launch_mm_cfg<MM_FWD, F16, 2, 2, 2, 4, 2>(a, st);
+        case 2:
+            if (a.kind == EPI_GLU) return launch_mm_cfg<MM_FWD, F16, 2, 4, 2, 3, 2>(a, st);
+            return launch_mm_cfg<MM_FWD, F16, 2, 2, 2, 4, 2>(a, st);
         case 4: return launch_mm_cfg<MM_FWD, F16, 4, 8, 2, 3, 1>(a, st);
         default: return launch_mm_rows(a, st);
     }
