@@ -287,7 +287,7 @@ __device__ __forceinline__ f32x4 load4(const void* p, int64_t i) {
 // next, so a tile's first stages arrive during the last one's products and stores. Every step loads the same number of pieces
 // (past the last tile from empty descriptors: zeros, no traffic), so the waits are constants.
 // EPI_GLU: the tile's columns are BJ / 2 of gate and the same of up, half by half for each wave, so that a lane holds both.
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, bool GATHER, int EPI>
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, bool GATHER, int EPI, bool LDS_OUT>
 struct MmKernel {
     static constexpr bool GLU = EPI == EPI_GLU;
     static constexpr bool ACC = FA * FB * 4 >= 256;   // the sums fill the accumulation registers
@@ -298,9 +298,43 @@ struct MmKernel {
     using B = Operand<BX, BJ, NW>;
     static constexpr int PA = A::PIECES, PB = B::PIECES;
     static constexpr int STAGE = A::BYTES + B::BYTES;
+    static constexpr bool LINES = MODE == MM_DW && LDS_OUT;
 
     // Stores (and the loads of bias and residual) go through buffer descriptors: lanes and columns past the tile's valid ones
     // get an offset past the end, absent operands an empty descriptor, so that the epilogue has no branches per element.
+    // 16-bit results without an epilogue go through LDS, 16 rows of a wave's columns at a time (private to the wave), so that
+    // every store instruction writes whole cache lines: from the matrix instruction's layout it would write half lines.
+    static constexpr int OUT_LD = 32 * FB + 16, OUT_BYTES = 16 * OUT_LD;   // of a wave
+    static __device__ __forceinline__ void store_lines(const MmArgs& g, const MmTile& t, f32x4 (&acc)[FA][FB], char* so, int lane,
+                                                       int wi, int wj) {
+        const int l = lane & 15, q = lane >> 4, jw = t.j0 + wj * FB * 16;
+        const int64_t row0 = MODE == MM_DW ? (int64_t)t.e * g.I + t.i0 : (int64_t)t.lo;
+        const auto yb = __builtin_amdgcn_make_buffer_rsrc((char*)g.y + row0 * g.J * 2, 0, (uint32_t)t.rows * (uint32_t)g.J * 2, 0x00027000);
+        constexpr int LPR = 2 * FB, RPI = 64 / LPR;   // lanes per row, rows per store
+        const int r = lane / LPR, c = lane % LPR * 8;
+        const bool ok = jw + c < g.J;
+        char *in = so + l * OUT_LD + q * 8, *out = so + r * OUT_LD + c * 2;
+#pragma unroll
+        for (int f = 0; f < FA; ++f) {
+            if (32 * f >= t.rows) break;
+            if constexpr (ACC) {   // read here, not where the branches to here begin: 256 copies would spill
+#pragma unroll
+                for (int h = 0; h < FB; ++h) asm volatile("" : "+a"(acc[f][h]));
+            }
+#pragma unroll
+            for (int h = 0; h < FB; ++h)
+                *(u32x2*)(in + h * 32) = (u32x2){pack16<F16>(acc[f][h][0], acc[f][h][1]), pack16<F16>(acc[f][h][2], acc[f][h][3])};
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int k = 0; k < 16 / RPI; ++k) {
+                const int i = 16 * (2 * f + wi) + k * RPI + r;
+                __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4*)(out + k * RPI * OUT_LD), yb,
+                                                       ok && i < t.rows ? ((uint32_t)i * (uint32_t)g.J + jw + c) * 2 : MM_OOB, 0, 2);
+            }
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
     static __device__ __forceinline__ void store(const MmArgs& g, const MmTile& t, f32x4 (&acc)[FA][FB], int lane, int wi, int wj) {
         const bool f32 = g.ydt == MOE_DTYPE_F32;
         const int ES = f32 ? 4 : 2;
@@ -716,6 +750,7 @@ struct MmKernel {
                     for (int h = 0; h < FB; ++h) asm volatile("" : "+a"(acc[f][h]));
             }
             if constexpr (GLU) store_glu(g, t, acc, lane, wi, wj);
+            else if (LINES && g.ydt != MOE_DTYPE_F32) store_lines(g, t, acc, sm + ST * STAGE + wave * OUT_BYTES, lane, wi, wj);
             else store(g, t, acc, lane, wi, wj);
             if constexpr (DB) {
                 if (bias && wj == 0) {
@@ -735,8 +770,11 @@ struct MmKernel {
 
 template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, bool GATHER, int EPI>
 __global__ void __launch_bounds__(128 * NWJ, OCC * NWJ / 2) k_mm(const MmArgs g) {
-    using K = MmKernel<MODE, F16, FA, FB, NWJ, ST, GATHER, EPI>;
-    __shared__ __attribute__((aligned(1024))) char sm[ST * K::STAGE];
+    // LDS of a CU's OCC workgroups: 160 KiB
+    constexpr int LDS = 160 * 1024 / OCC, STAGES = ST * 64 * (32 * FA + 16 * NWJ * FB) * 2, PRE = 4 * MM_MAX_E + 64;
+    constexpr bool LDS_OUT = OCC == 2 && STAGES + PRE + 2 * NWJ * 16 * (32 * FB + 16) <= LDS;
+    using K = MmKernel<MODE, F16, FA, FB, NWJ, ST, GATHER, EPI, LDS_OUT>;
+    __shared__ __attribute__((aligned(1024))) char sm[STAGES + (K::LINES ? K::NW * K::OUT_BYTES : 0)];
     __shared__ int pre[MODE == MM_DW ? 1 : MM_MAX_E + 1];
     K::block(g, sm, pre);
 }

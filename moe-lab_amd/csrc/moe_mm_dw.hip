@@ -2,19 +2,23 @@
 
 namespace moe {
 
+// Tiles of 128 x 128, two workgroups on a CU: while one stores its sums the other multiplies, and with sums over the slots of
+// one expert (often three steps of 64) stores are most of the traffic. With long sums and enough tiles, 256 x 256: half the LDS
+// reads per product. Measured, 128 x 128 against 256 x 256: 32 experts x 139 slots, [5760, 2880] 310 and 352 us; 64 x 256,
+// [2048, 2048] 268 and 313; 64 x 512 452 and 480; 8 x 1024, [4096, 4096] 304 and 278; one group of 8192, [8192, 2048] 263 and
+// 219; 4096, [4096, 4096] 132 and 118.
 template <bool F16>
 static int launch(const MmArgs& a, hipStream_t st) {
+    const int64_t big = (int64_t)a.E * ((a.I + 255) / 256) * ((a.J + 255) / 256);
     const int force = env_int("MM_CFG", -1);
-    auto tiles = [&](int bi, int bj) { return (int64_t)a.E * ((a.I + bi - 1) / bi) * ((a.J + bj - 1) / bj); };
-    int c = tiles(256, 256) >= 192 ? 0 : tiles(128, 128) >= 192 ? 1 : 2;
-    if (force >= 0) c = force;
-    switch (c) {
-        case 0: return launch_mm_cfg<MM_DW, F16, 8, 8, 2, 2, 1>(a, st);
+    switch (force) {
         case 5: return launch_mm_cfg<MM_DW, F16, 8, 4, 4, 2, 1>(a, st);
-        case 1: return launch_mm_cfg<MM_DW, F16, 4, 4, 2, 2, 2>(a, st);
-        case 4: return launch_mm_cfg<MM_DW, F16, 4, 8, 2, 3, 1>(a, st);
-        default: return launch_mm_cfg<MM_DW, F16, 2, 2, 2, 4, 2>(a, st);
+        case 2: return launch_mm_cfg<MM_DW, F16, 2, 2, 2, 4, 2>(a, st);
+        case 7: return launch_mm_cfg<MM_DW, F16, 4, 4, 2, 4, 1>(a, st);
+        default: break;
     }
+    if (force == 0 || (force < 0 && a.M / a.E >= 1024 && big >= 192)) return launch_mm_cfg<MM_DW, F16, 8, 8, 2, 2, 1>(a, st);
+    return launch_mm_cfg<MM_DW, F16, 4, 4, 2, 2, 2>(a, st);
 }
 int launch_mm_dw(const MmArgs& a, hipStream_t st) { return a.f16 ? launch<true>(a, st) : launch<false>(a, st); }
 

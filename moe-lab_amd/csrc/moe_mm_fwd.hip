@@ -15,11 +15,13 @@ static int launch(const MmArgs& a, hipStream_t st) {
     switch (c) {
         case 0: return launch_mm_cfg<MM_FWD, F16, 8, 8, 2, 2, 1>(a, st);
         case 5: return launch_mm_cfg<MM_FWD, F16, 8, 4, 4, 2, 1>(a, st);
+        case 6: return launch_mm_cfg<MM_FWD, F16, 4, 4, 4, 3, 1>(a, st);
         case 1: return launch_mm_cfg<MM_FWD, F16, 4, 4, 2, 2, 2>(a, st);
         case 2:
             if (a.kind == EPI_GLU) return launch_mm_cfg<MM_FWD, F16, 2, 4, 2, 3, 2>(a, st);
             return launch_mm_cfg<MM_FWD, F16, 2, 2, 2, 4, 2>(a, st);
-        case 4: return launch_mm_cfg<MM_FWD, F16, 4, 8, 2, 3, 1>(a, st);
+        case 7: return launch_mm_cfg<MM_FWD, F16, 4, 4, 2, 4, 1>(a, st);
+        case 8: return launch_mm_cfg<MM_FWD, F16, 2, 2, 2, 8, 1>(a, st);
         default: return launch_mm_rows(a, st);
     }
 }
