@@ -60,7 +60,7 @@ extern "C" {
 #define MOE_ACT_GEGLU 1       /* tanh-GELU(g) * u (Gemma-4) */
 #define MOE_ACT_GPTOSS 2      /* g = min(g,7), u = clip(u,-7,7), g * sigmoid(1.702 g) * (u + 1) */
 
-/* activations of moe_linear_run */
+/* activations of moe_linear */
 #define MOE_LIN_NONE 0
 #define MOE_LIN_SILU 1        /* z * sigmoid(z) */
 #define MOE_LIN_GELU 2        /* tanh-GELU(z) */
@@ -343,11 +343,19 @@ int moe_grouped_mm_dw(const void* dy, const void* x, const int32_t* offsets, con
  * One product with its epilogue: y = act(x w^T + bias) + residual, x [T, K] (ldx elements from row to row), w [N, K],
  * bias [N], residual and y [T, N]; types, alignment and sizes as moe_grouped_mm; act: MOE_LIN_*. The sums, bias, activation
  * and residual are fp32, rounded once. z [T, N] (or NULL): the sums with bias before the activation, in the operands' type,
- * what moe_linear_act_bwd takes. Gradients: dz = dy act'(z) by moe_linear_act_bwd (dz = dy without an activation), then
- * moe_grouped_mm_dx / _dw of dz with E = 1 and no offsets. residual may be y.
- * workspace: moe_linear_workspace_bytes(T, N, K) bytes, any contents (0: NULL will do).
+ * what moe_linear_act_bwd takes. residual may be y. Gradients: dz = dy act'(z) by moe_linear_act_bwd (dz = dy without an
+ * activation), then dx [T, K] = dz w by moe_linear_dx, and dw [N, K] = dz^T x and dbias [N] (or NULL), the sums of dz's
+ * columns, by moe_linear_dw, in the operands' type; lddz and ldx: elements from row to row.
+ * workspace: the call's _workspace_bytes(T, N, K), any contents (0: NULL will do). With few output tiles the sums are split
+ * into parts, whose results are added in a fixed order.
  */
 size_t moe_linear_workspace_bytes(int64_t T, int N, int K);
+size_t moe_linear_dx_workspace_bytes(int64_t T, int N, int K);
+size_t moe_linear_dw_workspace_bytes(int64_t T, int N, int K);
+int moe_linear_dx(const void* dz, const void* w, int64_t T, int64_t lddz, int N, int K, int dtype, void* dx, void* workspace,
+                  size_t workspace_bytes, void* stream);
+int moe_linear_dw(const void* dz, const void* x, int64_t T, int64_t lddz, int64_t ldx, int N, int K, int dtype, void* dw,
+                  void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 int moe_linear(const void* x, const void* w, const void* bias, const void* residual, int act, int64_t T, int64_t ldx, int N,
                int K, int dtype, void* y, int y_dtype, void* z, void* workspace, size_t workspace_bytes, void* stream);
 /* z [T, N] in 16 bits, or NULL and its 8-bit form codes, scales (moe_act8_pack). */

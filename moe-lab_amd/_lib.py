@@ -26,7 +26,8 @@ EXPORTS = ("moe_router", "moe_router_counter_count", "moe_topk", "moe_group", "m
            "moe_experts_run_static", "moe_layer_run", "moe_layer_workspace_bytes", "moe_experts_run_shared",
            "moe_experts_shared_workspace_bytes", "moe_router_group", "moe_layer_run_shared",
            "moe_layer_shared_workspace_bytes", "moe_probe_read", "moe_grouped_mm", "moe_grouped_mm_dx", "moe_grouped_mm_dw",
-           "moe_linear", "moe_linear_workspace_bytes", "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack",
+           "moe_linear", "moe_linear_workspace_bytes", "moe_linear_dx",
+           "moe_linear_dx_workspace_bytes", "moe_linear_dw", "moe_linear_dw_workspace_bytes", "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack",
            "moe_glu_fwd", "moe_glu_bwd", "moe_mlp_fwd", "moe_mlp_bwd", "moe_mlp_keep_bytes",
            "moe_mlp_fwd_workspace_bytes", "moe_mlp_bwd_workspace_bytes")
 PROBE_SINK = 1024   # MOE_PROBE_SINK
@@ -97,7 +98,11 @@ def lib():
         L.moe_grouped_mm_dx.argtypes = [vp, vp, vp, vp, i64, i64, i64, i, i, i, i, vp, i, i, vp]
         L.moe_grouped_mm_dw.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i, i, i, i, vp, i, vp, vp]
         L.moe_linear.argtypes = [vp, vp, vp, vp, i, i64, i64, i, i, i, vp, i, vp, vp, sz, vp]
-        L.moe_linear_workspace_bytes.argtypes = [i64, i, i]
+        L.moe_linear_dx.argtypes = [vp, vp, i64, i64, i, i, i, vp, vp, sz, vp]
+        L.moe_linear_dw.argtypes = [vp, vp, i64, i64, i64, i, i, i, vp, vp, vp, sz, vp]
+        for n in ("moe_linear_workspace_bytes", "moe_linear_dx_workspace_bytes", "moe_linear_dw_workspace_bytes"):
+            getattr(L, n).argtypes = [i64, i, i]
+            getattr(L, n).restype = sz
         L.moe_linear_act_bwd.argtypes = [vp, i64, vp, vp, vp, i, i64, i, i, vp, vp]
         L.moe_act8_pack.argtypes = [vp, i64, i64, i, i, vp, vp, vp]
         L.moe_act8_unpack.argtypes = [vp, vp, i64, i, vp, i, vp]
@@ -109,7 +114,6 @@ def lib():
         for n in ("moe_mlp_keep_bytes", "moe_mlp_fwd_workspace_bytes", "moe_mlp_bwd_workspace_bytes"):
             getattr(L, n).argtypes = [mlp, i, i]
             getattr(L, n).restype = sz
-        L.moe_linear_workspace_bytes.restype = sz
         L.moe_row_bytes.argtypes = [i, i]
         L.moe_row_bytes.restype = sz
         L.moe_tile_bytes.argtypes = [i, i, i]
@@ -126,7 +130,7 @@ def lib():
                   "moe_experts_run_stages", "moe_tiles_pack", "moe_shared_experts_run", "moe_experts_run_static",
                   "moe_layer_run", "moe_experts_run_shared", "moe_router_group", "moe_layer_run_shared",
                   "moe_probe_read", "moe_grouped_mm", "moe_grouped_mm_dx", "moe_grouped_mm_dw", "moe_linear",
-                  "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack", "moe_glu_fwd", "moe_glu_bwd", "moe_mlp_fwd",
+                  "moe_linear_dx", "moe_linear_dw", "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack", "moe_glu_fwd", "moe_glu_bwd", "moe_mlp_fwd",
                   "moe_mlp_bwd"):
             getattr(L, n).restype = ctypes.c_int
         _lib = L

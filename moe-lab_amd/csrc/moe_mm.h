@@ -27,7 +27,6 @@ __device__ __forceinline__ f32x4 mma(s16x8 a, s16x8 b, f32x4 c) {
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ void drain() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 template <bool F16>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
     if constexpr (F16) {
@@ -162,8 +161,10 @@ struct MmArgs {
     const int32_t* arows;    // row of a of each slot, or null: the slot itself
     const int32_t* brows;    // dw: the same for b
     void* y;
-    void* dbias;             // dw: [E, N] of the operands' type, or null
+    void* dbias;             // dw: [E, N] of the operands' type (parts: fp32), or null
     int M;                   // slots
+    // Without offsets: E = 1 group of all slots, or E parts of one product (split over r; y: the parts' fp32 sums, [E, rows, J]).
+    int part;                // slots (dw) or r (forward, dx) of a part, a multiple of 64; 0: no parts
     int a_n, b_n;            // rows of a and (dw) b
     int lda, ldb;            // elements between rows; ldb of forward and dx: K
     int E, I, J, R;          // dw: I = N, J = K; forward: J = N (EPI_GLU: F), R = K; dx: J = K, R = N
@@ -173,10 +174,11 @@ struct MmArgs {
 };
 
 // The slots of group e, inside [0, M) whatever offsets hold.
+template <int MODE>
 __device__ __forceinline__ void group_of(const MmArgs& a, int e, int& lo, int& hi) {
     if (!a.offsets) {
-        lo = 0;
-        hi = a.M;
+        lo = MODE == MM_DW ? e * a.part : 0;
+        hi = MODE == MM_DW && a.part && a.M - lo > a.part ? lo + a.part : a.M;
         return;
     }
     const int p = e ? a.offsets[e] : 0, q = a.offsets[e + 1];
@@ -204,7 +206,7 @@ __device__ __forceinline__ MmRun xcd_run(int tiles) {
 
 // Row tiles of the groups, counted on the device: pre[e] = tiles of the groups before e. Wave 0 scans 64 groups at a time.
 #define MM_MAX_E 1024
-template <int BI>
+template <int MODE, int BI>
 __device__ __forceinline__ void count_tiles(const MmArgs& a, int* pre) {
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x;
@@ -214,7 +216,7 @@ __device__ __forceinline__ void count_tiles(const MmArgs& a, int* pre) {
             int n = 0;
             if (base + lane < a.E) {
                 int lo, hi;
-                group_of(a, base + lane, lo, hi);
+                group_of<MODE>(a, base + lane, lo, hi);
                 n = (hi - lo) / BI + ((hi - lo) % BI > 0);
             }
             const int s = wave_incl_scan(n) + before;
@@ -225,16 +227,17 @@ __device__ __forceinline__ void count_tiles(const MmArgs& a, int* pre) {
     __syncthreads();
 }
 // Zeros into the rows behind the last group, 16 bytes a thread over the whole grid.
+template <int MODE>
 __device__ __forceinline__ void fill_rest(const MmArgs& a) {
     int lo, hi;
-    group_of(a, a.E - 1, lo, hi);
+    group_of<MODE>(a, a.E - 1, lo, hi);
     const int64_t row16 = (int64_t)a.J * (a.ydt == MOE_DTYPE_F32 ? 4 : 2) / 16, n = (a.M - hi) * row16;
     u32x4* y = (u32x4*)a.y + hi * row16;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) y[i] = (u32x4){0, 0, 0, 0};
 }
 // Tile id of the forward or dx product: its group by two 64-way searches in pre; inside a group down up to 4 row tiles before
 // the next column tile.
-template <int BI, int BJ>
+template <int MODE, int BI, int BJ>
 __device__ __forceinline__ void tile_at(const MmArgs& a, const int* pre, int id, MmTile& t) {
     const int lane = threadIdx.x & 63, nj = (a.J + BJ - 1) / BJ;
     constexpr int C = (MM_MAX_E + 63) / 64;
@@ -246,7 +249,7 @@ __device__ __forceinline__ void tile_at(const MmArgs& a, const int* pre, int id,
     const int first = __builtin_amdgcn_readfirstlane(pre[e]), nr = __builtin_amdgcn_readfirstlane(pre[e + 1]) - first;
     const int local = id - first * nj, sup = local / (4 * nj), in = local - sup * 4 * nj, h = min(4, nr - 4 * sup);
     int lo, hi;
-    group_of(a, e, lo, hi);
+    group_of<MODE>(a, e, lo, hi);
     t.e = e;
     t.j0 = in / h * BJ;
     t.lo = lo + (4 * sup + in % h) * BI;
@@ -261,7 +264,7 @@ __device__ __forceinline__ void tile_at_dw(const MmArgs& a, int id, MmTile& t) {
     t.e = id / (ni * nj);
     const int local = id - t.e * ni * nj, sup = local / (4 * nj), in = local - sup * 4 * nj, h = min(4, ni - 4 * sup);
     int hi;
-    group_of(a, t.e, t.lo, hi);
+    group_of<MM_DW>(a, t.e, t.lo, hi);
     t.cnt = hi - t.lo;
     t.i0 = (4 * sup + in % h) * BI;
     t.j0 = in / h * BJ;
@@ -308,7 +311,7 @@ struct MmKernel {
     static __device__ __forceinline__ void store_lines(const MmArgs& g, const MmTile& t, f32x4 (&acc)[FA][FB], char* so, int lane,
                                                        int wi, int wj) {
         const int l = lane & 15, q = lane >> 4, jw = t.j0 + wj * FB * 16;
-        const int64_t row0 = MODE == MM_DW ? (int64_t)t.e * g.I + t.i0 : (int64_t)t.lo;
+        const int64_t row0 = MODE == MM_DW ? (int64_t)t.e * g.I + t.i0 : (g.part ? (int64_t)t.e * g.M : 0) + t.lo;
         const auto yb = __builtin_amdgcn_make_buffer_rsrc((char*)g.y + row0 * g.J * 2, 0, (uint32_t)t.rows * (uint32_t)g.J * 2, 0x00027000);
         constexpr int LPR = 2 * FB, RPI = 64 / LPR;   // lanes per row, rows per store
         const int r = lane / LPR, c = lane % LPR * 8;
@@ -339,7 +342,7 @@ struct MmKernel {
         const bool f32 = g.ydt == MOE_DTYPE_F32;
         const int ES = f32 ? 4 : 2;
         const int l = lane & 15, q = lane >> 4, jw = t.j0 + wj * FB * 16;
-        const int64_t row0 = MODE == MM_DW ? (int64_t)t.e * g.I + t.i0 : (int64_t)t.lo;
+        const int64_t row0 = MODE == MM_DW ? (int64_t)t.e * g.I + t.i0 : (g.part ? (int64_t)t.e * g.M : 0) + t.lo;
         const auto rsrc = [&](const void* p, int es) {
             return __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<void*>(p) + row0 * g.J * es, 0,
                                                      p ? (uint32_t)t.rows * (uint32_t)g.J * es : 0u, 0x00027000);
@@ -509,19 +512,20 @@ struct MmKernel {
         if constexpr (MODE == MM_DW) {
             tiles = g.E * ((g.I + BI - 1) / BI) * nj;
         } else {
-            count_tiles<BI>(g, pre);
+            count_tiles<MODE, BI>(g, pre);
             tiles = __builtin_amdgcn_readfirstlane(pre[g.E]) * nj;
-            if (g.fill && g.offsets) fill_rest(g);
+            if (g.fill && g.offsets) fill_rest<MODE>(g);
         }
         const MmRun run = xcd_run(tiles);
         auto tile = [&](int id, MmTile& t) {
             if constexpr (MODE == MM_DW) tile_at_dw<BI, TJ>(g, id, t);
-            else tile_at<BI, TJ>(g, pre, id, t);
+            else tile_at<MODE, BI, TJ>(g, pre, id, t);
         };
-        auto steps_of = [&](const MmTile& t) -> int { return MODE == MM_DW ? (t.cnt + 63) / 64 : (g.R + 63) / 64; };
+        auto r_of = [&](const MmTile& t) -> int { return g.part ? min(g.part, g.R - t.e * g.part) : g.R; };   // forward, dx
+        auto steps_of = [&](const MmTile& t) -> int { return ((MODE == MM_DW ? t.cnt : r_of(t)) + 63) / 64; };
 
         // the stream of loads: its tile, the step in it, and where the operands' next pieces begin
-        int lid = run.id - run.stride, ls = 0, lsteps = 0, lrows = 0;
+        int lid = run.id - run.stride, ls = 0, lsteps = 0, lrows = 0, lr = 0;
         MmTile lt{};
         const char *pa = nullptr, *pb = nullptr;
         int rowa, cola, rowb, colb;
@@ -550,8 +554,11 @@ struct MmKernel {
                 lsteps = steps_of(lt);
             } while (lsteps == 0);
             lrows = 1;
+            lr = r_of(lt);
             pa = (const char*)g.a;
             pb = (const char*)g.b;
+            const int e = g.part ? 0 : lt.e, first = lt.e * g.part;   // group, and the part's first r
+            if constexpr (!AX) pa += (int64_t)first * 2;
             if constexpr (AX) pa += (int64_t)lt.i0 * 2 + (GATHER ? 0 : (int64_t)lt.lo * lda2);
             else if (!GATHER) pa += (int64_t)lt.lo * lda2;
 #pragma unroll
@@ -576,22 +583,22 @@ struct MmKernel {
                     offb[i] = j < g.J ? (uint32_t)((r % W < H ? j : g.J + j) * ldb2 + c * 2) : MM_OOB;
                 }
             }
-            if constexpr (MODE == MM_FWD) pb += GLU ? (int64_t)lt.e * 2 * g.J * ldb2 : ((int64_t)lt.e * g.J + lt.j0) * ldb2;
-            if constexpr (MODE == MM_DX) pb += (int64_t)lt.e * g.R * ldb2 + (int64_t)lt.j0 * 2;
+            if constexpr (MODE == MM_FWD) pb += GLU ? (int64_t)lt.e * 2 * g.J * ldb2 : ((int64_t)e * g.J + lt.j0) * ldb2 + first * 2;
+            if constexpr (MODE == MM_DX) pb += ((int64_t)e * g.R + first) * ldb2 + (int64_t)lt.j0 * 2;
             if constexpr (MODE == MM_DW) pb += (gath_b ? 0 : (int64_t)lt.lo * ldb2) + (int64_t)lt.j0 * 2;
             fetch_rows();
         };
         // bytes of the descriptors for load step ls: up to the end of the last valid row
         auto bytes_a = [&]() -> uint32_t {
             if (!lrows) return 0;
-            if constexpr (!AX) return (uint32_t)((GATHER ? g.a_n : lt.rows) - 1) * (uint32_t)lda2 + (uint32_t)(g.R - 64 * ls) * 2;
+            if constexpr (!AX) return (uint32_t)((GATHER ? g.a_n : lt.rows) - 1) * (uint32_t)lda2 + (uint32_t)(lr - 64 * ls) * 2;
             const int rows = GATHER ? g.a_n : min(64, lt.cnt - 64 * ls);
             return (uint32_t)(rows - 1) * (uint32_t)lda2 + (uint32_t)(g.I - lt.i0) * 2;
         };
         auto bytes_b = [&]() -> uint32_t {
             if (!lrows) return 0;
-            if constexpr (!BX) return (uint32_t)((GLU ? 2 * g.J : min(BJ, g.J - lt.j0)) - 1) * (uint32_t)ldb2 + (uint32_t)(g.R - 64 * ls) * 2;
-            const int rows = MODE == MM_DX ? min(64, g.R - 64 * ls) : gath_b ? g.b_n : min(64, lt.cnt - 64 * ls);
+            if constexpr (!BX) return (uint32_t)((GLU ? 2 * g.J : min(BJ, g.J - lt.j0)) - 1) * (uint32_t)ldb2 + (uint32_t)(lr - 64 * ls) * 2;
+            const int rows = MODE == MM_DX ? min(64, lr - 64 * ls) : gath_b ? g.b_n : min(64, lt.cnt - 64 * ls);
             return (uint32_t)(rows - 1) * (uint32_t)ldb2 + (uint32_t)(g.J - lt.j0) * 2;
         };
         // dw, gathered: the pieces' rows are other ones in every step
@@ -613,11 +620,11 @@ struct MmKernel {
                 }
             }
             // a step that ends past R: its pieces there (one with r contiguous has a single column per lane)
-            if (!AX && 64 * ls + 64 > g.R && lrows) {
-                if (64 * ls + cola >= g.R)
+            if (!AX && 64 * ls + 64 > lr && lrows) {
+                if (64 * ls + cola >= lr)
 #pragma unroll
                     for (int i = 0; i < PA; ++i) offa[i] = MM_OOB;
-                if (!BX && 64 * ls + colb >= g.R)
+                if (!BX && 64 * ls + colb >= lr)
 #pragma unroll
                     for (int i = 0; i < PB; ++i) offb[i] = MM_OOB;
             }
@@ -743,7 +750,6 @@ struct MmKernel {
                 wbuf = next_buf(wbuf);
             }
             if constexpr (ACC) {
-                drain();
 #pragma unroll
                 for (int f = 0; f < FA; ++f)
 #pragma unroll
@@ -759,7 +765,11 @@ struct MmKernel {
                         float v = sums[f] + __shfl_xor(sums[f], 16);
                         v += __shfl_xor(v, 32);
                         const int i = 16 * (2 * f + wi) + lane;
-                        if (lane < 16 && i < t.rows) ((uint16_t*)g.dbias)[(int64_t)t.e * g.I + t.i0 + i] = (uint16_t)pack16<F16>(v, 0.f);
+                        const int64_t at = (int64_t)t.e * g.I + t.i0 + i;
+                        if (lane < 16 && i < t.rows) {
+                            if (g.part) ((float*)g.dbias)[at] = v;
+                            else ((uint16_t*)g.dbias)[at] = (uint16_t)pack16<F16>(v, 0.f);
+                        }
                     }
                 }
             }
@@ -785,9 +795,25 @@ int launch_mm_dx(const MmArgs& a, hipStream_t st);
 int launch_mm_dw(const MmArgs& a, hipStream_t st);
 int launch_mm_rows(const MmArgs& a, hipStream_t st);   // forward, few rows (moe_mm_rows.hip)
 
+// Tiles of the product kernel: 256 x 256 with 4 waves; 128 x 256 with 8; 128 x 128 with 4, two workgroups on a CU; the same,
+// one on a CU with twice the stages; 64 x 64, two on a CU. MM_ROWS: dot products (moe_mm_rows.hip).
+enum MmShape { MM_256 = 0, MM_128x256 = 1, MM_128 = 2, MM_128_DEEP = 3, MM_64 = 4, MM_ROWS = 5 };
+// Shape and number of parts for a product without offsets: out [rows, J], sums of length R (moe_mm_parts.hip).
+struct MmPlan {
+    int shape, parts;
+};
+MmPlan mm_plan(int64_t rows, int64_t J, int64_t R, bool split);
+// Forward with up to 4 rows: dot products, whole (w [4096, 4096], T 1: 8.6 us, 64 x 64 in 4 parts 12.6; T 4: 10.0 and 12.6;
+// T 8: 14.4 and 12.8).
+constexpr int MM_FEW = 4;
+
+// A product without offsets in its plan's parts, and the parts' sum with the epilogue (part by part in order: the result does not
+// depend on which part ends first). ws: parts x rows x J floats, and for dbias parts x I behind them.
+int launch_mm_parts(int mode, const MmArgs& a, int parts, float* ws, hipStream_t st);
+
 // Workgroups for tiles of BI rows when the groups' sizes are known on the device only: every group can add a part tile.
 inline int64_t mm_row_tiles(const MmArgs& a, int BI) {
-    if (!a.offsets) return ((int64_t)a.M + BI - 1) / BI;
+    if (!a.offsets) return ((int64_t)a.M + BI - 1) / BI * a.E;
     return a.M / BI + (a.E + 1 < a.M ? a.E + 1 : a.M);
 }
 inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }

@@ -12,6 +12,12 @@ bool too_far(int64_t rows, int64_t ld) { return rows * ld * 2 > 0xB0000000ll; }
 bool two_byte(int dtype) { return dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16; }
 bool bad_act8(int64_t M, int64_t C) { return M < 0 || M > 0x7fffffff || C < 32 || C % 32 || C > (1 << 20); }
 bool bad_rows(const int32_t* idx, int64_t rows, int64_t M) { return rows > 0x7fffffff || rows < (idx ? 1 : M); }
+// Workspace of a product in parts, with `more` floats per part behind the sums.
+size_t parts_bytes(int64_t rows, int64_t J, int64_t R, int64_t more) {
+    if (rows < 1 || J < 1 || R < 1) return 0;
+    const int parts = moe::mm_plan(rows, J, R, true).parts;
+    return parts > 1 ? (size_t)parts * (rows * J + more) * 4 : 0;
+}
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Parts of the expert layer's buffers, in bytes from their start.
@@ -155,10 +161,9 @@ int moe_grouped_mm_dw(const void* dy, const void* x, const int32_t* offsets, con
     return moe::launch_mm_dw(a, (hipStream_t)stream);
 }
 
-size_t moe_linear_workspace_bytes(int64_t T, int N, int K) {
-    (void)T, (void)N, (void)K;
-    return 0;
-}
+size_t moe_linear_workspace_bytes(int64_t T, int N, int K) { return T <= moe::MM_FEW ? 0 : parts_bytes(T, N, K, 0); }
+size_t moe_linear_dx_workspace_bytes(int64_t T, int N, int K) { return parts_bytes(T, K, N, 0); }
+size_t moe_linear_dw_workspace_bytes(int64_t T, int N, int K) { return parts_bytes(N, K, T, N); }
 
 int moe_linear(const void* x, const void* w, const void* bias, const void* residual, int act, int64_t T, int64_t ldx, int N,
                int K, int dtype, void* y, int y_dtype, void* z, void* workspace, size_t workspace_bytes, void* stream) {
@@ -186,7 +191,62 @@ int moe_linear(const void* x, const void* w, const void* bias, const void* resid
     a.ydt = y_dtype;
     a.epi = moe::MmEpi{bias, residual, z, act, nullptr, nullptr, nullptr};
     a.kind = bias || residual || z || act != MOE_LIN_NONE ? moe::EPI_LIN : moe::EPI_PLAIN;
+    const int parts = T <= moe::MM_FEW ? 1 : moe::mm_plan(T, N, K, true).parts;
+    if (parts > 1) return moe::launch_mm_parts(moe::MM_FWD, a, parts, (float*)workspace, (hipStream_t)stream);
     return moe::launch_mm_fwd(a, (hipStream_t)stream);
+}
+
+int moe_linear_dx(const void* dy, const void* w, int64_t T, int64_t lddy, int N, int K, int dtype, void* dx, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+    if (!two_byte(dtype)) return MOE_ERR_DTYPE;
+    if (T < 0 || T > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
+    if (T == 0) return MOE_OK;
+    if (!dy || !w || !dx) return MOE_ERR_ARG;
+    if (misaligned(dy) || misaligned(w) || misaligned(dx) || misaligned(workspace)) return MOE_ERR_ALIGN;
+    if (workspace_bytes < moe_linear_dx_workspace_bytes(T, N, K)) return MOE_ERR_WORKSPACE;
+    moe::MmArgs a{};
+    a.a = dy;
+    a.b = w;
+    a.y = dx;
+    a.M = (int)T;
+    a.a_n = (int)T;
+    a.lda = (int)lddy;
+    a.ldb = K;
+    a.E = 1;
+    a.J = K;
+    a.R = N;
+    a.f16 = dtype == MOE_DTYPE_F16;
+    a.ydt = dtype;
+    const int parts = moe::mm_plan(T, K, N, true).parts;
+    if (parts > 1) return moe::launch_mm_parts(moe::MM_DX, a, parts, (float*)workspace, (hipStream_t)stream);
+    return moe::launch_mm_dx(a, (hipStream_t)stream);
+}
+
+int moe_linear_dw(const void* dy, const void* x, int64_t T, int64_t lddy, int64_t ldx, int N, int K, int dtype, void* dw,
+                  void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!two_byte(dtype)) return MOE_ERR_DTYPE;
+    if (T < 0 || T > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N) || bad_ld(ldx, K)) return MOE_ERR_ARG;
+    if (!dw || (T > 0 && (!dy || !x))) return MOE_ERR_ARG;
+    if (misaligned(dy) || misaligned(x) || misaligned(dw) || misaligned(workspace)) return MOE_ERR_ALIGN;
+    if (workspace_bytes < moe_linear_dw_workspace_bytes(T, N, K)) return MOE_ERR_WORKSPACE;
+    moe::MmArgs a{};
+    a.a = dy;
+    a.b = x;
+    a.y = dw;
+    a.dbias = dbias;
+    a.M = (int)T;
+    a.a_n = (int)T;
+    a.b_n = (int)T;
+    a.lda = (int)lddy;
+    a.ldb = (int)ldx;
+    a.E = 1;
+    a.I = N;
+    a.J = K;
+    a.f16 = dtype == MOE_DTYPE_F16;
+    a.ydt = dtype;
+    const int parts = moe::mm_plan(N, K, T, true).parts;
+    if (parts > 1) return moe::launch_mm_parts(moe::MM_DW, a, parts, (float*)workspace, (hipStream_t)stream);
+    return moe::launch_mm_dw(a, (hipStream_t)stream);
 }
 
 int moe_linear_act_bwd(const void* dy, int64_t lddy, const void* z, const void* codes, const void* scales, int act, int64_t T,

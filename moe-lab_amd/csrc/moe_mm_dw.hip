@@ -7,18 +7,28 @@ namespace moe {
 // reads per product. Measured, 128 x 128 against 256 x 256: 32 experts x 139 slots, [5760, 2880] 310 and 352 us; 64 x 256,
 // [2048, 2048] 268 and 313; 64 x 512 452 and 480; 8 x 1024, [4096, 4096] 304 and 278; one group of 8192, [8192, 2048] 263 and
 // 219; 4096, [4096, 4096] 132 and 118.
+static int grouped(const MmArgs& a) {
+    const int64_t big = (int64_t)a.E * ((a.I + 255) / 256) * ((a.J + 255) / 256);
+    return a.M / a.E >= 1024 && big >= 192 ? MM_256 : MM_128;
+}
+
+// One group: by the plan, but not with the larger tiles for short sums (256 slots, [4096, 4096]: 256 x 256 17.8 us, 128 x 128
+// 14.0; 237, [2048, 2816]: 128 x 256 11.4, 128 x 128 9.3; 1024, [4096, 4096]: 256 x 256 36.9, 128 x 128 39.7).
+static int dense(const MmArgs& a) {
+    const int s = mm_plan(a.I, a.J, a.M, a.part != 0).shape;
+    return !a.part && a.M < 1024 && (s == MM_256 || s == MM_128x256) ? MM_128 : s;
+}
+
 template <bool F16>
 static int launch(const MmArgs& a, hipStream_t st) {
-    const int64_t big = (int64_t)a.E * ((a.I + 255) / 256) * ((a.J + 255) / 256);
-    const int force = env_int("MM_CFG", -1);
-    switch (force) {
-        case 5: return launch_mm_cfg<MM_DW, F16, 8, 4, 4, 2, 1>(a, st);
-        case 2: return launch_mm_cfg<MM_DW, F16, 2, 2, 2, 4, 2>(a, st);
-        case 7: return launch_mm_cfg<MM_DW, F16, 4, 4, 2, 4, 1>(a, st);
-        default: break;
+    const int s = a.offsets ? grouped(a) : dense(a);
+    switch (s) {
+        case MM_256: return launch_mm_cfg<MM_DW, F16, 8, 8, 2, 2, 1>(a, st);
+        case MM_64: return launch_mm_cfg<MM_DW, F16, 2, 2, 2, 4, 2>(a, st);
+        case MM_128_DEEP: return launch_mm_cfg<MM_DW, F16, 4, 4, 2, 4, 1>(a, st);
+        case MM_128x256: return launch_mm_cfg<MM_DW, F16, 4, 4, 4, 3, 1>(a, st);
+        default: return launch_mm_cfg<MM_DW, F16, 4, 4, 2, 2, 2>(a, st);
     }
-    if (force == 0 || (force < 0 && a.M / a.E >= 1024 && big >= 192)) return launch_mm_cfg<MM_DW, F16, 8, 8, 2, 2, 1>(a, st);
-    return launch_mm_cfg<MM_DW, F16, 4, 4, 2, 2, 2>(a, st);
 }
 int launch_mm_dw(const MmArgs& a, hipStream_t st) { return a.f16 ? launch<true>(a, st) : launch<false>(a, st); }
 

@@ -23,18 +23,18 @@ __global__ void __launch_bounds__(256) k_mm_rows(const MmArgs g) {
         e = -1;
         for (int base = 0; base < g.E && e < 0; base += 64) {
             int l = -1, h = -1;
-            if (base + lane < g.E) group_of(g, base + lane, l, h);
+            if (base + lane < g.E) group_of<MM_FWD>(g, base + lane, l, h);
             const uint64_t hit = __ballot(l == p && h > l);
             if (hit) {
                 const int at = __builtin_ctzll(hit);
                 e = base + at;
-                group_of(g, e, lo, hi);
+                group_of<MM_FWD>(g, e, lo, hi);
             }
         }
         if (e < 0) {
             if (!g.fill) return;
             int l, h;
-            group_of(g, g.E - 1, l, h);
+            group_of<MM_FWD>(g, g.E - 1, l, h);
             if (p < h) return;
             if (lane < R && n0 + lane < g.J) {
                 if (g.ydt == MOE_DTYPE_F32) ((float*)g.y)[(int64_t)p * g.J + n0 + lane] = 0.f;

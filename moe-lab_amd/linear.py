@@ -8,13 +8,38 @@ once. The reference runs these as stock modules (reference e2e.py:66-68, 146-147
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib, act8, grouped
+from . import _lib, act8
 
 NONE, SILU, GELU = 0, 1, 2   # no activation; z * sigmoid(z); tanh-GELU
 
 
 def _rows(t, name, cols, device, dtype):
     return _lib.half_matrix(t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t, name, cols, device, dtype)
+
+
+def _workspace(size, T, N, K, device):
+    n = getattr(_lib.lib(), size)(T, N, K)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None, n
+
+
+def _dx(dz, w):
+    (T, N), K = dz.shape, w.shape[1]
+    w = _lib.plain(w, "w", (N, K), dz.device, dz.dtype)
+    dx = torch.empty((T, K), dtype=w.dtype, device=w.device)
+    ws, nws = _workspace("moe_linear_dx_workspace_bytes", T, N, K, w.device)
+    _lib.call("moe_linear_dx", w.device, dz.data_ptr(), w.data_ptr(), T, dz.stride(0), N, K, _lib.DTYPE[w.dtype], dx.data_ptr(),
+              _lib.ptr(ws), nws)
+    return dx
+
+
+def _dw(dz, x, bias):
+    (T, N), K = dz.shape, x.shape[1]
+    dw = torch.empty((N, K), dtype=dz.dtype, device=dz.device)
+    db = torch.empty(N, dtype=dz.dtype, device=dz.device) if bias else None
+    ws, nws = _workspace("moe_linear_dw_workspace_bytes", T, N, K, dz.device)
+    _lib.call("moe_linear_dw", dz.device, dz.data_ptr(), x.data_ptr(), T, dz.stride(0), x.stride(0), N, K, _lib.DTYPE[dz.dtype],
+              dw.data_ptr(), _lib.ptr(db), _lib.ptr(ws), nws)
+    return dw, db
 
 
 def _forward(x, w, bias, act, residual, out_dtype, keep_z):
@@ -38,8 +63,7 @@ def _forward(x, w, bias, act, residual, out_dtype, keep_z):
     T = x2.shape[0]
     y = _lib.result(None, (T, N), w.dtype, out_dtype, w.device)
     z = torch.empty((T, N), dtype=w.dtype, device=w.device) if keep_z else None
-    nws = _lib.lib().moe_linear_workspace_bytes(T, N, K)
-    ws = torch.empty(nws, dtype=torch.uint8, device=w.device) if nws else None
+    ws, nws = _workspace("moe_linear_workspace_bytes", T, N, K, w.device)
     _lib.call("moe_linear", w.device, x2.data_ptr(), w.data_ptr(), _lib.ptr(bias), _lib.ptr(residual), int(act), T,
               x2.stride(0), N, K, _lib.DTYPE[w.dtype], y.data_ptr(), _lib.DTYPE[y.dtype], _lib.ptr(z), _lib.ptr(ws), nws)
     return y.view(*x.shape[:-1], N), z
@@ -88,10 +112,10 @@ class _Linear(torch.autograd.Function):
             if ctx.act != NONE:
                 dz = act_backward(dz, z, ctx.act, codes, scales)
             if need_x:
-                dx = grouped.mm_dx(dz, w[None], None).view(x.shape)
+                dx = _dx(dz, w).view(x.shape)
             if need_w or need_b:
-                dw, db = grouped.mm_dw(dz, x.reshape(-1, x.shape[-1]), None, 1, bias=True)
-        return dx, dw[0] if need_w else None, db[0] if need_b else None, None, dy if ctx.needs_input_grad[4] else None, None, None
+                dw, db = _dw(dz, _rows(x, "x", w.shape[1], w.device, w.dtype), need_b)
+        return dx, dw if need_w else None, db, None, dy if ctx.needs_input_grad[4] else None, None, None
 
 
 def linear(x, w, bias=None, act=NONE, residual=None, out_dtype=None, checkpoint=False):
