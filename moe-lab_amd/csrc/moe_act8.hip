@@ -195,9 +195,9 @@ __global__ void __launch_bounds__(256) k_slots(const int32_t* idx, const int32_t
     if ((uint32_t)idx[p] >= (uint32_t)E) pos[p] = -1;
 }
 
-// y[t] = residual[t] + sum_j w[t][j] ys[pos[t k + j]] in fp32, slots in ascending j; 8 columns per item
-template <bool F16>
-__global__ void __launch_bounds__(256) k_slot_sum(const uint16_t* ys, const int32_t* pos, const float* wts, const uint16_t* residual,
+// y[t] = residual[t] + sum_j w[t][j] ys[pos[t k + j]] in fp32, slots in ascending j; 8 columns per item. S32: ys is fp32.
+template <bool F16, bool S32>
+__global__ void __launch_bounds__(256) k_slot_sum(const void* ys, const int32_t* pos, const float* wts, const uint16_t* residual,
                                                   int64_t M, int k, int d, uint32_t items, uint32_t per_row, void* y, int ydt) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
     if (i >= items) return;
@@ -210,7 +210,14 @@ __global__ void __launch_bounds__(256) k_slot_sum(const uint16_t* ys, const int3
         if (p < 0 || p >= M) continue;
         const float w = wts ? wts[(uint64_t)t * k + j] : 1.f;
         float v[8];
-        unpack8<F16>(*(const u32x4*)(ys + (uint64_t)p * d + c), v);
+        if constexpr (S32) {
+            const f32x4* s = (const f32x4*)((const float*)ys + (uint64_t)p * d + c);
+            const f32x4 lo = s[0], hi = s[1];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = lo[q], v[4 + q] = hi[q];
+        } else {
+            unpack8<F16>(*(const u32x4*)((const uint16_t*)ys + (uint64_t)p * d + c), v);
+        }
 #pragma unroll
         for (int q = 0; q < 8; ++q) acc[q] += w * v[q];
     }
@@ -299,15 +306,16 @@ int launch_slots(const int32_t* idx, const int32_t* sorted, const int32_t* offse
     k_slots<<<(n + 255) / 256, 256, 0, st>>>(idx, sorted, offsets, n, k, E, rows, pos);
     return done();
 }
-int launch_slot_sum(const void* ys, const int32_t* pos, const float* wts, const void* residual, int64_t M, int64_t T, int k, int d,
-                    bool f16, void* y, int ydt, hipStream_t st) {
+int launch_slot_sum(const void* ys, bool s32, const int32_t* pos, const float* wts, const void* residual, int64_t M, int64_t T, int k,
+                    int d, bool f16, void* y, int ydt, hipStream_t st) {
     return by_parts(T, d / 8, [&](int64_t r, uint32_t items, unsigned grid) {
         const int32_t* p = pos + r * k;
         const float* w = wts ? wts + r * k : nullptr;
         const uint16_t* res = residual ? (const uint16_t*)residual + r * d : nullptr;
         void* o = (char*)y + r * d * (ydt == MOE_DTYPE_F32 ? 4 : 2);
-        if (f16) k_slot_sum<true><<<grid, 256, 0, st>>>((const uint16_t*)ys, p, w, res, M, k, d, items, d / 8, o, ydt);
-        else k_slot_sum<false><<<grid, 256, 0, st>>>((const uint16_t*)ys, p, w, res, M, k, d, items, d / 8, o, ydt);
+        auto go = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(ys, p, w, res, M, k, d, items, d / 8, o, ydt); };
+        if (s32) f16 ? go(k_slot_sum<true, true>) : go(k_slot_sum<false, true>);
+        else f16 ? go(k_slot_sum<true, false>) : go(k_slot_sum<false, false>);
     });
 }
 
