@@ -194,14 +194,23 @@ struct MmTile {
     int j0;
 };
 
-// The tiles are dealt to the 8 XCDs in contiguous runs (workgroup b runs on XCD b % 8), so that tiles that share an expert's
-// weights share an L2; inside a run the XCD's workgroups take tiles in turn.
+// Workgroup b runs on XCD b % 8. The tiles go round by round, in each to the XCDs one after the other, as many as an XCD has
+// workgroups: neighbouring tiles, which share an expert's weights, share an L2, and a busy expert's tiles spread over all XCDs.
+// The tiles left after whole rounds are dealt evenly.
 struct MmRun {
-    int id, end, stride;
+    static constexpr int NONE = 0x7fffffff;
+    int first, step, whole, last;
+    __device__ __forceinline__ int next(int id) const { return id >= whole ? NONE : id + step < whole ? id + step : last; }
 };
 __device__ __forceinline__ MmRun xcd_run(int tiles) {
-    const int xcd = blockIdx.x & 7, rem = tiles & 7, q = tiles >> 3, start = xcd * q + min(xcd, rem);
-    return {start + (int)(blockIdx.x >> 3), start + q + (xcd < rem), (int)(gridDim.x >> 3)};
+    const int xcd = blockIdx.x & 7, w = blockIdx.x >> 3, per = gridDim.x >> 3;
+    MmRun r;
+    r.step = gridDim.x;
+    r.whole = tiles / r.step * r.step;
+    const int left = tiles - r.whole, q = left >> 3, rem = left & 7;
+    r.last = w < q + (xcd < rem) ? r.whole + xcd * q + min(xcd, rem) + w : MmRun::NONE;
+    r.first = r.whole ? xcd * per + w : r.last;
+    return r;
 }
 
 // Row tiles of the groups, counted on the device: pre[e] = tiles of the groups before e. Wave 0 scans 64 groups at a time.
@@ -525,7 +534,7 @@ struct MmKernel {
         auto steps_of = [&](const MmTile& t) -> int { return ((MODE == MM_DW ? t.cnt : r_of(t)) + 63) / 64; };
 
         // the stream of loads: its tile, the step in it, and where the operands' next pieces begin
-        int lid = run.id - run.stride, ls = 0, lsteps = 0, lrows = 0, lr = 0;
+        int lid = -1, ls = 0, lsteps = 0, lrows = 0, lr = 0;
         MmTile lt{};
         const char *pa = nullptr, *pb = nullptr;
         int rowa, cola, rowb, colb;
@@ -544,8 +553,8 @@ struct MmKernel {
         auto next_load_tile = [&]() {
             ls = 0;
             do {
-                lid += run.stride;
-                if (lid >= run.end) {   // no more: empty descriptors
+                lid = lid < 0 ? run.first : run.next(lid);
+                if (lid == MmRun::NONE) {   // no more: empty descriptors
                     lsteps = 0x7fffffff;
                     lrows = lt.cnt = 0;
                     return;
@@ -668,7 +677,7 @@ struct MmKernel {
             }
         };
 
-        if (run.id >= run.end) return;
+        if (run.first == MmRun::NONE) return;
         uint32_t rbuf = 0, wbuf = 0;   // stage buffers of the step that is multiplied, and of the load step
         auto next_buf = [](uint32_t b) -> uint32_t { return b == (ST - 1) * STAGE ? 0 : b + STAGE; };
 #pragma unroll
@@ -690,7 +699,7 @@ struct MmKernel {
 #pragma unroll
         for (int h = 0; h < FB; ++h) rb[0][h] = B::read(sm, frb, h, 1, 0);
 
-        for (int id = run.id; id < run.end; id += run.stride) {
+        for (int id = run.first; id != MmRun::NONE; id = run.next(id)) {
             MmTile t;
             tile(id, t);
             const int steps = steps_of(t), nf = (t.rows + 31) / 32;
