@@ -24,13 +24,18 @@ Two levels, as in the reference:
   its k-reduction, at T = 1), and the routing weights and the sum over a token's slots are applied afterwards,
   outside the kernels, so the model's own router and any extra terms stay as they are.
 
+* ``patch_dense`` puts the modules that hold the 16-bit weights, an experts module or a dense GLU MLP (a shared expert),
+  on the unquantised kernels (dense.experts_mlp, dense.glu_mlp): their own parameters, nothing packed, and gradients
+  to the parameters, the tokens and the routing weights, for a model that is trained or not quantised yet. With
+  ``patch_model(model, fmt="dense")`` every sparse MoE block's experts and shared experts; routers stay stock.
+
 The stock forwards are kept (``_moelab_stock_forward``); ``unpatch_block`` / ``unpatch_experts`` restore them.
 ``load_dequantised`` writes the state's dequantised weights back into the stock modules, so stock and patched
 forwards then differ by arithmetic only, not by quantisation.
 """
 import torch
 
-from . import _lib
+from . import _lib, dense
 from .experts import merge_shared, run_experts, run_layer, run_routed
 from .variants import hip_mxfp4_moe, hip_q4_moe
 
@@ -215,12 +220,57 @@ def unpatch_experts(experts):
     return experts
 
 
-def patch_model(model, fmt=None, universal=False):
+def _glu_linears(m):
+    """The gate, up and down weights of a dense GLU MLP without biases, or None."""
+    ls = [getattr(m, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+    ok = all(isinstance(x, torch.nn.Linear) and x.bias is None for x in ls) and hasattr(m, "act_fn")
+    return [x.weight for x in ls] if ok else None
+
+
+def patch_dense(module, checkpoint=True):
+    """Put a stacked experts module (forward(hidden_states [T, d], top_k_index [T, k], top_k_weights [T, k])) or a dense
+    GLU MLP (gate_proj, up_proj, down_proj, act_fn) on the 16-bit kernels, forward and backward, with the module's own
+    bf16 or fp16 parameters. checkpoint: activations are kept in 8 bits for the backward pass. unpatch_experts undoes it."""
+    stacked, glu = _stacked(module), _glu_linears(module)
+    if not stacked and glu is None:
+        raise ValueError(f"{type(module).__name__}: neither a stacked experts module nor a GLU MLP without biases")
+    act = _act_of(module)
+    ws = (module.gate_up_proj, module.down_proj) if stacked else glu
+    if any(w.dtype != ws[0].dtype or w.dtype not in (torch.bfloat16, torch.float16) for w in ws):
+        raise TypeError(f"weights in {', '.join(sorted({str(w.dtype) for w in ws}))}: all bf16 or all fp16 expected")
+    d, F = (ws[1].shape[1], ws[1].shape[2]) if stacked else (ws[0].shape[1], ws[0].shape[0])
+    _lib.multiple_of(d, 8, "the hidden size")
+    _lib.multiple_of(F, 32, "the intermediate size")
+
+    def experts_forward(hidden_states, top_k_index, top_k_weights):
+        return dense.experts_mlp(hidden_states, top_k_index, top_k_weights, module.gate_up_proj, module.down_proj, act=act,
+                                 checkpoint=checkpoint)
+
+    def mlp_forward(x):
+        return dense.glu_mlp(x, module.gate_proj.weight, module.up_proj.weight, module.down_proj.weight, act=act,
+                             checkpoint=checkpoint)
+
+    module._moelab_stock_forward = module.forward
+    module._moelab_state = {"fmt": "dense"}
+    module.forward = experts_forward if stacked else mlp_forward
+    return module
+
+
+def patch_model(model, fmt=None, universal=False, checkpoint=True):
     """Patch every sparse MoE block of a model (universal: every stacked experts module instead); returns how many
-    modules were patched."""
+    modules were patched. fmt "dense": patch_dense (with checkpoint) on each block's experts and shared experts
+    (universal: on every stacked experts module)."""
     n = 0
     for m in list(model.modules()):
         if hasattr(m, "_moelab_state"):
+            continue
+        if fmt == "dense":
+            parts = [m] if universal else [m.experts, getattr(m, "shared_expert", None), getattr(m, "shared_experts", None)] \
+                if is_moe_block(m) else []
+            for part in parts:
+                if part is not None and not hasattr(part, "_moelab_state") and (not universal or _stacked(part)):
+                    patch_dense(part, checkpoint)
+                    n += 1
             continue
         if universal:
             if _stacked(m) and not hasattr(m, "gate_up_proj_bias"):
@@ -242,6 +292,8 @@ def load_dequantised(module):
     """Write the patched module's dequantised weights back into its stock modules (experts, shared experts), so
     stock and patched forwards see the same weights."""
     s = module._moelab_state
+    if s["fmt"] == "dense":
+        raise ValueError("patch_dense packs nothing: the stock modules hold the weights it runs on")
     cfg = getattr(module, "_moelab_cfg", {"kind": "experts"})
     wg, wu, wd = _deq(s)
     kind = cfg["kind"]
