@@ -204,22 +204,34 @@ __global__ void __launch_bounds__(256) k_slot_sum(const void* ys, const int32_t*
     const uint32_t t = i / per_row, c = (i - t * per_row) * 8;
     float acc[8] = {};
     if (residual) unpack8<F16>(*(const u32x4*)(residual + (uint64_t)t * d + c), acc);
-#pragma unroll 4
-    for (int j = 0; j < k; ++j) {
-        const int p = pos[(uint64_t)t * k + j];
-        if (p < 0 || p >= M) continue;
-        const float w = wts ? wts[(uint64_t)t * k + j] : 1.f;
-        float v[8];
-        if constexpr (S32) {
-            const f32x4* s = (const f32x4*)((const float*)ys + (uint64_t)p * d + c);
-            const f32x4 lo = s[0], hi = s[1];
+    // eight slots' loads before their sums: a branch per slot would wait for each (5 tokens of 8 slots: 5.6 us)
+    for (int j0 = 0; j0 < k; j0 += 8) {
+        int p[8];
+        float w[8], v[8][8];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = lo[q], v[4 + q] = hi[q];
-        } else {
-            unpack8<F16>(*(const u32x4*)((const uint16_t*)ys + (uint64_t)p * d + c), v);
+        for (int j = 0; j < 8; ++j) {
+            const uint64_t s = (uint64_t)t * k + min(j0 + j, k - 1);
+            p[j] = pos[s];
+            w[j] = wts ? wts[s] : 1.f;
+            if (j0 + j >= k || p[j] >= M) p[j] = -1;
         }
 #pragma unroll
-        for (int q = 0; q < 8; ++q) acc[q] += w * v[q];
+        for (int j = 0; j < 8; ++j) {
+            const uint64_t at = (uint64_t)max(p[j], 0) * d + c;
+            if constexpr (S32) {
+                const f32x4 lo = *(const f32x4*)((const float*)ys + at), hi = *(const f32x4*)((const float*)ys + at + 4);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[j][q] = lo[q], v[j][4 + q] = hi[q];
+            } else {
+                unpack8<F16>(*(const u32x4*)((const uint16_t*)ys + at), v[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (p[j] < 0) continue;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) acc[q] += w[j] * v[j][q];
+        }
     }
     if (ydt == MOE_DTYPE_F32) {
         f32x4* o = (f32x4*)((float*)y + (uint64_t)i * 8);
