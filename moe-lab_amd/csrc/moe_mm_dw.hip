@@ -20,8 +20,13 @@ static int dense(const MmArgs& a) {
 }
 
 template <bool F16>
-static int launch(const MmArgs& a, hipStream_t st) {
+static int launch(const MmArgs& args, hipStream_t st) {
+    MmArgs a = args;
     const int s = a.offsets ? grouped(a) : dense(a);
+    // operands up to half of the memory cache, in groups of a few steps
+    const bool list = a.arows || a.brows;
+    const int64_t ra = list ? a.a_n : a.M, rb = list ? a.b_n : a.M;
+    a.touch = a.offsets && a.M > 0 && ra * a.lda + rb * a.ldb <= (64 << 20) && a.M / a.E <= 256;
     switch (s) {
         case MM_256: return launch_mm_cfg<MM_DW, F16, 8, 8, 2, 2, 1>(a, st);
         case MM_64: return launch_mm_cfg<MM_DW, F16, 2, 2, 2, 4, 2>(a, st);
