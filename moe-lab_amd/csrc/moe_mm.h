@@ -201,18 +201,25 @@ struct MmTile {
 
 // Workgroup b runs on XCD b % 8. The tiles go round by round, in each to the XCDs one after the other, as many as an XCD has
 // workgroups: neighbouring tiles, which share an expert's weights, share an L2, and a busy expert's tiles spread over all XCDs.
-// The tiles left after whole rounds are dealt evenly.
+// The tiles left after whole rounds are dealt evenly, in the forward and dx products cut into 2 or 4 pieces of their rows while
+// that leaves a piece or none to a CU: a piece's weights are read by its neighbours on the XCD too, its products are its own
+// (dx of 8 experts x 256, w [14336, 4096]: 442 -> 398 us, 16 x 64, [8192, 5120]: 313 -> 294).
 struct MmRun {
     static constexpr int NONE = 0x7fffffff;
-    int first, step, whole, last;
+    int first, step, whole, last, cut;   // cut: log2 of the pieces
     __device__ __forceinline__ int next(int id) const { return id >= whole ? NONE : id + step < whole ? id + step : last; }
+    __device__ __forceinline__ int tile(int id) const { return id < whole ? id : whole + ((id - whole) >> cut); }
 };
+template <int MAX_CUT>
 __device__ __forceinline__ MmRun xcd_run(int tiles) {
     const int xcd = blockIdx.x & 7, w = blockIdx.x >> 3, per = gridDim.x >> 3;
     MmRun r;
     r.step = gridDim.x;
     r.whole = tiles / r.step * r.step;
-    const int left = tiles - r.whole, q = left >> 3, rem = left & 7;
+    int left = tiles - r.whole;
+    r.cut = 0;
+    while (r.cut < MAX_CUT && left * 2 <= min(r.step, 256)) left *= 2, ++r.cut;
+    const int q = left >> 3, rem = left & 7;
     r.last = w < q + (xcd < rem) ? r.whole + xcd * q + min(xcd, rem) + w : MmRun::NONE;
     r.first = r.whole ? xcd * per + w : r.last;
     return r;
@@ -530,13 +537,20 @@ struct MmKernel {
             tiles = __builtin_amdgcn_readfirstlane(pre[g.E]) * nj;
             if (g.fill && g.offsets) fill_rest<MODE>(g);
         }
-        const MmRun run = xcd_run(tiles);
+        const MmRun run = xcd_run<MODE == MM_DW ? 0 : FA >= 4 ? 2 : 1>(tiles);
         auto tile = [&](int id, MmTile& t) {
             if constexpr (MODE == MM_DW) tile_at_dw<BI, TJ>(g, id, t);
-            else tile_at<MODE, BI, TJ>(g, pre, id, t);
+            else tile_at<MODE, BI, TJ>(g, pre, run.tile(id), t);
+            if constexpr (MODE != MM_DW) {
+                if (id >= run.whole) {   // a piece (the last ones of a tile with few rows are empty)
+                    const int n = BI >> run.cut, lo = ((id - run.whole) & ((1 << run.cut) - 1)) * n;
+                    t.lo += lo;
+                    t.rows = max(0, min(n, t.rows - lo));
+                }
+            }
         };
         auto r_of = [&](const MmTile& t) -> int { return g.part ? min(g.part, g.R - t.e * g.part) : g.R; };   // forward, dx
-        auto steps_of = [&](const MmTile& t) -> int { return ((MODE == MM_DW ? t.cnt : r_of(t)) + 63) / 64; };
+        auto steps_of = [&](const MmTile& t) -> int { return MODE == MM_DW ? (t.cnt + 63) / 64 : t.rows ? (r_of(t) + 63) / 64 : 0; };
 
         // the stream of loads: its tile, the step in it, and where the operands' next pieces begin
         int lid = -1, ls = 0, lsteps = 0, lrows = 0, lr = 0;
@@ -858,7 +872,8 @@ int launch_mm_cfg(const MmArgs& a, hipStream_t st) {
     const int64_t ni = MODE == MM_DW ? (int64_t)a.E * ((a.I + 32 * FA - 1) / (32 * FA)) : mm_row_tiles(a, 32 * FA);
     if (ni * nj == 0) return MOE_OK;
     if (ni * nj > 0x7fffffff) return MOE_ERR_ARG;
-    const int64_t most = 256 * OCC, grid = round8(ni * nj) < most ? round8(ni * nj) : most;   // 256 CUs
+    constexpr int CUT = MODE == MM_DW ? 1 : FA >= 4 ? 4 : 2;   // pieces that a tile can be cut into
+    const int64_t most = 256 * OCC, grid = round8(CUT * ni * nj) < most ? round8(CUT * ni * nj) : most;   // 256 CUs
     auto go = [&](auto epi) {
         constexpr int EPI = decltype(epi)::value;
         if (gather) k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, true, EPI><<<(unsigned)grid, 128 * NWJ, 0, st>>>(a);
