@@ -227,8 +227,9 @@ __device__ __forceinline__ MmRun xcd_run(int tiles) {
 
 // Row tiles of the groups, counted on the device: pre[e] = tiles of the groups before e. Wave 0 scans 64 groups at a time.
 #define MM_MAX_E 1024
+// most: offsets that overlap (which the caller should not pass) could count past 32 bits.
 template <int MODE, int BI>
-__device__ __forceinline__ void count_tiles(const MmArgs& a, int* pre) {
+__device__ __forceinline__ void count_tiles(const MmArgs& a, int* pre, int most) {
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x;
         int before = 0;
@@ -240,7 +241,7 @@ __device__ __forceinline__ void count_tiles(const MmArgs& a, int* pre) {
                 group_of<MODE>(a, base + lane, lo, hi);
                 n = (hi - lo) / BI + ((hi - lo) % BI > 0);
             }
-            const int s = wave_incl_scan(n) + before;
+            const int s = min(wave_incl_scan(n) + before, most);
             if (base + lane < a.E) pre[base + lane + 1] = s;
             before = __builtin_amdgcn_readlane(s, 63);
         }
@@ -533,7 +534,7 @@ struct MmKernel {
         if constexpr (MODE == MM_DW) {
             tiles = g.E * ((g.I + BI - 1) / BI) * nj;
         } else {
-            count_tiles<MODE, BI>(g, pre);
+            count_tiles<MODE, BI>(g, pre, 0x70000000 / nj);
             tiles = __builtin_amdgcn_readfirstlane(pre[g.E]) * nj;
             if (g.fill && g.offsets) fill_rest<MODE>(g);
         }
@@ -871,7 +872,7 @@ int launch_mm_cfg(const MmArgs& a, hipStream_t st) {
     const int64_t nj = (a.J + bj - 1) / bj;
     const int64_t ni = MODE == MM_DW ? (int64_t)a.E * ((a.I + 32 * FA - 1) / (32 * FA)) : mm_row_tiles(a, 32 * FA);
     if (ni * nj == 0) return MOE_OK;
-    if (ni * nj > 0x7fffffff) return MOE_ERR_ARG;
+    if (ni * nj > 0x70000000) return MOE_ERR_ARG;
     constexpr int CUT = MODE == MM_DW ? 1 : FA >= 4 ? 4 : 2;   // pieces that a tile can be cut into
     const int64_t most = 256 * OCC, grid = round8(CUT * ni * nj) < most ? round8(CUT * ni * nj) : most;   // 256 CUs
     auto go = [&](auto epi) {

@@ -175,7 +175,8 @@ int moe_linear(const void* x, const void* w, const void* bias, const void* resid
     if (misaligned(x) || misaligned(w) || misaligned(y) || misaligned(bias) || misaligned(residual) || misaligned(z) ||
         misaligned(workspace))
         return MOE_ERR_ALIGN;
-    if (workspace_bytes < moe_linear_workspace_bytes(T, N, K)) return MOE_ERR_WORKSPACE;
+    const size_t need = moe_linear_workspace_bytes(T, N, K);
+    if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE;
     moe::MmArgs a{};
     a.a = x;
     a.b = w;
@@ -203,7 +204,8 @@ int moe_linear_dx(const void* dy, const void* w, int64_t T, int64_t lddy, int N,
     if (T == 0) return MOE_OK;
     if (!dy || !w || !dx) return MOE_ERR_ARG;
     if (misaligned(dy) || misaligned(w) || misaligned(dx) || misaligned(workspace)) return MOE_ERR_ALIGN;
-    if (workspace_bytes < moe_linear_dx_workspace_bytes(T, N, K)) return MOE_ERR_WORKSPACE;
+    const size_t need = moe_linear_dx_workspace_bytes(T, N, K);
+    if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE;
     moe::MmArgs a{};
     a.a = dy;
     a.b = w;
@@ -228,7 +230,8 @@ int moe_linear_dw(const void* dy, const void* x, int64_t T, int64_t lddy, int64_
     if (T < 0 || T > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N) || bad_ld(ldx, K)) return MOE_ERR_ARG;
     if (!dw || (T > 0 && (!dy || !x))) return MOE_ERR_ARG;
     if (misaligned(dy) || misaligned(x) || misaligned(dw) || misaligned(workspace)) return MOE_ERR_ALIGN;
-    if (workspace_bytes < moe_linear_dw_workspace_bytes(T, N, K)) return MOE_ERR_WORKSPACE;
+    const size_t need = moe_linear_dw_workspace_bytes(T, N, K);
+    if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE;
     moe::MmArgs a{};
     a.a = dy;
     a.b = x;
