@@ -10,6 +10,10 @@ Modules:
     router                      fused gate GEMV + router tail, stable slot grouping
     experts, fallback           the expert-path call and the per-slot stock-style path
     variants/                   drop-in variant modules (prepare / run / dequant contract)
+    grouped, linear             16-bit products by expert, and with an epilogue, with their gradients
+    act8                        activations kept in 8 bits for a backward pass; the GLU on them
+    dense                       the expert layer on 16-bit weights, forward and backward
+    patch                       transformers' MoE blocks onto the kernels, quantised or in 16 bits
     backend                     torch-ROCm harness: fp32 reference, errors, chained timing
 """
 __version__ = "0.1.0"

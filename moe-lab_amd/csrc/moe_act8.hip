@@ -1,6 +1,7 @@
 // Elementwise passes of the 16-bit expert layer: the GLU with its input kept in 8 bits, its backward pass from those codes,
 // the activation's backward pass of the linear layer, and the weighted sum of a token's slots. Each is one pass over its
-// data, 16 bytes per lane and load, and bound by HBM.
+// data, 16 bytes per lane and load, and bound by HBM (traced: GLU with codes, 32768 rows of F 768, 33 us for 203 MB; from codes
+// back to 16 bits 24 us for 153 MB; backward, 16383 rows of F 1024, 30 us for 169 MB).
 #include "moe_mm.h"
 #include "moe_rows.h"
 

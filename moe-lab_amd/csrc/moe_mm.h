@@ -311,6 +311,9 @@ __device__ __forceinline__ f32x4 load4(const void* p, int64_t i) {
 // A workgroup goes through its tiles with two streams: loads run ST steps ahead of the products and pass from one tile into the
 // next, so a tile's first stages arrive during the last one's products and stores. Every step loads the same number of pieces
 // (past the last tile from empty descriptors: zeros, no traffic), so the waits are constants.
+// What bounds it (4096^3, 256 x 256: 117 us, 1.17 PFLOP/s; a library product 92-104): with no loads 84 us, with no products 93,
+// so reads of LDS and loads into it take as long as the matrix cores and overlap them in part; with ragged groups loads alone,
+// at 3.5-5.6 TB/s of weights (a tile reads 128 bytes of a row at a time in the forward pass).
 // EPI_GLU: the tile's columns are BJ / 2 of gate and the same of up, half by half for each wave, so that a lane holds both.
 template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, bool GATHER, int EPI, bool LDS_OUT>
 struct MmKernel {

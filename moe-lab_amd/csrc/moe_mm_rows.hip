@@ -9,7 +9,8 @@ __device__ __forceinline__ float dot2(uint32_t a, uint32_t b, float c) {
 }
 
 // A group's rows are multiplied MR at a time; the weights come from HBM once and, for the further passes of a group with more
-// rows, from the caches. Bound by the weights' bytes: every 16-byte load of a wave is a contiguous 1 KiB of a weight row.
+// rows, from the caches. Bound by the weights' bytes: every 16-byte load of a wave is a contiguous 1 KiB of a weight row
+// (traced: w [14336, 4096], one row: 19.6 us, 6.0 TB/s; 8 experts' [1536, 2048]: 10.6 us, 4.7 TB/s).
 // GLU: a wave takes R rows of gate and the same R of up, and writes h.
 // Workgroups go by slot, not by group: with few slots most groups are empty. The one at a group's first slot does the group.
 template <bool F16, int R, int MR, bool GLU>
