@@ -22,9 +22,9 @@ def _workspace(size, T, N, K, device):
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None, n
 
 
+# dz, x and w as half_matrix and plain return them
 def _dx(dz, w):
     (T, N), K = dz.shape, w.shape[1]
-    w = _lib.plain(w, "w", (N, K), dz.device, dz.dtype)
     dx = torch.empty((T, K), dtype=w.dtype, device=w.device)
     ws, nws = _workspace("moe_linear_dx_workspace_bytes", T, N, K, w.device)
     _lib.call("moe_linear_dx", w.device, dz.data_ptr(), w.data_ptr(), T, dz.stride(0), N, K, _lib.DTYPE[w.dtype], dx.data_ptr(),
@@ -43,7 +43,12 @@ def _dw(dz, x, bias):
 
 
 def _forward(x, w, bias, act, residual, out_dtype, keep_z):
-    """y [T, N] and z (None unless keep_z)."""
+    """y [..., N] and z [T, N] (None unless keep_z)."""
+    return _run(x, w, bias, act, residual, out_dtype, keep_z)[:2]
+
+
+def _run(x, w, bias, act, residual, out_dtype, keep_z):
+    """y, z, and x [T, K] and w as the kernels read them."""
     _lib.require_device(w, "w")
     if w.dim() != 2:
         raise ValueError(f"w has shape {tuple(w.shape)}: [N, K] expected")
@@ -66,7 +71,7 @@ def _forward(x, w, bias, act, residual, out_dtype, keep_z):
     ws, nws = _workspace("moe_linear_workspace_bytes", T, N, K, w.device)
     _lib.call("moe_linear", w.device, x2.data_ptr(), w.data_ptr(), _lib.ptr(bias), _lib.ptr(residual), int(act), T,
               x2.stride(0), N, K, _lib.DTYPE[w.dtype], y.data_ptr(), _lib.DTYPE[y.dtype], _lib.ptr(z), _lib.ptr(ws), nws)
-    return y.view(*x.shape[:-1], N), z
+    return y.view(*x.shape[:-1], N), z, x2, w
 
 
 def act_backward(dy, z, act, codes=None, scales=None):
@@ -81,6 +86,11 @@ def act_backward(dy, z, act, codes=None, scales=None):
     z = _lib.plain(z, "z", (T, N), dy.device, dy.dtype)
     if codes is not None:
         codes, scales = act8.check_codes(codes, scales, (T, N), dy.device)
+    return _act_backward(dy, z, act, codes, scales)
+
+
+def _act_backward(dy, z, act, codes, scales):
+    T, N = dy.shape
     dz = torch.empty((T, N), dtype=dy.dtype, device=dy.device)
     _lib.call("moe_linear_act_bwd", dy.device, dy.data_ptr(), dy.stride(0), _lib.ptr(z), _lib.ptr(codes), _lib.ptr(scales),
               int(act), T, N, _lib.DTYPE[dy.dtype], dz.data_ptr())
@@ -91,13 +101,15 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, act, residual, out_dtype, checkpoint):
         need_z = act != NONE and any(ctx.needs_input_grad[:3])
-        y, z = _forward(x, w, bias, act, residual, out_dtype, need_z)
+        y, z, x2, w2 = _run(x, w, bias, act, residual, out_dtype, need_z)
         codes = scales = None
         if need_z and checkpoint:
             codes, scales = act8.pack(z)
             z = None
-        ctx.save_for_backward(x, w, z, codes, scales)
-        ctx.act = act
+        # the inputs themselves where the kernels read them in place, so that a change before the backward pass is noticed
+        in_place = x2.data_ptr() == x.data_ptr() and x.is_contiguous()
+        ctx.save_for_backward(x if in_place else x2, w2, z, codes, scales)
+        ctx.act, ctx.x_shape = act, x.shape
         return y
 
     @staticmethod
@@ -110,11 +122,11 @@ class _Linear(torch.autograd.Function):
         if need_x or need_w or need_b:
             dz = _rows(dy, "dy", w.shape[0], w.device, w.dtype)
             if ctx.act != NONE:
-                dz = act_backward(dz, z, ctx.act, codes, scales)
+                dz = _act_backward(dz, z, ctx.act, codes, scales)
             if need_x:
-                dx = _dx(dz, w).view(x.shape)
+                dx = _dx(dz, w).view(ctx.x_shape)
             if need_w or need_b:
-                dw, db = _dw(dz, _rows(x, "x", w.shape[1], w.device, w.dtype), need_b)
+                dw, db = _dw(dz, x.view(-1, w.shape[1]) if x.dim() != 2 else x, need_b)
         return dx, dw if need_w else None, db, None, dy if ctx.needs_input_grad[4] else None, None, None
 
 
