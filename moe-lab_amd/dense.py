@@ -46,6 +46,8 @@ def _slot_lists(x, idx, wts):
         raise TypeError(f"idx {idx.dtype} and wts {wts.dtype}: int32 (or int64) and a floating type expected")
     if idx.device != x.device or wts.device != x.device:
         raise ValueError("idx and wts must be on x's device")
+    if idx.dtype == torch.int64:   # an id past 32 bits stays outside [0, E)
+        idx = idx.clamp(-1, 2 ** 31 - 1)
     return _lib.dense(idx, torch.int32), _lib.dense(wts, torch.float32)
 
 

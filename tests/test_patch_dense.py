@@ -134,3 +134,15 @@ def test_an_update_in_place_is_seen():
         a = block.experts(x, idx, wts)
         block.experts.down_proj.mul_(2.0)
         assert torch.equal(block.experts(x, idx, wts), 2 * a)
+
+
+@pytest.mark.gpu
+def test_ids_past_32_bits_are_outside():
+    e = make_block("mixtral", "cuda").experts
+    x = H.randn(3, D, dtype=torch.bfloat16)
+    far = torch.tensor([[0, 2 ** 32 + 1], [2 ** 32, 2 ** 33], [-2 ** 32, 3]], device="cuda")
+    near = torch.tensor([[0, -1], [-1, 4], [-1, 3]], device="cuda")
+    wts = torch.full((3, 2), 0.5, device="cuda")
+    with torch.no_grad():
+        y = dense.experts_mlp(x, far, wts, e.gate_up_proj, e.down_proj)
+        assert torch.equal(y, dense.experts_mlp(x, near, wts, e.gate_up_proj, e.down_proj)) and not y[1].any() and y[0].any()
