@@ -311,16 +311,20 @@ __device__ __forceinline__ f32x4 load4(const void* p, int64_t i) {
 // A workgroup goes through its tiles with two streams: loads run ST steps ahead of the products and pass from one tile into the
 // next, so a tile's first stages arrive during the last one's products and stores. Every step loads the same number of pieces
 // (past the last tile from empty descriptors: zeros, no traffic), so the waits are constants.
-// What bounds it (4096^3, 256 x 256: 117 us, 1.17 PFLOP/s; a library product 92-104): with no loads 84 us, with no products 93,
-// so reads of LDS and loads into it take as long as the matrix cores and overlap them in part; with ragged groups loads alone,
-// at 3.5-5.6 TB/s of weights (a tile reads 128 bytes of a row at a time in the forward pass).
+// NL > 0: as many waves beside the others only load. A wave's loads wait for their turn to be issued, and the products behind
+// them with it (4096^3 without any loads: 84 us of 117): 128 x 256 went from 131 to 109 us for 4096^3, 197 to 178 for dx of
+// 64 experts x 256 slots, 128 x 128 from 48 to 40 for 1024 x 4096 x 4096. 12 waves leave 168 registers each, enough for 64 x 64
+// outputs of a wave; 256 x 256 tiles with 4 waves of all registers are no faster and are gone. With two workgroups of 6 waves on a
+// CU they do not pay (128 x 128: the second one does not fit).
+// What bounds it: dense, LDS reads and loads into LDS beside the matrix cores (4096^3: 1.17-1.26 PFLOP/s, a library product
+// 1.3-1.5); ragged groups, loads, at 3.6-5.8 TB/s of weights.
 // EPI_GLU: the tile's columns are BJ / 2 of gate and the same of up, half by half for each wave, so that a lane holds both.
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, bool GATHER, int EPI, bool LDS_OUT>
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, bool GATHER, int EPI, bool LDS_OUT, int NL>
 struct MmKernel {
     static constexpr bool GLU = EPI == EPI_GLU;
-    static constexpr bool ACC = FA * FB * 4 >= 256;   // the sums fill the accumulation registers
     static constexpr bool AX = MODE == MM_DW, BX = MODE != MM_FWD;   // operand with its own index contiguous
-    static constexpr int NW = 2 * NWJ, BI = 32 * FA, BJ = 16 * NWJ * FB;
+    static constexpr int NWC = 2 * NWJ, NW = NL ? NL : NWC;   // waves that multiply, waves that load
+    static constexpr int BI = 32 * FA, BJ = 16 * NWJ * FB;
     static constexpr int TJ = GLU ? BJ / 2 : BJ;   // output columns of a tile
     using A = Operand<AX, BI, NW>;
     using B = Operand<BX, BJ, NW>;
@@ -345,10 +349,6 @@ struct MmKernel {
 #pragma unroll
         for (int f = 0; f < FA; ++f) {
             if (32 * f >= t.rows) break;
-            if constexpr (ACC) {   // read here, not where the branches to here begin: 256 copies would spill
-#pragma unroll
-                for (int h = 0; h < FB; ++h) asm volatile("" : "+a"(acc[f][h]));
-            }
 #pragma unroll
             for (int h = 0; h < FB; ++h)
                 *(u32x2*)(in + h * 32) = (u32x2){pack16<F16>(acc[f][h][0], acc[f][h][1]), pack16<F16>(acc[f][h][2], acc[f][h][3])};
@@ -380,10 +380,6 @@ struct MmKernel {
 #pragma unroll
         for (int f = 0; f < FA; ++f) {
             if (32 * f >= t.rows) break;
-            if constexpr (ACC) {   // read here, not where the branches to here begin: 256 copies would spill
-#pragma unroll
-                for (int h = 0; h < FB; ++h) asm volatile("" : "+a"(acc[f][h]));
-            }
             const int i = 16 * (2 * f + wi) + l;
             const uint32_t row = i < t.rows ? (uint32_t)i * (uint32_t)g.J : MM_OOB / 4;
 #pragma unroll
@@ -457,10 +453,6 @@ struct MmKernel {
 #pragma unroll
         for (int f = 0; f < FA; ++f) {
             if (32 * f >= t.rows) break;
-            if constexpr (ACC) {
-#pragma unroll
-                for (int h = 0; h < FB; ++h) asm volatile("" : "+a"(acc[f][h]));
-            }
             const int i = 16 * (2 * f + wi) + l;
             const bool in = i < t.rows;
 #pragma unroll
@@ -528,6 +520,7 @@ struct MmKernel {
         constexpr int L = PA + PB;
         constexpr bool DB = MODE == MM_DW;   // also dbias
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave & 1, wj = wave >> 1;
+        const int lw = NL ? wave - NWC : wave;   // among the waves that load
         constexpr bool gath_b = MODE == MM_DW && GATHER;
         const int lda2 = g.lda * 2, ldb2 = g.ldb * 2;
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)sm;
@@ -561,8 +554,8 @@ struct MmKernel {
         MmTile lt{};
         const char *pa = nullptr, *pb = nullptr;
         int rowa, cola, rowb, colb;
-        A::at(wave, lane, rowa, cola);
-        B::at(wave, lane, rowb, colb);
+        A::at(lw, lane, rowa, cola);
+        B::at(lw, lane, rowb, colb);
         uint32_t offa[PA], offb[PB];   // each lane's offsets of a step's pieces
         int ia = -1, ib = -1;          // dw, gathered: the step's 64 source rows, one per lane
         auto fetch_rows = [&]() {
@@ -663,9 +656,9 @@ struct MmKernel {
         };
         // pieces i0 .. of either operand, for load step ls into stage buffer `buf`
         constexpr int NA = PA < 4 ? PA : 4, NB = PB < 4 ? PB : 4;
-        auto load_a = [&](uint32_t buf, srd_t d, int i) { dma16<NA, NW * 1024>(d, offa + i, lds0 + buf + (uint32_t)((i * NW + wave) * 1024)); };
+        auto load_a = [&](uint32_t buf, srd_t d, int i) { dma16<NA, NW * 1024>(d, offa + i, lds0 + buf + (uint32_t)((i * NW + lw) * 1024)); };
         auto load_b = [&](uint32_t buf, srd_t d, int i) {
-            dma16<NB, NW * 1024>(d, offb + i, lds0 + buf + (uint32_t)(A::BYTES + (i * NW + wave) * 1024));
+            dma16<NB, NW * 1024>(d, offb + i, lds0 + buf + (uint32_t)(A::BYTES + (i * NW + lw) * 1024));
         };
         auto srd_a = [&]() { return srd_of(pa, bytes_a()); };
         auto srd_b = [&]() { return srd_of(pb, bytes_b()); };
@@ -721,20 +714,46 @@ struct MmKernel {
         }
         uint32_t rbuf = 0, wbuf = 0;   // stage buffers of the step that is multiplied, and of the load step
         auto next_buf = [](uint32_t b) -> uint32_t { return b == (ST - 1) * STAGE ? 0 : b + STAGE; };
+const bool loads = !NL || wave >= NWC;
+        if (loads) {
 #pragma unroll
-        for (int s = 0; s < ST; ++s) {
-            if (ls >= lsteps) next_load_tile();
-            step_offsets();
-            const srd_t da = srd_a(), db = srd_b();
+            for (int s = 0; s < ST; ++s) {
+                if (ls >= lsteps) next_load_tile();
+                step_offsets();
+                const srd_t da = srd_a(), db = srd_b();
 #pragma unroll
-            for (int i = 0; i < PA; i += NA) load_a(wbuf, da, i);
+                for (int i = 0; i < PA; i += NA) load_a(wbuf, da, i);
 #pragma unroll
-            for (int i = 0; i < PB; i += NB) load_b(wbuf, db, i);
-            step_loads();
-            wbuf = next_buf(wbuf);
+                for (int i = 0; i < PB; i += NB) load_b(wbuf, db, i);
+                step_loads();
+                wbuf = next_buf(wbuf);
+            }
+            wait_vm<(ST - 1) * L>();
         }
-        wait_vm<(ST - 1) * L>();
         barrier_raw();
+        if constexpr (NL > 0) {
+            if (loads) {
+                for (int id = run.first; id != MmRun::NONE; id = run.next(id)) {
+                    MmTile t;
+                    tile(id, t);
+                    for (int s = steps_of(t); s > 0; --s) {
+                        if (ls >= lsteps) next_load_tile();
+                        step_offsets();
+                        const srd_t da = srd_a(), db = srd_b();
+                        wait_vm<(ST - 2) * L>();
+                        barrier_raw();
+#pragma unroll
+                        for (int i = 0; i < PB; i += NB) load_b(wbuf, db, i);
+#pragma unroll
+                        for (int i = 0; i < PA; i += NA) load_a(wbuf, da, i);
+                        step_loads();
+                        wbuf = next_buf(wbuf);
+                    }
+                }
+                wait_vm<0>();
+                return;
+            }
+        }
 #pragma unroll
         for (int f = 0; f < FA; ++f) ra[0][f] = A::read(sm, fra, f, 2, 0);
 #pragma unroll
@@ -769,13 +788,16 @@ struct MmKernel {
                 if constexpr (DB) {
                     if (bias) add_rows(0);
                 }
-                if (ls >= lsteps) next_load_tile();
-                step_offsets();
-                const srd_t da = srd_a(), db = srd_b();
+                srd_t da = {}, db = {};
+                if constexpr (!NL) {
+                    if (ls >= lsteps) next_load_tile();
+                    step_offsets();
+                    da = srd_a(), db = srd_b();
+                }
                 // every read of this stage is done, so once all waves are here it is free for the load stream; and the next
                 // stage has landed for all waves
                 wait_lds();
-                wait_vm<(ST - 2) * L>();
+                if constexpr (!NL) wait_vm<(ST - 2) * L>();
                 barrier_raw();
                 rbuf = next_buf(rbuf);
 #pragma unroll
@@ -786,7 +808,7 @@ struct MmKernel {
                     // the pieces, four at a time, over the row blocks
                     constexpr int CALLS = PA / NA + PB / NB;
 #pragma unroll
-                    for (int c = f * CALLS / FA; c < (f + 1) * CALLS / FA; ++c) {
+                    for (int c = NL ? CALLS : f * CALLS / FA; c < (f + 1) * CALLS / FA; ++c) {
                         if (c < PB / NB) load_b(wbuf, db, c * NB);
                         else load_a(wbuf, da, (c - PB / NB) * NA);
                     }
@@ -796,14 +818,10 @@ struct MmKernel {
                 if constexpr (DB) {
                     if (bias) add_rows(1);
                 }
-                step_loads();
-                wbuf = next_buf(wbuf);
-            }
-            if constexpr (ACC) {
-#pragma unroll
-                for (int f = 0; f < FA; ++f)
-#pragma unroll
-                    for (int h = 0; h < FB; ++h) asm volatile("" : "+a"(acc[f][h]));
+                if constexpr (!NL) {
+                    step_loads();
+                    wbuf = next_buf(wbuf);
+                }
             }
             if constexpr (GLU) store_glu(g, t, acc, lane, wi, wj);
             else if (LINES && g.ydt != MOE_DTYPE_F32) store_lines(g, t, acc, sm + ST * STAGE + wave * OUT_BYTES, lane, wi, wj);
@@ -828,12 +846,12 @@ struct MmKernel {
     }
 };
 
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, bool GATHER, int EPI>
-__global__ void __launch_bounds__(128 * NWJ, OCC * NWJ / 2) k_mm(const MmArgs g) {
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, bool GATHER, int EPI, int NL>
+__global__ void __launch_bounds__(128 * NWJ + 64 * NL, OCC * (2 * NWJ + NL) / 4) k_mm(const MmArgs g) {
     // LDS of a CU's OCC workgroups: 160 KiB
     constexpr int LDS = 160 * 1024 / OCC, STAGES = ST * 64 * (32 * FA + 16 * NWJ * FB) * 2, PRE = 4 * MM_MAX_E + 64;
     constexpr bool LDS_OUT = OCC == 2 && STAGES + PRE + 2 * NWJ * 16 * (32 * FB + 16) <= LDS;
-    using K = MmKernel<MODE, F16, FA, FB, NWJ, ST, GATHER, EPI, LDS_OUT>;
+    using K = MmKernel<MODE, F16, FA, FB, NWJ, ST, GATHER, EPI, LDS_OUT, NL>;
     __shared__ __attribute__((aligned(1024))) char sm[STAGES + (K::LINES ? K::NW * K::OUT_BYTES : 0)];
     __shared__ int pre[MODE == MM_DW ? 1 : MM_MAX_E + 1];
     K::block(g, sm, pre);
@@ -845,14 +863,15 @@ int launch_mm_dx(const MmArgs& a, hipStream_t st);
 int launch_mm_dw(const MmArgs& a, hipStream_t st);
 int launch_mm_rows(const MmArgs& a, hipStream_t st);   // forward, few rows (moe_mm_rows.hip)
 
-// Tiles of the product kernel: 256 x 256 with 4 waves; 128 x 256 with 8; 128 x 128 with 4, two workgroups on a CU; the same,
-// one on a CU with twice the stages; 64 x 64, two on a CU. MM_ROWS: dot products (moe_mm_rows.hip).
-enum MmShape { MM_256 = 0, MM_128x256 = 1, MM_128 = 2, MM_128_DEEP = 3, MM_64 = 4, MM_ROWS = 5 };
+// Tiles of the product kernel: 128 x 256 with 8 waves that multiply and 4 that load; 128 x 128 with 4 and 4, one workgroup on a
+// CU, 4 stages; 128 x 128 with 4 waves that do both, two workgroups on a CU (dw, and dx of few rows); 64 x 64, two on a CU.
+// MM_ROWS: dot products (moe_mm_rows.hip).
+enum MmShape { MM_128x256 = 0, MM_128_DEEP = 1, MM_128 = 2, MM_64 = 3, MM_ROWS = 4 };
 // Shape and number of parts for a product without offsets: out [rows, J], sums of length R (moe_mm_parts.hip).
 struct MmPlan {
     int shape, parts;
 };
-MmPlan mm_plan(int64_t rows, int64_t J, int64_t R, bool split);
+MmPlan mm_plan(int mode, int64_t rows, int64_t J, int64_t R, bool split);
 // Forward with up to 4 rows: dot products, whole (w [4096, 4096], T 1: 8.6 us, 64 x 64 in 4 parts 12.6; T 4: 10.0 and 12.6;
 // T 8: 14.4 and 12.8).
 constexpr int MM_FEW = 4;
@@ -868,7 +887,7 @@ inline int64_t mm_row_tiles(const MmArgs& a, int BI) {
 }
 inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC>
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, int NL = 0>
 int launch_mm_cfg(const MmArgs& a, hipStream_t st) {
     const bool glu = MODE == MM_FWD && a.kind == EPI_GLU, gather = a.arows || (MODE == MM_DW && a.brows);
     const int bj = 16 * NWJ * FB / (glu ? 2 : 1);
@@ -880,8 +899,8 @@ int launch_mm_cfg(const MmArgs& a, hipStream_t st) {
     const int64_t most = 256 * OCC, grid = round8(CUT * ni * nj) < most ? round8(CUT * ni * nj) : most;   // 256 CUs
     auto go = [&](auto epi) {
         constexpr int EPI = decltype(epi)::value;
-        if (gather) k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, true, EPI><<<(unsigned)grid, 128 * NWJ, 0, st>>>(a);
-        else k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, false, EPI><<<(unsigned)grid, 128 * NWJ, 0, st>>>(a);
+        if (gather) k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, true, EPI, NL><<<(unsigned)grid, 128 * NWJ + 64 * NL, 0, st>>>(a);
+        else k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, false, EPI, NL><<<(unsigned)grid, 128 * NWJ + 64 * NL, 0, st>>>(a);
     };
     if constexpr (MODE == MM_FWD) {
         if (glu) {

@@ -13,9 +13,9 @@ bool two_byte(int dtype) { return dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_
 bool bad_act8(int64_t M, int64_t C) { return M < 0 || M > 0x7fffffff || C < 32 || C % 32 || C > (1 << 20); }
 bool bad_rows(const int32_t* idx, int64_t rows, int64_t M) { return rows > 0x7fffffff || rows < (idx ? 1 : M); }
 // Workspace of a product in parts, with `more` floats per part behind the sums.
-size_t parts_bytes(int64_t rows, int64_t J, int64_t R, int64_t more) {
+size_t parts_bytes(int mode, int64_t rows, int64_t J, int64_t R, int64_t more) {
     if (rows < 1 || J < 1 || R < 1) return 0;
-    const int parts = moe::mm_plan(rows, J, R, true).parts;
+    const int parts = moe::mm_plan(mode, rows, J, R, true).parts;
     return parts > 1 ? (size_t)parts * (rows * J + more) * 4 : 0;
 }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -161,9 +161,9 @@ int moe_grouped_mm_dw(const void* dy, const void* x, const int32_t* offsets, con
     return moe::launch_mm_dw(a, (hipStream_t)stream);
 }
 
-size_t moe_linear_workspace_bytes(int64_t T, int N, int K) { return T <= moe::MM_FEW ? 0 : parts_bytes(T, N, K, 0); }
-size_t moe_linear_dx_workspace_bytes(int64_t T, int N, int K) { return parts_bytes(T, K, N, 0); }
-size_t moe_linear_dw_workspace_bytes(int64_t T, int N, int K) { return parts_bytes(N, K, T, N); }
+size_t moe_linear_workspace_bytes(int64_t T, int N, int K) { return T <= moe::MM_FEW ? 0 : parts_bytes(moe::MM_FWD, T, N, K, 0); }
+size_t moe_linear_dx_workspace_bytes(int64_t T, int N, int K) { return parts_bytes(moe::MM_DX, T, K, N, 0); }
+size_t moe_linear_dw_workspace_bytes(int64_t T, int N, int K) { return parts_bytes(moe::MM_DW, N, K, T, N); }
 
 int moe_linear(const void* x, const void* w, const void* bias, const void* residual, int act, int64_t T, int64_t ldx, int N,
                int K, int dtype, void* y, int y_dtype, void* z, void* workspace, size_t workspace_bytes, void* stream) {
@@ -192,7 +192,7 @@ int moe_linear(const void* x, const void* w, const void* bias, const void* resid
     a.ydt = y_dtype;
     a.epi = moe::MmEpi{bias, residual, z, act, nullptr, nullptr, nullptr};
     a.kind = bias || residual || z || act != MOE_LIN_NONE ? moe::EPI_LIN : moe::EPI_PLAIN;
-    const int parts = T <= moe::MM_FEW ? 1 : moe::mm_plan(T, N, K, true).parts;
+    const int parts = T <= moe::MM_FEW ? 1 : moe::mm_plan(moe::MM_FWD, T, N, K, true).parts;
     if (parts > 1) return moe::launch_mm_parts(moe::MM_FWD, a, parts, (float*)workspace, (hipStream_t)stream);
     return moe::launch_mm_fwd(a, (hipStream_t)stream);
 }
@@ -219,7 +219,7 @@ int moe_linear_dx(const void* dy, const void* w, int64_t T, int64_t lddy, int N,
     a.R = N;
     a.f16 = dtype == MOE_DTYPE_F16;
     a.ydt = dtype;
-    const int parts = moe::mm_plan(T, K, N, true).parts;
+    const int parts = moe::mm_plan(moe::MM_DX, T, K, N, true).parts;
     if (parts > 1) return moe::launch_mm_parts(moe::MM_DX, a, parts, (float*)workspace, (hipStream_t)stream);
     return moe::launch_mm_dx(a, (hipStream_t)stream);
 }
@@ -247,7 +247,7 @@ int moe_linear_dw(const void* dy, const void* x, int64_t T, int64_t lddy, int64_
     a.J = K;
     a.f16 = dtype == MOE_DTYPE_F16;
     a.ydt = dtype;
-    const int parts = moe::mm_plan(N, K, T, true).parts;
+    const int parts = moe::mm_plan(moe::MM_DW, N, K, T, true).parts;
     if (parts > 1) return moe::launch_mm_parts(moe::MM_DW, a, parts, (float*)workspace, (hipStream_t)stream);
     return moe::launch_mm_dw(a, (hipStream_t)stream);
 }

@@ -4,29 +4,29 @@
 namespace moe {
 
 // Which of the shapes, and into how many parts: the shortest of estimates that take a step of 64 r at its measured time with
-// every CU busy (in us: 256 x 256 1.75, 128 x 256 1.02, 128 x 128 1.05 with two workgroups on a CU, 0.92 alone and 0.72 with
-// the deeper stages, 64 x 64 0.55 and 0.41), workgroups in rounds over the 256 CUs, a tile's start and stores as two steps,
-// and the join as a launch and one pass over the parts at 4.5 TB/s. Measured, parts against one whole:
-//   T 64, w [4096, 4096]     64 x 64 in 4:     14.4 us, whole 26.8      T 237, w [2048, 2816]    64 x 64 in 2: 16.9 and 19.8
-//   T 512, w [4096, 4096]    128 x 256 in 4:   34.1 us, whole 38.2      dx, T 1024, w [14336, 4096]  128 x 256 in 2: 131 and 156
-//   dw of 16384 slots, [512, 512]  128 x 128 in 16: 23 us, whole 107    dw of 65536, [1024, 1024]  128 x 128 in 8: 155 and 426
-MmPlan mm_plan(int64_t rows, int64_t J, int64_t R, bool split) {
-    static const struct { int bi, bj, slots; float busy, alone; } S[] = {
-        {256, 256, 256, 1.75f, 1.75f}, {128, 256, 256, 1.02f, 1.02f}, {128, 128, 512, 1.05f, 0.92f}, {128, 128, 256, 0.72f, 0.72f},
-        {64, 64, 512, 0.55f, 0.41f}};
-    MmPlan best{MM_128, 1};
+// every CU busy, workgroups in rounds over the 256 CUs, a tile's start and stores as two steps, and the join as a launch and one
+// pass over the parts at 4.5 TB/s. Measured, parts against one whole:
+//   T 64, w [4096, 4096] 16.2 us, whole 24.5      T 512, w [4096, 4096] 31.3, whole 36.7      dx, T 1024, w [14336, 4096] 116, whole 157
+//   dw of 16384 slots, [512, 512] 22.0, whole 107      dw of 65536 slots, [1024, 1024] 133, whole 426
+MmPlan mm_plan(int mode, int64_t rows, int64_t J, int64_t R, bool split) {
+    // us of a step: with two workgroups on each CU that takes two, and with one
+    static const struct { int shape, bi, bj, slots; float busy, alone; } S[] = {
+        {MM_128x256, 128, 256, 256, 0.83f, 0.83f}, {MM_128_DEEP, 128, 128, 256, 0.52f, 0.52f}, {MM_128, 128, 128, 512, 1.05f, 0.92f},
+        {MM_64, 64, 64, 512, 0.55f, 0.41f}};
+    MmPlan best{MM_128x256, 1};
     float least = 3e38f;
-    for (int s = 0; s < 5; ++s) {
-        const int64_t tiles = ((rows + S[s].bi - 1) / S[s].bi) * ((J + S[s].bj - 1) / S[s].bj), steps = (R + 63) / 64;
+    for (const auto& c : S) {
+        if (c.shape == MM_128 && mode != MM_DW) continue;
+        const int64_t tiles = ((rows + c.bi - 1) / c.bi) * ((J + c.bj - 1) / c.bj), steps = (R + 63) / 64;
         for (int parts = 1; parts <= 64 && parts <= steps; parts *= 2) {
             const int64_t n = tiles * parts;
-            if (parts > 1 && (!split || n > S[s].slots)) break;
-            const float rounds = (float)((n + S[s].slots - 1) / S[s].slots);
-            float us = rounds * (float)((steps + parts - 1) / parts + 2) * (n <= 256 ? S[s].alone : S[s].busy);
-            if (parts > 1) us += 3.5f + (float)parts * rows * J * 8.f / 4.5e6f;
+            if (parts > 1 && (!split || n > c.slots)) break;
+            const float rounds = (float)((n + c.slots - 1) / c.slots);
+            float us = rounds * (float)((steps + parts - 1) / parts + 2) * (n <= 256 ? c.alone : c.busy);
+            if (parts > 1) us += 5.f + (float)parts * rows * J * 8.f / 4.5e6f;
             if (us < least) {
                 least = us;
-                best = {s, parts};
+                best = {c.shape, parts};
             }
         }
     }
