@@ -388,7 +388,7 @@ int moe_glu_bwd(const void* codes, const void* scales, const void* gu, int64_t l
  *   y[t] = residual[t] + sum_j wts[t][j] w_down[e] . act(w_gate_up[e] . x[t]),  e = idx[t][j]
  * w_gate_up [E, 2 F, d] (gate rows, then up), w_down [E, d, F]; x, residual [T, d] and the weights of m->dtype, y too or
  * MOE_DTYPE_F32; idx [T, k] int32 (a slot with an id outside [0, E) adds nothing), wts [T, k] fp32.
- * h and the slots' outputs are rounded to the 16-bit type between the launches; the GLU takes the gate/up sums in fp32.
+ * h is rounded to the 16-bit type between the launches; the GLU takes the gate/up sums, and the sum over slots their rows, in fp32.
  *   keep [moe_mlp_keep_bytes]: the slots' grouping, which the backward pass reads; written in every case.
  *   gu [T k, 2 F], or codes [T k, 2 F] and scales [T k, F / 16]: what the backward pass needs of the gate/up rows, in 16 or in
  *   8 bits (forward: each may be NULL; backward: one of the two forms).

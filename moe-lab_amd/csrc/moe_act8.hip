@@ -196,9 +196,9 @@ __global__ void __launch_bounds__(256) k_slots(const int32_t* idx, const int32_t
     if ((uint32_t)idx[p] >= (uint32_t)E) pos[p] = -1;
 }
 
-// y[t] = residual[t] + sum_j w[t][j] ys[pos[t k + j]] in fp32, slots in ascending j; 8 columns per item. S32: ys is fp32.
-template <bool F16, bool S32>
-__global__ void __launch_bounds__(256) k_slot_sum(const void* ys, const int32_t* pos, const float* wts, const uint16_t* residual,
+// y[t] = residual[t] + sum_j w[t][j] ys[pos[t k + j]] in fp32, slots in ascending j; 8 columns per item
+template <bool F16>
+__global__ void __launch_bounds__(256) k_slot_sum(const float* ys, const int32_t* pos, const float* wts, const uint16_t* residual,
                                                   int64_t M, int k, int d, uint32_t items, uint32_t per_row, void* y, int ydt) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
     if (i >= items) return;
@@ -219,13 +219,9 @@ __global__ void __launch_bounds__(256) k_slot_sum(const void* ys, const int32_t*
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint64_t at = (uint64_t)max(p[j], 0) * d + c;
-            if constexpr (S32) {
-                const f32x4 lo = *(const f32x4*)((const float*)ys + at), hi = *(const f32x4*)((const float*)ys + at + 4);
+            const f32x4 lo = *(const f32x4*)(ys + at), hi = *(const f32x4*)(ys + at + 4);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) v[j][q] = lo[q], v[j][4 + q] = hi[q];
-            } else {
-                unpack8<F16>(*(const u32x4*)((const uint16_t*)ys + at), v[j]);
-            }
+            for (int q = 0; q < 4; ++q) v[j][q] = lo[q], v[j][4 + q] = hi[q];
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -319,7 +315,7 @@ int launch_slots(const int32_t* idx, const int32_t* sorted, const int32_t* offse
     k_slots<<<(n + 255) / 256, 256, 0, st>>>(idx, sorted, offsets, n, k, E, rows, pos);
     return done();
 }
-int launch_slot_sum(const void* ys, bool s32, const int32_t* pos, const float* wts, const void* residual, int64_t M, int64_t T, int k,
+int launch_slot_sum(const float* ys, const int32_t* pos, const float* wts, const void* residual, int64_t M, int64_t T, int k,
                     int d, bool f16, void* y, int ydt, hipStream_t st) {
     return by_parts(T, d / 8, [&](int64_t r, uint32_t items, unsigned grid) {
         const int32_t* p = pos + r * k;
@@ -327,8 +323,7 @@ int launch_slot_sum(const void* ys, bool s32, const int32_t* pos, const float* w
         const uint16_t* res = residual ? (const uint16_t*)residual + r * d : nullptr;
         void* o = (char*)y + r * d * (ydt == MOE_DTYPE_F32 ? 4 : 2);
         auto go = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(ys, p, w, res, M, k, d, items, d / 8, o, ydt); };
-        if (s32) f16 ? go(k_slot_sum<true, true>) : go(k_slot_sum<false, true>);
-        else f16 ? go(k_slot_sum<true, false>) : go(k_slot_sum<false, false>);
+        f16 ? go(k_slot_sum<true>) : go(k_slot_sum<false>);
     });
 }
 

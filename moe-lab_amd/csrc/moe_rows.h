@@ -33,7 +33,7 @@ int launch_lin_act_bwd(const void* dy, int64_t ldy, const void* z, const uint8_t
                        int act, bool f16, void* dz, hipStream_t st);
 int launch_slots(const int32_t* idx, const int32_t* sorted, const int32_t* offsets, int n, int k, int E, int32_t* rows, int32_t* pos,
                  hipStream_t st);
-int launch_slot_sum(const void* ys, bool s32, const int32_t* pos, const float* wts, const void* residual, int64_t M, int64_t T, int k,
+int launch_slot_sum(const float* ys, const int32_t* pos, const float* wts, const void* residual, int64_t M, int64_t T, int k,
                     int d, bool f16, void* y, int ydt, hipStream_t st);
 
 }  // namespace moe

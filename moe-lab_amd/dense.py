@@ -6,8 +6,8 @@ packed weights, for a model before it is quantised, or in training.
 
 The forward call groups the slots by expert (the stable grouping of router.group), multiplies gate and up for each slot with
 token rows read through the slot list (no gathered copy of x), applies the GLU, multiplies down, and sums each token's slots
-in fp32 in their order; the backward call reads dy through the same list. Between two launches h, the slots' rows of y, and
-the gradients of gate and up are in 16 bits (the matrix cores' operands); dh and the slots' rows of dx are fp32. For the
+in fp32 in their order; the backward call reads dy through the same list. Between two launches h and the gradients
+of gate and up are in 16 bits (the matrix cores' operands); dh and the slots' rows of y and dx are fp32. For the
 backward pass the gate/up rows are kept in 8 bits (act8) or 16.
 """
 import torch
