@@ -319,7 +319,10 @@ __device__ __forceinline__ f32x4 load4(const void* p, int64_t i) {
 // What bounds it: dense, LDS reads and loads into LDS beside the matrix cores (4096^3: 1.17-1.26 PFLOP/s, a library product
 // 1.3-1.5); ragged groups, loads, at 3.6-5.8 TB/s of weights.
 // EPI_GLU: the tile's columns are BJ / 2 of gate and the same of up, half by half for each wave, so that a lane holds both.
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, bool GATHER, int EPI, bool LDS_OUT, int NL>
+// GATHER: operands that are read through index lists, bit 0: a, bit 1 (dw): b. Such an operand is addressed with 32 bits from its
+// start; one in slot order from its group's first slot, in 64 bits, so that its own size has no bound (one flag for both made
+// weight gradients of slot-ordered rows past 4 GiB wrong).
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int GATHER, int EPI, bool LDS_OUT, int NL>
 struct MmKernel {
     static constexpr bool GLU = EPI == EPI_GLU;
     static constexpr bool AX = MODE == MM_DW, BX = MODE != MM_FWD;   // operand with its own index contiguous
@@ -521,7 +524,8 @@ struct MmKernel {
         constexpr bool DB = MODE == MM_DW;   // also dbias
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave & 1, wj = wave >> 1;
         const int lw = NL ? wave - NWC : wave;   // among the waves that load
-        constexpr bool gath_b = MODE == MM_DW && GATHER;
+        constexpr bool gath_a = GATHER & 1, gath_b = GATHER & 2;
+        static_assert(MODE == MM_DW || !gath_b, "b is weights");
         const int lda2 = g.lda * 2, ldb2 = g.ldb * 2;
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)sm;
 
@@ -562,8 +566,8 @@ struct MmKernel {
             if constexpr (MODE == MM_DW && GATHER) {
                 const int p = 64 * ls + lane;
                 const bool in = p < lt.cnt;
-                ia = !in ? -1 : g.arows ? g.arows[lt.lo + p] : lt.lo + p;
-                ib = !in ? -1 : g.brows ? g.brows[lt.lo + p] : lt.lo + p;
+                if constexpr (gath_a) ia = in ? g.arows[lt.lo + p] : -1;
+                if constexpr (gath_b) ib = in ? g.brows[lt.lo + p] : -1;
             }
         };
         auto next_load_tile = [&]() {
@@ -584,15 +588,15 @@ struct MmKernel {
             pb = (const char*)g.b;
             const int e = g.part ? 0 : lt.e, first = lt.e * g.part;   // group, and the part's first r
             if constexpr (!AX) pa += (int64_t)first * 2;
-            if constexpr (AX) pa += (int64_t)lt.i0 * 2 + (GATHER ? 0 : (int64_t)lt.lo * lda2);
-            else if (!GATHER) pa += (int64_t)lt.lo * lda2;
+            if constexpr (AX) pa += (int64_t)lt.i0 * 2 + (gath_a ? 0 : (int64_t)lt.lo * lda2);
+            else if (!gath_a) pa += (int64_t)lt.lo * lda2;
 #pragma unroll
             for (int i = 0; i < PA; ++i) {
                 const int r = rowa + A::ROWS * i, c = A::col_of(cola, i);
                 offa[i] = (uint32_t)(r * lda2 + c * 2);
                 if constexpr (AX) {
                     if (lt.i0 + c >= g.I) offa[i] = MM_OOB;
-                } else if constexpr (GATHER) {
+                } else if constexpr (gath_a) {
                     const int src = r < lt.rows ? g.arows[lt.lo + r] : -1;
                     offa[i] = (uint32_t)src < (uint32_t)g.a_n ? (uint32_t)src * (uint32_t)lda2 + c * 2 : MM_OOB;
                 }
@@ -616,8 +620,8 @@ struct MmKernel {
         // bytes of the descriptors for load step ls: up to the end of the last valid row
         auto bytes_a = [&]() -> uint32_t {
             if (!lrows) return 0;
-            if constexpr (!AX) return (uint32_t)((GATHER ? g.a_n : lt.rows) - 1) * (uint32_t)lda2 + (uint32_t)(lr - 64 * ls) * 2;
-            const int rows = GATHER ? g.a_n : min(64, lt.cnt - 64 * ls);
+            if constexpr (!AX) return (uint32_t)((gath_a ? g.a_n : lt.rows) - 1) * (uint32_t)lda2 + (uint32_t)(lr - 64 * ls) * 2;
+            const int rows = gath_a ? g.a_n : min(64, lt.cnt - 64 * ls);
             return (uint32_t)(rows - 1) * (uint32_t)lda2 + (uint32_t)(g.I - lt.i0) * 2;
         };
         auto bytes_b = [&]() -> uint32_t {
@@ -632,12 +636,14 @@ struct MmKernel {
             return in && (uint32_t)src < (uint32_t)n ? (uint32_t)src * (uint32_t)ld2 + c * 2 : MM_OOB;
         };
         auto step_offsets = [&]() {
-            if constexpr (MODE == MM_DW && GATHER) {
+            if constexpr (MODE == MM_DW && gath_a) {
 #pragma unroll
                 for (int i = 0; i < PA; ++i) {
                     const int c = A::col_of(cola, i);
                     offa[i] = row_off(ia, rowa + A::ROWS * i, g.a_n, lda2, c, lt.i0 + c < g.I);
                 }
+            }
+            if constexpr (gath_b) {
 #pragma unroll
                 for (int i = 0; i < PB; ++i) {
                     const int c = B::col_of(colb, i);
@@ -664,7 +670,7 @@ struct MmKernel {
         auto srd_b = [&]() { return srd_of(pb, bytes_b()); };
         auto step_loads = [&]() {
             ++ls;
-            if (!(AX && GATHER)) pa += AX ? 64 * (int64_t)lda2 : 128;
+            if (!(AX && gath_a)) pa += AX ? 64 * (int64_t)lda2 : 128;
             if (!gath_b) pb += BX ? 64 * (int64_t)ldb2 : 128;
             fetch_rows();
         };
@@ -708,8 +714,8 @@ struct MmKernel {
                         dma4(d, i < n ? r * (uint32_t)ld2 + (i - r * lines) * 128 : MM_OOB, lds0 + ST * STAGE + wave * OUT_BYTES);
                     }
                 };
-                touch(g.a, GATHER ? g.a_n : g.M, g.I, lda2);
-                touch(g.b, GATHER ? g.b_n : g.M, g.J, ldb2);
+                touch(g.a, gath_a ? g.a_n : g.M, g.I, lda2);
+                touch(g.b, gath_b ? g.b_n : g.M, g.J, ldb2);
             }
         }
         uint32_t rbuf = 0, wbuf = 0;   // stage buffers of the step that is multiplied, and of the load step
@@ -846,7 +852,7 @@ const bool loads = !NL || wave >= NWC;
     }
 };
 
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, bool GATHER, int EPI, int NL>
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, int GATHER, int EPI, int NL>
 __global__ void __launch_bounds__(128 * NWJ + 64 * NL, OCC * (2 * NWJ + NL) / 4) k_mm(const MmArgs g) {
     // LDS of a CU's OCC workgroups: 160 KiB
     constexpr int LDS = 160 * 1024 / OCC, STAGES = ST * 64 * (32 * FA + 16 * NWJ * FB) * 2, PRE = 4 * MM_MAX_E + 64;
@@ -889,7 +895,7 @@ inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
 template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, int NL = 0>
 int launch_mm_cfg(const MmArgs& a, hipStream_t st) {
-    const bool glu = MODE == MM_FWD && a.kind == EPI_GLU, gather = a.arows || (MODE == MM_DW && a.brows);
+    const bool glu = MODE == MM_FWD && a.kind == EPI_GLU;
     const int bj = 16 * NWJ * FB / (glu ? 2 : 1);
     const int64_t nj = (a.J + bj - 1) / bj;
     const int64_t ni = MODE == MM_DW ? (int64_t)a.E * ((a.I + 32 * FA - 1) / (32 * FA)) : mm_row_tiles(a, 32 * FA);
@@ -897,10 +903,17 @@ int launch_mm_cfg(const MmArgs& a, hipStream_t st) {
     if (ni * nj > 0x70000000) return MOE_ERR_ARG;
     constexpr int CUT = MODE == MM_DW ? 1 : FA >= 4 ? 4 : 2;   // pieces that a tile can be cut into
     const int64_t most = 256 * OCC, grid = round8(CUT * ni * nj) < most ? round8(CUT * ni * nj) : most;   // 256 CUs
+    auto run = [&](auto epi, auto lists) {
+        k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, decltype(lists)::value, decltype(epi)::value, NL>
+            <<<(unsigned)grid, 128 * NWJ + 64 * NL, 0, st>>>(a);
+    };
     auto go = [&](auto epi) {
-        constexpr int EPI = decltype(epi)::value;
-        if (gather) k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, true, EPI, NL><<<(unsigned)grid, 128 * NWJ + 64 * NL, 0, st>>>(a);
-        else k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, false, EPI, NL><<<(unsigned)grid, 128 * NWJ + 64 * NL, 0, st>>>(a);
+        if constexpr (MODE == MM_DW) {
+            if (a.arows && a.brows) return run(epi, std::integral_constant<int, 3>{});
+            if (a.brows) return run(epi, std::integral_constant<int, 2>{});
+        }
+        if (a.arows) return run(epi, std::integral_constant<int, 1>{});
+        run(epi, std::integral_constant<int, 0>{});
     };
     if constexpr (MODE == MM_FWD) {
         if (glu) {

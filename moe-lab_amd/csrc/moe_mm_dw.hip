@@ -23,8 +23,7 @@ static int launch(const MmArgs& args, hipStream_t st) {
     MmArgs a = args;
     const int s = a.offsets ? grouped(a) : dense(a);
     // operands up to half of the memory cache, in groups of a few steps
-    const bool list = a.arows || a.brows;
-    const int64_t ra = list ? a.a_n : a.M, rb = list ? a.b_n : a.M;
+    const int64_t ra = a.arows ? a.a_n : a.M, rb = a.brows ? a.b_n : a.M;
     a.touch = a.offsets && a.M > 0 && ra * a.lda + rb * a.ldb <= (64 << 20) && a.M / a.E <= 256;
     switch (s) {
         case MM_128x256: return launch_mm_cfg<MM_DW, F16, 4, 4, 4, 3, 1, 4>(a, st);
