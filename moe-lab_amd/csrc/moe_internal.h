@@ -71,7 +71,10 @@ int launch_router_logits(const uint16_t* x, const uint16_t* wr, const float* bia
 // lstride: elements between logit rows (0: E)
 int launch_topk(const void* logits, int dtype, int T, int E, int k, int norm, float scale, int32_t* idx, float* wts,
                 hipStream_t st, int lstride = 0);
-// stable grouping of the ids idx[n] into o (with o.items / o.items2 also the grouped kernels' pass lists, passes of P and
+// Slots that a grouping can hold: the chunks that the workgroups of its launches take, and the steps past their ends, are
+// counted in 32 bits (at 128 chunks the last one's shares begin up to n / 32 slots behind n).
+constexpr int GROUP_MAX_SLOTS = 0x78000000;
+// stable grouping of the ids idx[n], n <= GROUP_MAX_SLOTS, into o (with o.items / o.items2 also the grouped kernels' pass lists, passes of P and
 // P2 slots); with sc.chunks and many slots in two launches, else in one workgroup
 int launch_group(const int32_t* idx, int n, int E, const GroupBufs& o, const GroupScratch& sc, hipStream_t st, int P = 0,
                  int P2 = 0);

@@ -10,6 +10,8 @@ bool bad_ld(int64_t ld, int64_t cols) { return ld < cols || ld % 8 || ld > (1 <<
 // Rows reached through a list are addressed with 32 bits from the matrix's start.
 bool too_far(int64_t rows, int64_t ld) { return rows * ld * 2 > 0xB0000000ll; }
 bool two_byte(int dtype) { return dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16; }
+// Slots are counted in 32 bits, in steps of up to 64 past the last one and pieces of up to 128.
+constexpr int64_t MAX_SLOTS = 0x7fffff00;
 bool bad_act8(int64_t M, int64_t C) { return M < 0 || M > 0x7fffffff || C < 32 || C % 32 || C > (1 << 20); }
 bool bad_rows(const int32_t* idx, int64_t rows, int64_t M) { return rows > 0x7fffffff || rows < (idx ? 1 : M); }
 // Workspace of a product in parts, with `more` floats per part behind the sums.
@@ -54,7 +56,7 @@ struct MlpLayout {
     }
 };
 int check_mlp(const moe_mlp_t* m, int T, int k) {
-    if (!m || T < 0 || k < 1 || m->E < 1 || m->E > MM_MAX_E || (int64_t)T * k > 0x7fffffff) return MOE_ERR_ARG;
+    if (!m || T < 0 || k < 1 || m->E < 1 || m->E > MM_MAX_E || (int64_t)T * k > moe::GROUP_MAX_SLOTS) return MOE_ERR_ARG;
     if (!two_byte(m->dtype)) return MOE_ERR_DTYPE;
     if (m->act < 0 || m->act > MOE_ACT_GPTOSS || bad_dim(m->d) || bad_act8(0, m->F) || bad_dim(2 * (int64_t)m->F)) return MOE_ERR_ARG;
     if (!m->w_gate_up || !m->w_down) return MOE_ERR_ARG;
@@ -71,7 +73,7 @@ int moe_grouped_mm(const void* x, const void* w, const void* bias, const int32_t
                    void* stream) {
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return MOE_ERR_DTYPE;
     if (y_dtype != dtype && y_dtype != MOE_DTYPE_F32) return MOE_ERR_DTYPE;
-    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(ldx, K)) return MOE_ERR_ARG;
+    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > MAX_SLOTS || bad_dim(N) || bad_dim(K) || bad_ld(ldx, K)) return MOE_ERR_ARG;
     if (M == 0) return MOE_OK;
     if (!x || !w || !y || bad_rows(rows, x_rows, M)) return MOE_ERR_ARG;
     if (misaligned(x) || misaligned(w) || misaligned(y) || misaligned(bias)) return MOE_ERR_ALIGN;
@@ -103,7 +105,7 @@ int moe_grouped_mm_dx(const void* dy, const void* w, const int32_t* offsets, con
                       void* stream) {
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return MOE_ERR_DTYPE;
     if (dx_dtype != dtype && dx_dtype != MOE_DTYPE_F32) return MOE_ERR_DTYPE;
-    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
+    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > MAX_SLOTS || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
     if (M == 0) return MOE_OK;
     if (!dy || !w || !dx || bad_rows(rows, dy_rows, M)) return MOE_ERR_ARG;
     if (misaligned(dy) || misaligned(w) || misaligned(dx)) return MOE_ERR_ALIGN;
@@ -132,7 +134,7 @@ int moe_grouped_mm_dw(const void* dy, const void* x, const int32_t* offsets, con
                       void* dw, int dw_dtype, void* dbias, void* stream) {
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return MOE_ERR_DTYPE;
     if (dw_dtype != dtype && dw_dtype != MOE_DTYPE_F32) return MOE_ERR_DTYPE;
-    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N) ||
+    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > MAX_SLOTS || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N) ||
         bad_ld(ldx, K))
         return MOE_ERR_ARG;
     if (!dw || (M > 0 && (!dy || !x))) return MOE_ERR_ARG;
@@ -168,7 +170,7 @@ size_t moe_linear_dw_workspace_bytes(int64_t T, int N, int K) { return parts_byt
 int moe_linear(const void* x, const void* w, const void* bias, const void* residual, int act, int64_t T, int64_t ldx, int N,
                int K, int dtype, void* y, int y_dtype, void* z, void* workspace, size_t workspace_bytes, void* stream) {
     if (!two_byte(dtype) || (y_dtype != dtype && y_dtype != MOE_DTYPE_F32)) return MOE_ERR_DTYPE;
-    if (act < MOE_LIN_NONE || act > MOE_LIN_GELU || T < 0 || T > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(ldx, K))
+    if (act < MOE_LIN_NONE || act > MOE_LIN_GELU || T < 0 || T > MAX_SLOTS || bad_dim(N) || bad_dim(K) || bad_ld(ldx, K))
         return MOE_ERR_ARG;
     if (T == 0) return MOE_OK;
     if (!x || !w || !y) return MOE_ERR_ARG;
@@ -200,7 +202,7 @@ int moe_linear(const void* x, const void* w, const void* bias, const void* resid
 int moe_linear_dx(const void* dy, const void* w, int64_t T, int64_t lddy, int N, int K, int dtype, void* dx, void* workspace,
                   size_t workspace_bytes, void* stream) {
     if (!two_byte(dtype)) return MOE_ERR_DTYPE;
-    if (T < 0 || T > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
+    if (T < 0 || T > MAX_SLOTS || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
     if (T == 0) return MOE_OK;
     if (!dy || !w || !dx) return MOE_ERR_ARG;
     if (misaligned(dy) || misaligned(w) || misaligned(dx) || misaligned(workspace)) return MOE_ERR_ALIGN;
@@ -227,7 +229,7 @@ int moe_linear_dx(const void* dy, const void* w, int64_t T, int64_t lddy, int N,
 int moe_linear_dw(const void* dy, const void* x, int64_t T, int64_t lddy, int64_t ldx, int N, int K, int dtype, void* dw,
                   void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
     if (!two_byte(dtype)) return MOE_ERR_DTYPE;
-    if (T < 0 || T > 0x7fffffff || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N) || bad_ld(ldx, K)) return MOE_ERR_ARG;
+    if (T < 0 || T > MAX_SLOTS || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N) || bad_ld(ldx, K)) return MOE_ERR_ARG;
     if (!dw || (T > 0 && (!dy || !x))) return MOE_ERR_ARG;
     if (misaligned(dy) || misaligned(x) || misaligned(dw) || misaligned(workspace)) return MOE_ERR_ALIGN;
     const size_t need = moe_linear_dw_workspace_bytes(T, N, K);

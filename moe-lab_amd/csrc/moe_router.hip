@@ -535,6 +535,7 @@ int launch_shared_route(const void* x, int xdt, const uint16_t* gate, int T, int
 
 int launch_group(const int32_t* idx, int n, int E, const GroupBufs& o, const GroupScratch& sc, hipStream_t st, int P,
                  int P2) {
+    if (n > GROUP_MAX_SLOTS) return MOE_ERR_ARG;
     if ((o.items && (P < 1 || (P & (P - 1)))) || (o.items2 && (P2 < 1 || (P2 & (P2 - 1))))) return MOE_ERR_ARG;
     const int cs = n > 0 ? group_chunk(n, 128) : 128, nchunk = (n + cs - 1) / cs;   // no slots: no chunk
     if (n > 0 && group_split(n, E, nchunk, sc)) {
