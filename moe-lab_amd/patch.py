@@ -33,6 +33,9 @@ The stock forwards are kept (``_moelab_stock_forward``); ``unpatch_block`` / ``u
 ``load_dequantised`` writes the state's dequantised weights back into the stock modules, so stock and patched
 forwards then differ by arithmetic only, not by quantisation.
 """
+import copy
+import math
+
 import torch
 
 from . import _lib, dense
@@ -71,11 +74,40 @@ def is_moe_block(m):
     return block_kind(m) is not None
 
 
-def _act_of(module):
-    name = getattr(getattr(module, "act_fn", None), "__class__", type(None)).__name__.lower()
+def _act(act, z):
+    """The kernels' SiLU or tanh-GELU."""
+    return z * torch.sigmoid(z if act == _lib.ACT_SWIGLU else 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+
+
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+def _bare(module):
+    """A copy of a small module on the CPU, without hooks."""
+    c = copy.deepcopy(module).cpu()
+    for m in c.modules():
+        for n in _HOOKS:
+            getattr(m, n).clear()
+    return c
+
+
+def _act_of(module, tol=1e-3):
+    """The GLU of a module with this act_fn, which may differ from the kernels' function by tol: by default as far as the exact
+    GELU does from the tanh form (4.7e-4, below what 4-bit weights do to a layer), but not as far as a function of another kind
+    with a similar name (QuickGELU 2e-2, Hardswish 0.14)."""
+    fn = getattr(module, "act_fn", None)
+    name = type(fn).__name__.lower()
     for k, v in (("silu", _lib.ACT_SWIGLU), ("swish", _lib.ACT_SWIGLU), ("gelu", _lib.ACT_GEGLU)):
         if k in name:
-            return v
+            z = torch.linspace(-12, 12, 4097, dtype=torch.float64, device="cpu")
+            if isinstance(fn, torch.nn.Module):
+                fn = _bare(fn)
+            with torch.no_grad():
+                gap = float((fn(z) - _act(v, z)).abs().max())
+            if gap <= tol:
+                return v
+            name += f", {gap:.1e} off"
+            break
     raise NotImplementedError(f"activation {name}: the kernels take SiLU, tanh-GELU or gpt-oss's clamped GLU")
 
 
@@ -227,20 +259,95 @@ def _glu_linears(m):
     return [x.weight for x in ls] if ok else None
 
 
+def _probe(module, d, F, E, dtype, act):
+    """The largest error of a module's own forward against the plain GLU layer, relative to the magnitudes that its sums add,
+    on small random weights in its parameters' place (E None: a dense GLU MLP). Gates reach the hundreds, so that a clamp shows;
+    routing weights are not 1, so that a weight at another place does."""
+    g = torch.Generator().manual_seed(0)
+
+    def rand(*shape):
+        return torch.randn(shape, generator=g, dtype=torch.float64, device="cpu").to(dtype)
+    scales = torch.tensor([0.25, 2.0, 8.0] if dtype.itemsize == 2 else [0.25, 2.0, 16.0, 128.0], device="cpu")
+    x = rand(4 * len(scales), d) * scales.repeat(4)[:, None].to(dtype)
+    cls = torch.nn.utils.parametrize.type_before_parametrizations(module)
+    m = cls.__new__(cls)   # the module with other parameters, without its hooks
+    torch.nn.Module.__init__(m)
+    names = ("gate_up_proj", "down_proj") if E else ("gate_proj", "up_proj", "down_proj")
+    kept = {n: _bare(c) for n, c in module._modules.items() if n not in names + ("parametrizations",)}
+    m.__dict__.update({n: v for n, v in module.__dict__.items() if n not in m.__dict__ and n not in ("forward", "_moelab_stock_forward")})
+    m._buffers, m._modules = dict(module._buffers), kept
+    if E:
+        n = E if F <= 32 else 1   # at the module's own sizes its experts are one and the same
+        gu, dn = rand(n, 2 * F, d).expand(E, 2 * F, d), rand(n, d, F).expand(E, d, F)
+        m._parameters = {n: torch.nn.Parameter(t, requires_grad=False) for n, t in zip(names, (gu, dn))}
+        k = min(2, E)
+        idx = torch.stack([torch.randperm(E, generator=g, device="cpu")[:k] for _ in range(len(x))])
+        wts = (torch.rand(len(x), k, generator=g, device="cpu") + 0.3).to(dtype)
+        args = (x, idx, wts)
+    else:
+        for n, t in zip(names, (rand(F, d), rand(F, d), rand(d, F))):
+            m._modules[n] = torch.nn.Linear(t.shape[1], t.shape[0], bias=False, device="meta", dtype=dtype)
+            m._modules[n].weight = torch.nn.Parameter(t, requires_grad=False)
+        gu = torch.cat([m.gate_proj.weight, m.up_proj.weight])[None]
+        dn, idx, wts = m.down_proj.weight[None], torch.zeros(len(x), 1, dtype=torch.int64, device="cpu"), torch.ones(len(x), 1, device="cpu")
+        args = (x,)
+    got = cls.forward(m.train(), *args)   # as in training: a dropout shows too
+    if E:
+        # ids past the experts: most forwards raise, some skip them as the kernels do, some take the last expert instead; but
+        # some have experts without weights there
+        try:
+            past = cls.forward(m, x, torch.full_like(idx, E), wts)
+        except (IndexError, RuntimeError):
+            past = torch.zeros_like(x)
+        if past.any() and not torch.equal(past, cls.forward(m, x, torch.full_like(idx, E - 1), wts)):
+            return math.inf
+    ref, mags = torch.zeros(2, len(x), d, dtype=torch.float64, device="cpu")
+    for t in range(len(x)):
+        for j in range(idx.shape[1]):
+            e = int(idx[t, j])
+            z = gu[e].double() @ x[t].double()
+            h = wts[t, j].double() * _act(act, z[:F]) * z[F:]
+            ref[t] += dn[e].double() @ h
+            mags[t] += dn[e].double().abs() @ h.abs()
+    return float(((got.double() - ref).abs() / mags).max())   # a NaN or another shape fails too
+
+
+def _check_glu(module, act, stacked, d, F, E):
+    """Raises unless the module's own forward is the plain GLU layer that the kernels compute."""
+    tried = []
+    own = (module.down_proj if stacked else module.down_proj.weight).dtype
+    for size in ((16, 32), (d, F)):   # some forwards know their sizes
+        for dtype, tol in ((torch.float64, 1e-6), (torch.float32, 1e-4), (own, 0.05)):
+            try:
+                with torch.no_grad():
+                    gap = _probe(module, *size, E if stacked else None, dtype, act)
+            except Exception as e:   # a type or a size that this forward does not take
+                tried.append(f"{type(e).__name__}: {e}")
+                continue
+            if gap <= tol:
+                return
+            raise ValueError(f"{type(module).__name__} computes something else than the plain GLU layer of the kernels (off by {gap:.1e} of "
+                             f"its sums on random weights): a clamp, another gate or another place of the routing weights")
+    raise ValueError(f"{type(module).__name__}: its forward could not be checked against the kernels' GLU layer ({tried[0]})")
+
+
 def patch_dense(module, checkpoint=True):
     """Put a stacked experts module (forward(hidden_states [T, d], top_k_index [T, k], top_k_weights [T, k])) or a dense
     GLU MLP (gate_proj, up_proj, down_proj, act_fn) on the 16-bit kernels, forward and backward, with the module's own
-    bf16 or fp16 parameters. checkpoint: activations are kept in 8 bits for the backward pass. unpatch_experts undoes it."""
+    bf16 or fp16 parameters. checkpoint: activations are kept in 8 bits for the backward pass. unpatch_experts undoes it.
+    A module whose forward computes anything else (clamped gates, exact GELU, QuickGELU, dropout) is refused: its forward is
+    run on a few random rows and small random weights on the CPU, and compared."""
     stacked, glu = _stacked(module), _glu_linears(module)
     if not stacked and glu is None:
         raise ValueError(f"{type(module).__name__}: neither a stacked experts module nor a GLU MLP without biases")
-    act = _act_of(module)
+    act = _act_of(module, 1e-6)
     ws = (module.gate_up_proj, module.down_proj) if stacked else glu
     if any(w.dtype != ws[0].dtype or w.dtype not in (torch.bfloat16, torch.float16) for w in ws):
         raise TypeError(f"weights in {', '.join(sorted({str(w.dtype) for w in ws}))}: all bf16 or all fp16 expected")
     d, F = (ws[1].shape[1], ws[1].shape[2]) if stacked else (ws[0].shape[1], ws[0].shape[0])
     _lib.multiple_of(d, 8, "the hidden size")
     _lib.multiple_of(F, 32, "the intermediate size")
+    _check_glu(module, act, stacked, d, F, ws[1].shape[0])
 
     def experts_forward(hidden_states, top_k_index, top_k_weights):
         return dense.experts_mlp(hidden_states, top_k_index, top_k_weights, module.gate_up_proj, module.down_proj, act=act,
