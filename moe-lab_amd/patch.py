@@ -35,6 +35,7 @@ forwards then differ by arithmetic only, not by quantisation.
 """
 import copy
 import math
+import types
 
 import torch
 
@@ -331,6 +332,19 @@ def _check_glu(module, act, stacked, d, F, E):
     raise ValueError(f"{type(module).__name__}: its forward could not be checked against the kernels' GLU layer ({tried[0]})")
 
 
+# patch_dense's forwards are bound methods: a deep copy of a patched module computes with its own parameters
+def _experts_forward(self, hidden_states, top_k_index, top_k_weights):
+    s = self._moelab_state
+    return dense.experts_mlp(hidden_states, top_k_index, top_k_weights, self.gate_up_proj, self.down_proj, act=s["act"],
+                             checkpoint=s["checkpoint"])
+
+
+def _mlp_forward(self, x):
+    s = self._moelab_state
+    return dense.glu_mlp(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, act=s["act"],
+                         checkpoint=s["checkpoint"])
+
+
 def patch_dense(module, checkpoint=True):
     """Put a stacked experts module (forward(hidden_states [T, d], top_k_index [T, k], top_k_weights [T, k])) or a dense
     GLU MLP (gate_proj, up_proj, down_proj, act_fn) on the 16-bit kernels, forward and backward, with the module's own
@@ -349,17 +363,9 @@ def patch_dense(module, checkpoint=True):
     _lib.multiple_of(F, 32, "the intermediate size")
     _check_glu(module, act, stacked, d, F, ws[1].shape[0])
 
-    def experts_forward(hidden_states, top_k_index, top_k_weights):
-        return dense.experts_mlp(hidden_states, top_k_index, top_k_weights, module.gate_up_proj, module.down_proj, act=act,
-                                 checkpoint=checkpoint)
-
-    def mlp_forward(x):
-        return dense.glu_mlp(x, module.gate_proj.weight, module.up_proj.weight, module.down_proj.weight, act=act,
-                             checkpoint=checkpoint)
-
     module._moelab_stock_forward = module.forward
-    module._moelab_state = {"fmt": "dense"}
-    module.forward = experts_forward if stacked else mlp_forward
+    module._moelab_state = {"fmt": "dense", "act": act, "checkpoint": checkpoint}
+    module.forward = types.MethodType(_experts_forward if stacked else _mlp_forward, module)
     return module
 
 

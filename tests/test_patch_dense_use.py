@@ -1,0 +1,71 @@
+"""What a program does with a module under patch_dense besides calling it: copies, second patches, models that are refused in the
+middle, hooks on and replacements of its parts. The expert layer's calls are recorded here, not run."""
+import copy
+
+import pytest
+import torch
+
+import __graft_entry__
+
+__graft_entry__.load_package()
+import dense_helpers as H  # noqa: E402
+from moelab_amd import dense, patch  # noqa: E402
+from test_patch import D, make_block  # noqa: E402
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """The arguments of the expert layer's calls, which return their first one."""
+    seen = []
+
+    def record(*a, **k):
+        seen.append(a)
+        return a[0]
+    monkeypatch.setattr(dense, "experts_mlp", record)
+    monkeypatch.setattr(dense, "glu_mlp", record)
+    return seen
+
+
+def tokens(T=3, dtype=torch.bfloat16):
+    return torch.randn(T, D, generator=torch.Generator().manual_seed(T)).to(dtype)
+
+
+def slots(T=3):
+    return torch.zeros(T, 2, dtype=torch.int64), torch.ones(T, 2)
+
+
+def test_a_copy_uses_its_own_parameters(calls):
+    block = make_block("deepseek", "cpu")
+    patch.patch_model(torch.nn.ModuleList([block]), fmt="dense")
+    other = copy.deepcopy(block)
+    for b in (block, other):
+        b.experts(tokens(), *slots())
+        b.shared_experts(tokens())
+        e, m = b.experts, b.shared_experts
+        used = [*calls[-2][3:5], *calls[-1][1:4]]
+        assert all(p is q for p, q in zip(used, [e.gate_up_proj, e.down_proj, *(getattr(m, n).weight for n in ("gate_proj", "up_proj", "down_proj"))]))
+    x = tokens(dtype=torch.float32)
+    other.float()
+    patch.unpatch_experts(other.shared_experts)
+    with torch.no_grad():
+        other.shared_experts.down_proj.weight.mul_(2)
+        assert torch.equal(other.shared_experts(x), 2 * make_block("deepseek", "cpu").float().shared_experts(x))
+    assert hasattr(block.shared_experts, "_moelab_state")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("part", ["experts", "shared_experts"])
+def test_gradients_of_a_copy(part):
+    """A copy trains its own parameters, as an average or a reference model made by copying does."""
+    block = make_block("deepseek", "cuda")
+    patch.patch_model(torch.nn.ModuleList([block]), fmt="dense")
+    other = copy.deepcopy(block)
+    args = (H.randn(5, D, dtype=torch.bfloat16),) + (() if part != "experts" else
+                                                     (torch.tensor([[0, 1]] * 5, device="cuda"), torch.full((5, 2), 0.5, device="cuda")))
+    y = getattr(block, part)(*args)
+    with torch.no_grad():
+        for p in getattr(other, part).parameters():
+            p.mul_(0.5)
+        assert not torch.equal(getattr(other, part)(*args), y)
+    getattr(other, part)(*args).sum().backward()
+    assert all(p.grad is not None for p in getattr(other, part).parameters()) and all(p.grad is None for p in block.parameters())
