@@ -180,6 +180,15 @@ def _route_stock(block, hidden):
     return idx.to(torch.int32).contiguous(), wts.float().contiguous()
 
 
+def _install(module, forward, state):
+    """The patched forward and its state; a second patch keeps the stock forward of the first."""
+    if not hasattr(module, "_moelab_stock_forward"):
+        module._moelab_stock_forward = module.forward
+    module._moelab_state = state
+    module.forward = forward
+    return module
+
+
 def patch_block(block, fmt=None):
     """Replace a sparse MoE block's forward by the kernels (router inside the layer call). fmt: "int4" (default for
     the stacked families) or "mxfp4" (default for gpt-oss)."""
@@ -200,11 +209,8 @@ def patch_block(block, fmt=None):
             return y, wts.to(hidden_states.dtype)
         return y
 
-    block._moelab_stock_forward = block.forward
-    block._moelab_state = s
     block._moelab_cfg = cfg
-    block.forward = forward
-    return block
+    return _install(block, forward, s)
 
 
 def unpatch_block(block):
@@ -241,10 +247,7 @@ def patch_experts(experts, fmt="int4"):
         y = (slots.reshape(T, k, d) * top_k_weights.float().reshape(T, k, 1)).sum(1)
         return y.to(hidden_states.dtype)
 
-    experts._moelab_stock_forward = experts.forward
-    experts._moelab_state = s
-    experts.forward = forward
-    return experts
+    return _install(experts, forward, s)
 
 
 def unpatch_experts(experts):
@@ -363,10 +366,8 @@ def patch_dense(module, checkpoint=True):
     _lib.multiple_of(F, 32, "the intermediate size")
     _check_glu(module, act, stacked, d, F, ws[1].shape[0])
 
-    module._moelab_stock_forward = module.forward
-    module._moelab_state = {"fmt": "dense", "act": act, "checkpoint": checkpoint}
-    module.forward = types.MethodType(_experts_forward if stacked else _mlp_forward, module)
-    return module
+    return _install(module, types.MethodType(_experts_forward if stacked else _mlp_forward, module),
+                    {"fmt": "dense", "act": act, "checkpoint": checkpoint})
 
 
 def patch_model(model, fmt=None, universal=False, checkpoint=True):

@@ -69,3 +69,41 @@ def test_gradients_of_a_copy(part):
         assert not torch.equal(getattr(other, part)(*args), y)
     getattr(other, part)(*args).sum().backward()
     assert all(p.grad is not None for p in getattr(other, part).parameters()) and all(p.grad is None for p in block.parameters())
+
+
+def test_a_second_patch_keeps_the_stock_forward(calls):
+    """With other settings, say: the last one holds, and undoing it gives the stock forward."""
+    e = make_block("mixtral", "cpu").experts
+    stock, x = e.forward, tokens()
+    want = e(x, *slots())
+    patch.patch_dense(e, checkpoint=True)
+    patch.patch_dense(e, checkpoint=False)
+    assert e._moelab_state["checkpoint"] is False
+    e(x, *slots())
+    assert len(calls) == 1
+    patch.unpatch_experts(e)
+    assert e.forward == stock and torch.equal(e(x, *slots()), want) and len(calls) == 1
+    assert not any(n.startswith("_moelab") for n in e.__dict__)
+
+
+@pytest.mark.gpu
+def test_patches_onto_4_bits_and_back():
+    """patch_experts over patch_dense and the other way round, and patch_block twice."""
+    block = make_block("mixtral", "cuda")
+    e, stock = block.experts, block.experts.forward
+    args = (H.randn(5, D, dtype=torch.bfloat16), torch.tensor([[0, 1]] * 5, device="cuda"), torch.full((5, 2), 0.5, device="cuda"))
+    with torch.no_grad():
+        for first, second in ((patch.patch_dense, patch.patch_experts), (patch.patch_experts, patch.patch_dense)):
+            first(e)
+            second(e)
+            y = e(*args)
+            patch.unpatch_experts(e)
+            assert e.forward == stock
+            second(e)
+            assert torch.equal(e(*args), y)
+            patch.unpatch_experts(e)
+        stock = block.forward
+        patch.patch_block(block)
+        patch.patch_block(block)
+        patch.unpatch_block(block)
+        assert block.forward == stock and not any(n.startswith("_moelab") for n in block.__dict__)
