@@ -348,12 +348,8 @@ def _mlp_forward(self, x):
                          checkpoint=s["checkpoint"])
 
 
-def patch_dense(module, checkpoint=True):
-    """Put a stacked experts module (forward(hidden_states [T, d], top_k_index [T, k], top_k_weights [T, k])) or a dense
-    GLU MLP (gate_proj, up_proj, down_proj, act_fn) on the 16-bit kernels, forward and backward, with the module's own
-    bf16 or fp16 parameters. checkpoint: activations are kept in 8 bits for the backward pass. unpatch_experts undoes it.
-    A module whose forward computes anything else (clamped gates, exact GELU, QuickGELU, dropout) is refused: its forward is
-    run on a few random rows and small random weights on the CPU, and compared."""
+def _dense_act(module):
+    """The activation of a module that patch_dense takes; raises for any other."""
     stacked, glu = _stacked(module), _glu_linears(module)
     if not stacked and glu is None:
         raise ValueError(f"{type(module).__name__}: neither a stacked experts module nor a GLU MLP without biases")
@@ -365,26 +361,49 @@ def patch_dense(module, checkpoint=True):
     _lib.multiple_of(d, 8, "the hidden size")
     _lib.multiple_of(F, 32, "the intermediate size")
     _check_glu(module, act, stacked, d, F, ws[1].shape[0])
+    return act
 
-    return _install(module, types.MethodType(_experts_forward if stacked else _mlp_forward, module),
+
+def _install_dense(module, act, checkpoint):
+    return _install(module, types.MethodType(_experts_forward if _stacked(module) else _mlp_forward, module),
                     {"fmt": "dense", "act": act, "checkpoint": checkpoint})
+
+
+def patch_dense(module, checkpoint=True):
+    """Put a stacked experts module (forward(hidden_states [T, d], top_k_index [T, k], top_k_weights [T, k])) or a dense
+    GLU MLP (gate_proj, up_proj, down_proj, act_fn) on the 16-bit kernels, forward and backward, with the module's own
+    bf16 or fp16 parameters. checkpoint: activations are kept in 8 bits for the backward pass. unpatch_experts undoes it.
+    A module whose forward computes anything else (clamped gates, exact GELU, QuickGELU, dropout) is refused: its forward is
+    run on a few random rows and small random weights on the CPU, and compared."""
+    return _install_dense(module, _dense_act(module), checkpoint)
+
+
+def _patch_model_dense(model, universal, checkpoint):
+    """All parts are checked before the first is patched: a model that is refused is left as it was."""
+    parts = {}
+    for m in model.modules():
+        if hasattr(m, "_moelab_state"):
+            continue
+        if universal:
+            found = [m] if _stacked(m) else []
+        else:
+            found = [m.experts, getattr(m, "shared_expert", None), getattr(m, "shared_experts", None)] if is_moe_block(m) else []
+        parts |= {id(p): p for p in found if p is not None and not hasattr(p, "_moelab_state")}
+    acts = [_dense_act(p) for p in parts.values()]
+    for p, act in zip(parts.values(), acts):
+        _install_dense(p, act, checkpoint)
+    return len(parts)
 
 
 def patch_model(model, fmt=None, universal=False, checkpoint=True):
     """Patch every sparse MoE block of a model (universal: every stacked experts module instead); returns how many
     modules were patched. fmt "dense": patch_dense (with checkpoint) on each block's experts and shared experts
-    (universal: on every stacked experts module)."""
+    (universal: on every stacked experts module); if it refuses one of them, none is patched."""
+    if fmt == "dense":
+        return _patch_model_dense(model, universal, checkpoint)
     n = 0
     for m in list(model.modules()):
         if hasattr(m, "_moelab_state"):
-            continue
-        if fmt == "dense":
-            parts = [m] if universal else [m.experts, getattr(m, "shared_expert", None), getattr(m, "shared_experts", None)] \
-                if is_moe_block(m) else []
-            for part in parts:
-                if part is not None and not hasattr(part, "_moelab_state") and (not universal or _stacked(part)):
-                    patch_dense(part, checkpoint)
-                    n += 1
             continue
         if universal:
             if _stacked(m) and not hasattr(m, "gate_up_proj_bias"):

@@ -107,3 +107,26 @@ def test_patches_onto_4_bits_and_back():
         patch.patch_block(block)
         patch.unpatch_block(block)
         assert block.forward == stock and not any(n.startswith("_moelab") for n in block.__dict__)
+
+
+@pytest.mark.parametrize("odd", ["gpt-oss", "biased shared experts", "another activation", "fp32"])
+def test_a_refused_model_is_left_as_it_was(odd):
+    blocks = [make_block("deepseek", "cpu"), make_block("gpt-oss" if odd == "gpt-oss" else "deepseek", "cpu")]
+    if odd == "biased shared experts":
+        blocks[1].shared_experts.up_proj.bias = torch.nn.Parameter(torch.zeros(512, dtype=torch.bfloat16))
+    if odd == "another activation":
+        blocks[1].shared_experts.act_fn = torch.nn.GELU()
+    if odd == "fp32":
+        blocks[1].experts.float()
+    model = torch.nn.ModuleList(blocks)
+    with pytest.raises((ValueError, TypeError, NotImplementedError)):
+        patch.patch_model(model, fmt="dense")
+    assert not any(n.startswith("_moelab") or n == "forward" for m in model.modules() for n in m.__dict__)
+    assert patch.patch_model(model[:1], fmt="dense") == 2 and patch.patch_model(model[:1], fmt="dense") == 0
+
+
+def test_shared_modules_count_once():
+    block = make_block("mixtral", "cpu")
+    other = make_block("mixtral", "cpu")
+    other.experts = block.experts
+    assert patch.patch_model(torch.nn.ModuleList([block, other]), fmt="dense") == 1
