@@ -256,11 +256,24 @@ def unpatch_experts(experts):
     return experts
 
 
+_PROJ = ("gate_proj", "up_proj", "down_proj")
+
+
+def _plain_linear(x):
+    """Whether x multiplies by its weight and does nothing else (a subclass with a forward of its own, as of 4-bit weights or
+    adapters, does)."""
+    return (isinstance(x, torch.nn.Linear) and x.bias is None and "forward" not in x.__dict__
+            and type(x).forward is torch.nn.Linear.forward)
+
+
 def _glu_linears(m):
     """The gate, up and down weights of a dense GLU MLP without biases, or None."""
-    ls = [getattr(m, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
-    ok = all(isinstance(x, torch.nn.Linear) and x.bias is None for x in ls) and hasattr(m, "act_fn")
-    return [x.weight for x in ls] if ok else None
+    ls = [getattr(m, n, None) for n in _PROJ]
+    return [x.weight for x in ls] if all(_plain_linear(x) for x in ls) and hasattr(m, "act_fn") else None
+
+
+def _hooked(x):
+    return any(getattr(x, n, None) for n in _HOOKS)
 
 
 def _probe(module, d, F, E, dtype, act):
@@ -335,17 +348,23 @@ def _check_glu(module, act, stacked, d, F, E):
     raise ValueError(f"{type(module).__name__}: its forward could not be checked against the kernels' GLU layer ({tried[0]})")
 
 
-# patch_dense's forwards are bound methods: a deep copy of a patched module computes with its own parameters
+# patch_dense's forwards are bound methods: a deep copy of a patched module computes with its own parameters. The kernels call
+# none of the module's parts, so where one would do more than it did when the module was patched (a hook on it, an adapter or
+# another module in its place), the stock forward runs.
 def _experts_forward(self, hidden_states, top_k_index, top_k_weights):
     s = self._moelab_state
+    if self.act_fn is not s["act_fn"] or _hooked(self.act_fn):
+        return self._moelab_stock_forward(hidden_states, top_k_index, top_k_weights)
     return dense.experts_mlp(hidden_states, top_k_index, top_k_weights, self.gate_up_proj, self.down_proj, act=s["act"],
                              checkpoint=s["checkpoint"])
 
 
 def _mlp_forward(self, x):
     s = self._moelab_state
-    return dense.glu_mlp(x, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, act=s["act"],
-                         checkpoint=s["checkpoint"])
+    parts = [getattr(self, n) for n in _PROJ]
+    if self.act_fn is not s["act_fn"] or _hooked(self.act_fn) or not all(_plain_linear(p) and not _hooked(p) for p in parts):
+        return self._moelab_stock_forward(x)
+    return dense.glu_mlp(x, *(p.weight for p in parts), act=s["act"], checkpoint=s["checkpoint"])
 
 
 def _dense_act(module):
@@ -366,7 +385,7 @@ def _dense_act(module):
 
 def _install_dense(module, act, checkpoint):
     return _install(module, types.MethodType(_experts_forward if _stacked(module) else _mlp_forward, module),
-                    {"fmt": "dense", "act": act, "checkpoint": checkpoint})
+                    {"fmt": "dense", "act": act, "act_fn": module.act_fn, "checkpoint": checkpoint})
 
 
 def patch_dense(module, checkpoint=True):
@@ -374,7 +393,8 @@ def patch_dense(module, checkpoint=True):
     GLU MLP (gate_proj, up_proj, down_proj, act_fn) on the 16-bit kernels, forward and backward, with the module's own
     bf16 or fp16 parameters. checkpoint: activations are kept in 8 bits for the backward pass. unpatch_experts undoes it.
     A module whose forward computes anything else (clamped gates, exact GELU, QuickGELU, dropout) is refused: its forward is
-    run on a few random rows and small random weights on the CPU, and compared."""
+    run on a few random rows and small random weights on the CPU, and compared. While a projection or the activation has
+    hooks or another module in its place, the stock forward runs."""
     return _install_dense(module, _dense_act(module), checkpoint)
 
 

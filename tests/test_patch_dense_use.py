@@ -130,3 +130,89 @@ def test_shared_modules_count_once():
     other = make_block("mixtral", "cpu")
     other.experts = block.experts
     assert patch.patch_model(torch.nn.ModuleList([block, other]), fmt="dense") == 1
+
+
+class Adapter(torch.nn.Module):
+    """What a finetune puts in a projection's place: the frozen product and a low-rank one beside it, with the base's weight in view."""
+
+    def __init__(self, base):
+        super().__init__()
+        self.base = base
+        self.a = torch.nn.Parameter(torch.ones(4, base.in_features, dtype=base.weight.dtype))
+        self.b = torch.nn.Parameter(torch.ones(base.out_features, 4, dtype=base.weight.dtype))
+
+    @property
+    def weight(self):
+        return self.base.weight
+
+    bias = None
+
+    def forward(self, x):
+        return self.base(x) + x @ self.a.T @ self.b.T
+
+
+class Scaled(torch.nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+@pytest.mark.parametrize("name", ["gate_proj", "up_proj", "down_proj"])
+def test_adapters_and_subclasses_run(calls, name):
+    m, x = make_block("deepseek", "cpu").shared_experts, tokens()
+    patch.patch_dense(m)
+    assert m(x) is x and len(calls) == 1
+    stock = copy.deepcopy(m)
+    patch.unpatch_experts(stock)
+    p = getattr(m, name)
+    setattr(m, name, Adapter(p))
+    setattr(stock, name, Adapter(getattr(stock, name)))
+    assert torch.equal(m(x), stock(x)) and len(calls) == 1
+    sub = Scaled(p.in_features, p.out_features, bias=False, dtype=p.weight.dtype)
+    sub.weight = p.weight
+    setattr(m, name, sub)
+    setattr(stock, name, sub)
+    assert torch.equal(m(x), stock(x)) and len(calls) == 1
+    patch.unpatch_experts(m)
+    with pytest.raises(ValueError, match="neither"):   # and when it is there before
+        patch.patch_dense(m)
+    setattr(m, name, p)
+    patch.patch_dense(m)
+    assert m(x) is x and len(calls) == 2
+    p.bias = torch.nn.Parameter(torch.ones(p.out_features, dtype=p.weight.dtype))
+    m(x)
+    p.bias = None
+    p.forward = lambda t: torch.nn.functional.linear(t, p.weight)   # an instance's own
+    m(x)
+    assert len(calls) == 2
+
+
+@pytest.mark.parametrize("part", ["gate_proj", "up_proj", "down_proj", "act_fn"])
+def test_hooks_run(calls, part):
+    m, x, seen = make_block("deepseek", "cpu").shared_experts, tokens(), []
+    patch.patch_dense(m)
+    for register in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook", "register_full_backward_pre_hook"):
+        h = getattr(getattr(m, part), register)(lambda *a: seen.append(1))
+        xs = x.clone().requires_grad_()
+        m(xs).sum().backward()
+        assert len(seen) == 1 and not calls, register
+        h.remove()
+        seen.clear()
+    assert m(x) is x and len(calls) == 1   # and without hooks the kernels again
+
+
+def test_another_activation_runs(calls):
+    for m, args in ((make_block("mixtral", "cpu").experts, (tokens(), *slots())), (make_block("deepseek", "cpu").shared_experts, (tokens(),))):
+        patch.patch_dense(m)
+        n = len(calls)
+        assert m(*args) is args[0] and len(calls) == n + 1
+        act, m.act_fn = m.act_fn, torch.nn.GELU()
+        y = m(*args)
+        patch.unpatch_experts(m)
+        assert torch.equal(m(*args), y) and len(calls) == n + 1
+        m.act_fn = act
+        patch.patch_dense(m)
+        h = m.act_fn.register_forward_hook(lambda *a: None)
+        m(*args)
+        assert len(calls) == n + 1
+        h.remove()
+        assert copy.deepcopy(m)(*args) is args[0] and len(calls) == n + 2
