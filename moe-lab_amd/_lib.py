@@ -9,6 +9,7 @@ import ctypes
 import os
 
 import torch  # noqa: F401  (loads the HIP runtime before the library)
+import torch.autograd.forward_ad as _fw
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # MOELAB_AMD_LIB names another build of the same library (e.g. one compiled with different tuning macros)
@@ -259,6 +260,9 @@ def result(out, shape, dtype, out_dtype, device):
 
 
 def wants_grad(*ts):
+    """Whether the call's result is differentiable. A forward-mode derivative would be lost in the library: that raises."""
+    if _fw._current_level >= 0 and any(t is not None and _fw.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError("no forward-mode derivative: the 16-bit operators have backward passes only")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
