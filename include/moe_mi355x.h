@@ -368,7 +368,7 @@ int moe_linear_act_bwd(const void* dy, int64_t lddy, const void* z, const void* 
  * scale = biased exponent of the block's largest magnitude, one more if that would round to 128 (254 at most: there the
  * code stays 127); 255: the block holds an infinity or NaN and reads as NaN.
  *   moe_act8_pack, _unpack: 16-bit values to that form, and back (to bf16, fp16 or fp32; into the type they came from it is
- *                           exact).
+ *                           exact, but for 65536, the form of fp16 values from 65280 on, which becomes fp16's 65504).
  *   moe_glu_fwd: gu [M, 2 F] (gate columns, then up; ldgu elements from row to row) -> h [M, F] = act(gate, up) and, codes not
  *                NULL, gu's 8-bit form (codes [M, 2 F], scales [M, 2 F / 32]). act: MOE_ACT_*; F % 32 == 0.
  *   moe_glu_bwd: from that form (or gu itself with codes NULL), dh [M, F] (16-bit or MOE_DTYPE_F32) and row weights wts [M]

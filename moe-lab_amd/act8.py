@@ -38,7 +38,8 @@ def pack(x):
 
 
 def unpack(codes, scales, dtype=torch.bfloat16):
-    """The values that codes and scales stand for, in bf16, fp16 or fp32 (exact in the type they came from and in fp32)."""
+    """The values that codes and scales stand for, in bf16, fp16 or fp32: exact in the type they came from and in fp32, but
+    for 65536 in fp16, to which fp16 values from 65280 on are kept: 65504 there, not infinity."""
     if dtype not in _lib.DTYPE:
         raise TypeError(f"dtype {dtype}: bf16, fp16 or fp32 expected")
     if codes.dim() != 2:

@@ -152,6 +152,10 @@ __global__ void __launch_bounds__(256) k_unpack8(const uint8_t* codes, const uin
     if (i >= items) return;
     float v[8];
     values8(*(const u32x2*)(codes + (uint64_t)i * 8), scales[i / 4], v);
+    // fp16 values from 65280 on are kept as 64 steps of 1024, past fp16's range by one rounding
+    if constexpr (F16)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = fabsf(v[j]) == 65536.f ? copysignf(65504.f, v[j]) : v[j];
     if (f32) {
         f32x4* o = (f32x4*)((float*)out + (uint64_t)i * 8);
         o[0] = (f32x4){v[0], v[1], v[2], v[3]};
