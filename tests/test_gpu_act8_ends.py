@@ -33,11 +33,13 @@ def test_every_largest_value(dtype):
 
 
 def test_other_values_in_fp16():
-    """Codes of bf16 values: past fp16's range they are infinite, 65536 apart. (65024 is 63.5 steps of its block: 64.)"""
-    x = torch.zeros(1, 128, dtype=torch.bfloat16, device=DEV)
-    x[0, 0], x[0, 32], x[0, 33], x[0, 64], x[0, 96] = 65536, -65536, 65024, 66048, float("nan")
+    """Codes of bf16 values: past fp16's range they are infinite, 65536 apart. (65024 and 66048 are 63.5 and 64.5 steps of
+    1024, 66560 is 65: ties go to the even 64.)"""
+    x = torch.zeros(1, 160, dtype=torch.bfloat16, device=DEV)
+    x[0, 0], x[0, 32], x[0, 33], x[0, 64], x[0, 96], x[0, 128] = 65536, -65536, 65024, 66048, float("nan"), 66560
     v = act8.unpack(*act8.pack(x), torch.float16)[0]
-    assert v[0] == 65504 and v[32] == -65504 and v[33] == 65504 and v[64] == float("inf") and torch.isnan(v[96:]).all()
+    assert v[0] == 65504 and v[32] == -65504 and v[33] == 65504 and v[64] == 65504
+    assert torch.isnan(v[96:128]).all() and v[128] == float("inf") and not v[129:].any()
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=["bf16", "fp16"])
