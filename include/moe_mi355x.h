@@ -326,8 +326,8 @@ int moe_probe_read(const void* src, size_t nbytes, uint32_t* sink, void* stream)
  * sums in a fixed order, or MOE_DTYPE_F32 (dbias: the operands' type). x [x_rows, K] with ldx elements from row to row
  * (dy alike); w [E, N, K], results and bias contiguous. Slots behind the last group are left as they were, or set to zero
  * with fill = 1. An index outside its matrix reads as a row of zeros.
- * Requirements: M <= 0x7fffff00, E <= 1024, N % 8 == 0, K % 8 == 0, strides % 8 == 0, N, K <= 2^20, strides <= 2^21; pointers 16-byte aligned; a matrix
- * read through an index list (for dw: either, then both) at most 0xB0000000 bytes.
+ * Requirements: M <= 0x7fffff00, E <= 1024, N % 8 == 0, K % 8 == 0, strides % 8 == 0, N, K <= 2^20, strides <= 2^21; pointers
+ * 16-byte aligned; a matrix read through an index list (for dw: either, then both) at most 0xB0000000 bytes.
  */
 int moe_grouped_mm(const void* x, const void* w, const void* bias, const int32_t* offsets, const int32_t* rows, int64_t M,
                    int64_t x_rows, int64_t ldx, int E, int N, int K, int dtype, void* y, int y_dtype, int fill,
@@ -394,8 +394,8 @@ int moe_glu_bwd(const void* codes, const void* scales, const void* gu, int64_t l
  *   8 bits (forward: each may be NULL; backward: one of the two forms).
  *   moe_mlp_bwd: dx [T, d], dwts [T, k] fp32, dw_gate_up, dw_down (as the weights), each may be NULL. dwts of slots with an id
  *   outside [0, E) is left as it was. From the kept 8-bit values, gradients are those of the function at these values.
- * Requirements: E <= 1024, d % 8 == 0, F % 32 == 0, T d and 2 F d at most 0x58000000, T k <= 0x78000000; pointers 16-byte aligned. workspace: any contents;
- * forward and backward sizes from their queries. moe_mlp_bwd takes T > 0.
+ * Requirements: E <= 1024, d % 8 == 0, F % 32 == 0, T d and 2 F d at most 0x58000000, T k <= 0x78000000; pointers 16-byte
+ * aligned. workspace: any contents; forward and backward sizes from their queries. moe_mlp_bwd takes T > 0.
  */
 typedef struct {
     int32_t E, d, F, act, dtype;

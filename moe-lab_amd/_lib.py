@@ -28,8 +28,8 @@ EXPORTS = ("moe_router", "moe_router_counter_count", "moe_topk", "moe_group", "m
            "moe_experts_shared_workspace_bytes", "moe_router_group", "moe_layer_run_shared",
            "moe_layer_shared_workspace_bytes", "moe_probe_read", "moe_grouped_mm", "moe_grouped_mm_dx", "moe_grouped_mm_dw",
            "moe_linear", "moe_linear_workspace_bytes", "moe_linear_dx",
-           "moe_linear_dx_workspace_bytes", "moe_linear_dw", "moe_linear_dw_workspace_bytes", "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack",
-           "moe_glu_fwd", "moe_glu_bwd", "moe_mlp_fwd", "moe_mlp_bwd", "moe_mlp_keep_bytes",
+           "moe_linear_dx_workspace_bytes", "moe_linear_dw", "moe_linear_dw_workspace_bytes", "moe_linear_act_bwd",
+           "moe_act8_pack", "moe_act8_unpack", "moe_glu_fwd", "moe_glu_bwd", "moe_mlp_fwd", "moe_mlp_bwd", "moe_mlp_keep_bytes",
            "moe_mlp_fwd_workspace_bytes", "moe_mlp_bwd_workspace_bytes")
 PROBE_SINK = 1024   # MOE_PROBE_SINK
 STATIC_SCRATCH_BYTES = 32 << 20   # MOE_STATIC_SCRATCH_BYTES: the workspace array of moe_experts_run_static
@@ -131,8 +131,8 @@ def lib():
                   "moe_experts_run_stages", "moe_tiles_pack", "moe_shared_experts_run", "moe_experts_run_static",
                   "moe_layer_run", "moe_experts_run_shared", "moe_router_group", "moe_layer_run_shared",
                   "moe_probe_read", "moe_grouped_mm", "moe_grouped_mm_dx", "moe_grouped_mm_dw", "moe_linear",
-                  "moe_linear_dx", "moe_linear_dw", "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack", "moe_glu_fwd", "moe_glu_bwd", "moe_mlp_fwd",
-                  "moe_mlp_bwd"):
+                  "moe_linear_dx", "moe_linear_dw", "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack", "moe_glu_fwd",
+                  "moe_glu_bwd", "moe_mlp_fwd", "moe_mlp_bwd"):
             getattr(L, n).restype = ctypes.c_int
         _lib = L
     return _lib
@@ -220,7 +220,8 @@ def half_matrix(t, name, cols=None, device=None, dtype=None):
     bytes aligned with a stride of whole 16 bytes; any other layout is copied. Wrong types and shapes raise."""
     require_device(t, name)
     if t.dtype not in (torch.bfloat16, torch.float16) or (dtype is not None and t.dtype != dtype):
-        raise TypeError(f"{name} is {t.dtype}: " + ("bf16 or fp16 expected" if dtype is None else f"{dtype} expected, as the other operands"))
+        want = "bf16 or fp16 expected" if dtype is None else f"{dtype} expected, as the other operands"
+        raise TypeError(f"{name} is {t.dtype}: {want}")
     if t.dim() != 2 or (cols is not None and t.shape[1] != cols):
         raise ValueError(f"{name} has shape {tuple(t.shape)}: [rows, {'columns' if cols is None else cols}] expected")
     if device is not None and t.device != device:

@@ -4,8 +4,9 @@
     x = unpack(codes, scales, dtype)
     h = glu(gu)                              act(gate) * up of rows [gate | up], differentiable: its backward pass reads 8 bits
 
-A value is code * 2^(scale - 133). The exponent is the block's largest, so an element is off by at most 1/128 of that one
-(half a step), and a block is as exact at 1e-30 as at 1e30; 255 marks a block that held an infinity or NaN and reads as NaN.
+A value is code * 2^(scale - 133), off by at most half a step 2^(scale - 134). The exponent is the block's largest, one more
+where that one would round to 128 steps, so half a step is at most 1/127.5 of the block's largest value, and a block is as
+exact at 1e-30 as at 1e30; 255 marks a block that held an infinity or NaN and reads as NaN.
 Against 16 bits this halves what a GLU keeps: 8.25 bits per value. int8 rather than an 8-bit float: activations of one
 neighbourhood are of one size, and over a block a uniform step errs by about 0.7% of its rms, e4m3 by 2.6%.
 """
@@ -82,7 +83,8 @@ def glu_forward(gu, act=_lib.ACT_SWIGLU, keep=True):
 def glu_backward(codes, scales, dh, act=_lib.ACT_SWIGLU, wts=None, gu=None):
     """The GLU's backward pass from its kept input (codes and scales, or both None and gu itself), dh [M, F] in bf16, fp16 or,
     with codes, fp32, and a weight per row wts fp32 [M] (None: 1), for rows that are summed with these weights later on:
-    (dgu [M, 2 F] = wts dh act'(gate, up), h [M, F] times wts, dwts fp32 [M] = sum of dh h). Results in dh's type (bf16 for fp32 dh)."""
+    (dgu [M, 2 F] = wts dh act'(gate, up), h [M, F] times wts, dwts fp32 [M] = sum of dh h). Results in gu's type, from codes in
+    dh's (bf16 for fp32 dh)."""
     _lib.require_device(dh, "dh")
     if dh.dim() != 2 or dh.dtype not in _lib.DTYPE:
         raise TypeError(f"dh is {dh.dtype} {tuple(dh.shape)}: [M, F] in bf16, fp16 or fp32 expected")

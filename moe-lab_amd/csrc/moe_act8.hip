@@ -101,7 +101,8 @@ __global__ void __launch_bounds__(256) k_glu_bwd(const GluBwd a) {
             unpack8<F16>(*(const u32x4*)(p + F), u);
         }
         if (a.dh32) {
-            const f32x4 d0 = *(const f32x4*)((const float*)a.dh + row * F + c), d1 = *(const f32x4*)((const float*)a.dh + row * F + c + 4);
+            const f32x4* p = (const f32x4*)((const float*)a.dh + row * F + c);
+            const f32x4 d0 = p[0], d1 = p[1];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 d[j] = d0[j];
@@ -303,8 +304,8 @@ int launch_unpack8(const uint8_t* codes, const uint8_t* scales, int64_t M, int64
         else k_unpack8<false><<<grid, 256, 0, st>>>(codes + r * C, scales + r * (C / 32), items, o, dtype == MOE_DTYPE_F32);
     });
 }
-int launch_lin_act_bwd(const void* dy, int64_t ldy, const void* z, const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t N,
-                       int act, bool f16, void* dz, hipStream_t st) {
+int launch_lin_act_bwd(const void* dy, int64_t ldy, const void* z, const uint8_t* codes, const uint8_t* scales, int64_t M,
+                       int64_t N, int act, bool f16, void* dz, hipStream_t st) {
     return by_parts(M, N / 8, [&](int64_t r, uint32_t items, unsigned grid) {
         const uint16_t *d = (const uint16_t*)dy + r * ldy, *v = z ? (const uint16_t*)z + r * N : nullptr;
         const uint8_t *q = codes ? codes + r * N : nullptr, *s = codes ? scales + r * (N / 32) : nullptr;
@@ -313,8 +314,8 @@ int launch_lin_act_bwd(const void* dy, int64_t ldy, const void* z, const uint8_t
         else k_lin_act_bwd<false><<<grid, 256, 0, st>>>(d, ldy, v, q, s, items, (uint32_t)(N / 8), act, o);
     });
 }
-int launch_slots(const int32_t* idx, const int32_t* sorted, const int32_t* offsets, int n, int k, int E, int32_t* rows, int32_t* pos,
-                 hipStream_t st) {
+int launch_slots(const int32_t* idx, const int32_t* sorted, const int32_t* offsets, int n, int k, int E, int32_t* rows,
+                 int32_t* pos, hipStream_t st) {
     if (n == 0) return MOE_OK;
     k_slots<<<(n + 255) / 256, 256, 0, st>>>(idx, sorted, offsets, n, k, E, rows, pos);
     return done();

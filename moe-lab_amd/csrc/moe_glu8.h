@@ -8,8 +8,8 @@ namespace moe {
 // Blocks of 32 neighbours share one exponent byte s: value = q 2^(s - 133), q in [-127, 127]. s is the biased exponent of
 // the block's largest magnitude (so that one keeps 7 bits, 64 <= |q| <= 127), one more where it would round to 128; 0 for a
 // block below 2^-126 (whose 16-bit values stay exact), 255 marks a block that holds an infinity or NaN and reads as NaN.
-// With a power of two the scaling is exact, so an element is off by its rounding alone, at most half a step 2^(s - 133):
-// 1/128 to 1/256 of the block's largest.
+// With a power of two the scaling is exact, so an element is off by its rounding alone, at most half a step 2^(s - 134). The
+// block's largest is 63.75 (s one more) to 127.5 steps, so that is at most 1/127.5 of it.
 __device__ __forceinline__ uint32_t exponent8(uint32_t top) {   // of the bits of a block's largest magnitude (fp32)
     const uint32_t s = top >> 23;
     return s > 0 && s < 254 && (top & 0x7fffffu) >= 0x7f0000u ? s + 1 : s;   // 127.5 and up

@@ -59,23 +59,22 @@ __device__ __forceinline__ srd_t srd_of(const char* p, uint32_t bytes) {
 // vector instruction just before; s_nop 0: M0.
 template <int N, int STRIDE>
 __device__ __forceinline__ void dma16(srd_t s, const uint32_t* off, uint32_t lds) {
-    static_assert(N == 1 || N == 2 || N == 4, "");
+    static_assert(N == 2 || N == 4, "");
     if constexpr (N == 4)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
                      "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %5, 0 offen lds\n\t"
                      "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, 0 offen lds\n\t"
                      "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %5, 0 offen lds"
                      ::"s"(lds), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(s), "n"(STRIDE) : "memory", "m0", "scc");
-    else if constexpr (N == 2)
+    else
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
                      "s_add_u32 m0, m0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
                      ::"s"(lds), "v"(off[0]), "v"(off[1]), "s"(s), "n"(STRIDE) : "memory", "m0", "scc");
-    else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off[0]), "s"(s) : "memory", "m0");
 }
 // 4 bytes per lane, to LDS at lds + 4 lane
 __device__ __forceinline__ void dma4(srd_t s, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(s) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 ::"s"(lds), "v"(off), "s"(s) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void wait_vm() {
@@ -255,7 +254,8 @@ __device__ __forceinline__ void fill_rest(const MmArgs& a) {
     group_of<MODE>(a, a.E - 1, lo, hi);
     const int64_t row16 = (int64_t)a.J * (a.ydt == MOE_DTYPE_F32 ? 4 : 2) / 16, n = (a.M - hi) * row16;
     u32x4* y = (u32x4*)a.y + hi * row16;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) y[i] = (u32x4){0, 0, 0, 0};
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
+        y[i] = (u32x4){0, 0, 0, 0};
 }
 // Tile id of the forward or dx product: its group by two 64-way searches in pre; inside a group down up to 4 row tiles before
 // the next column tile.
@@ -344,7 +344,8 @@ struct MmKernel {
                                                        int wi, int wj) {
         const int l = lane & 15, q = lane >> 4, jw = t.j0 + wj * FB * 16;
         const int64_t row0 = MODE == MM_DW ? (int64_t)t.e * g.I + t.i0 : (g.part ? (int64_t)t.e * g.M : 0) + t.lo;
-        const auto yb = __builtin_amdgcn_make_buffer_rsrc((char*)g.y + row0 * g.J * 2, 0, (uint32_t)t.rows * (uint32_t)g.J * 2, 0x00027000);
+        const auto yb = __builtin_amdgcn_make_buffer_rsrc((char*)g.y + row0 * g.J * 2, 0, (uint32_t)t.rows * (uint32_t)g.J * 2,
+                                                          0x00027000);
         constexpr int LPR = 2 * FB, RPI = 64 / LPR;   // lanes per row, rows per store
         const int r = lane / LPR, c = lane % LPR * 8;
         const bool ok = jw + c < g.J;
@@ -359,8 +360,8 @@ struct MmKernel {
 #pragma unroll
             for (int k = 0; k < 16 / RPI; ++k) {
                 const int i = 16 * (2 * f + wi) + k * RPI + r;
-                __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4*)(out + k * RPI * OUT_LD), yb,
-                                                       ok && i < t.rows ? ((uint32_t)i * (uint32_t)g.J + jw + c) * 2 : MM_OOB, 0, 2);
+                const uint32_t to = ok && i < t.rows ? ((uint32_t)i * (uint32_t)g.J + jw + c) * 2 : MM_OOB;
+                __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4*)(out + k * RPI * OUT_LD), yb, to, 0, 2);
             }
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_sched_barrier(0);
@@ -402,8 +403,8 @@ struct MmKernel {
                         zz[u][1] = pack16<F16>(v[u][2], v[u][3]);
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
-                            const float z = v[u][c];
-                            v[u][c] = (lin ? z : z * sigmoid_fast(z * (c1 + c3 * (z * z)))) + un16<F16>(rw[c >> 1] >> (16 * (c & 1)));
+                            const float z = v[u][c], r = un16<F16>(rw[c >> 1] >> (16 * (c & 1)));
+                            v[u][c] = (lin ? z : z * sigmoid_fast(z * (c1 + c3 * (z * z)))) + r;
                         }
                     }
                 }
@@ -416,7 +417,8 @@ struct MmKernel {
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const int j = jw + 16 * (h + u) + 4 * q;
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[u]), yb, j < g.J ? (row + j) * 4 : MM_OOB, 0, 0);
+                        const uint32_t at = j < g.J ? (row + j) * 4 : MM_OOB;
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[u]), yb, at, 0, 0);
                     }
                 } else {
                     put(yb, pack16<F16>(v[0][0], v[0][1]), pack16<F16>(v[0][2], v[0][3]), pack16<F16>(v[1][0], v[1][1]),
@@ -441,9 +443,10 @@ struct MmKernel {
         const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
         return p[0] > p[1] ? p[0] : p[1];
     }
-    // EPI_GLU. Two column blocks (32 columns: one block of the 8-bit form) at a time: h = act(gate, up) from the fp32 sums; the kept
-    // rows from the sums rounded to 16 bits, as a pass over 16-bit rows would find them.
-    static __device__ __forceinline__ void store_glu(const MmArgs& g, const MmTile& t, f32x4 (&acc)[FA][FB], int lane, int wi, int wj) {
+    // EPI_GLU. Two column blocks (32 columns: one block of the 8-bit form) at a time: h = act(gate, up) from the fp32 sums; the
+    // kept rows from the sums rounded to 16 bits, as a pass over 16-bit rows would find them.
+    static __device__ __forceinline__ void store_glu(const MmArgs& g, const MmTile& t, f32x4 (&acc)[FA][FB], int lane, int wi,
+                                                     int wj) {
         constexpr int H = FB / 2;
         static_assert(!GLU || H % 2 == 0, "a block of 32 columns per wave");
         const int l = lane & 15, q = lane >> 4, jw = t.j0 + wj * H * 16, F = g.J;
@@ -509,9 +512,10 @@ struct MmKernel {
 #pragma unroll
                                 for (int c = 0; c < 4; ++c) k[u] |= code8(v[u][c], e) << (8 * c);
                         const auto p = __builtin_amdgcn_permlane16_swap(k[0], k[1], false, false);
-                        __builtin_amdgcn_raw_buffer_store_b64((u32x2){p[0], p[1]}, cb, ok ? (uint32_t)i * 2 * F + s * F + jj : MM_OOB, 0, 0);
-                        if (q == 0)
-                            __builtin_amdgcn_raw_buffer_store_b8((uint8_t)e, sb, ok ? (uint32_t)i * (F / 16) + (s * F + jw + 16 * h) / 32 : MM_OOB, 0, 0);
+                        const uint32_t to = ok ? (uint32_t)i * 2 * F + s * F + jj : MM_OOB;
+                        __builtin_amdgcn_raw_buffer_store_b64((u32x2){p[0], p[1]}, cb, to, 0, 0);
+                        const uint32_t block = ok ? (uint32_t)i * (F / 16) + (s * F + jw + 16 * h) / 32 : MM_OOB;
+                        if (q == 0) __builtin_amdgcn_raw_buffer_store_b8((uint8_t)e, sb, block, 0, 0);
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -551,7 +555,9 @@ struct MmKernel {
             }
         };
         auto r_of = [&](const MmTile& t) -> int { return g.part ? min(g.part, g.R - t.e * g.part) : g.R; };   // forward, dx
-        auto steps_of = [&](const MmTile& t) -> int { return MODE == MM_DW ? (t.cnt + 63) / 64 : t.rows ? (r_of(t) + 63) / 64 : 0; };
+        auto steps_of = [&](const MmTile& t) -> int {
+            return MODE == MM_DW ? (t.cnt + 63) / 64 : t.rows ? (r_of(t) + 63) / 64 : 0;
+        };
 
         // the stream of loads: its tile, the step in it, and where the operands' next pieces begin
         int lid = -1, ls = 0, lsteps = 0, lrows = 0, lr = 0;
@@ -612,7 +618,8 @@ struct MmKernel {
                     offb[i] = j < g.J ? (uint32_t)((r % W < H ? j : g.J + j) * ldb2 + c * 2) : MM_OOB;
                 }
             }
-            if constexpr (MODE == MM_FWD) pb += GLU ? (int64_t)lt.e * 2 * g.J * ldb2 : ((int64_t)e * g.J + lt.j0) * ldb2 + first * 2;
+            if constexpr (GLU) pb += (int64_t)lt.e * 2 * g.J * ldb2;
+            else if constexpr (MODE == MM_FWD) pb += ((int64_t)e * g.J + lt.j0) * ldb2 + first * 2;
             if constexpr (MODE == MM_DX) pb += ((int64_t)e * g.R + first) * ldb2 + (int64_t)lt.j0 * 2;
             if constexpr (MODE == MM_DW) pb += (gath_b ? 0 : (int64_t)lt.lo * ldb2) + (int64_t)lt.j0 * 2;
             fetch_rows();
@@ -626,7 +633,10 @@ struct MmKernel {
         };
         auto bytes_b = [&]() -> uint32_t {
             if (!lrows) return 0;
-            if constexpr (!BX) return (uint32_t)((GLU ? 2 * g.J : min(BJ, g.J - lt.j0)) - 1) * (uint32_t)ldb2 + (uint32_t)(lr - 64 * ls) * 2;
+            if constexpr (!BX) {
+                const int rows = GLU ? 2 * g.J : min(BJ, g.J - lt.j0);
+                return (uint32_t)(rows - 1) * (uint32_t)ldb2 + (uint32_t)(lr - 64 * ls) * 2;
+            }
             const int rows = MODE == MM_DX ? min(64, lr - 64 * ls) : gath_b ? g.b_n : min(64, lt.cnt - 64 * ls);
             return (uint32_t)(rows - 1) * (uint32_t)ldb2 + (uint32_t)(g.J - lt.j0) * 2;
         };
@@ -662,7 +672,9 @@ struct MmKernel {
         };
         // pieces i0 .. of either operand, for load step ls into stage buffer `buf`
         constexpr int NA = PA < 4 ? PA : 4, NB = PB < 4 ? PB : 4;
-        auto load_a = [&](uint32_t buf, srd_t d, int i) { dma16<NA, NW * 1024>(d, offa + i, lds0 + buf + (uint32_t)((i * NW + lw) * 1024)); };
+        auto load_a = [&](uint32_t buf, srd_t d, int i) {
+            dma16<NA, NW * 1024>(d, offa + i, lds0 + buf + (uint32_t)((i * NW + lw) * 1024));
+        };
         auto load_b = [&](uint32_t buf, srd_t d, int i) {
             dma16<NB, NW * 1024>(d, offb + i, lds0 + buf + (uint32_t)(A::BYTES + (i * NW + lw) * 1024));
         };
@@ -689,13 +701,16 @@ struct MmKernel {
                 acc[f][h] = mma<F16>(rb[set][h], ra[set][f], acc[f][h]);
             }
         };
-        // dbias: this lane's share (8 of 32 r) of its rows' sums over r
+        // dbias: this lane's share (8 of 32 r) of its rows' sums over r, in fp32, of dy as it lies in the fragments: in 16 bits. A
+        // linear layer's dz is rounded to them for the products; its rows' errors are independent and even, so that of T rows they
+        // add sqrt(T) half steps / sqrt(3) of a row's to a sum, below its own rounding unless the rows cancel to less than that.
         auto add_rows = [&](int set) {
 #pragma unroll
             for (int f = 0; f < FA; ++f) {
                 const u32x4 w = __builtin_bit_cast(u32x4, ra[set][f]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) sums[f] = F16 ? dot2_f16(w[c], 0x3C003C00u, sums[f]) : dot2_bf16(w[c], 0x3F803F80u, sums[f]);
+                for (int c = 0; c < 4; ++c)
+                    sums[f] = F16 ? dot2_f16(w[c], 0x3C003C00u, sums[f]) : dot2_bf16(w[c], 0x3F803F80u, sums[f]);
             }
         };
 
@@ -720,7 +735,7 @@ struct MmKernel {
         }
         uint32_t rbuf = 0, wbuf = 0;   // stage buffers of the step that is multiplied, and of the load step
         auto next_buf = [](uint32_t b) -> uint32_t { return b == (ST - 1) * STAGE ? 0 : b + STAGE; };
-const bool loads = !NL || wave >= NWC;
+        const bool loads = !NL || wave >= NWC;
         if (loads) {
 #pragma unroll
             for (int s = 0; s < ST; ++s) {

@@ -12,6 +12,9 @@ bool too_far(int64_t rows, int64_t ld) { return rows * ld * 2 > 0xB0000000ll; }
 bool two_byte(int dtype) { return dtype == MOE_DTYPE_BF16 || dtype == MOE_DTYPE_F16; }
 // Slots are counted in 32 bits, in steps of up to 64 past the last one and pieces of up to 128.
 constexpr int64_t MAX_SLOTS = 0x7fffff00;
+bool bad_groups(const int32_t* offsets, int E, int64_t M) {
+    return E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > MAX_SLOTS;
+}
 bool bad_act8(int64_t M, int64_t C) { return M < 0 || M > 0x7fffffff || C < 32 || C % 32 || C > (1 << 20); }
 bool bad_rows(const int32_t* idx, int64_t rows, int64_t M) { return rows > 0x7fffffff || rows < (idx ? 1 : M); }
 // Workspace of a product in parts, with `more` floats per part behind the sums.
@@ -58,7 +61,8 @@ struct MlpLayout {
 int check_mlp(const moe_mlp_t* m, int T, int k) {
     if (!m || T < 0 || k < 1 || m->E < 1 || m->E > MM_MAX_E || (int64_t)T * k > moe::GROUP_MAX_SLOTS) return MOE_ERR_ARG;
     if (!two_byte(m->dtype)) return MOE_ERR_DTYPE;
-    if (m->act < 0 || m->act > MOE_ACT_GPTOSS || bad_dim(m->d) || bad_act8(0, m->F) || bad_dim(2 * (int64_t)m->F)) return MOE_ERR_ARG;
+    if (m->act < 0 || m->act > MOE_ACT_GPTOSS || bad_dim(m->d) || bad_act8(0, m->F) || bad_dim(2 * (int64_t)m->F))
+        return MOE_ERR_ARG;
     if (!m->w_gate_up || !m->w_down) return MOE_ERR_ARG;
     if (misaligned(m->w_gate_up) || misaligned(m->w_down)) return MOE_ERR_ALIGN;
     if (too_far(T, m->d) || too_far(2 * (int64_t)m->F, m->d)) return MOE_ERR_ARG;
@@ -73,7 +77,7 @@ int moe_grouped_mm(const void* x, const void* w, const void* bias, const int32_t
                    void* stream) {
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return MOE_ERR_DTYPE;
     if (y_dtype != dtype && y_dtype != MOE_DTYPE_F32) return MOE_ERR_DTYPE;
-    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > MAX_SLOTS || bad_dim(N) || bad_dim(K) || bad_ld(ldx, K)) return MOE_ERR_ARG;
+    if (bad_groups(offsets, E, M) || bad_dim(N) || bad_dim(K) || bad_ld(ldx, K)) return MOE_ERR_ARG;
     if (M == 0) return MOE_OK;
     if (!x || !w || !y || bad_rows(rows, x_rows, M)) return MOE_ERR_ARG;
     if (misaligned(x) || misaligned(w) || misaligned(y) || misaligned(bias)) return MOE_ERR_ALIGN;
@@ -105,7 +109,7 @@ int moe_grouped_mm_dx(const void* dy, const void* w, const int32_t* offsets, con
                       void* stream) {
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return MOE_ERR_DTYPE;
     if (dx_dtype != dtype && dx_dtype != MOE_DTYPE_F32) return MOE_ERR_DTYPE;
-    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > MAX_SLOTS || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
+    if (bad_groups(offsets, E, M) || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
     if (M == 0) return MOE_OK;
     if (!dy || !w || !dx || bad_rows(rows, dy_rows, M)) return MOE_ERR_ARG;
     if (misaligned(dy) || misaligned(w) || misaligned(dx)) return MOE_ERR_ALIGN;
@@ -134,9 +138,7 @@ int moe_grouped_mm_dw(const void* dy, const void* x, const int32_t* offsets, con
                       void* dw, int dw_dtype, void* dbias, void* stream) {
     if (dtype != MOE_DTYPE_BF16 && dtype != MOE_DTYPE_F16) return MOE_ERR_DTYPE;
     if (dw_dtype != dtype && dw_dtype != MOE_DTYPE_F32) return MOE_ERR_DTYPE;
-    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || M < 0 || M > MAX_SLOTS || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N) ||
-        bad_ld(ldx, K))
-        return MOE_ERR_ARG;
+    if (bad_groups(offsets, E, M) || bad_dim(N) || bad_dim(K) || bad_ld(lddy, N) || bad_ld(ldx, K)) return MOE_ERR_ARG;
     if (!dw || (M > 0 && (!dy || !x))) return MOE_ERR_ARG;
     if (M > 0 && (bad_rows(dy_idx, dy_rows, M) || bad_rows(x_idx, x_rows, M))) return MOE_ERR_ARG;
     if (misaligned(dy) || misaligned(x) || misaligned(dw)) return MOE_ERR_ALIGN;
@@ -257,13 +259,14 @@ int moe_linear_dw(const void* dy, const void* x, int64_t T, int64_t lddy, int64_
 int moe_linear_act_bwd(const void* dy, int64_t lddy, const void* z, const void* codes, const void* scales, int act, int64_t T,
                        int N, int dtype, void* dz, void* stream) {
     if (!two_byte(dtype)) return MOE_ERR_DTYPE;
-    if ((act != MOE_LIN_SILU && act != MOE_LIN_GELU) || T < 0 || T > 0x7fffffff || bad_dim(N) || bad_ld(lddy, N)) return MOE_ERR_ARG;
+    if ((act != MOE_LIN_SILU && act != MOE_LIN_GELU) || T < 0 || T > 0x7fffffff || bad_dim(N) || bad_ld(lddy, N))
+        return MOE_ERR_ARG;
     if (codes && bad_act8(T, N)) return MOE_ERR_ARG;
     if (T == 0) return MOE_OK;
     if (!dy || !dz || (!z && (!codes || !scales)) || (z && codes)) return MOE_ERR_ARG;
     if (misaligned(dy) || misaligned(z) || misaligned(codes) || misaligned(dz)) return MOE_ERR_ALIGN;
-    return moe::launch_lin_act_bwd(dy, lddy, z, (const uint8_t*)codes, (const uint8_t*)scales, T, N, act, dtype == MOE_DTYPE_F16, dz,
-                                   (hipStream_t)stream);
+    return moe::launch_lin_act_bwd(dy, lddy, z, (const uint8_t*)codes, (const uint8_t*)scales, T, N, act, dtype == MOE_DTYPE_F16,
+                                   dz, (hipStream_t)stream);
 }
 
 int moe_act8_pack(const void* x, int64_t ldx, int64_t M, int C, int dtype, void* codes, void* scales, void* stream) {
@@ -291,7 +294,8 @@ int moe_glu_fwd(const void* gu, int64_t ldgu, int64_t M, int F, int act, int dty
     if (M == 0) return MOE_OK;
     if (!gu || !h || !codes != !scales) return MOE_ERR_ARG;
     if (misaligned(gu) || misaligned(h) || misaligned(codes)) return MOE_ERR_ALIGN;
-    return moe::launch_glu_fwd(gu, ldgu, M, F, act, dtype == MOE_DTYPE_F16, h, (uint8_t*)codes, (uint8_t*)scales, (hipStream_t)stream);
+    return moe::launch_glu_fwd(gu, ldgu, M, F, act, dtype == MOE_DTYPE_F16, h, (uint8_t*)codes, (uint8_t*)scales,
+                               (hipStream_t)stream);
 }
 
 int moe_glu_bwd(const void* codes, const void* scales, const void* gu, int64_t ldgu, const void* dh, int dh_dtype,
@@ -301,12 +305,14 @@ int moe_glu_bwd(const void* codes, const void* scales, const void* gu, int64_t l
     if (M == 0) return MOE_OK;
     if (!dh || !dgu || (codes ? !scales || gu : !gu || bad_ld(ldgu, 2 * (int64_t)F))) return MOE_ERR_ARG;
     if (misaligned(codes) || misaligned(gu) || misaligned(dh) || misaligned(dgu) || misaligned(hw)) return MOE_ERR_ALIGN;
-    const moe::GluBwd a{(const uint8_t*)codes, (const uint8_t*)scales, (const uint16_t*)gu, ldgu, dh, dh_dtype == MOE_DTYPE_F32, wts,
-                        nullptr, nullptr, M, F, act, (uint16_t*)dgu, (uint16_t*)hw, dwts};
+    const moe::GluBwd a{(const uint8_t*)codes, (const uint8_t*)scales, (const uint16_t*)gu, ldgu, dh, dh_dtype == MOE_DTYPE_F32,
+                        wts, nullptr, nullptr, M, F, act, (uint16_t*)dgu, (uint16_t*)hw, dwts};
     return moe::launch_glu_bwd(a, dtype == MOE_DTYPE_F16, (hipStream_t)stream);
 }
 
-size_t moe_mlp_keep_bytes(const moe_mlp_t* m, int T, int k) { return m && T >= 0 && k > 0 ? MlpLayout(*m, (int64_t)T * k).keep : 0; }
+size_t moe_mlp_keep_bytes(const moe_mlp_t* m, int T, int k) {
+    return m && T >= 0 && k > 0 ? MlpLayout(*m, (int64_t)T * k).keep : 0;
+}
 size_t moe_mlp_fwd_workspace_bytes(const moe_mlp_t* m, int T, int k) {
     return m && T >= 0 && k > 0 ? MlpLayout(*m, (int64_t)T * k).fwd : 0;
 }
@@ -417,8 +423,8 @@ int moe_mlp_bwd(const moe_mlp_t* m, const void* x, const float* wts, const void*
     rc = moe::launch_mm_dx(a, st);
     if (rc) return rc;
     const moe::GluBwd b{(const uint8_t*)codes, (const uint8_t*)scales, (const uint16_t*)gu, 2 * (int64_t)m->F, ws + L.dh, 1, wts,
-                        sorted, offsets + m->E, n, m->F, m->act, (uint16_t*)(ws + L.dgu), dw_down ? (uint16_t*)(ws + L.hw) : nullptr,
-                        dwts};
+                        sorted, offsets + m->E, n, m->F, m->act, (uint16_t*)(ws + L.dgu),
+                        dw_down ? (uint16_t*)(ws + L.hw) : nullptr, dwts};
     rc = moe::launch_glu_bwd(b, f16, st);
     if (rc) return rc;
     // the slots' rows of dx in fp32: rounded to 16 bits before their sum, they took dx's error from 2.4e-3 to 2.9e-3

@@ -6,13 +6,14 @@ namespace moe {
 // Which of the shapes, and into how many parts: the shortest of estimates that take a step of 64 r at its measured time with
 // every CU busy, workgroups in rounds over the 256 CUs, a tile's start and stores as a few more, and the join as a launch and one
 // pass over the parts at 4.5 TB/s. Measured, parts against one whole:
-//   T 64, w [4096, 4096] 16.2 us, whole 24.5      T 512, w [4096, 4096] 31.3, whole 36.7      dx, T 1024, w [14336, 4096] 116, whole 157
+//   T 64, w [4096, 4096] 16.2 us, whole 24.5      T 512, w [4096, 4096] 31.3, whole 36.7
+//   dx, T 1024, w [14336, 4096] 116, whole 157
 //   dw of 16384 slots, [512, 512] 22.0, whole 107      dw of 65536 slots, [1024, 1024] 133, whole 426
 MmPlan mm_plan(int mode, int64_t rows, int64_t J, int64_t R, bool split) {
     // us of a step: with two workgroups on each CU that takes two, and with one; steps that a tile's start and stores take
     static const struct { int shape, bi, bj, slots; float busy, alone; int more; } S[] = {
-        {MM_128x256, 128, 256, 256, 0.83f, 0.83f, 3}, {MM_128_DEEP, 128, 128, 256, 0.52f, 0.52f, 6}, {MM_128, 128, 128, 512, 1.05f, 0.92f, 2},
-        {MM_64, 64, 64, 512, 0.55f, 0.41f, 3}};
+        {MM_128x256, 128, 256, 256, 0.83f, 0.83f, 3}, {MM_128_DEEP, 128, 128, 256, 0.52f, 0.52f, 6},
+        {MM_128, 128, 128, 512, 1.05f, 0.92f, 2}, {MM_64, 64, 64, 512, 0.55f, 0.41f, 3}};
     MmPlan best{MM_128x256, 1};
     float least = 3e38f;
     for (const auto& c : S) {

@@ -65,7 +65,8 @@ __global__ void __launch_bounds__(256) k_mm_rows(const MmArgs g) {
             u32x4 wv[S * R], xv[MR];
 #pragma unroll
             for (int r = 0; r < S * R; ++r)
-                wv[r] = in && n0 + r % R < g.J ? *(const u32x4*)(w + (r < R ? 0 : up) + (int64_t)(r % R) * g.ldb + k) : (u32x4){0, 0, 0, 0};
+                wv[r] = in && n0 + r % R < g.J ? *(const u32x4*)(w + (r < R ? 0 : up) + (int64_t)(r % R) * g.ldb + k)
+                                               : (u32x4){0, 0, 0, 0};
 #pragma unroll
             for (int m = 0; m < MR; ++m) xv[m] = in ? *(const u32x4*)(x[m] + k) : (u32x4){0, 0, 0, 0};
 #pragma unroll

@@ -29,10 +29,10 @@ int launch_glu_fwd(const void* gu, int64_t ldg, int64_t M, int F, int act, bool 
 int launch_glu_bwd(const GluBwd& a, bool f16, hipStream_t st);
 int launch_pack8(const void* x, int64_t ld, int64_t M, int64_t C, bool f16, uint8_t* codes, uint8_t* scales, hipStream_t st);
 int launch_unpack8(const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t C, int dtype, void* out, hipStream_t st);
-int launch_lin_act_bwd(const void* dy, int64_t ldy, const void* z, const uint8_t* codes, const uint8_t* scales, int64_t M, int64_t N,
-                       int act, bool f16, void* dz, hipStream_t st);
-int launch_slots(const int32_t* idx, const int32_t* sorted, const int32_t* offsets, int n, int k, int E, int32_t* rows, int32_t* pos,
-                 hipStream_t st);
+int launch_lin_act_bwd(const void* dy, int64_t ldy, const void* z, const uint8_t* codes, const uint8_t* scales, int64_t M,
+                       int64_t N, int act, bool f16, void* dz, hipStream_t st);
+int launch_slots(const int32_t* idx, const int32_t* sorted, const int32_t* offsets, int n, int k, int E, int32_t* rows,
+                 int32_t* pos, hipStream_t st);
 int launch_slot_sum(const float* ys, const int32_t* pos, const float* wts, const void* residual, int64_t M, int64_t T, int k,
                     int d, bool f16, void* y, int ydt, hipStream_t st);
 

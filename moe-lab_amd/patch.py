@@ -291,7 +291,8 @@ def _probe(module, d, F, E, dtype, act):
     torch.nn.Module.__init__(m)
     names = ("gate_up_proj", "down_proj") if E else ("gate_proj", "up_proj", "down_proj")
     kept = {n: _bare(c) for n, c in module._modules.items() if n not in names + ("parametrizations",)}
-    m.__dict__.update({n: v for n, v in module.__dict__.items() if n not in m.__dict__ and n not in ("forward", "_moelab_stock_forward")})
+    own = {n: v for n, v in module.__dict__.items() if n not in m.__dict__}
+    m.__dict__.update({n: v for n, v in own.items() if n not in ("forward", "_moelab_stock_forward")})
     m._buffers, m._modules = dict(module._buffers), kept
     if E:
         n = E if F <= 32 else 1   # at the module's own sizes its experts are one and the same
@@ -306,7 +307,8 @@ def _probe(module, d, F, E, dtype, act):
             m._modules[n] = torch.nn.Linear(t.shape[1], t.shape[0], bias=False, device="meta", dtype=dtype)
             m._modules[n].weight = torch.nn.Parameter(t, requires_grad=False)
         gu = torch.cat([m.gate_proj.weight, m.up_proj.weight])[None]
-        dn, idx, wts = m.down_proj.weight[None], torch.zeros(len(x), 1, dtype=torch.int64, device="cpu"), torch.ones(len(x), 1, device="cpu")
+        dn = m.down_proj.weight[None]
+        idx, wts = torch.zeros(len(x), 1, dtype=torch.int64, device="cpu"), torch.ones(len(x), 1, device="cpu")
         args = (x,)
     got = cls.forward(m.train(), *args)   # as in training: a dropout shows too
     if E:
@@ -343,8 +345,8 @@ def _check_glu(module, act, stacked, d, F, E):
                 continue
             if gap <= tol:
                 return
-            raise ValueError(f"{type(module).__name__} computes something else than the plain GLU layer of the kernels (off by {gap:.1e} of "
-                             f"its sums on random weights): a clamp, another gate or another place of the routing weights")
+            raise ValueError(f"{type(module).__name__} computes something else than the plain GLU layer of the kernels (off by "
+                             f"{gap:.1e} of its sums on random weights): a clamp, another gate or other routing weights")
     raise ValueError(f"{type(module).__name__}: its forward could not be checked against the kernels' GLU layer ({tried[0]})")
 
 
