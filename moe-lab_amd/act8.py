@@ -3,6 +3,7 @@
     codes, scales = pack(x)                  int8 codes like x, one exponent byte per 32 neighbours of a row (uint8)
     x = unpack(codes, scales, dtype)
     h = glu(gu)                              act(gate) * up of rows [gate | up], differentiable: its backward pass reads 8 bits
+                                             (pack, unpack, glu_forward and glu_backward have no gradient themselves)
 
 A value is code * 2^(scale - 133), off by at most half a step 2^(scale - 134). The exponent is the block's largest, one more
 where that one would round to 128 steps, so half a step is at most 1/127.5 of the block's largest value, and a block is as

@@ -124,7 +124,8 @@ def experts_mlp(x, idx, wts, w_gate_up, w_down, act=_lib.ACT_SWIGLU, residual=No
     int32 (int64 is converted), wts [T, k] floating. d a multiple of 8, F of 32. A slot whose id is outside [0, E) adds
     nothing. out_dtype: x's type or fp32.
     Differentiable; checkpoint: the gate/up rows are kept in 8 bits for the backward pass (half the memory; its gradients are
-    the layer's at these values), else in 16."""
+    the layer's at these values, about 1% off its own in the norm), else in 16 (0.3% off in bf16, 0.04% in fp16). Gradients of
+    a result in fp32 are rounded to x's type first."""
     if not _lib.wants_grad(x, wts, w_gate_up, w_down, residual):
         idx, wts = _slot_lists(x, idx, wts)
         y = _forward(x, idx, wts, w_gate_up, w_down, act, residual, out_dtype, None)[0]
