@@ -280,7 +280,7 @@ def _probe(module, d, F, E, dtype, act):
     """The largest error of a module's own forward against the plain GLU layer, relative to the magnitudes that its sums add,
     on small random weights in its parameters' place (E None: a dense GLU MLP). Gates reach the hundreds, so that a clamp shows;
     routing weights are not 1, so that a weight at another place does."""
-    g = torch.Generator().manual_seed(0)
+    g = torch.Generator("cpu").manual_seed(0)
 
     def rand(*shape):
         return torch.randn(shape, generator=g, dtype=torch.float64, device="cpu").to(dtype)
@@ -338,7 +338,7 @@ def _check_glu(module, act, stacked, d, F, E):
     for size in ((16, 32), (d, F)):   # some forwards know their sizes
         for dtype, tol in ((torch.float64, 1e-6), (torch.float32, 1e-4), (own, 0.05)):
             try:
-                with torch.no_grad():
+                with torch.no_grad(), torch.device("cpu"):   # whatever the program's default device is
                     gap = _probe(module, *size, E if stacked else None, dtype, act)
             except Exception as e:   # a type or a size that this forward does not take
                 tried.append(f"{type(e).__name__}: {e}")

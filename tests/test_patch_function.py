@@ -149,3 +149,19 @@ def test_the_check_leaves_the_module_alone():
     m = Experts()
     torch.nn.utils.parametrize.register_parametrization(m, "down_proj", Twice())
     patch.patch_dense(m)
+
+
+@pytest.mark.parametrize("device", ["meta", "cpu"])
+def test_under_a_default_device(device):
+    """The check runs on the CPU whatever device a program makes its tensors on by default (and in a model built on none)."""
+    m, e, s = Experts(), experts(), mlp()
+    with torch.device(device):
+        patch.patch_dense(m)
+        patch.patch_dense(e)
+        patch.patch_dense(s)
+    with torch.device("meta"):
+        m = Experts(how="plain")
+        patch.patch_dense(m)
+        with pytest.raises(ValueError, match="something else"):
+            patch.patch_dense(Experts(how="clamped"))
+    assert all(p.is_meta for p in m.parameters())
