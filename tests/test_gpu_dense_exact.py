@@ -18,10 +18,10 @@ pytestmark = pytest.mark.gpu
 EPS = 2.0 ** -23
 
 # T, k, E, d, F, act: dot products of single slots; 64-row tiles; 128-row tiles of few experts and of uneven ones; 128 x 256
-# tiles with rounds and rests; 300 and 1024 experts
+# tiles with rounds and rests; 300 and 1024 experts; the smallest d; more slots a token than are summed at once
 SIZES = [(1, 4, 8, 128, 96, 0), (5, 3, 16, 136, 64, 1), (33, 2, 4, 72, 160, 2), (150, 2, 3, 264, 128, 0), (600, 4, 8, 136, 96, 1),
          (900, 4, 12, 264, 544, 0), (2100, 2, 16, 72, 800, 2), (1500, 8, 64, 136, 160, 0), (40, 8, 300, 72, 64, 1), (3, 8, 1024, 64, 32, 0),
-         (700, 8, 1024, 64, 64, 0)]
+         (700, 8, 1024, 64, 64, 0), (7, 1, 1, 8, 32, 1), (60, 13, 24, 72, 64, 0), (9, 40, 48, 8, 96, 1)]
 IDS = ["-".join(map(str, s)) for s in SIZES]
 
 
