@@ -34,8 +34,8 @@ The stock forwards are kept (``_moelab_stock_forward``); ``unpatch_block`` / ``u
 forwards then differ by arithmetic only, not by quantisation.
 """
 import copy
+import functools
 import math
-import types
 
 import torch
 
@@ -350,9 +350,10 @@ def _check_glu(module, act, stacked, d, F, E):
     raise ValueError(f"{type(module).__name__}: its forward could not be checked against the kernels' GLU layer ({tried[0]})")
 
 
-# patch_dense's forwards are bound methods: a deep copy of a patched module computes with its own parameters. The kernels call
-# none of the module's parts, so where one would do more than it did when the module was patched (a hook on it, an adapter or
-# another module in its place), the stock forward runs.
+# patch_dense's forwards are bound to their module by a partial call: a deep copy of a patched module computes with its own
+# parameters, and a saved one loads (a bound method would be looked up in the module when it loads). The kernels call none of
+# the module's parts, so where one would do more than it did when the module was patched (a hook on it, an adapter or another
+# module in its place), the stock forward runs.
 def _experts_forward(self, hidden_states, top_k_index, top_k_weights):
     s = self._moelab_state
     if self.act_fn is not s["act_fn"] or _hooked(self.act_fn):
@@ -386,7 +387,7 @@ def _dense_act(module):
 
 
 def _install_dense(module, act, checkpoint):
-    return _install(module, types.MethodType(_experts_forward if _stacked(module) else _mlp_forward, module),
+    return _install(module, functools.partial(_experts_forward if _stacked(module) else _mlp_forward, module),
                     {"fmt": "dense", "act": act, "act_fn": module.act_fn, "checkpoint": checkpoint})
 
 

@@ -249,3 +249,28 @@ def test_default_gradients_against_the_stock_module(kind):
     got = torch.autograd.grad(e(b[0], idx, b[1]), [*b, e.gate_up_proj, e.down_proj], dy)
     for name, g, w in zip(("dx", "dwts", "dw_gate_up", "dw_down"), got, want):
         assert float((g.cpu().double() - w).norm() / w.norm()) <= 2 * H.half_step(dt) / 3 ** 0.5, name
+
+
+@pytest.mark.parametrize("how", ["pickle", "torch.save"])
+def test_a_saved_module_loads(calls, how):
+    """Patched, with its own parameters, and its stock forward behind it."""
+    import io
+    import pickle
+    block = make_block("deepseek", "cpu")
+    patch.patch_model(torch.nn.ModuleList([block]), fmt="dense", checkpoint=True)
+    for m, args in ((block.experts, (tokens(), *slots())), (block.shared_experts, (tokens(),))):
+        if how == "pickle":
+            other = pickle.loads(pickle.dumps(m))
+        else:
+            f = io.BytesIO()
+            torch.save(m, f)
+            f.seek(0)
+            other = torch.load(f, weights_only=False)   # written two lines above
+        n = len(calls)
+        assert other(*args) is args[0] and len(calls) == n + 1 and other._moelab_state["checkpoint"] is True
+        w = other.down_proj if m is block.experts else other.down_proj.weight
+        assert any(t is w for t in calls[-1])
+        patch.unpatch_experts(other)
+        stock = copy.deepcopy(m)
+        patch.unpatch_experts(stock)
+        assert torch.equal(other(*args), stock(*args)) and len(calls) == n + 1
