@@ -412,6 +412,74 @@ int moe_mlp_bwd(const moe_mlp_t* m, const void* x, const float* wts, const void*
                 const void* codes, const void* scales, void* dx, float* dwts, void* dw_gate_up, void* dw_down, void* workspace,
                 size_t workspace_bytes, void* stream);
 
+/*
+ * Routing by scores and groups (the reference's router is the softmax top-k of moe_topk, moelab/router.py:1-66; it leaves
+ * group-limited gates to the stock module, e2e.py:129-150):
+ *   s = sigmoid(logit) or softmax(logits) (MOE_SCORE_*); an expert ranks by s + bias[e], without a bias by its logit;
+ *   groups > 1: experts E / groups * g ... form group g, its value is the largest ranking value in it (MOE_GROUP_MAX) or the sum
+ *   of the two largest (MOE_GROUP_TOP2; without a bias the scores'); the top_groups groups of largest value stay;
+ *   idx [T, k]: the k experts of largest ranking value in the groups that stay, of equals the lowest id first (groups alike);
+ *   wts [T, k] fp32 = scale s, with norm scale s / (sum of the k experts' s) (0 where that is 0; a softmax's from the chosen
+ *   logits alone).
+ * A NaN logit counts as -inf. Experts whose logit is -inf or whose ranking value is -inf or NaN are chosen after all others,
+ * lowest id first, with weight 0. Scores and their sums are fp64: of two experts the better one is chosen also where fp32
+ * scores are equal.
+ *   moe_topk_scored: logits [T, E] of dtype MOE_DTYPE_*, contiguous.
+ *   moe_topk_scored_bwd: dlogits [T, E] of the logits' type from dwts [T, k] fp32 and the call's idx; the bias and the choice
+ *   have no gradient.
+ *   moe_router_scored: moe_router's logits x . wr^T + wr_bias (x [T, d], wr [E, d] bf16, wr_bias [E] fp32 or NULL; logits
+ *   [T, E] fp32 out), then moe_topk_scored.
+ * Requirements: E <= 1024, groups <= 64, E % groups == 0, k <= min(32, top_groups E / groups); MOE_GROUP_TOP2: groups of 2
+ * experts at least.
+ */
+#define MOE_SCORE_SOFTMAX 0
+#define MOE_SCORE_SIGMOID 1
+#define MOE_GROUP_MAX 0
+#define MOE_GROUP_TOP2 1
+typedef struct {
+    int32_t E, k, score, groups, top_groups, group_score, norm;
+    float scale;
+    const float* bias;   /* [E] fp32 or NULL */
+} moe_scored_t;
+int moe_topk_scored(const moe_scored_t* r, const void* logits, int dtype, int T, int32_t* idx, float* wts, void* stream);
+int moe_topk_scored_bwd(const moe_scored_t* r, const void* logits, int dtype, int T, const int32_t* idx, const float* dwts,
+                        void* dlogits, void* stream);
+int moe_router_scored(const moe_scored_t* r, const void* x, const void* wr, const float* wr_bias, int T, int d, float* logits,
+                      int32_t* idx, float* wts, void* stream);
+
+/*
+ * MXFP4 operands made on the device, and their products (the reference multiplies MXFP4 weights by 16-bit activations inside
+ * its expert kernels only, metal_mxfp4_moe.py). A matrix of `rows` rows and K columns (K % 32 == 0):
+ *   codes  [rows, K / 2]: an E2M1 code per element, two to a byte, the low half first (the packed words of MOE_FMT_MXFP4);
+ *   scales [ceil(K / 256), rows, 8]: byte b of (s, row) is the E8M0 exponent of columns 256 s + 32 b .. + 31, 127 past K.
+ * value = e2m1(code) 2^(byte - 127); 255 is NaN. `matrices` of them follow each other, codes and scales alike; the scales'
+ * buffer has moe_mx4_scale_bytes(matrices, rows, K) bytes (8 per row and step, and 16 that are read but not used).
+ *   moe_mx4_quantize: x (bf16, fp16 or fp32; ldx elements between rows, = K with several matrices). byte = biased exponent of
+ *       the block's largest magnitude less 2; codes to nearest, ties to even, past 6 to 6; a zero keeps its sign. Blocks below
+ *       2^-124 become zeros of byte 0, blocks with an infinity or NaN codes of 0 and byte 255. (formats.py's rule.)
+ *   moe_mx4_dequantize: the values, to bf16, fp16 or fp32, rounded to nearest (bf16, fp32: exact but below 2^-126).
+ *   moe_mx4_linear: y = act(x w^T + bias) + residual with w [N, K] in that form, and x either 16-bit rows [T, K] (ldx; then xc
+ *       and xs receive its form, or are NULL) or, x NULL, its form xc, xs. bias [N], residual and z [T, N] of `dtype`, bf16 or
+ *       fp16 (x's type); y of dtype or MOE_DTYPE_F32; act, z, workspace as moe_linear.
+ *   moe_mx4_grouped_mm: moe_grouped_mm on w [E, N, K] and x [x_rows, K] in that form (x alike: 16-bit rows, or its form).
+ * Products of codes and powers of two are exact, their sums fp32; bias, activation and residual fp32, rounded once.
+ * Requirements: K % 32 == 0, N % 8 == 0, K, N <= 2^20, rows <= 0x7fffff00, ldx % 8 == 0 and <= 2^21, E <= 1024; pointers 16-byte
+ * aligned; x_rows K / 2 <= 0xB0000000 with an index list.
+ */
+size_t moe_mx4_scale_bytes(int64_t matrices, int64_t rows, int K);
+int moe_mx4_quantize(const void* x, int64_t ldx, int64_t matrices, int64_t rows, int K, int dtype, void* codes, void* scales,
+                     void* stream);
+int moe_mx4_dequantize(const void* codes, const void* scales, int64_t matrices, int64_t rows, int K, void* out, int dtype,
+                       void* stream);
+size_t moe_mx4_linear_workspace_bytes(int64_t T, int N, int K);
+int moe_mx4_linear(const void* x, int64_t ldx, void* xc, void* xs, const void* wc, const void* ws, const void* bias,
+                   const void* residual, int act, int64_t T, int N, int K, int dtype, void* y, int y_dtype, void* z,
+                   void* workspace, size_t workspace_bytes, void* stream);
+size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int K, int indexed);
+int moe_mx4_grouped_mm(const void* x, int64_t ldx, void* xc, void* xs, int64_t x_rows, const void* wc, const void* ws,
+                       const void* bias, const int32_t* offsets, const int32_t* rows, int64_t M, int E, int N, int K, int dtype,
+                       void* y, int y_dtype, int fill, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Library version and build target, for logs. */
 const char* moe_version(void);
 

@@ -30,7 +30,9 @@ EXPORTS = ("moe_router", "moe_router_counter_count", "moe_topk", "moe_group", "m
            "moe_linear", "moe_linear_workspace_bytes", "moe_linear_dx",
            "moe_linear_dx_workspace_bytes", "moe_linear_dw", "moe_linear_dw_workspace_bytes", "moe_linear_act_bwd",
            "moe_act8_pack", "moe_act8_unpack", "moe_glu_fwd", "moe_glu_bwd", "moe_mlp_fwd", "moe_mlp_bwd", "moe_mlp_keep_bytes",
-           "moe_mlp_fwd_workspace_bytes", "moe_mlp_bwd_workspace_bytes")
+           "moe_mlp_fwd_workspace_bytes", "moe_mlp_bwd_workspace_bytes", "moe_topk_scored", "moe_topk_scored_bwd",
+           "moe_router_scored", "moe_mx4_scale_bytes", "moe_mx4_quantize", "moe_mx4_dequantize", "moe_mx4_linear_workspace_bytes",
+           "moe_mx4_linear", "moe_mx4_grouped_mm_workspace_bytes", "moe_mx4_grouped_mm")
 PROBE_SINK = 1024   # MOE_PROBE_SINK
 STATIC_SCRATCH_BYTES = 32 << 20   # MOE_STATIC_SCRATCH_BYTES: the workspace array of moe_experts_run_static
 STAGE_GATE_UP, STAGE_DOWN, STAGE_ALL = 1, 2, 3
@@ -62,6 +64,12 @@ class Experts(ctypes.Structure):
 class Mlp(ctypes.Structure):
     _fields_ = [("E", ctypes.c_int32), ("d", ctypes.c_int32), ("F", ctypes.c_int32), ("act", ctypes.c_int32),
                 ("dtype", ctypes.c_int32), ("w_gate_up", ctypes.c_void_p), ("w_down", ctypes.c_void_p)]
+
+
+class Scored(ctypes.Structure):
+    _fields_ = [("E", ctypes.c_int32), ("k", ctypes.c_int32), ("score", ctypes.c_int32), ("groups", ctypes.c_int32),
+                ("top_groups", ctypes.c_int32), ("group_score", ctypes.c_int32), ("norm", ctypes.c_int32),
+                ("scale", ctypes.c_float), ("bias", ctypes.c_void_p)]
 
 
 _lib = None
@@ -115,6 +123,19 @@ def lib():
         for n in ("moe_mlp_keep_bytes", "moe_mlp_fwd_workspace_bytes", "moe_mlp_bwd_workspace_bytes"):
             getattr(L, n).argtypes = [mlp, i, i]
             getattr(L, n).restype = sz
+        scored = ctypes.POINTER(Scored)
+        L.moe_topk_scored.argtypes = [scored, vp, i, i, vp, vp, vp]
+        L.moe_topk_scored_bwd.argtypes = [scored, vp, i, i, vp, vp, vp, vp]
+        L.moe_router_scored.argtypes = [scored, vp, vp, vp, i, i, vp, vp, vp, vp]
+        L.moe_mx4_scale_bytes.argtypes = [i64, i64, i]
+        L.moe_mx4_quantize.argtypes = [vp, i64, i64, i64, i, i, vp, vp, vp]
+        L.moe_mx4_dequantize.argtypes = [vp, vp, i64, i64, i, vp, i, vp]
+        L.moe_mx4_linear_workspace_bytes.argtypes = [i64, i, i]
+        L.moe_mx4_linear.argtypes = [vp, i64, vp, vp, vp, vp, vp, vp, i, i64, i, i, i, vp, i, vp, vp, sz, vp]
+        L.moe_mx4_grouped_mm_workspace_bytes.argtypes = [i64, i64, i, i]
+        L.moe_mx4_grouped_mm.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, vp, vp, i64, i, i, i, i, vp, i, i, vp, sz, vp]
+        for n in ("moe_mx4_scale_bytes", "moe_mx4_linear_workspace_bytes", "moe_mx4_grouped_mm_workspace_bytes"):
+            getattr(L, n).restype = sz
         L.moe_row_bytes.argtypes = [i, i]
         L.moe_row_bytes.restype = sz
         L.moe_tile_bytes.argtypes = [i, i, i]
@@ -132,7 +153,8 @@ def lib():
                   "moe_layer_run", "moe_experts_run_shared", "moe_router_group", "moe_layer_run_shared",
                   "moe_probe_read", "moe_grouped_mm", "moe_grouped_mm_dx", "moe_grouped_mm_dw", "moe_linear",
                   "moe_linear_dx", "moe_linear_dw", "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack", "moe_glu_fwd",
-                  "moe_glu_bwd", "moe_mlp_fwd", "moe_mlp_bwd"):
+                  "moe_glu_bwd", "moe_mlp_fwd", "moe_mlp_bwd", "moe_topk_scored", "moe_topk_scored_bwd", "moe_router_scored",
+                  "moe_mx4_quantize", "moe_mx4_dequantize", "moe_mx4_linear", "moe_mx4_grouped_mm"):
             getattr(L, n).restype = ctypes.c_int
         _lib = L
     return _lib

@@ -27,6 +27,9 @@ static int launch(const MmArgs& a, hipStream_t st) {
         default: return launch_mm_rows(a, st);
     }
 }
-int launch_mm_fwd(const MmArgs& a, hipStream_t st) { return a.f16 ? launch<true>(a, st) : launch<false>(a, st); }
+int launch_mm_fwd(const MmArgs& a, hipStream_t st) {
+    if (a.sa) return launch_mm_mx4(a, st);
+    return a.f16 ? launch<true>(a, st) : launch<false>(a, st);
+}
 
 }  // namespace moe

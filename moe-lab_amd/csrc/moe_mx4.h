@@ -1,0 +1,35 @@
+// MXFP4 operands made on the device: E2M1 codes, two to a byte, the low half first, with an E8M0 byte per 32 neighbours.
+// A matrix of `rows` rows and K columns is codes [rows, K / 2] and scales [steps, rows, 8], steps = ceil(K / 256): byte b of
+// (s, row) belongs to the columns 256 s + 32 b ... The products take a step of all rows of a tile at a time, so those bytes lie
+// together (in rows of their own, K / 32 bytes each, a tile's step would be a hundred lines for 8 bytes of each).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "moe_mm.h"
+
+namespace moe {
+
+struct Mx4 {
+    uint8_t* codes;
+    uint8_t* scales;
+};
+// Bytes of a matrix's scales. Reads of 16 bytes may start at any row, so 8 more lie behind the last one (16: whole pieces).
+inline int64_t mx4_steps(int64_t K) { return (K + 255) / 256; }
+inline size_t mx4_scale_bytes(int64_t rows, int64_t K) { return (size_t)(mx4_steps(K) * rows * 8 + 16); }
+
+// x: G matrices of `rows` rows each, ld elements between rows (G > 1: contiguous)
+int launch_mx4_quantize(const void* x, int64_t ld, int64_t G, int64_t rows, int64_t K, int dtype, Mx4 out, hipStream_t st);
+int launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t G, int64_t rows, int64_t K, int dtype, void* out,
+                          hipStream_t st);
+// scales of the rows idx[0 .. M) of a matrix with n rows, in their order (an index outside it: any finite scale)
+int launch_mx4_take_scales(const uint8_t* scales, int64_t n, int64_t K, const int32_t* idx, int64_t M, uint8_t* out, hipStream_t st);
+// Products of few rows per group. x16 not null: a.a's rows are 16-bit numbers of the result's type there (ldx elements between
+// them), quantised by every workgroup for itself; else a.a, a.sa (not gathered: row arows[p]).
+int launch_mx4_rows(const MmArgs& a, const void* x16, int64_t ldx, hipStream_t st);
+constexpr int MX4_ROWS = 16;      // rows of a group that one pass multiplies
+inline bool mx4_few(const MmArgs& a) { return a.offsets ? a.M / (a.E < a.M ? a.E : a.M) <= 1 : a.M <= MX4_ROWS; }
+constexpr int MX4_FUSE = 4;       // rows that are quantised inside the product
+constexpr int64_t MX4_FUSE_K = 1 << 16;   // and their elements in all, at most (LDS)
+
+}  // namespace moe

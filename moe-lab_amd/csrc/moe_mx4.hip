@@ -1,0 +1,314 @@
+// MXFP4 quantisation and its inverse, and products of few rows.
+#include "moe_mx4.h"
+
+namespace moe {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t max4(uint32_t v) {   // over the 4 lanes of 8 values that make a block of 32
+    v = dpp_umax<0xB1>(v);
+    return dpp_umax<0x4E>(v);
+}
+// The block's exponent byte from the bits of its largest magnitude (fp32): that of the largest power of two in it, less 2, so that
+// the largest lies in [4, 8) of E2M1's 6. Below 2^-124 (a byte of 0) the block is zeros; 255: it holds an infinity or NaN.
+__device__ __forceinline__ uint32_t exponent4(uint32_t top) {
+    const uint32_t e = top >> 23;
+    return e == 255 ? 255 : e > 2 ? e - 2 : 0;
+}
+// Eight values of type DT as a lane holds them: u32x4 of 16-bit pairs, or two f32x4.
+template <int DT>
+struct Eight {
+    u32x4 w[DT == MOE_DTYPE_F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const char* p) {
+#pragma unroll
+        for (int i = 0; i < (DT == MOE_DTYPE_F32 ? 2 : 1); ++i) w[i] = ((const u32x4*)p)[i];
+    }
+    __device__ __forceinline__ uint32_t top() const {   // bits of the largest magnitude in fp32
+        uint32_t m = 0;
+        if constexpr (DT == MOE_DTYPE_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, w[i >> 2][i & 3] & 0x7fffffffu);
+            return m;
+        } else {
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 p = {0, 0};   // magnitudes of 16-bit floats compare as integers
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p = __builtin_elementwise_max(p, __builtin_bit_cast(u16x2, w[0][i] & 0x7fff7fffu));
+            const uint32_t h = max((uint32_t)p[0], (uint32_t)p[1]);
+            return DT == MOE_DTYPE_BF16 ? h << 16 : __float_as_uint(un16<true>(h));
+        }
+    }
+    // Their codes at the scale of byte e in [1, 254]. The instruction rounds to nearest, ties to even, and saturates.
+    __device__ __forceinline__ uint32_t codes(uint32_t e) const {
+        const float s = __uint_as_float(e << 23);
+        uint32_t q = 0;
+        if constexpr (DT == MOE_DTYPE_F32) {
+            const auto f = [&](int i) { return __uint_as_float(w[i >> 2][i & 3]); };
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f(0), f(1), s, 0);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f(2), f(3), s, 1);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f(4), f(5), s, 2);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f(6), f(7), s, 3);
+        } else if constexpr (DT == MOE_DTYPE_BF16) {
+            const auto f = [&](int i) { return __builtin_bit_cast(moe_bf16x2, (uint32_t)w[0][i]); };
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, f(0), s, 0);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, f(1), s, 1);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, f(2), s, 2);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, f(3), s, 3);
+        } else {
+            const auto f = [&](int i) { return __builtin_bit_cast(moe_f16x2, (uint32_t)w[0][i]); };
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, f(0), s, 0);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, f(1), s, 1);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, f(2), s, 2);
+            q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, f(3), s, 3);
+        }
+        return q;
+    }
+};
+
+// Bytes of the values in memory.
+__host__ __device__ constexpr int size_of(int dt) { return dt == MOE_DTYPE_F32 ? 4 : 2; }
+
+// One item: 8 columns of a row, its 4-lane neighbours the rest of its block. The lane with a row's last block also writes the
+// bytes that fill its last step (1.0: they meet codes of zero in the products).
+template <int DT>
+__global__ void __launch_bounds__(256) k_mx4_quantize(const char* x, int64_t ld, uint32_t items, uint32_t per_row, uint32_t row0,
+                                                      uint32_t rows, int64_t scale_stride, uint8_t* codes, uint8_t* scales) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= items) return;   // items % 4 == 0: a block's four lanes leave together
+    const uint32_t r = i / per_row, c = i - r * per_row;
+    const uint32_t row = row0 + r, g = row / rows, n = row - g * rows;
+    Eight<DT> v;
+    v.load(x + ((int64_t)row * ld + c * 8) * size_of(DT));
+    const uint32_t e = exponent4(max4(v.top()));
+    const uint32_t q = v.codes(e - 1 < 254 ? e : 127);
+    *(uint32_t*)(codes + ((int64_t)row * per_row + c) * 4) = e - 1 < 254 ? q : 0;
+    if ((c & 3) == 0) {
+        const uint32_t b = c >> 2;
+        uint8_t* s = scales + g * scale_stride + ((int64_t)(b >> 3) * rows + n) * 8;
+        s[b & 7] = (uint8_t)e;
+        if (c + 4 == per_row)
+            for (uint32_t p = (b & 7) + 1; p < 8; ++p) s[p] = 127;
+    }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, uint32_t items,
+                                                        uint32_t per_row, uint32_t row0, uint32_t rows, int64_t scale_stride,
+                                                        char* out) {
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= items) return;
+    const uint32_t r = i / per_row, c = i - r * per_row;
+    const uint32_t row = row0 + r, g = row / rows, n = row - g * rows, b = c >> 2;
+    const uint32_t e = scales[g * scale_stride + ((int64_t)(b >> 3) * rows + n) * 8 + (b & 7)];
+    const int64_t at = (int64_t)row * per_row + c;
+    const uint32_t q = *(const uint32_t*)(codes + at * 4);
+    // codes as fp32 (exact), then the power of two: 2^-127 is subnormal, and 255 stands for NaN
+    const float s = e == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(1.f, (int)e - 127);
+    f32x2 v[4];
+    v[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 0);
+    v[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 1);
+    v[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 2);
+    v[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, 1.f, 3);
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = v[j >> 1][j & 1] * s;
+    if constexpr (DT == MOE_DTYPE_F32) {
+        ((f32x4*)out)[2 * at] = (f32x4){f[0], f[1], f[2], f[3]};
+        ((f32x4*)out)[2 * at + 1] = (f32x4){f[4], f[5], f[6], f[7]};
+    } else {
+        constexpr bool H = DT == MOE_DTYPE_F16;
+        ((u32x4*)out)[at] = (u32x4){pack16<H>(f[0], f[1]), pack16<H>(f[2], f[3]), pack16<H>(f[4], f[5]), pack16<H>(f[6], f[7])};
+    }
+}
+
+__global__ void __launch_bounds__(256) k_mx4_take_scales(const uint8_t* scales, uint32_t n, const int32_t* idx, uint32_t M,
+                                                         uint8_t* out) {
+    const uint32_t p = blockIdx.x * 256 + threadIdx.x, s = blockIdx.y;
+    if (p >= M) return;
+    const int32_t r = idx[p];
+    const uint64_t ones = 0x7f7f7f7f7f7f7f7full;
+    ((uint64_t*)out)[(int64_t)s * M + p] = (uint32_t)r < n ? ((const uint64_t*)scales)[(int64_t)s * n + r] : ones;
+}
+
+// Rows that a launch takes: its items are counted in 32 bits.
+static int64_t rows_at_once(int64_t rows, int64_t per_row) {
+    const int64_t fit = ((int64_t)1 << 31) / per_row;
+    return rows < fit ? rows : fit;
+}
+
+int launch_mx4_quantize(const void* x, int64_t ld, int64_t G, int64_t rows, int64_t K, int dtype, Mx4 out, hipStream_t st) {
+    const int64_t all = G * rows, per_row = K / 8, step = rows_at_once(all, per_row), stride = (int64_t)mx4_steps(K) * rows * 8;
+    for (int64_t r = 0; r < all; r += step) {
+        const uint32_t items = (uint32_t)((all - r < step ? all - r : step) * per_row);
+        auto go = [&](auto kernel) {
+            kernel<<<(items + 255) / 256, 256, 0, st>>>((const char*)x, ld, items, (uint32_t)per_row, (uint32_t)r, (uint32_t)rows, stride,
+                                                        out.codes, out.scales);
+        };
+        if (dtype == MOE_DTYPE_F32) go(k_mx4_quantize<MOE_DTYPE_F32>);
+        else if (dtype == MOE_DTYPE_F16) go(k_mx4_quantize<MOE_DTYPE_F16>);
+        else go(k_mx4_quantize<MOE_DTYPE_BF16>);
+        if (hipGetLastError() != hipSuccess) return MOE_ERR_LAUNCH;
+    }
+    return MOE_OK;
+}
+
+int launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t G, int64_t rows, int64_t K, int dtype, void* out,
+                          hipStream_t st) {
+    const int64_t all = G * rows, per_row = K / 8, step = rows_at_once(all, per_row), stride = (int64_t)mx4_steps(K) * rows * 8;
+    for (int64_t r = 0; r < all; r += step) {
+        const uint32_t items = (uint32_t)((all - r < step ? all - r : step) * per_row);
+        auto go = [&](auto kernel) {
+            kernel<<<(items + 255) / 256, 256, 0, st>>>(codes, scales, items, (uint32_t)per_row, (uint32_t)r, (uint32_t)rows, stride,
+                                                        (char*)out);
+        };
+        if (dtype == MOE_DTYPE_F32) go(k_mx4_dequantize<MOE_DTYPE_F32>);
+        else if (dtype == MOE_DTYPE_F16) go(k_mx4_dequantize<MOE_DTYPE_F16>);
+        else go(k_mx4_dequantize<MOE_DTYPE_BF16>);
+        if (hipGetLastError() != hipSuccess) return MOE_ERR_LAUNCH;
+    }
+    return MOE_OK;
+}
+
+int launch_mx4_take_scales(const uint8_t* scales, int64_t n, int64_t K, const int32_t* idx, int64_t M, uint8_t* out,
+                           hipStream_t st) {
+    const dim3 grid((unsigned)((M + 255) / 256), (unsigned)mx4_steps(K));
+    k_mx4_take_scales<<<grid, 256, 0, st>>>(scales, (uint32_t)n, idx, (uint32_t)M, out);
+    return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;
+}
+
+// Few rows: a workgroup multiplies 16 rows of the weights by up to 16 rows of x. Its waves share K, 128 columns at a time, with
+// the weights' codes straight from memory as the matrix instruction's first operand, and their sums meet in LDS, in the waves'
+// order. FUSE: x's rows are quantised here first, while the first weights are on their way.
+// Workgroups go by slot, not by group (as k_mm_rows): the one at a group's first slot does the group.
+constexpr int MXR_WAVES = 8;
+template <bool F16, bool FUSE>
+__global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, const uint16_t* x16, int64_t ldx) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t sx[];   // FUSE: codes [MX4_FUSE, K / 2], scale bytes [MX4_FUSE, K / 32]
+    __shared__ f32x4 sums[MXR_WAVES][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int l = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16, p = blockIdx.y;
+    int e = 0, lo = 0, hi = g.M;
+    if (g.offsets) {
+        e = -1;   // the group whose first slot is p
+        for (int base = 0; base < g.E && e < 0; base += 64) {
+            int a = -1, b = -1;
+            if (base + lane < g.E) group_of<MM_FWD>(g, base + lane, a, b);
+            const uint64_t hit = __ballot(a == p && b > a);
+            if (hit) {
+                e = base + __builtin_ctzll(hit);
+                group_of<MM_FWD>(g, e, lo, hi);
+            }
+        }
+        if (e < 0) {
+            if (!g.fill) return;
+            int a, b;
+            group_of<MM_FWD>(g, g.E - 1, a, b);
+            if (p < b) return;
+            if (threadIdx.x < 16 && n0 + threadIdx.x < g.J) {
+                const int64_t at = (int64_t)p * g.J + n0 + threadIdx.x;
+                if (g.ydt == MOE_DTYPE_F32) ((float*)g.y)[at] = 0.f;
+                else ((uint16_t*)g.y)[at] = 0;
+            }
+            return;
+        }
+    }
+    const int K = g.R * 4, KB = K / 2, steps = (g.R + 63) / 64, chunks = (K + 127) / 128;
+    const int n = min(n0 + l, g.J - 1);   // rows past the last: multiplied, not stored
+    const uint8_t* wc = (const uint8_t*)g.b + ((int64_t)e * g.J + n) * KB + q * 16;
+    const uint8_t* ws = g.sb + ((int64_t)e * steps * g.J + n) * 8;
+    constexpr int AHEAD = 4;   // chunks of a wave whose weights are loaded together
+    s16x8 w[AHEAD];
+    uint32_t we[AHEAD];
+    const s16x8 zero = {};
+    auto load_w = [&](int c0) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int c = c0 + u * MXR_WAVES;
+            const bool in = c * 128 + q * 32 < K;
+            w[u] = in ? *(const s16x8*)(wc + (int64_t)c * 64) : zero;
+            we[u] = in ? *(const uint32_t*)(ws + (int64_t)(c >> 1) * g.J * 8 + (c & 1) * 4) >> (8 * q) : 127;
+        }
+    };
+    load_w(wave);
+    for (int m0 = lo; m0 < hi; m0 += FUSE ? MX4_FUSE : MX4_ROWS) {
+        const int rows = min(hi - m0, FUSE ? MX4_FUSE : MX4_ROWS);
+        int src = -1;   // this lane's row of x
+        if (l < rows) {
+            src = g.arows ? g.arows[m0 + l] : m0 + l;
+            if ((uint32_t)src >= (uint32_t)g.a_n) src = -1;
+        }
+        if constexpr (FUSE) {
+            if (m0 > lo) __syncthreads();   // the last rows are multiplied
+            const int per_row = K / 8;
+            for (int i = threadIdx.x; i < rows * per_row; i += 64 * MXR_WAVES) {   // a block's four lanes together: K % 32 == 0
+                const int r = i / per_row, c = i - r * per_row;
+                int s = g.arows ? g.arows[m0 + r] : m0 + r;
+                Eight<F16 ? MOE_DTYPE_F16 : MOE_DTYPE_BF16> v;
+                const bool live = (uint32_t)s < (uint32_t)g.a_n;
+                v.load((const char*)(x16 + (live ? s : 0) * ldx + c * 8));
+                const uint32_t ex = exponent4(max4(v.top()));
+                const uint32_t code = v.codes(ex - 1 < 254 ? ex : 127);
+                *(uint32_t*)(sx + (r * per_row + c) * 4) = live && ex - 1 < 254 ? code : 0;
+                if ((c & 3) == 0) sx[MX4_FUSE * KB + r * (K / 32) + (c >> 2)] = live ? (uint8_t)ex : 127;
+            }
+            __syncthreads();
+        }
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int c0 = wave; c0 < chunks; c0 += AHEAD * MXR_WAVES) {
+            if (c0 != wave || m0 > lo) load_w(c0);
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const int c = c0 + u * MXR_WAVES;
+                if (c >= chunks) break;
+                s16x8 x = zero;
+                uint32_t xe = 127;
+                if (src >= 0 && c * 128 + q * 32 < K) {
+                    if constexpr (FUSE) {
+                        x = *(const s16x8*)(sx + l * KB + c * 64 + q * 16);
+                        xe = sx[MX4_FUSE * KB + l * (K / 32) + c * 4 + q];
+                    } else {
+                        x = *(const s16x8*)((const uint8_t*)g.a + (int64_t)src * KB + c * 64 + q * 16);
+                        xe = g.sa[((int64_t)(c >> 1) * g.a_n + src) * 8 + (c & 1) * 4 + q];
+                    }
+                }
+                acc = mma4(w[u], we[u], x, xe, acc);
+            }
+        }
+        sums[wave][lane] = acc;
+        __syncthreads();
+        if (wave == 0) {
+            acc = sums[0][lane];
+#pragma unroll
+            for (int i = 1; i < MXR_WAVES; ++i) acc += sums[i][lane];
+            const int j = n0 + 4 * q;   // four neighbours of J (a multiple of 8)
+            if (l < rows && j < g.J) {
+                const int64_t at = (int64_t)(m0 + l) * g.J + j;
+                if (g.epi.bias) acc += load4<F16>(g.epi.bias, (int64_t)e * g.J + j);
+                if (g.epi.z) *(u32x2*)((uint16_t*)g.epi.z + at) = (u32x2){pack16<F16>(acc[0], acc[1]), pack16<F16>(acc[2], acc[3])};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] = lin_act(g.epi.act, acc[i]);
+                if (g.epi.residual) acc += load4<F16>(g.epi.residual, at);
+                if (g.ydt == MOE_DTYPE_F32) *(f32x4*)((float*)g.y + at) = acc;
+                else *(u32x2*)((uint16_t*)g.y + at) = (u32x2){pack16<F16>(acc[0], acc[1]), pack16<F16>(acc[2], acc[3])};
+            }
+        }
+        __syncthreads();   // the sums are read
+    }
+}
+
+int launch_mx4_rows(const MmArgs& a, const void* x16, int64_t ldx, hipStream_t st) {
+    const dim3 grid((unsigned)((a.J + 15) / 16), a.offsets ? (unsigned)a.M : 1);
+    const size_t lds = x16 ? (size_t)MX4_FUSE * a.R * 4 * 17 / 32 : 0;
+    auto go = [&](auto kernel) { kernel<<<grid, 64 * MXR_WAVES, lds, st>>>(a, (const uint16_t*)x16, ldx); };
+    if (x16) {
+        if (a.f16) go(k_mx4_rows<true, true>);
+        else go(k_mx4_rows<false, true>);
+    } else {
+        if (a.f16) go(k_mx4_rows<true, false>);
+        else go(k_mx4_rows<false, false>);
+    }
+    return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;
+}
+
+}  // namespace moe

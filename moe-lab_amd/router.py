@@ -6,13 +6,21 @@ Mirrors reference moelab/router.py (semantics :1-12, ``topk_norm`` :71-80):
   * ties: the lowest expert id wins; NaN logits count as -inf; with fewer than k finite logits the
     remaining slots take the lowest unused ids with weight 0;
   * E <= 1024, k <= min(E, 32).
+``topk_scored`` and ``route_scored`` are the routers that the reference leaves to the stock gate (reference e2e.py:129-150):
+softmax or sigmoid scores, a bias that only ranks, groups of experts of which the best few are kept, and a gradient.
 ``route`` adds what the reference leaves to the stock gate GEMV (reference e2e.py:57-59): the logits
 x . Wr^T (+ bias) are computed in the same kernel, in fp32, in one fixed reduction order, so a CPU
 restatement reproduces them bit for bit and the chosen ids are exact.
 """
+import math
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
+
+_SCORES = {"softmax": 0, "sigmoid": 1}   # MOE_SCORE_*
+_GROUP_SCORES = {"max": 0, "top2": 1}    # MOE_GROUP_*
 
 
 def topk_norm(logits, k, norm=True, scale=1.0):
@@ -103,3 +111,109 @@ def group(idx, E):
                               _lib.ptr(active), _lib.ptr(meta), _lib.stream_of(dev))
     _lib.check("moe_group", rc)
     return counts, offsets, srt[:n], active, meta
+
+
+def _scored(E, k, score, bias, groups, top_groups, group_score, norm, scale, device):
+    """The call's descriptor, its arguments checked, and the bias that it points to."""
+    if score not in _SCORES or group_score not in _GROUP_SCORES:
+        raise ValueError(f"score {score!r}, group_score {group_score!r}: one of {list(_SCORES)}, one of {list(_GROUP_SCORES)} expected")
+    if not 1 <= E <= 1024 or not 1 <= groups <= 64 or E % groups or not 1 <= top_groups <= groups:
+        raise ValueError(f"{E} experts in {groups} groups, {top_groups} kept: at most 1024 in at most 64 equal groups expected")
+    if groups > 1 and group_score == "top2" and E < 2 * groups:
+        raise ValueError("group_score 'top2': groups of two experts at least expected")
+    if not 1 <= k <= min(32, top_groups * (E // groups)):
+        raise ValueError(f"k = {k}: 1 to {min(32, top_groups * (E // groups))} expected (32, or the experts in the kept groups)")
+    if not math.isfinite(scale):
+        raise ValueError(f"scale {scale}: a finite number expected")
+    if bias is not None:
+        if bias.dtype not in _lib.DTYPE or tuple(bias.shape) != (E,) or bias.device != device:
+            raise ValueError(f"bias {bias.dtype} {tuple(bias.shape)} on {bias.device}: floating [{E}] on {device} expected")
+        bias = _lib.dense(bias.detach(), torch.float32)
+    return _lib.Scored(E, k, _SCORES[score], groups, top_groups, _GROUP_SCORES[group_score], int(bool(norm)), float(scale),
+                       _lib.ptr(bias)), bias
+
+
+def _topk_scored(lg, desc):
+    T = lg.shape[0]
+    idx = torch.empty((T, desc.k), dtype=torch.int32, device=lg.device)
+    wts = torch.empty((T, desc.k), dtype=torch.float32, device=lg.device)
+    _lib.call("moe_topk_scored", lg.device, desc, lg.data_ptr(), _lib.DTYPE[lg.dtype], T, idx.data_ptr(), wts.data_ptr())
+    return idx, wts
+
+
+class _TopkScored(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, settings):
+        desc, bias = _scored(logits.shape[1], *settings[:2], bias, *settings[2:], logits.device)
+        lg = _lib.dense(logits)
+        idx, wts = _topk_scored(lg, desc)
+        ctx.save_for_backward(logits if lg is logits else lg, bias, idx)
+        ctx.settings = settings
+        ctx.mark_non_differentiable(idx)
+        ctx.set_materialize_grads(False)
+        return idx, wts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _, dwts):
+        if dwts is None:
+            return None, None, None
+        logits, bias, idx = ctx.saved_tensors
+        lg = _lib.dense(logits)
+        desc, bias = _scored(lg.shape[1], *ctx.settings[:2], bias, *ctx.settings[2:], lg.device)
+        dw = _lib.dense(dwts, torch.float32)
+        dl = torch.empty_like(lg)
+        _lib.call("moe_topk_scored_bwd", lg.device, desc, lg.data_ptr(), _lib.DTYPE[lg.dtype], lg.shape[0], idx.data_ptr(),
+                  dw.data_ptr(), dl.data_ptr())
+        return dl, None, None
+
+
+def topk_scored(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_score="max", norm=True, scale=1.0):
+    """logits [..., E] (fp32, bf16 or fp16) -> (idx [T, k] int32, wts [T, k] fp32); differentiable: wts in logits.
+    score: "softmax" or "sigmoid" of the logits. bias [E]: added to the scores for ranking only (without one the logits rank).
+    groups: experts E / groups * g .. form group g; only the top_groups groups of largest value stay, a group's value being its
+    largest ranking value (group_score "max") or the sum of its two largest ("top2"). idx: the k experts that rank highest, best
+    first, of equals the lowest id. wts: scale * score, with norm divided by the k scores' sum (0 where that is 0).
+    NaN logits count as -inf; experts at -inf are chosen last, with weight 0 and no gradient. E <= 1024, groups <= 64, k <= 32.
+    Scores are ranked in fp64. The bias and the choice have no gradient."""
+    _lib.require_device(logits, "logits")
+    if logits.dim() < 1:
+        raise ValueError("logits [..., E] expected")
+    if logits.dtype not in _lib.DTYPE:
+        raise TypeError(f"logits are {logits.dtype}: fp32, bf16 or fp16 expected")
+    lg = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
+    settings = (k, score, groups, top_groups, group_score, norm, scale)
+    if _lib.wants_grad(logits):
+        return _TopkScored.apply(lg, bias, settings)
+    desc, bias = _scored(lg.shape[1], k, score, bias, groups, top_groups, group_score, norm, scale, lg.device)
+    return _topk_scored(_lib.dense(lg), desc)
+
+
+def route_scored(x, wr, k, wr_bias=None, score="softmax", bias=None, groups=1, top_groups=1, group_score="max", norm=True,
+                 scale=1.0, return_logits=False):
+    """topk_scored on the logits x . wr^T (+ wr_bias), which are route's: fp32, in one fixed order. x [T, d] bf16, wr [E, d]
+    bf16, wr_bias [E] (any float) or None, the other arguments as topk_scored's. Returns (idx, wts[, logits [T, E] fp32]).
+    No gradient: for training, topk_scored on logits of linear.linear(x, wr, out_dtype=torch.float32)."""
+    _lib.require_device(x, "x")
+    if x.dim() != 2 or wr.dim() != 2 or x.shape[1] != wr.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} and wr {tuple(wr.shape)}: [T, d] and [E, d] expected")
+    if x.dtype != torch.bfloat16 or wr.dtype != torch.bfloat16:
+        raise TypeError(f"x {x.dtype} and wr {wr.dtype}: bf16 expected")
+    if wr.device != x.device:
+        raise ValueError(f"wr is on {wr.device}, x on {x.device}")
+    if _lib.wants_grad(x, wr, wr_bias):
+        raise NotImplementedError("route_scored has no gradient: topk_scored on linear.linear's logits has one")
+    (T, d), E = x.shape, wr.shape[0]
+    _lib.multiple_of(d, 8, "d")
+    desc, bias = _scored(E, k, score, bias, groups, top_groups, group_score, norm, scale, x.device)
+    x, wr = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format) for t in (x, wr))
+    if wr_bias is not None:
+        if wr_bias.dtype not in _lib.DTYPE or tuple(wr_bias.shape) != (E,) or wr_bias.device != x.device:
+            raise ValueError(f"wr_bias {wr_bias.dtype} {tuple(wr_bias.shape)} on {wr_bias.device}: floating [{E}] on {x.device} expected")
+        wr_bias = _lib.dense(wr_bias, torch.float32)
+    logits = torch.empty((T, E), dtype=torch.float32, device=x.device)
+    idx = torch.empty((T, k), dtype=torch.int32, device=x.device)
+    wts = torch.empty((T, k), dtype=torch.float32, device=x.device)
+    _lib.call("moe_router_scored", x.device, desc, x.data_ptr(), wr.data_ptr(), _lib.ptr(wr_bias), T, d, logits.data_ptr(),
+              idx.data_ptr(), wts.data_ptr())
+    return (idx, wts, logits) if return_logits else (idx, wts)
