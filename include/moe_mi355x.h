@@ -451,7 +451,8 @@ int moe_router_scored(const moe_scored_t* r, const void* x, const void* wr, cons
  * MXFP4 operands made on the device, and their products (the reference multiplies MXFP4 weights by 16-bit activations inside
  * its expert kernels only, metal_mxfp4_moe.py). A matrix of `rows` rows and K columns (K % 32 == 0):
  *   codes  [rows, K / 2]: an E2M1 code per element, two to a byte, the low half first (the packed words of MOE_FMT_MXFP4);
- *   scales [ceil(K / 256), rows, 8]: byte b of (s, row) is the E8M0 exponent of columns 256 s + 32 b .. + 31, 127 past K.
+ *   scales [ceil(K / 256), rows, 8]: byte 4 (b % 2) + b / 2 of (s, row) is the E8M0 exponent of columns 256 s + 32 b .. + 31, 127
+ *   past K.
  * value = e2m1(code) 2^(byte - 127); 255 is NaN. `matrices` of them follow each other, codes and scales alike; the scales'
  * buffer has moe_mx4_scale_bytes(matrices, rows, K) bytes (8 per row and step, and 16 that are read but not used).
  *   moe_mx4_quantize: x (bf16, fp16 or fp32; ldx elements between rows, = K with several matrices). byte = biased exponent of

@@ -42,17 +42,6 @@ __device__ __forceinline__ float un16(uint32_t h) {   // the low half
     return __uint_as_float(h << 16);
 }
 
-// Both operands MXFP4: 32 codes of a lane times its E8M0 scale (byte 0 of s), 128 of r in one instruction of the same 16 cycles.
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ f32x4 mma4(s16x8 a, uint32_t sa, s16x8 b, uint32_t sb, f32x4 c) {
-    typedef int i32x4 __attribute__((ext_vector_type(4)));
-    const auto wide = [](s16x8 v) {   // the upper half is not read
-        const i32x4 w = __builtin_bit_cast(i32x4, v);
-        return __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
-    };
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a), wide(b), c, 4, 4, 0, (int)sa, 0, (int)sb);
-}
-
 // Buffer descriptor of `bytes` from p on; loads past the end deliver zeros. Offsets from MM_OOB on are always past it.
 #define MM_OOB 0xC0000000u
 __device__ __forceinline__ srd_t srd_of(const char* p, uint32_t bytes) {
@@ -189,8 +178,8 @@ struct MmArgs {
     int touch;               // dw: read the operands through once at the start (set by the launcher)
     int f16, ydt, fill;      // ydt: MOE_DTYPE_*; fill: rows behind the last group are set to zero
     MmEpi epi;
-    // MXFP4 operands (forward): a and b are codes, their sizes along r counted in 16-bit words of four, and these the exponents,
-    // 8 bytes per row and step of 64 words: a's [steps, M, 8] in slot order, b's [E, steps, rows of b, 8]; else null.
+    // MXFP4 operands (forward, moe_mx4.h): a and b are codes, their sizes along r counted in 16-bit words of four, and these the
+    // exponents: a's in slot order, b's of E matrices; else null.
     const uint8_t* sa;
     const uint8_t* sb;
 };
@@ -340,10 +329,7 @@ __device__ __forceinline__ f32x4 load4(const void* p, int64_t i) {
 // GATHER: operands that are read through index lists, bit 0: a, bit 1 (dw): b. Such an operand is addressed with 32 bits from its
 // start; one in slot order from its group's first slot, in 64 bits, so that its own size has no bound (one flag for both made
 // weight gradients of slot-ordered rows past 4 GiB wrong).
-// MX: both operands are MXFP4. A step's 64 words hold 256 of r, and a fragment the 32 codes that one lane of the block-scaled
-// instruction takes, so the tiles, loads and fragments are those of 16-bit operands; only each fragment's scale byte comes with
-// it. The scales of a step lie together (moe_mx4_quantize), so that a tile's arrive as 1 KiB pieces, one to each loading wave.
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int GATHER, int EPI, bool LDS_OUT, int NL, bool MX>
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int GATHER, int EPI, bool LDS_OUT, int NL>
 struct MmKernel {
     static constexpr bool GLU = EPI == EPI_GLU;
     static constexpr bool AX = MODE == MM_DW, BX = MODE != MM_FWD;   // operand with its own index contiguous
@@ -353,10 +339,7 @@ struct MmKernel {
     using A = Operand<AX, BI, NW>;
     using B = Operand<BX, BJ, NW>;
     static constexpr int PA = A::PIECES, PB = B::PIECES;
-    static_assert(!MX || (MODE == MM_FWD && !GLU), "");
-    static constexpr int SCA = MX ? (BI * 8 + 1023) / 1024 : 0, SCB = MX ? (BJ * 8 + 1023) / 1024 : 0;   // pieces of scales
-    static_assert(SCA + SCB <= NW, "one to a wave");
-    static constexpr int STAGE = A::BYTES + B::BYTES + (SCA + SCB) * 1024;
+    static constexpr int STAGE = A::BYTES + B::BYTES;
     static constexpr bool LINES = MODE == MM_DW && LDS_OUT;
 
     // Stores (and the loads of bias and residual) go through buffer descriptors: lanes and columns past the tile's valid ones
@@ -548,7 +531,7 @@ struct MmKernel {
     }
 
     static __device__ __forceinline__ void block(const MmArgs& g, char* sm, int* pre) {
-        constexpr int L = PA + PB + (MX ? 1 : 0);
+        constexpr int L = PA + PB;
         constexpr bool DB = MODE == MM_DW;   // also dbias
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave & 1, wj = wave >> 1;
         const int lw = NL ? wave - NWC : wave;   // among the waves that load
@@ -702,21 +685,6 @@ struct MmKernel {
         auto load_b = [&](uint32_t buf, srd_t d, int i) {
             dma16<NB, NW * 1024>(d, offb + i, lds0 + buf + (uint32_t)(A::BYTES + (i * NW + lw) * 1024));
         };
-        // the step's scales: this wave's piece of a's or b's (waves past the last piece load one again)
-        auto load_scales = [&](uint32_t buf) {
-            if constexpr (MX) {
-                const int p = lw % (SCA + SCB), step = ls + (g.part ? lt.e * (g.part / 64) : 0), e = g.part ? 0 : lt.e;
-                const uint8_t* base = g.sa + ((int64_t)step * g.M + lt.lo) * 8;
-                int n = (lt.rows * 8 + 15) / 16 * 16;
-                uint32_t off = (p * 64 + lane) * 16;
-                if (p >= SCA) {
-                    base = g.sb + (((int64_t)e * ((g.R + 63) / 64) + step) * g.J + lt.j0) * 8;
-                    n = (g.J - lt.j0) * 8;
-                    off = ((p - SCA) * 64 + lane) * 16;
-                }
-                dma16<1, 0>(srd_of((const char*)base, lrows ? n : 0), &off, lds0 + buf + A::BYTES + B::BYTES + p * 1024);
-            }
-        };
         auto srd_a = [&]() { return srd_of(pa, bytes_a()); };
         auto srd_b = [&]() { return srd_of(pb, bytes_b()); };
         auto step_loads = [&]() {
@@ -734,23 +702,11 @@ struct MmKernel {
         f32x4 acc[FA][FB];
         float sums[DB ? FA : 1];
         s16x8 ra[2][FA], rb[2][FB];   // fragments of the half step that is multiplied and of the next one
-        uint32_t ea[2][MX ? FA : 1], eb[2][MX ? FB : 1];   // their scales
         auto mul = [&](int set, int f) {
 #pragma unroll
             for (int h = 0; h < FB; ++h) {
-                if constexpr (MX) acc[f][h] = mma4(rb[set][h], eb[set][h], ra[set][f], ea[set][f], acc[f][h]);
-                else acc[f][h] = mma<F16>(rb[set][h], ra[set][f], acc[f][h]);
+                acc[f][h] = mma<F16>(rb[set][h], ra[set][f], acc[f][h]);
             }
-        };
-        // half a step's fragments; of a scale word's four bytes (blocks of 32 codes) a lane takes that of its own block
-        const uint32_t sc = (uint32_t)(A::BYTES + B::BYTES + (lane & 15) * 8), sh = (uint32_t)(lane >> 4) * 8;
-        auto read_a = [&](const char* st, int set, int f) {
-            ra[set][f] = A::read(st, fra, f, 2, set);
-            if constexpr (MX) ea[set][f] = *(const uint32_t*)(st + sc + (2 * f + wi) * 128 + set * 4) >> sh;
-        };
-        auto read_b = [&](const char* st, int set, int h) {
-            rb[set][h] = B::read(st, frb, h, 1, set);
-            if constexpr (MX) eb[set][h] = *(const uint32_t*)(st + sc + SCA * 1024 + (wj * FB + h) * 128 + set * 4) >> sh;
         };
         // dbias: this lane's share (8 of 32 r) of its rows' sums over r, in fp32, of dy as it lies in the fragments: in 16 bits. A
         // linear layer's dz is rounded to them for the products; its rows' errors are independent and even, so that of T rows they
@@ -797,7 +753,6 @@ struct MmKernel {
                 for (int i = 0; i < PA; i += NA) load_a(wbuf, da, i);
 #pragma unroll
                 for (int i = 0; i < PB; i += NB) load_b(wbuf, db, i);
-                load_scales(wbuf);
                 step_loads();
                 wbuf = next_buf(wbuf);
             }
@@ -819,7 +774,6 @@ struct MmKernel {
                         for (int i = 0; i < PB; i += NB) load_b(wbuf, db, i);
 #pragma unroll
                         for (int i = 0; i < PA; i += NA) load_a(wbuf, da, i);
-                        load_scales(wbuf);
                         step_loads();
                         wbuf = next_buf(wbuf);
                     }
@@ -829,9 +783,9 @@ struct MmKernel {
             }
         }
 #pragma unroll
-        for (int f = 0; f < FA; ++f) read_a(sm, 0, f);
+        for (int f = 0; f < FA; ++f) ra[0][f] = A::read(sm, fra, f, 2, 0);
 #pragma unroll
-        for (int h = 0; h < FB; ++h) read_b(sm, 0, h);
+        for (int h = 0; h < FB; ++h) rb[0][h] = B::read(sm, frb, h, 1, 0);
 
         for (int id = run.first; id != MmRun::NONE; id = run.next(id)) {
             MmTile t;
@@ -852,9 +806,9 @@ struct MmKernel {
 #pragma unroll
                 for (int f = 0; f < FA; ++f) {
 #pragma unroll
-                    for (int h = f * FB / FA; h < (f + 1) * FB / FA; ++h) read_b(sm + rbuf, 1, h);
+                    for (int h = f * FB / FA; h < (f + 1) * FB / FA; ++h) rb[1][h] = B::read(sm + rbuf, frb, h, 1, 1);
                     if (f < nf) {
-                        read_a(sm + rbuf, 1, f);
+                        ra[1][f] = A::read(sm + rbuf, fra, f, 2, 1);
                         mul(0, f);
                     }
                     __builtin_amdgcn_sched_barrier(0);
@@ -877,8 +831,8 @@ struct MmKernel {
 #pragma unroll
                 for (int f = 0; f < FA; ++f) {
 #pragma unroll
-                    for (int h = f * FB / FA; h < (f + 1) * FB / FA; ++h) read_b(sm + rbuf, 0, h);
-                    read_a(sm + rbuf, 0, f);
+                    for (int h = f * FB / FA; h < (f + 1) * FB / FA; ++h) rb[0][h] = B::read(sm + rbuf, frb, h, 1, 0);
+                    ra[0][f] = A::read(sm + rbuf, fra, f, 2, 0);
                     // the pieces, four at a time, over the row blocks
                     constexpr int CALLS = PA / NA + PB / NB;
 #pragma unroll
@@ -893,7 +847,6 @@ struct MmKernel {
                     if (bias) add_rows(1);
                 }
                 if constexpr (!NL) {
-                    load_scales(wbuf);
                     step_loads();
                     wbuf = next_buf(wbuf);
                 }
@@ -921,13 +874,13 @@ struct MmKernel {
     }
 };
 
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, int GATHER, int EPI, int NL, bool MX>
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, int GATHER, int EPI, int NL>
 __global__ void __launch_bounds__(128 * NWJ + 64 * NL, OCC * (2 * NWJ + NL) / 4) k_mm(const MmArgs g) {
     // LDS of a CU's OCC workgroups: 160 KiB
     constexpr int LDS = 160 * 1024 / OCC, STAGES = ST * 64 * (32 * FA + 16 * NWJ * FB) * 2, PRE = 4 * MM_MAX_E + 64;
     constexpr bool LDS_OUT = OCC == 2 && STAGES + PRE + 2 * NWJ * 16 * (32 * FB + 16) <= LDS;
-    using K = MmKernel<MODE, F16, FA, FB, NWJ, ST, GATHER, EPI, LDS_OUT, NL, MX>;
-    __shared__ __attribute__((aligned(1024))) char sm[ST * K::STAGE + (K::LINES ? K::NW * K::OUT_BYTES : 0)];
+    using K = MmKernel<MODE, F16, FA, FB, NWJ, ST, GATHER, EPI, LDS_OUT, NL>;
+    __shared__ __attribute__((aligned(1024))) char sm[STAGES + (K::LINES ? K::NW * K::OUT_BYTES : 0)];
     __shared__ int pre[MODE == MM_DW ? 1 : MM_MAX_E + 1];
     K::block(g, sm, pre);
 }
@@ -963,7 +916,7 @@ inline int64_t mm_row_tiles(const MmArgs& a, int BI) {
 }
 inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
-template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, int NL = 0, bool MX = false>
+template <int MODE, bool F16, int FA, int FB, int NWJ, int ST, int OCC, int NL = 0>
 int launch_mm_cfg(const MmArgs& a, hipStream_t st) {
     const bool glu = MODE == MM_FWD && a.kind == EPI_GLU;
     const int bj = 16 * NWJ * FB / (glu ? 2 : 1);
@@ -974,7 +927,7 @@ int launch_mm_cfg(const MmArgs& a, hipStream_t st) {
     constexpr int CUT = MODE == MM_DW ? 1 : FA >= 4 ? 4 : 2;   // pieces that a tile can be cut into
     const int64_t most = 256 * OCC, grid = round8(CUT * ni * nj) < most ? round8(CUT * ni * nj) : most;   // 256 CUs
     auto run = [&](auto epi, auto lists) {
-        k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, decltype(lists)::value, decltype(epi)::value, NL, MX>
+        k_mm<MODE, F16, FA, FB, NWJ, ST, OCC, decltype(lists)::value, decltype(epi)::value, NL>
             <<<(unsigned)grid, 128 * NWJ + 64 * NL, 0, st>>>(a);
     };
     auto go = [&](auto epi) {
@@ -987,7 +940,7 @@ int launch_mm_cfg(const MmArgs& a, hipStream_t st) {
     };
     if constexpr (MODE == MM_FWD) {
         if (glu) {
-            if constexpr (FB % 4 == 0 && !MX) go(std::integral_constant<int, EPI_GLU>{});
+            if constexpr (FB % 4 == 0) go(std::integral_constant<int, EPI_GLU>{});
             else return MOE_ERR_ARG;
         } else if (a.kind == EPI_LIN) {
             go(std::integral_constant<int, EPI_LIN>{});

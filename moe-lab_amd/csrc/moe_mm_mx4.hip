@@ -1,8 +1,409 @@
-#include "moe_mm.h"
+// Products of MXFP4 operands in tiles: y[p][n] = sum_k x[p][k] w[e][n][k], both operands codes with an exponent per 32 of k.
+#include "moe_mx4.h"
 
 namespace moe {
 
-// The tiles of the 16-bit products on MXFP4 operands: a step of the same bytes holds four times as much of r.
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// 32 x 32 outputs, 64 of k: lane l holds 32 codes of row l & 31 (k from 32 (l >> 5) on) and in byte KS of s their exponent.
+// The codes fill half of the operand's registers.
+template <int KS>
+__device__ __forceinline__ f32x16 mma32(s16x8 a, uint32_t sa, s16x8 b, uint32_t sb, f32x16 c) {
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const auto wide = [](s16x8 v) {
+        const i32x4 w = __builtin_bit_cast(i32x4, v);
+        return __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
+    };
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, KS, (int)sa, KS, (int)sb);
+}
+// A lane's four 32-bit words from lane ^ X of its quad.
+template <int X>
+__device__ __forceinline__ u32x4 quad_xor(u32x4 v) {
+    constexpr int P = X == 1 ? 0xB1 : 0x4E;
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[i], P, 0xF, 0xF, false);
+    return o;
+}
+// W x W transposition (W 2 or 4) over W neighbouring lanes: afterwards lane q holds in c[j] what lane j held in c[q].
+template <int W>
+__device__ __forceinline__ void transpose(u32x4* c, int lane) {
+#pragma unroll
+    for (int i = 0; i < W; i += 2) {
+        const bool odd = lane & 1;
+        const u32x4 got = quad_xor<1>(odd ? c[i] : c[i + 1]);
+        if (odd) c[i] = got;
+        else c[i + 1] = got;
+    }
+    if constexpr (W == 4) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool high = lane & 2;
+            const u32x4 got = quad_xor<2>(high ? c[i] : c[i + 2]);
+            if (high) c[i] = got;
+            else c[i + 2] = got;
+        }
+    }
+}
+
+// The epilogue: none, bias and residual, or those with an activation. A kernel of its own for each: a branch on the activation
+// inside one made the compiler hold both sides' values and spill.
+enum MxEpi { MX_PLAIN = 0, MX_LIN = 1, MX_ACT = 2 };
+
+// Tiles of 32 FA NWI x 32 FB NWJ outputs, NWI x NWJ waves that multiply FA x FB blocks of 32 x 32 each (wave (wi, wj): row blocks
+// NWI f + wi, columns 32 FB wj ..) and NL waves that only load, k in steps of 256 through ST stages of LDS. The streams of loads
+// and products, the tiles' order and the pieces of the last round are those of the 16-bit products (moe_mm.h): sizes along k are
+// counted in 16-bit words, four codes each, so that a step is 64 words.
+// A stage is the operands' codes, 128 bytes a row, its 16-byte pieces XORed so that a fragment's rows spread over the banks, and
+// their exponents, 8 bytes a row. These lie in memory by steps (moe_mx4.h), so that a tile's are 1 KiB pieces, one to a loading
+// wave; their bytes are ordered so that a lane's four of a step are one word, which the instruction picks from.
+// The matrix instruction takes w's rows as its first operand, and row m of it is w's row column(m) of the wave's 32 FB, so that
+// a lane's sums of one row of x are 16 FB neighbours; a transposition over four lanes then makes every store instruction write
+// whole lines.
+template <bool F16, int FA, int FB, int NWI, int NWJ, int ST, int GATHER, int EPI, int NL>
+struct MxKernel {
+    static constexpr bool LIN = EPI != MX_PLAIN;
+    static constexpr int NWC = NWI * NWJ;
+    static constexpr int BI = 32 * FA * NWI, BJ = 32 * FB * NWJ;
+    static constexpr int PA = BI / 8 / NL, PB = BJ / 8 / NL;                                  // 1 KiB pieces of a loading wave
+    static constexpr int SCA = (BI * 8 + 1023) / 1024, SCB = (BJ * 8 + 1023) / 1024;   // pieces of exponents
+    static_assert(SCA + SCB <= NL, "one to a wave");
+    static constexpr int CODES = (BI + BJ) * 128, STAGE = CODES + (SCA + SCB) * 1024;
+    static constexpr int L = PA + PB + 1;
+
+    // XOR of the 16-byte pieces of a row: eight lanes that read at once have eight different ones. Rows of x go by lane; of w by
+    // column(): rows 0 .. 3 and 16 FB .. 16 FB + 3.
+    static __device__ __forceinline__ int swz_a(int r) { return r & 7; }
+    static __device__ __forceinline__ int swz_b(int r) { return (r & 3) | ((r >> 2 ^ r / (16 * FB)) & 1) << 2; }
+    static __device__ __forceinline__ int column(int h, int m) { return (m >> 2 & 1) * 16 * FB + h * 16 + (m >> 3) * 4 + (m & 3); }
+
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* p, int64_t row0, int rows, int J, int es) {
+        return __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<void*>(p) + row0 * J * es, 0,
+                                                 p ? (uint32_t)rows * (uint32_t)J * es : 0u, 0x00027000);
+    }
+    // Everything goes through buffer descriptors: rows and columns past the tile's valid ones get an offset past the end, absent
+    // operands an empty descriptor. Residual rows are loaded as lines, like the stores, all before the first is needed.
+    static __device__ __forceinline__ void store(const MmArgs& g, const MmTile& t, f32x16 (&acc)[FA][FB], int lane, int wi, int wj) {
+        const bool f32 = g.ydt == MOE_DTYPE_F32;
+        const int ES = f32 ? 4 : 2, hb = lane >> 5;
+        const int jw = t.j0 + wj * 32 * FB + hb * 16 * FB;   // this lane's columns
+        const int64_t row0 = (g.part ? (int64_t)t.e * g.M : 0) + t.lo;
+        const auto yb = rows_of(g.y, row0, t.rows, g.J, ES), zb = rows_of(g.epi.z, row0, t.rows, g.J, 2),
+                   rb = rows_of(g.epi.residual, row0, t.rows, g.J, 2);
+        constexpr int NC = 2 * FB, W = NC < 4 ? NC : 4;   // 16-bit: pieces of 8 columns of a lane; lanes that exchange
+        const int q = lane & (W - 1), first = lane & 31 & ~(W - 1);
+        // of piece u, W at a time: row j of the W, columns 8 (u & ~(W - 1)) + 8 q
+        const auto at = [&](int f, int u, int j) -> uint32_t {
+            const int i = 32 * (NWI * f + wi) + first + j, c = jw + 8 * ((u & ~(W - 1)) + q);
+            return i < t.rows && c < g.J ? ((uint32_t)i * (uint32_t)g.J + c) * 2 : MM_OOB;
+        };
+        u32x4 res[LIN ? FA : 1][NC];
+        if constexpr (LIN) {
+#pragma unroll
+            for (int f = 0; f < FA; ++f)
+#pragma unroll
+                for (int u = 0; u < NC; ++u) res[f][u] = __builtin_amdgcn_raw_buffer_load_b128(rb, at(f, u, u & (W - 1)), 0, 0);
+        }
+        const bool gelu = g.epi.act == MOE_LIN_GELU;
+        const float c1 = gelu ? 1.5957691216057308f : 1.f, c3 = gelu ? 1.5957691216057308f * 0.044715f : 0.f;
+#pragma unroll
+        for (int f = 0; f < FA; ++f) {
+            if (32 * (NWI * f + wi) >= t.rows) break;
+            if constexpr (LIN) {
+                u32x4 zz[NC], bias[NC];   // loaded for each row block: its 32 values kept in fp32 would spill others
+                const auto bb = rows_of(g.epi.bias, t.e, 1, g.J, 2);
+#pragma unroll
+                for (int u = 0; u < NC; ++u)
+                    bias[u] = __builtin_amdgcn_raw_buffer_load_b128(bb, jw + 8 * u < g.J ? (jw + 8 * u) * 2 : MM_OOB, 0, 0);
+#pragma unroll
+                for (int u = 0; u < NC; u += W) transpose<W>(res[f] + u, lane);
+#pragma unroll
+                for (int u = 0; u < NC; ++u) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {   // two neighbours
+                        const int i = (u & 1) * 8 + 2 * c;
+                        float v[2];
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) v[p] = acc[f][u >> 1][i + p] + un16<F16>(bias[u][c] >> (16 * p));
+                        zz[u][c] = pack16<F16>(v[0], v[1]);
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            if constexpr (EPI == MX_ACT) v[p] *= sigmoid_fast(v[p] * (c1 + c3 * (v[p] * v[p])));
+                            acc[f][u >> 1][i + p] = v[p] + un16<F16>(res[f][u][c] >> (16 * p));
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);   // not all pieces at once: they would spill
+                }
+                if (g.epi.z) {
+#pragma unroll
+                    for (int u = 0; u < NC; u += W) transpose<W>(zz + u, lane);
+#pragma unroll
+                    for (int u = 0; u < NC; ++u) __builtin_amdgcn_raw_buffer_store_b128(zz[u], zb, at(f, u, u & (W - 1)), 0, 2);
+                }
+            }
+            if (f32) {   // pieces of 4 columns
+                constexpr int NF = 4 * FB;
+                const int qf = lane & 3, rf = 32 * (NWI * f + wi) + (lane & 28);
+#pragma unroll
+                for (int u = 0; u < NF; u += 4) {
+                    u32x4 o[4];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[v][c] = __float_as_uint(acc[f][(u + v) >> 2][((u + v) & 3) * 4 + c]);
+                    transpose<4>(o, lane);
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        const int i = rf + v, c = jw + 4 * (u + qf);
+                        __builtin_amdgcn_raw_buffer_store_b128(
+                            o[v], yb, i < t.rows && c < g.J ? ((uint32_t)i * (uint32_t)g.J + c) * 4 : MM_OOB, 0, 0);
+                    }
+                }
+            } else {
+                u32x4 o[NC];
+#pragma unroll
+                for (int u = 0; u < NC; ++u)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        o[u][c] = pack16<F16>(acc[f][u >> 1][(u & 1) * 8 + 2 * c], acc[f][u >> 1][(u & 1) * 8 + 2 * c + 1]);
+#pragma unroll
+                for (int u = 0; u < NC; u += W) transpose<W>(o + u, lane);
+#pragma unroll
+                for (int u = 0; u < NC; ++u) __builtin_amdgcn_raw_buffer_store_b128(o[u], yb, at(f, u, u & (W - 1)), 0, 2);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+
+    static __device__ __forceinline__ void block(const MmArgs& g, char* sm, int* pre) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wi = wave % NWI, wj = wave / NWI;
+        const int ld2 = g.R * 2;   // bytes of a row of codes
+        const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)sm;
+        const int nj = (g.J + BJ - 1) / BJ, ksteps = (g.R + 63) / 64;
+        count_tiles<MM_FWD, BI>(g, pre, 0x70000000 / nj);
+        const int tiles = __builtin_amdgcn_readfirstlane(pre[g.E]) * nj;
+        if (g.fill && g.offsets) fill_rest<MM_FWD>(g);
+        const MmRun run = xcd_run<BI >= 128 ? 2 : 1>(tiles);
+        auto tile = [&](int id, MmTile& t) {
+            tile_at<MM_FWD, BI, BJ>(g, pre, run.tile(id), t);
+            if (id >= run.whole) {   // a piece (the last ones of a tile with few rows are empty)
+                const int n = BI >> run.cut, lo = ((id - run.whole) & ((1 << run.cut) - 1)) * n;
+                t.lo += lo;
+                t.rows = max(0, min(n, t.rows - lo));
+            }
+        };
+        auto r_of = [&](const MmTile& t) -> int { return g.part ? min(g.part, g.R - t.e * g.part) : g.R; };
+        auto steps_of = [&](const MmTile& t) -> int { return t.rows ? (r_of(t) + 63) / 64 : 0; };
+        auto next_buf = [](uint32_t b) -> uint32_t { return b == (ST - 1) * STAGE ? 0 : b + STAGE; };
+        if (run.first == MmRun::NONE) return;
+
+        if (wave >= NWC) {   // loads: ST stages ahead, past the last tile from empty descriptors
+            const int lw = wave - NWC, row = 8 * lw + (lane >> 3), piece = lane & 7;
+            int lid = -1, ls = 0, lsteps = 0, lrows = 0, lr = 0;
+            MmTile lt{};
+            const char *pa = nullptr, *pb = nullptr;
+            uint32_t offa[PA], offb[PB];
+            auto next_tile = [&]() {
+                ls = 0;
+                do {
+                    lid = lid < 0 ? run.first : run.next(lid);
+                    if (lid == MmRun::NONE) {
+                        lsteps = 0x7fffffff;
+                        lrows = 0;
+                        return;
+                    }
+                    tile(lid, lt);
+                    lsteps = steps_of(lt);
+                } while (lsteps == 0);
+                lrows = lt.rows;
+                lr = r_of(lt);
+                const int first = lt.e * g.part;   // the part's first word
+                pa = (const char*)g.a + (GATHER ? 0 : (int64_t)lt.lo * ld2) + (int64_t)first * 2;
+                pb = (const char*)g.b + ((int64_t)(g.part ? 0 : lt.e) * g.J + lt.j0) * ld2 + (int64_t)first * 2;
+#pragma unroll
+                for (int i = 0; i < PA; ++i) {
+                    const int r = row + 8 * NL * i, c = (piece ^ swz_a(r)) * 16;
+                    int src = r;
+                    if constexpr (GATHER) src = r < lt.rows ? g.arows[lt.lo + r] : -1;
+                    offa[i] = !GATHER || (uint32_t)src < (uint32_t)g.a_n ? (uint32_t)src * (uint32_t)ld2 + c : MM_OOB;
+                }
+#pragma unroll
+                for (int i = 0; i < PB; ++i) {
+                    const int r = row + 8 * NL * i;
+                    offb[i] = (uint32_t)r * (uint32_t)ld2 + (piece ^ swz_b(r)) * 16;
+                }
+            };
+            auto load = [&](uint32_t buf) {   // step ls
+                const int left = (lr - 64 * ls) * 2;   // bytes of a row from here on
+                if (left < 128 && lrows) {             // the last step ends inside a row: its pieces past the end
+#pragma unroll
+                    for (int i = 0; i < PA; ++i)
+                        if ((piece ^ swz_a(row + 8 * NL * i)) * 16 >= left) offa[i] = MM_OOB;
+#pragma unroll
+                    for (int i = 0; i < PB; ++i)
+                        if ((piece ^ swz_b(row + 8 * NL * i)) * 16 >= left) offb[i] = MM_OOB;
+                }
+                const uint32_t na = lrows ? (uint32_t)((GATHER ? g.a_n : lrows) - 1) * (uint32_t)ld2 + (uint32_t)left : 0,
+                               nb = lrows ? (uint32_t)(min(BJ, g.J - lt.j0) - 1) * (uint32_t)ld2 + (uint32_t)left : 0;
+                const srd_t da = srd_of(pa, na), db = srd_of(pb, nb);
+                constexpr int NA = PA < 4 ? PA : 4, NB = PB < 4 ? PB : 4;
+#pragma unroll
+                for (int i = 0; i < PB; i += NB) dma16<NB, NL * 1024>(db, offb + i, lds0 + buf + (uint32_t)(BI * 128 + (i * NL + lw) * 1024));
+#pragma unroll
+                for (int i = 0; i < PA; i += NA) dma16<NA, NL * 1024>(da, offa + i, lds0 + buf + (uint32_t)((i * NL + lw) * 1024));
+                // this wave's piece of a's or b's exponents (waves past the last piece load one again)
+                const int p = lw % (SCA + SCB), step = ls + (g.part ? lt.e * (g.part / 64) : 0), e = g.part ? 0 : lt.e;
+                const uint8_t* s = g.sa + ((int64_t)step * g.M + lt.lo) * 8 + p * 1024;
+                int n = (lrows * 8 + 15) / 16 * 16 - p * 1024;
+                if (p >= SCA) {
+                    s = g.sb + (((int64_t)e * ksteps + step) * g.J + lt.j0) * 8 + (p - SCA) * 1024;
+                    n = (g.J - lt.j0) * 8 - (p - SCA) * 1024;
+                }
+                const uint32_t off = lane * 16;
+                dma16<1, 0>(srd_of((const char*)s, lrows && n > 0 ? n : 0), &off, lds0 + buf + CODES + p * 1024);
+                ++ls;
+                pa += 128;
+                pb += 128;
+            };
+            uint32_t wbuf = 0;
+#pragma unroll
+            for (int s = 0; s < ST; ++s) {
+                if (ls >= lsteps) next_tile();
+                load(wbuf);
+                wbuf = next_buf(wbuf);
+            }
+            wait_vm<(ST - 1) * L>();
+            barrier_raw();
+            for (int id = run.first; id != MmRun::NONE; id = run.next(id)) {
+                MmTile t;
+                tile(id, t);
+                for (int s = steps_of(t); s > 0; --s) {
+                    if (ls >= lsteps) next_tile();
+                    wait_vm<(ST - 2) * L>();
+                    barrier_raw();   // the stage that is multiplied next has landed, the last one is free
+                    load(wbuf);
+                    wbuf = next_buf(wbuf);
+                }
+            }
+            wait_vm<0>();   // no load may still write this workgroup's LDS when it ends
+            return;
+        }
+
+        const int r = lane & 31, hb = lane >> 5;
+        uint32_t fa[FA], fb[FB], xa[FA], xb[FB];   // LDS offsets: the fragments of k 0 .. 63, and the exponents' words
+#pragma unroll
+        for (int f = 0; f < FA; ++f) {
+            const int i = 32 * (NWI * f + wi) + r;
+            fa[f] = i * 128 + (hb ^ swz_a(i)) * 16;
+            xa[f] = CODES + i * 8 + hb * 4;
+        }
+#pragma unroll
+        for (int h = 0; h < FB; ++h) {
+            const int j = 32 * FB * wj + column(h, r);
+            fb[h] = BI * 128 + j * 128 + (hb ^ swz_b(j)) * 16;
+            xb[h] = CODES + SCA * 1024 + j * 8 + hb * 4;
+        }
+        f32x16 acc[FA][FB];
+        s16x8 ra[2][FA], rb[2][FB];        // fragments of the quarter step that is multiplied and of the next one
+        uint32_t ea[2][FA], eb[2][FB];   // exponents of the step that is multiplied and of the next one
+        auto read = [&](const char* st, int set, int ks) {
+#pragma unroll
+            for (int h = 0; h < FB; ++h) rb[set][h] = *(const s16x8*)(st + (fb[h] ^ (ks * 32)));
+#pragma unroll
+            for (int f = 0; f < FA; ++f) ra[set][f] = *(const s16x8*)(st + (fa[f] ^ (ks * 32)));
+        };
+        auto read_exponents = [&](const char* st, int set) {
+#pragma unroll
+            for (int h = 0; h < FB; ++h) eb[set][h] = *(const uint32_t*)(st + xb[h]);
+#pragma unroll
+            for (int f = 0; f < FA; ++f) ea[set][f] = *(const uint32_t*)(st + xa[f]);
+        };
+        barrier_raw();
+        uint32_t rbuf = 0;
+        for (int id = run.first; id != MmRun::NONE; id = run.next(id)) {
+            MmTile t;
+            tile(id, t);
+            const int steps = steps_of(t), nf = (t.rows + 32 * NWI - 1) / (32 * NWI);
+            float zero;   // opaque: zeros kept in accumulation registers for the next tile would take them from the sums
+            asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
+#pragma unroll
+            for (int f = 0; f < FA; ++f)
+#pragma unroll
+                for (int h = 0; h < FB; ++h)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[f][h][i] = zero;
+            read(sm + rbuf, 0, 0);   // again after the last tile's stores, which need the registers
+            read_exponents(sm + rbuf, 0);
+            auto mul = [&](auto ks) {
+                constexpr int K = decltype(ks)::value, set = K & 1;
+#pragma unroll
+                for (int f = 0; f < FA; ++f)
+                    if (f < nf) {
+#pragma unroll
+                        for (int h = 0; h < FB; ++h) acc[f][h] = mma32<K>(rb[set][h], eb[0][h], ra[set][f], ea[0][f], acc[f][h]);
+                    }
+            };
+#pragma nounroll
+            for (int s = 0; s < steps; ++s) {
+                read(sm + rbuf, 1, 1);
+                mul(std::integral_constant<int, 0>{});
+                __builtin_amdgcn_sched_barrier(0);
+                read(sm + rbuf, 0, 2);
+                mul(std::integral_constant<int, 1>{});
+                __builtin_amdgcn_sched_barrier(0);
+                read(sm + rbuf, 1, 3);
+                mul(std::integral_constant<int, 2>{});
+                // every read of this stage is done, so once all waves are here it is free for the loads; and the next stage has
+                // landed
+                wait_lds();
+                barrier_raw();
+                rbuf = next_buf(rbuf);
+                read(sm + rbuf, 0, 0);
+                read_exponents(sm + rbuf, 1);
+                mul(std::integral_constant<int, 3>{});
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int h = 0; h < FB; ++h) eb[0][h] = eb[1][h];
+#pragma unroll
+                for (int f = 0; f < FA; ++f) ea[0][f] = ea[1][f];
+            }
+            store(g, t, acc, lane, wi, wj);
+        }
+    }
+};
+
+template <bool F16, int FA, int FB, int NWI, int NWJ, int ST, int OCC, int GATHER, int EPI, int NL>
+__global__ void __launch_bounds__(64 * (NWI * NWJ + NL), OCC * (NWI * NWJ + NL) / 4) k_mm_mx4(const MmArgs g) {
+    using K = MxKernel<F16, FA, FB, NWI, NWJ, ST, GATHER, EPI, NL>;
+    __shared__ __attribute__((aligned(1024))) char sm[ST * K::STAGE];
+    __shared__ int pre[MM_MAX_E + 1];
+    static_assert(sizeof(sm) + sizeof(pre) <= 160 * 1024 / OCC, "");
+    K::block(g, sm, pre);
+}
+
+template <bool F16, int FA, int FB, int NWI, int NWJ, int ST, int OCC, int NL>
+static int launch_cfg(const MmArgs& a, hipStream_t st) {
+    constexpr int BI = 32 * FA * NWI, BJ = 32 * FB * NWJ;
+    const int64_t ni = mm_row_tiles(a, BI), nj = (a.J + BJ - 1) / BJ;
+    if (ni * nj == 0) return MOE_OK;
+    if (ni * nj > 0x70000000) return MOE_ERR_ARG;
+    constexpr int CUT = BI >= 128 ? 4 : 2;   // pieces that a tile can be cut into
+    const int64_t most = 256 * OCC, grid = round8(CUT * ni * nj) < most ? round8(CUT * ni * nj) : most;   // 256 CUs
+    auto run = [&](auto lists, auto epi) {
+        k_mm_mx4<F16, FA, FB, NWI, NWJ, ST, OCC, decltype(lists)::value, decltype(epi)::value, NL>
+            <<<(unsigned)grid, 64 * (NWI * NWJ + NL), 0, st>>>(a);
+    };
+    auto go = [&](auto lists) {
+        if (a.kind != EPI_LIN) run(lists, std::integral_constant<int, MX_PLAIN>{});
+        else run(lists, std::integral_constant<int, MX_LIN>{});
+    };
+    if (a.arows) go(std::integral_constant<int, 1>{});   // moe_mx4_grouped_mm: no activation
+    else if (a.epi.act != MOE_LIN_NONE) run(std::integral_constant<int, 0>{}, std::integral_constant<int, MX_ACT>{});
+    else go(std::integral_constant<int, 0>{});
+    return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;
+}
+
 static int grouped(const MmArgs& a) {
     const int64_t live = a.E < a.M ? a.E : a.M;
     if (a.M / live <= 32) return MM_64;
@@ -12,9 +413,9 @@ static int grouped(const MmArgs& a) {
 template <bool F16>
 static int launch(const MmArgs& a, hipStream_t st) {
     switch (a.offsets ? grouped(a) : mm_plan(MM_FWD, a.M, a.J, a.R, a.part != 0).shape) {
-        case MM_128x256: return launch_mm_cfg<MM_FWD, F16, 4, 4, 4, 3, 1, 4, true>(a, st);
-        case MM_128_DEEP: return launch_mm_cfg<MM_FWD, F16, 4, 4, 2, 4, 1, 4, true>(a, st);
-        default: return launch_mm_cfg<MM_FWD, F16, 2, 2, 2, 4, 2, 4, true>(a, st);
+        case MM_128x256: return launch_cfg<F16, 2, 2, 2, 4, 3, 1, 4>(a, st);
+        case MM_128_DEEP: return launch_cfg<F16, 2, 2, 2, 2, 4, 1, 4>(a, st);
+        default: return launch_cfg<F16, 1, 1, 2, 2, 4, 2, 4>(a, st);
     }
 }
 int launch_mm_mx4(const MmArgs& a, hipStream_t st) { return a.f16 ? launch<true>(a, st) : launch<false>(a, st); }

@@ -1,7 +1,8 @@
 // MXFP4 operands made on the device: E2M1 codes, two to a byte, the low half first, with an E8M0 byte per 32 neighbours.
-// A matrix of `rows` rows and K columns is codes [rows, K / 2] and scales [steps, rows, 8], steps = ceil(K / 256): byte b of
-// (s, row) belongs to the columns 256 s + 32 b ... The products take a step of all rows of a tile at a time, so those bytes lie
-// together (in rows of their own, K / 32 bytes each, a tile's step would be a hundred lines for 8 bytes of each).
+// A matrix of `rows` rows and K columns is codes [rows, K / 2] and scales [steps, rows, 8], steps = ceil(K / 256): byte
+// mx4_byte(b) of (s, row) belongs to the columns 256 s + 32 b ... The products take a step of all rows of a tile at a time, so
+// those bytes lie together (in rows of their own, K / 32 bytes each, a tile's step would be a hundred lines for 8 bytes of each),
+// the even blocks' before the odd ones': a lane of the matrix instruction holds every second block, so its four bytes are a word.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -15,6 +16,7 @@ struct Mx4 {
     uint8_t* scales;
 };
 // Bytes of a matrix's scales. Reads of 16 bytes may start at any row, so 8 more lie behind the last one (16: whole pieces).
+__host__ __device__ constexpr int mx4_byte(int b) { return (b & 1) * 4 + (b >> 1); }
 inline int64_t mx4_steps(int64_t K) { return (K + 255) / 256; }
 inline size_t mx4_scale_bytes(int64_t rows, int64_t K) { return (size_t)(mx4_steps(K) * rows * 8 + 16); }
 

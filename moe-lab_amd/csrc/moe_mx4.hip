@@ -68,8 +68,15 @@ struct Eight {
 // Bytes of the values in memory.
 __host__ __device__ constexpr int size_of(int dt) { return dt == MOE_DTYPE_F32 ? 4 : 2; }
 
-// One item: 8 columns of a row, its 4-lane neighbours the rest of its block. The lane with a row's last block also writes the
-// bytes that fill its last step (1.0: they meet codes of zero in the products).
+// Block b's byte of the eight of its row and step. With a row's last block also those that fill its step, with 1.0: they meet
+// codes of zero in the products, whose product with a NaN would be one.
+__device__ __forceinline__ void write_exponent(uint8_t* s, int b, uint32_t e, bool last) {
+    s[mx4_byte(b)] = (uint8_t)e;
+    if (last)
+        for (int p = b + 1; p < 8; ++p) s[mx4_byte(p)] = 127;
+}
+
+// One item: 8 columns of a row, its 4-lane neighbours the rest of its block.
 template <int DT>
 __global__ void __launch_bounds__(256) k_mx4_quantize(const char* x, int64_t ld, uint32_t items, uint32_t per_row, uint32_t row0,
                                                       uint32_t rows, int64_t scale_stride, uint8_t* codes, uint8_t* scales) {
@@ -85,9 +92,7 @@ __global__ void __launch_bounds__(256) k_mx4_quantize(const char* x, int64_t ld,
     if ((c & 3) == 0) {
         const uint32_t b = c >> 2;
         uint8_t* s = scales + g * scale_stride + ((int64_t)(b >> 3) * rows + n) * 8;
-        s[b & 7] = (uint8_t)e;
-        if (c + 4 == per_row)
-            for (uint32_t p = (b & 7) + 1; p < 8; ++p) s[p] = 127;
+        write_exponent(s, b & 7, e, c + 4 == per_row);
     }
 }
 
@@ -99,7 +104,7 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* codes, co
     if (i >= items) return;
     const uint32_t r = i / per_row, c = i - r * per_row;
     const uint32_t row = row0 + r, g = row / rows, n = row - g * rows, b = c >> 2;
-    const uint32_t e = scales[g * scale_stride + ((int64_t)(b >> 3) * rows + n) * 8 + (b & 7)];
+    const uint32_t e = scales[g * scale_stride + ((int64_t)(b >> 3) * rows + n) * 8 + mx4_byte(b & 7)];
     const int64_t at = (int64_t)row * per_row + c;
     const uint32_t q = *(const uint32_t*)(codes + at * 4);
     // codes as fp32 (exact), then the power of two: 2^-127 is subnormal, and 255 stands for NaN
@@ -176,18 +181,30 @@ int launch_mx4_take_scales(const uint8_t* scales, int64_t n, int64_t K, const in
     return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;
 }
 
-// Few rows: a workgroup multiplies 16 rows of the weights by up to 16 rows of x. Its waves share K, 128 columns at a time, with
-// the weights' codes straight from memory as the matrix instruction's first operand, and their sums meet in LDS, in the waves'
+// Both operands MXFP4, 16 x 16 outputs and 128 of k: lane l holds 32 codes of row l & 15 (k from 32 (l >> 4) on), and in byte B of
+// its word their exponent.
+template <int B>
+__device__ __forceinline__ f32x4 mma16(s16x8 a, uint32_t sa, s16x8 b, uint32_t sb, f32x4 c) {
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    const auto wide = [](s16x8 v) {   // the upper half is not read
+        const i32x4 w = __builtin_bit_cast(i32x4, v);
+        return __builtin_shufflevector(w, w, 0, 1, 2, 3, -1, -1, -1, -1);
+    };
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a), wide(b), c, 4, 4, B, (int)sa, B, (int)sb);
+}
+
+// Few rows: a wave multiplies 16 rows of the weights by up to 16 rows of x, with the weights' codes straight from memory as the
+// matrix instruction's first operand. ks waves of a workgroup share the steps of K, and their sums meet in LDS, in the waves'
 // order. FUSE: x's rows are quantised here first, while the first weights are on their way.
 // Workgroups go by slot, not by group (as k_mm_rows): the one at a group's first slot does the group.
 constexpr int MXR_WAVES = 8;
 template <bool F16, bool FUSE>
-__global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, const uint16_t* x16, int64_t ldx) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t sx[];   // FUSE: codes [MX4_FUSE, K / 2], scale bytes [MX4_FUSE, K / 32]
+__global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, const uint16_t* x16, int64_t ldx, int ks) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t sx[];   // FUSE: codes [MX4_FUSE, K / 2], exponents [MX4_FUSE, steps, 8]
     __shared__ f32x4 sums[MXR_WAVES][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % ks;
     const int l = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * 16, p = blockIdx.y;
+    const int wg0 = blockIdx.x * 16 * (MXR_WAVES / ks), n0 = wg0 + wave / ks * 16, p = blockIdx.y;
     int e = 0, lo = 0, hi = g.M;
     if (g.offsets) {
         e = -1;   // the group whose first slot is p
@@ -197,7 +214,8 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, con
             const uint64_t hit = __ballot(a == p && b > a);
             if (hit) {
                 e = base + __builtin_ctzll(hit);
-                group_of<MM_FWD>(g, e, lo, hi);
+                lo = p;
+                hi = __builtin_amdgcn_readlane(b, __builtin_ctzll(hit));
             }
         }
         if (e < 0) {
@@ -205,32 +223,35 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, con
             int a, b;
             group_of<MM_FWD>(g, g.E - 1, a, b);
             if (p < b) return;
-            if (threadIdx.x < 16 && n0 + threadIdx.x < g.J) {
-                const int64_t at = (int64_t)p * g.J + n0 + threadIdx.x;
+            const int n = wg0 + threadIdx.x;
+            if (threadIdx.x < 16 * (MXR_WAVES / ks) && n < g.J) {
+                const int64_t at = (int64_t)p * g.J + n;
                 if (g.ydt == MOE_DTYPE_F32) ((float*)g.y)[at] = 0.f;
                 else ((uint16_t*)g.y)[at] = 0;
             }
             return;
         }
     }
-    const int K = g.R * 4, KB = K / 2, steps = (g.R + 63) / 64, chunks = (K + 127) / 128;
+    const int K = g.R * 4, KB = K / 2, steps = (K + 255) / 256;
     const int n = min(n0 + l, g.J - 1);   // rows past the last: multiplied, not stored
     const uint8_t* wc = (const uint8_t*)g.b + ((int64_t)e * g.J + n) * KB + q * 16;
-    const uint8_t* ws = g.sb + ((int64_t)e * steps * g.J + n) * 8;
-    constexpr int AHEAD = 4;   // chunks of a wave whose weights are loaded together
-    s16x8 w[AHEAD];
+    const uint8_t* ws = g.sb + ((int64_t)e * steps * g.J + n) * 8 + (q & 1) * 4;
+    const int sh = (q >> 1) * 8;   // the first half step's exponent in byte 0, the second's in byte 2
+    constexpr int AHEAD = 4;       // steps of a wave whose weights are loaded together
+    s16x8 w[AHEAD][2];
     uint32_t we[AHEAD];
     const s16x8 zero = {};
-    auto load_w = [&](int c0) {
+    auto load_w = [&](int s0) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const int c = c0 + u * MXR_WAVES;
-            const bool in = c * 128 + q * 32 < K;
-            w[u] = in ? *(const s16x8*)(wc + (int64_t)c * 64) : zero;
-            we[u] = in ? *(const uint32_t*)(ws + (int64_t)(c >> 1) * g.J * 8 + (c & 1) * 4) >> (8 * q) : 127;
+            const int s = min(s0 + u * ks, steps - 1);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                w[u][c] = s * 256 + c * 128 + q * 32 < K ? *(const s16x8*)(wc + (int64_t)s * 128 + c * 64) : zero;
+            we[u] = *(const uint32_t*)(ws + (int64_t)s * g.J * 8) >> sh;
         }
     };
-    load_w(wave);
+    if (n0 < g.J) load_w(part);
     for (int m0 = lo; m0 < hi; m0 += FUSE ? MX4_FUSE : MX4_ROWS) {
         const int rows = min(hi - m0, FUSE ? MX4_FUSE : MX4_ROWS);
         int src = -1;   // this lane's row of x
@@ -242,65 +263,68 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, con
             if (m0 > lo) __syncthreads();   // the last rows are multiplied
             const int per_row = K / 8;
             for (int i = threadIdx.x; i < rows * per_row; i += 64 * MXR_WAVES) {   // a block's four lanes together: K % 32 == 0
-                const int r = i / per_row, c = i - r * per_row;
-                int s = g.arows ? g.arows[m0 + r] : m0 + r;
+                const int r = i / per_row, c = i - r * per_row, b = c >> 2;
+                const int s = g.arows ? g.arows[m0 + r] : m0 + r;
                 Eight<F16 ? MOE_DTYPE_F16 : MOE_DTYPE_BF16> v;
                 const bool live = (uint32_t)s < (uint32_t)g.a_n;
                 v.load((const char*)(x16 + (live ? s : 0) * ldx + c * 8));
                 const uint32_t ex = exponent4(max4(v.top()));
                 const uint32_t code = v.codes(ex - 1 < 254 ? ex : 127);
                 *(uint32_t*)(sx + (r * per_row + c) * 4) = live && ex - 1 < 254 ? code : 0;
-                if ((c & 3) == 0) sx[MX4_FUSE * KB + r * (K / 32) + (c >> 2)] = live ? (uint8_t)ex : 127;
+                if ((c & 3) == 0) write_exponent(sx + MX4_FUSE * KB + (r * steps + (b >> 3)) * 8, b & 7, live ? ex : 127, c + 4 == per_row);
             }
             __syncthreads();
         }
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int c0 = wave; c0 < chunks; c0 += AHEAD * MXR_WAVES) {
-            if (c0 != wave || m0 > lo) load_w(c0);
+        if (n0 < g.J)
+            for (int s0 = part; s0 < steps; s0 += AHEAD * ks) {
+                if (s0 != part || m0 > lo) load_w(s0);
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
-                const int c = c0 + u * MXR_WAVES;
-                if (c >= chunks) break;
-                s16x8 x = zero;
-                uint32_t xe = 127;
-                if (src >= 0 && c * 128 + q * 32 < K) {
-                    if constexpr (FUSE) {
-                        x = *(const s16x8*)(sx + l * KB + c * 64 + q * 16);
-                        xe = sx[MX4_FUSE * KB + l * (K / 32) + c * 4 + q];
-                    } else {
-                        x = *(const s16x8*)((const uint8_t*)g.a + (int64_t)src * KB + c * 64 + q * 16);
-                        xe = g.sa[((int64_t)(c >> 1) * g.a_n + src) * 8 + (c & 1) * 4 + q];
+                for (int u = 0; u < AHEAD; ++u) {
+                    const int s = s0 + u * ks;
+                    if (s >= steps) break;
+                    s16x8 x[2] = {zero, zero};
+                    uint32_t xe = 0x7f7f7f7f;
+                    if (src >= 0) {
+                        const uint8_t* xc = FUSE ? sx + l * KB : (const uint8_t*)g.a + (int64_t)src * KB;
+                        const uint8_t* xs = FUSE ? sx + MX4_FUSE * KB + (l * steps + s) * 8 : g.sa + ((int64_t)s * g.a_n + src) * 8;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            if (s * 256 + c * 128 + q * 32 < K) x[c] = *(const s16x8*)(xc + s * 128 + c * 64 + q * 16);
+                        xe = *(const uint32_t*)(xs + (q & 1) * 4) >> sh;
                     }
+                    acc = mma16<0>(w[u][0], we[u], x[0], xe, acc);
+                    acc = mma16<2>(w[u][1], we[u], x[1], xe, acc);
                 }
-                acc = mma4(w[u], we[u], x, xe, acc);
             }
+        if (ks > 1) {
+            sums[wave][lane] = acc;
+            __syncthreads();
         }
-        sums[wave][lane] = acc;
-        __syncthreads();
-        if (wave == 0) {
-            acc = sums[0][lane];
+        const int j = n0 + 4 * q;   // four neighbours of J (a multiple of 8)
+        if (part == 0 && l < rows && j < g.J) {
+            for (int i = 1; i < ks; ++i) acc += sums[wave + i][lane];
+            const int64_t at = (int64_t)(m0 + l) * g.J + j;
+            if (g.epi.bias) acc += load4<F16>(g.epi.bias, (int64_t)e * g.J + j);
+            if (g.epi.z) *(u32x2*)((uint16_t*)g.epi.z + at) = (u32x2){pack16<F16>(acc[0], acc[1]), pack16<F16>(acc[2], acc[3])};
 #pragma unroll
-            for (int i = 1; i < MXR_WAVES; ++i) acc += sums[i][lane];
-            const int j = n0 + 4 * q;   // four neighbours of J (a multiple of 8)
-            if (l < rows && j < g.J) {
-                const int64_t at = (int64_t)(m0 + l) * g.J + j;
-                if (g.epi.bias) acc += load4<F16>(g.epi.bias, (int64_t)e * g.J + j);
-                if (g.epi.z) *(u32x2*)((uint16_t*)g.epi.z + at) = (u32x2){pack16<F16>(acc[0], acc[1]), pack16<F16>(acc[2], acc[3])};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] = lin_act(g.epi.act, acc[i]);
-                if (g.epi.residual) acc += load4<F16>(g.epi.residual, at);
-                if (g.ydt == MOE_DTYPE_F32) *(f32x4*)((float*)g.y + at) = acc;
-                else *(u32x2*)((uint16_t*)g.y + at) = (u32x2){pack16<F16>(acc[0], acc[1]), pack16<F16>(acc[2], acc[3])};
-            }
+            for (int i = 0; i < 4; ++i) acc[i] = lin_act(g.epi.act, acc[i]);
+            if (g.epi.residual) acc += load4<F16>(g.epi.residual, at);
+            if (g.ydt == MOE_DTYPE_F32) *(f32x4*)((float*)g.y + at) = acc;
+            else *(u32x2*)((uint16_t*)g.y + at) = (u32x2){pack16<F16>(acc[0], acc[1]), pack16<F16>(acc[2], acc[3])};
         }
-        __syncthreads();   // the sums are read
+        if (ks > 1 && m0 + (FUSE ? MX4_FUSE : MX4_ROWS) < hi) __syncthreads();   // the sums are read
     }
 }
 
 int launch_mx4_rows(const MmArgs& a, const void* x16, int64_t ldx, hipStream_t st) {
-    const dim3 grid((unsigned)((a.J + 15) / 16), a.offsets ? (unsigned)a.M : 1);
-    const size_t lds = x16 ? (size_t)MX4_FUSE * a.R * 4 * 17 / 32 : 0;
-    auto go = [&](auto kernel) { kernel<<<grid, 64 * MXR_WAVES, lds, st>>>(a, (const uint16_t*)x16, ldx); };
+    const int64_t K = (int64_t)a.R * 4, steps = mx4_steps(K), blocks = (int64_t)((a.J + 15) / 16) * (a.offsets ? a.M : 1);
+    int ks = 1;   // waves that share K
+    while (ks < MXR_WAVES && ks < steps && blocks * ks < 2048) ks *= 2;
+    const int rows = 16 * (MXR_WAVES / ks);
+    const dim3 grid((unsigned)((a.J + rows - 1) / rows), a.offsets ? (unsigned)a.M : 1);
+    const size_t lds = x16 ? (size_t)MX4_FUSE * (K / 2 + steps * 8) : 0;
+    auto go = [&](auto kernel) { kernel<<<grid, 64 * MXR_WAVES, lds, st>>>(a, (const uint16_t*)x16, ldx, ks); };
     if (x16) {
         if (a.f16) go(k_mx4_rows<true, true>);
         else go(k_mx4_rows<false, true>);

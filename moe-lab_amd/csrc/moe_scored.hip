@@ -33,15 +33,28 @@ __device__ __forceinline__ uint32_t key_of(float v) {
     const uint32_t b = __float_as_uint(v + 0.f);
     return b >> 31 ? ~b : b | 1u << 31;
 }
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+// Sums and maxima over lanes by DPP moves: a move through LDS (ds_bpermute) takes about ten times as long, and a token is a chain
+// of them (256 experts, k 8, one token: 10.0 us with those, 5.1 so; 4096 tokens 17.6 and 9.8).
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double moved64(double v) {   // lanes without a source: 0
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const u32x2 o = {(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[0], CTRL, ROWS, 0xF, false),
+                     (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[1], CTRL, ROWS, 0xF, false)};
+    return __builtin_bit_cast(double, o);
 }
-__device__ __forceinline__ float wave_max32(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
+__device__ __forceinline__ double lane64(double v, int lane) {   // of one lane, wave-uniform
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    const u32x2 o = {(uint32_t)__builtin_amdgcn_readlane((int)w[0], lane), (uint32_t)__builtin_amdgcn_readlane((int)w[1], lane)};
+    return __builtin_bit_cast(double, o);
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+    v += moved64<0xB1>(v);
+    v += moved64<0x4E>(v);
+    v += moved64<0x141>(v);
+    v += moved64<0x140>(v);
+    v += moved64<0x142, 0xA>(v);
+    v += moved64<0x143, 0xC>(v);
+    return lane64(v, 63);
 }
 
 // The value by which an expert ranks, or -inf (behind all others, weight 0) where the logit or its bias says so.
@@ -52,8 +65,23 @@ __device__ __forceinline__ double ranked(float l, double s, const float* bias, i
     return c == c ? c : -INFINITY;
 }
 
+// The larger two of a lane's pair and another's.
+__device__ __forceinline__ void join2(double& top, double& next, double t2, double n2) {
+    next = fmax(fmax(next, n2), fmin(top, t2));
+    top = fmax(top, t2);
+}
+// The two largest over aligned groups of `share` lanes (a power of two), in every lane.
+__device__ __forceinline__ void largest2(double& top, double& next, int share) {
+    if (share > 1) join2(top, next, moved64<0xB1>(top), moved64<0xB1>(next));
+    if (share > 2) join2(top, next, moved64<0x4E>(top), moved64<0x4E>(next));
+    if (share > 4) join2(top, next, moved64<0x141>(top), moved64<0x141>(next));
+    if (share > 8) join2(top, next, moved64<0x140>(top), moved64<0x140>(next));
+    if (share > 16) join2(top, next, __shfl_xor(top, 16), __shfl_xor(next, 16));
+}
+
+// WIDE: with a bias, 64-bit ranks.
 constexpr int SC_WAVES = 4;   // tokens of a workgroup
-template <typename LT, int JM>
+template <typename LT, int JM, bool WIDE>
 __global__ void __launch_bounds__(64 * SC_WAVES) k_topk_scored(const LT* logits, const ScoredArgs a, int32_t* idx, float* wts) {
     __shared__ double val[SC_WAVES][JM * 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -70,8 +98,8 @@ __global__ void __launch_bounds__(64 * SC_WAVES) k_topk_scored(const LT* logits,
     if (soft) {
 #pragma unroll
         for (int j = 0; j < JM; ++j) m = fmaxf(m, l[j]);
-        m = wave_max32(m);
-        if (a.bias || sums || !a.norm) {
+        m = wave_max_dpp(m);
+        if (WIDE || sums || !a.norm) {
             double p = 0.0;
 #pragma unroll
             for (int j = 0; j < JM; ++j) p += share64(l[j], m);
@@ -79,89 +107,99 @@ __global__ void __launch_bounds__(64 * SC_WAVES) k_topk_scored(const LT* logits,
             total = total > 0.0 ? total : 1.0;
         }
     }
-    double c[JM];
+    // keys: the high words, and (WIDE) the low ones; 0: not to be chosen (any more)
+    uint32_t hi[JM], lo[WIDE ? JM : 1];
 #pragma unroll
     for (int j = 0; j < JM; ++j) {
         const int e = 64 * j + lane;
         double s = 0.0;
-        if (a.bias || sums) s = soft ? share64(l[j], m) / total : sigmoid64(l[j]);
-        c[j] = e < E ? ranked(l[j], s, a.bias, e) : -INFINITY;
-        if (a.groups > 1) val[wave][e] = a.bias || !sums ? c[j] : l[j] == -INFINITY ? -INFINITY : s;
+        if (WIDE || sums) s = soft ? share64(l[j], m) / total : sigmoid64(l[j]);
+        if constexpr (WIDE) {
+            const double c = e < E ? ranked(l[j], s, a.bias, e) : -INFINITY;
+            const uint64_t k = key_of(c);
+            hi[j] = (uint32_t)(k >> 32);
+            lo[j] = (uint32_t)k;
+            if (a.groups > 1) val[wave][e] = c;
+        } else {
+            hi[j] = key_of(l[j]);
+            if (a.groups > 1) val[wave][e] = sums && l[j] != -INFINITY ? s : (double)l[j];
+        }
+        if (e >= E) hi[j] = 0;
     }
-    uint64_t live = ~0ull;   // bit g: group g stays
-    const int size = E / a.groups;
     if (a.groups > 1) {
+        const int size = E / a.groups;
         __builtin_amdgcn_wave_barrier();
-        int share = 64;   // lanes of a group: a power of two
+        int share = 64;   // lanes of a group
         while (share * a.groups > 64) share >>= 1;
-        const int g = lane / share, sub = lane & (share - 1);
+        const int g = lane / share;
         double top = -INFINITY, next = -INFINITY;
         if (g < a.groups)
-            for (int i = sub; i < size; i += share) {
+            for (int i = lane & (share - 1); i < size; i += share) {
                 const double v = val[wave][g * size + i];
                 next = fmax(next, fmin(top, v));
                 top = fmax(top, v);
             }
-        for (int d = share >> 1; d; d >>= 1) {
-            const double t2 = __shfl_xor(top, d), n2 = __shfl_xor(next, d);
-            next = fmax(fmax(next, n2), fmin(top, t2));
-            top = fmax(top, t2);
-        }
+        largest2(top, next, share);
         double v = sums ? top + next : top;
         v = v == v ? v : -INFINITY;
         int before = 0;
         for (int h = 0; h < a.groups; ++h) {
-            const double o = __shfl(v, h * share);
+            const double o = lane64(v, h * share);
             before += o > v || (o == v && h < g);
         }
-        const uint64_t stay = __ballot(g < a.groups && before < a.top_groups);
-        live = 0;
-        for (int h = 0; h < a.groups; ++h) live |= (stay >> (h * share) & 1ull) << h;
-    }
-    uint64_t key[JM];   // 0: not to be chosen (any more)
+        const uint64_t stay = __ballot(g < a.groups && before < a.top_groups);   // all of a group's lanes
 #pragma unroll
-    for (int j = 0; j < JM; ++j) {
-        const int e = 64 * j + lane;
-        key[j] = e < E && live >> (e / size) & 1 ? key_of(c[j]) : 0;
+        for (int j = 0; j < JM; ++j) {
+            const int e = 64 * j + lane;
+            if (e < E && !(stay >> (e / size * share) & 1)) hi[j] = 0;
+        }
     }
-    const uint64_t none = key_of(-(double)INFINITY);
+    const uint64_t none64 = key_of(-(double)INFINITY);
+    const uint32_t none = WIDE ? (uint32_t)(none64 >> 32) : key_of(-INFINITY), none_lo = (uint32_t)none64;
     int mine = 0;        // lane r holds round r's expert
     float ml = -INFINITY;
     for (int r = 0; r < a.k; ++r) {
-        uint64_t best = 0;
-        int id = 0x7fffffff;
+        uint32_t bh = hi[0], bl = WIDE ? lo[0] : 0;
+        int bj = 0;
 #pragma unroll
-        for (int j = 0; j < JM; ++j)
-            if (key[j] > best) {
-                best = key[j];
-                id = 64 * j + lane;
-            }
-#pragma unroll
-        for (int d = 32; d; d >>= 1) {
-            const uint64_t o = __shfl_xor(best, d);
-            const int oi = __shfl_xor(id, d);
-            if (o > best || (o == best && oi < id)) {
-                best = o;
-                id = oi;
+        for (int j = 1; j < JM; ++j) {
+            const bool more = hi[j] > bh || (WIDE && hi[j] == bh && lo[j] > bl);
+            bh = more ? hi[j] : bh;
+            if constexpr (WIDE) bl = more ? lo[j] : bl;
+            bj = more ? j : bj;
+        }
+        const uint32_t mh = wave_umax_dpp(bh);
+        uint64_t hit = __ballot(bh == mh);
+        uint32_t id;
+        if constexpr (WIDE) {
+            if (hit & (hit - 1)) {
+                const uint32_t low = wave_umax_dpp(bh == mh ? bl : 0);   // by all lanes
+                hit &= __ballot(bl == low);
             }
         }
+        if (hit & (hit - 1)) id = wave_min_dpp(hit >> lane & 1 ? (uint32_t)(64 * bj + lane) : 0xffffffffu);
+        else id = 64 * __builtin_amdgcn_readlane(bj, __builtin_ctzll(hit)) + __builtin_ctzll(hit);
+        const uint32_t ml_lo = WIDE ? (uint32_t)__builtin_amdgcn_readlane((int)bl, id & 63) : 0;
+        const bool out = mh == none && (!WIDE || ml_lo == none_lo);
         float lv = -INFINITY;
 #pragma unroll
         for (int j = 0; j < JM; ++j)
-            if (id == 64 * j + lane) {
-                key[j] = 0;
-                lv = l[j];
+            if (j == (int)(id >> 6)) {   // wave-uniform
+                lv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l[j]), id & 63));
+                if ((int)(id & 63) == lane) {
+                    hi[j] = 0;
+                    if constexpr (WIDE) lo[j] = 0;
+                }
             }
-        lv = __shfl(lv, id & 63);
         if (lane == r) {
             mine = id;
-            ml = best == none ? -INFINITY : lv;
+            ml = out ? -INFINITY : lv;
         }
     }
     double s = 0.0;
     if (ml != -INFINITY) s = !soft ? sigmoid64(ml) : a.norm ? 1.0 : share64(ml, m) / total;
     if (a.norm) {
-        if (soft) s = share64(ml, wave_max32(ml));
+        if (soft) s = share64(ml, wave_max_dpp(ml));
         const double sum = wave_sum64(s);
         s = sum > 0.0 ? s / sum : 0.0;
     }
@@ -201,13 +239,13 @@ __global__ void __launch_bounds__(64 * SC_WAVES) k_topk_scored_bwd(const LT* log
             v[j] = 64 * j + lane < E ? clean(as_f32<LT>(row[64 * j + lane])) : -INFINITY;
             m = fmaxf(m, v[j]);
         }
-        m = wave_max32(m);
+        m = wave_max_dpp(m);
 #pragma unroll
         for (int j = 0; j < JM; ++j) p += share64(v[j], m);
         total = wave_sum64(p);
         total = total > 0.0 ? total : 1.0;
     } else if (soft) {
-        m = wave_max32(l);
+        m = wave_max_dpp(l);
     }
     double s = 0.0, mean = 0.0;   // this lane's score (with norm: its share), and sum_j dw_j s_j
     if (l != -INFINITY) s = soft ? share64(l, m) : sigmoid64(l);
@@ -227,8 +265,8 @@ __global__ void __launch_bounds__(64 * SC_WAVES) k_topk_scored_bwd(const LT* log
 #pragma unroll
     for (int j = 0; j < JM; ++j) out[j] = dense ? -share64(v[j], m) / total * mean : 0.0;
     for (int r = 0; r < a.k; ++r) {
-        const int i = __shfl(id, r);
-        const double o = __shfl(g, r);
+        const int i = __builtin_amdgcn_readlane(id, r);
+        const double o = lane64(g, r);
 #pragma unroll
         for (int j = 0; j < JM; ++j) out[j] += i == 64 * j + lane ? o : 0.0;
     }
@@ -255,7 +293,9 @@ static int by_size(const ScoredArgs& a, F run) {
 template <typename LT>
 static int forward(const void* logits, const ScoredArgs& a, int32_t* idx, float* wts, hipStream_t st) {
     return by_size<LT>(a, [&](auto jm) {
-        k_topk_scored<LT, decltype(jm)::value><<<(a.T + SC_WAVES - 1) / SC_WAVES, 64 * SC_WAVES, 0, st>>>((const LT*)logits, a, idx, wts);
+        const unsigned grid = (a.T + SC_WAVES - 1) / SC_WAVES;
+        if (a.bias) k_topk_scored<LT, decltype(jm)::value, true><<<grid, 64 * SC_WAVES, 0, st>>>((const LT*)logits, a, idx, wts);
+        else k_topk_scored<LT, decltype(jm)::value, false><<<grid, 64 * SC_WAVES, 0, st>>>((const LT*)logits, a, idx, wts);
     });
 }
 template <typename LT>
