@@ -178,8 +178,8 @@ struct MmArgs {
     int touch;               // dw: read the operands through once at the start (set by the launcher)
     int f16, ydt, fill;      // ydt: MOE_DTYPE_*; fill: rows behind the last group are set to zero
     MmEpi epi;
-    // MXFP4 operands (forward, moe_mx4.h): a and b are codes, their sizes along r counted in 16-bit words of four, and these the
-    // exponents: a's in slot order, b's of E matrices; else null.
+    // MXFP4 operands (moe_mx4.h), else null. Forward: a and b are codes, their sizes along r counted in 16-bit words of four, and
+    // these the exponents, a's in slot order, b's of E matrices. dx: sb alone, b is codes.
     const uint8_t* sa;
     const uint8_t* sb;
 };
@@ -891,6 +891,7 @@ int launch_mm_dx(const MmArgs& a, hipStream_t st);
 int launch_mm_dw(const MmArgs& a, hipStream_t st);
 int launch_mm_rows(const MmArgs& a, hipStream_t st);   // forward, few rows (moe_mm_rows.hip)
 int launch_mm_mx4(const MmArgs& a, hipStream_t st);    // forward, MXFP4 operands (moe_mm_mx4.hip)
+int launch_mm_mx4_dx(const MmArgs& a, hipStream_t st); // dx, MXFP4 weights (moe_mm_mx4_dx.hip)
 
 // Tiles of the product kernel: 128 x 256 with 8 waves that multiply and 4 that load; 128 x 128 with 4 and 4, one workgroup on a
 // CU, 4 stages; 128 x 128 with 4 waves that do both, two workgroups on a CU (dw, and dx of few rows); 64 x 64, two on a CU.

@@ -21,6 +21,9 @@ static int launch(const MmArgs& a, hipStream_t st) {
         default: return launch_mm_cfg<MM_DX, F16, 2, 2, 2, 4, 2, 4>(a, st);
     }
 }
-int launch_mm_dx(const MmArgs& a, hipStream_t st) { return a.f16 ? launch<true>(a, st) : launch<false>(a, st); }
+int launch_mm_dx(const MmArgs& a, hipStream_t st) {
+    if (a.sb) return launch_mm_mx4_dx(a, st);
+    return a.f16 ? launch<true>(a, st) : launch<false>(a, st);
+}
 
 }  // namespace moe

@@ -60,6 +60,23 @@ moe::MmArgs product(const Problem& p, int64_t M, int E, int N, int dtype, void* 
     a.ydt = y_dtype;
     return a;
 }
+moe::MmArgs gradient(const void* dy, int64_t ld, const void* wc, const void* ws, int64_t M, int E, int N, int K, int dtype, void* dx,
+                     int dx_dtype) {
+    moe::MmArgs a{};
+    a.a = dy;
+    a.b = wc;
+    a.sb = (const uint8_t*)ws;
+    a.y = dx;
+    a.M = a.a_n = (int)M;
+    a.lda = (int)ld;
+    a.ldb = K;
+    a.E = E;
+    a.J = K;
+    a.R = N;
+    a.f16 = dtype == MOE_DTYPE_F16;
+    a.ydt = dx_dtype;
+    return a;
+}
 size_t linear_parts(int64_t T, int N, int K) {
     if (T <= moe::MX4_ROWS) return 0;
     const int parts = moe::mm_plan(moe::MM_FWD, T, N, K / 4, true).parts;
@@ -126,6 +143,40 @@ int moe_mx4_linear(const void* x, int64_t ldx, void* xc, void* xs, const void* w
     const int parts = moe::mm_plan(moe::MM_FWD, T, N, K / 4, true).parts;
     if (parts > 1) return moe::launch_mm_parts(moe::MM_FWD, a, parts, (float*)w, st);
     return moe::launch_mm_fwd(a, st);
+}
+
+size_t moe_mx4_linear_dx_workspace_bytes(int64_t T, int N, int K) {
+    if (bad_rows(T) || T == 0 || bad_n(N) || bad_k(K)) return 0;
+    const int parts = moe::mx4_dx_parts(T, N, K);
+    return parts > 1 ? (size_t)parts * T * K * 4 : 0;
+}
+
+int moe_mx4_linear_dx(const void* dz, int64_t lddz, const void* wc, const void* ws, int64_t T, int N, int K, int dtype, void* dx,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+    if (!two_byte(dtype)) return MOE_ERR_DTYPE;
+    if (bad_rows(T) || bad_n(N) || bad_k(K) || bad_ld(lddz, N)) return MOE_ERR_ARG;
+    if (T == 0) return MOE_OK;
+    if (!dz || !wc || !ws || !dx) return MOE_ERR_ARG;
+    if (misaligned(dz) || misaligned(wc) || misaligned(ws) || misaligned(dx) || misaligned(workspace)) return MOE_ERR_ALIGN;
+    const size_t need = moe_mx4_linear_dx_workspace_bytes(T, N, K);
+    if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE;
+    const moe::MmArgs a = gradient(dz, lddz, wc, ws, T, 1, N, K, dtype, dx, dtype);
+    const int parts = moe::mx4_dx_parts(T, N, K);
+    if (parts > 1) return moe::launch_mm_parts(moe::MM_DX, a, parts, (float*)workspace, (hipStream_t)stream);
+    return moe::launch_mm_dx(a, (hipStream_t)stream);
+}
+
+int moe_mx4_grouped_mm_dx(const void* dy, int64_t lddy, const void* wc, const void* ws, const int32_t* offsets, int64_t M, int E,
+                          int N, int K, int dtype, void* dx, int dx_dtype, int fill, void* stream) {
+    if (!two_byte(dtype) || (dx_dtype != dtype && dx_dtype != MOE_DTYPE_F32)) return MOE_ERR_DTYPE;
+    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || bad_rows(M) || bad_n(N) || bad_k(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
+    if (M == 0) return MOE_OK;
+    if (!dy || !wc || !ws || !dx) return MOE_ERR_ARG;
+    if (misaligned(dy) || misaligned(wc) || misaligned(ws) || misaligned(dx)) return MOE_ERR_ALIGN;
+    moe::MmArgs a = gradient(dy, lddy, wc, ws, M, E, N, K, dtype, dx, dx_dtype);
+    a.offsets = offsets;
+    a.fill = fill;
+    return moe::launch_mm_dx(a, (hipStream_t)stream);
 }
 
 size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int K, int indexed) {

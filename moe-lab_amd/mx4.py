@@ -25,23 +25,33 @@ STEP = 256                 # columns whose exponents lie together: 8 bytes of a 
 
 class Mx4:
     """A matrix [rows, K], or several [E, rows, K], in MXFP4. codes: uint8 [..., rows, K / 2], two codes to a byte, the low half
-    first; scales: the E8M0 bytes as the products read them (include/moe_mi355x.h)."""
-    __slots__ = ("codes", "scales")
+    first; scales: the E8M0 bytes as the products read them (include/moe_mi355x.h). Neither can be replaced."""
+    __slots__ = ("codes", "scales", "shape", "device")
 
     def __init__(self, codes, scales):
-        self.codes, self.scales = codes, scales
-        _check(self, "codes")
+        shape = (*codes.shape[:-1], 2 * codes.shape[-1])
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() not in (2, 3) or shape[-1] % BLOCK or not shape[-1]:
+            raise ValueError(f"uint8 codes [rows, K / 2] or [E, rows, K / 2] with K a multiple of {BLOCK}, and uint8 scales expected")
+        n = _scale_bytes(shape)
+        if scales.device != codes.device or tuple(scales.shape) != (n,) or not codes.is_contiguous() or not scales.is_contiguous():
+            raise ValueError(f"contiguous codes, and {n} bytes of scales on the same device expected")
+        if codes.data_ptr() % 16 or scales.data_ptr() % 16:
+            raise ValueError("16-byte aligned codes and scales expected")
+        _set(self, codes, scales, shape)
 
-    @property
-    def shape(self):
-        return (*self.codes.shape[:-1], 2 * self.codes.shape[-1])
+    def __setattr__(self, name, value):
+        raise AttributeError("an Mx4 is not changed: its products rely on the sizes it was made with")
 
-    @property
-    def device(self):
-        return self.codes.device
+    def __reduce__(self):
+        return Mx4, (self.codes, self.scales)
 
     def __repr__(self):
         return f"Mx4({list(self.shape)}, device='{self.device}')"
+
+
+def _set(q, codes, scales, shape):
+    for name, value in (("codes", codes), ("scales", scales), ("shape", shape), ("device", codes.device)):
+        object.__setattr__(q, name, value)
 
 
 def _scale_bytes(shape):
@@ -49,20 +59,10 @@ def _scale_bytes(shape):
     return 8 * E * shape[-2] * (-(-shape[-1] // STEP)) + 16
 
 
-def _check(q, name):
-    c, s = q.codes, q.scales
-    if c.dtype != torch.uint8 or s.dtype != torch.uint8 or c.dim() not in (2, 3) or c.shape[-1] % 16 or c.shape[-1] < 16:
-        raise ValueError(f"{name}: uint8 codes [rows, K / 2] or [E, rows, K / 2] with K a multiple of {BLOCK} expected")
-    if s.device != c.device or s.numel() != _scale_bytes(q.shape) or not c.is_contiguous() or not s.is_contiguous():
-        raise ValueError(f"{name}: contiguous codes, and {_scale_bytes(q.shape)} bytes of scales on the same device expected")
-    if c.data_ptr() % 16 or s.data_ptr() % 16:
-        raise ValueError(f"{name}: 16-byte aligned codes and scales expected")
-
-
 def _new(shape, device):
     q = Mx4.__new__(Mx4)
-    q.codes = torch.empty((*shape[:-1], shape[-1] // 2), dtype=torch.uint8, device=device)
-    q.scales = torch.empty(_scale_bytes(shape), dtype=torch.uint8, device=device)
+    _set(q, torch.empty((*shape[:-1], shape[-1] // 2), dtype=torch.uint8, device=device),
+         torch.empty(_scale_bytes(shape), dtype=torch.uint8, device=device), tuple(shape))
     return q
 
 
@@ -99,7 +99,6 @@ def quantize(x):
 
 def dequantize(q, dtype=torch.bfloat16):
     """The values of an Mx4, in its shape: exact in bf16 and fp32 (from 2^-126 on), rounded to fp16."""
-    _check(q, "q")
     _lib.require_device(q.codes, "q")
     if dtype not in _lib.DTYPE:
         raise TypeError(f"dtype {dtype}: bf16, fp16 or fp32 expected")
@@ -135,7 +134,6 @@ def from_packed(codes, scales):
 
 def to_packed(q):
     """(codes int32 [..., K / 8], scales uint8 [..., K / 32]) of an Mx4."""
-    _check(q, "q")
     E, N, S = q.shape[0] if len(q.shape) == 3 else 1, q.shape[-2], _steps_of(q.shape)
     s = q.scales[:-16].reshape(E, S, N, 2, 4).permute(0, 2, 1, 4, 3).reshape(E, N, 8 * S)[..., :q.shape[-1] // BLOCK]
     return q.codes.clone().view(torch.int32), s.reshape(*q.shape[:-1], -1).contiguous()
@@ -145,7 +143,6 @@ def to_packed(q):
 def _weights(w, dims, what):
     """w as an Mx4 of that many dimensions (16-bit numbers are quantised), and its type if it was 16-bit."""
     if isinstance(w, Mx4):
-        _check(w, "w")
         _lib.require_device(w.codes, "w")
         if len(w.shape) != dims:
             raise ValueError(f"w has shape {w.shape}: {what} expected")
@@ -163,7 +160,9 @@ def _weights(w, dims, what):
 
 def _type_of(x, w_type, out_dtype, *others):
     """The call's 16-bit type: x's, or for an Mx4 that of w or the other operands, else out_dtype if that is one, else bf16."""
-    types = {t.dtype for t in others if t is not None} | ({w_type} if w_type else set())
+    types = {t.dtype for t in others if t is not None}
+    if w_type is not None:
+        types.add(w_type)
     if not isinstance(x, Mx4):
         types.add(x.dtype)
     if len(types) > 1:
@@ -177,7 +176,6 @@ def _type_of(x, w_type, out_dtype, *others):
 def _operand(x, K, device, dims=None):
     """x as the library takes it: (16-bit rows or None, Mx4 or None, rows)."""
     if isinstance(x, Mx4):
-        _check(x, "x")
         if len(x.shape) != 2 or x.shape[1] != K:
             raise ValueError(f"x has shape {x.shape}: [rows, {K}] expected")
         if x.device != device:
@@ -239,18 +237,42 @@ class _Linear(torch.autograd.Function):
             if ctx.act != NONE:
                 dz = _linear._act_backward(dz, z, ctx.act, None, None)
             if need_x:
-                dx = _linear._dx(dz, dequantize(Mx4(wc, ws), ctx.dtype)).view(ctx.x_shape)
+                dx = _linear_dx(dz, Mx4(wc, ws)).view(ctx.x_shape)
             if need_w:
                 dw, db = _linear._dw(dz, dequantize(Mx4(xc, xs), ctx.dtype), need_b)
             elif need_b:
-                db = _sums(dz, None, 1)[0]
+                db = _linear._dw(dz, _no_columns(dz), True)[1]
         return dx, dw, None, db, None, dy if ctx.needs_input_grad[5] else None, None
 
 
-def _sums(dz, offsets, E):
-    """The bias gradient alone, [E, N]: dz's rows summed by group (the weight gradient's call on eight columns of zeros)."""
-    none = torch.zeros((dz.shape[0], 8), dtype=dz.dtype, device=dz.device)
-    return _grouped.mm_dw(dz, none, offsets, E, bias=True)[1]
+def _no_columns(dz):
+    """What the weight gradient's calls multiply where only the bias's is wanted: eight columns of zeros."""
+    return torch.zeros((dz.shape[0], 8), dtype=dz.dtype, device=dz.device)
+
+
+# Rows from which a dense dx multiplies by the weights' values, written out once, and not by the codes, which each tile of 128 rows
+# decodes anew (us from codes and values, w [4096, 4096]: 2048 rows 68 and 73, 4096 rows 130 and 124, 8192 rows 250 and 231).
+DECODE_ONCE = 4096
+
+
+def _linear_dx(dz, w4):
+    (T, N), K = dz.shape, w4.shape[1]
+    if T >= DECODE_ONCE:
+        return _linear._dx(dz, dequantize(w4, dz.dtype))
+    dx = torch.empty((T, K), dtype=dz.dtype, device=dz.device)
+    nws = _lib.lib().moe_mx4_linear_dx_workspace_bytes(T, N, K)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dz.device) if nws else None
+    _lib.call("moe_mx4_linear_dx", dz.device, dz.data_ptr(), dz.stride(0), w4.codes.data_ptr(), w4.scales.data_ptr(), T, N, K,
+              _lib.DTYPE[dz.dtype], dx.data_ptr(), _lib.ptr(ws), nws)
+    return dx
+
+
+def _grouped_dx(dy, w4, offsets):
+    M, (E, N, K) = dy.shape[0], w4.shape
+    dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
+    _lib.call("moe_mx4_grouped_mm_dx", dy.device, dy.data_ptr(), dy.stride(0), w4.codes.data_ptr(), w4.scales.data_ptr(),
+              _lib.ptr(offsets), M, E, N, K, _lib.DTYPE[dy.dtype], dx.data_ptr(), _lib.DTYPE[dy.dtype], 1)
+    return dx
 
 
 def linear(x, w, bias=None, act=NONE, residual=None, out_dtype=None):
@@ -312,11 +334,11 @@ class _GroupedMm(torch.autograd.Function):
         dy = _lib.half_matrix(dy.to(ctx.dtype), "dy")
         dx = dw = db = None
         if need_x:
-            dx = _grouped.mm_dx(dy, dequantize(Mx4(wc, ws), ctx.dtype), offsets)
+            dx = _grouped_dx(dy, Mx4(wc, ws), offsets)
         if need_w:
             dw, db = _grouped.mm_dw(dy, dequantize(Mx4(xc, xs), ctx.dtype), offsets, wc.shape[0], x_rows=rows, bias=True)
         elif need_b:
-            db = _sums(dy, offsets, wc.shape[0])
+            db = _grouped.mm_dw(dy, _no_columns(dy), offsets, wc.shape[0], bias=True)[1]
         return dx, dw, None, None, db if need_b else None, None, None
 
 
