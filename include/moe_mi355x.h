@@ -462,7 +462,8 @@ int moe_router_scored(const moe_scored_t* r, const void* x, const void* wr, cons
  *   moe_mx4_linear: y = act(x w^T + bias) + residual with w [N, K] in that form, and x either 16-bit rows [T, K] (ldx; then xc
  *       and xs receive its form, or are NULL) or, x NULL, its form xc, xs. bias [N], residual and z [T, N] of `dtype`, bf16 or
  *       fp16 (x's type); y of dtype or MOE_DTYPE_F32; act, z, workspace as moe_linear.
- *   moe_mx4_grouped_mm: moe_grouped_mm on w [E, N, K] and x [x_rows, K] in that form (x alike: 16-bit rows, or its form).
+ *   moe_mx4_grouped_mm: moe_grouped_mm on w [E, N, K] and x [x_rows, K] in that form (x alike: 16-bit rows, or its form). For the
+ *       workspace: indexed, an index list is given; has_form, xc and xs are.
  *   moe_mx4_linear_dx, moe_mx4_grouped_mm_dx: dx = dz w with w's values as `dtype` numbers (fp16: rounded to it), dz [T, N] (dy
  *       [M, N]) of `dtype`, as moe_linear_dx and moe_grouped_mm_dx without an index list.
  * Products of codes and powers of two are exact, their sums fp32; bias, activation and residual fp32, rounded once.
@@ -483,7 +484,7 @@ int moe_mx4_linear_dx(const void* dz, int64_t lddz, const void* wc, const void* 
                       void* workspace, size_t workspace_bytes, void* stream);
 int moe_mx4_grouped_mm_dx(const void* dy, int64_t lddy, const void* wc, const void* ws, const int32_t* offsets, int64_t M, int E,
                           int N, int K, int dtype, void* dx, int dx_dtype, int fill, void* stream);
-size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int K, int indexed);
+size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int E, int K, int indexed, int has_form);
 int moe_mx4_grouped_mm(const void* x, int64_t ldx, void* xc, void* xs, int64_t x_rows, const void* wc, const void* ws,
                        const void* bias, const int32_t* offsets, const int32_t* rows, int64_t M, int E, int N, int K, int dtype,
                        void* y, int y_dtype, int fill, void* workspace, size_t workspace_bytes, void* stream);

@@ -31,7 +31,6 @@ int launch_mx4_take_scales(const uint8_t* scales, int64_t n, int64_t K, const in
 int launch_mx4_rows(const MmArgs& a, const void* x16, int64_t ldx, hipStream_t st);
 constexpr int MX4_ROWS = 16;      // rows of a group that one pass multiplies
 int mx4_dx_parts(int64_t rows, int64_t N, int64_t K);   // parts of a dense product of dx (moe_mm_mx4_dx.hip)
-inline bool mx4_few(const MmArgs& a) { return a.offsets ? a.M / (a.E < a.M ? a.E : a.M) <= 1 : a.M <= MX4_ROWS; }
 constexpr int MX4_FUSE = 4;       // rows that are quantised inside the product
 constexpr int64_t MX4_FUSE_K = 1 << 16;   // and their elements in all, at most (LDS)
 

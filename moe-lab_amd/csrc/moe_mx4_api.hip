@@ -15,6 +15,9 @@ size_t x_bytes(int64_t rows, int64_t K) { return up256((size_t)rows * (K / 2)) +
 // whether x's rows are quantised inside the product of few rows
 bool fused(int64_t rows, int64_t K) { return rows <= moe::MX4_FUSE && moe::MX4_FUSE * K <= moe::MX4_FUSE_K; }
 
+// grouped: whether a group has one slot on average, of those that can have any
+bool few_slots(int64_t M, int64_t E) { return M / (E < M ? E : M) <= 1; }
+
 struct Problem {
     const void *x, *xc, *xs, *wc, *ws;
     int64_t x_rows, ldx;
@@ -139,7 +142,7 @@ int moe_mx4_linear(const void* x, int64_t ldx, void* xc, void* xs, const void* w
     char* w = (char*)workspace;
     rc = operand(p, dtype, w, a, st);
     if (rc) return rc;
-    if (moe::mx4_few(a)) return moe::launch_mx4_rows(a, nullptr, 0, st);
+    if (T <= moe::MX4_ROWS) return moe::launch_mx4_rows(a, nullptr, 0, st);
     const int parts = moe::mm_plan(moe::MM_FWD, T, N, K / 4, true).parts;
     if (parts > 1) return moe::launch_mm_parts(moe::MM_FWD, a, parts, (float*)w, st);
     return moe::launch_mm_fwd(a, st);
@@ -179,9 +182,10 @@ int moe_mx4_grouped_mm_dx(const void* dy, int64_t lddy, const void* wc, const vo
     return moe::launch_mm_dx(a, (hipStream_t)stream);
 }
 
-size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int K, int indexed) {
-    if (bad_rows(M) || bad_rows(x_rows) || M == 0 || bad_k(K)) return 0;
-    return x_bytes(x_rows, K) + (indexed ? up256(moe::mx4_scale_bytes(M, K)) : 0);
+size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int E, int K, int indexed, int has_form) {
+    if (bad_rows(M) || bad_rows(x_rows) || M == 0 || E < 1 || bad_k(K)) return 0;
+    if (few_slots(M, E) && !has_form && fused(1, K)) return 0;
+    return (has_form ? 0 : x_bytes(x_rows, K)) + (indexed && !few_slots(M, E) ? up256(moe::mx4_scale_bytes(M, K)) : 0);
 }
 
 int moe_mx4_grouped_mm(const void* x, int64_t ldx, void* xc, void* xs, int64_t x_rows, const void* wc, const void* ws,
@@ -197,8 +201,8 @@ int moe_mx4_grouped_mm(const void* x, int64_t ldx, void* xc, void* xs, int64_t x
     if (x_rows < (rows ? 1 : M)) return MOE_ERR_ARG;
     if (rows && x_rows * (K / 2) > 0xB0000000ll) return MOE_ERR_ARG;   // addressed with 32 bits from its start
     if (misaligned(bias) || misaligned(workspace)) return MOE_ERR_ALIGN;
-    const size_t need = moe_mx4_grouped_mm_workspace_bytes(M, x_rows, K, rows != nullptr);
-    if (workspace_bytes < need || !workspace) return MOE_ERR_WORKSPACE;
+    const size_t need = moe_mx4_grouped_mm_workspace_bytes(M, x_rows, E, K, rows != nullptr, xc != nullptr);
+    if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE;
     const hipStream_t st = (hipStream_t)stream;
     moe::MmArgs a = product(p, M, E, N, dtype, y, y_dtype);
     a.offsets = offsets;
@@ -206,7 +210,7 @@ int moe_mx4_grouped_mm(const void* x, int64_t ldx, void* xc, void* xs, int64_t x
     a.fill = fill;
     a.epi.bias = bias;
     a.kind = bias ? moe::EPI_LIN : moe::EPI_PLAIN;
-    const bool few = moe::mx4_few(a);
+    const bool few = few_slots(M, E);
     if (few && x && !xc && fused(1, K)) return moe::launch_mx4_rows(a, x, ldx, st);
     char* w = (char*)workspace;
     rc = operand(p, dtype, w, a, st);

@@ -13,6 +13,8 @@ metal_mxfp4_moe.py); experts.run_experts is that form.
 Gradients go straight through the roundings, in 16 bits: dx = dz w and dw = dz^T x at the values that the product used, of which
 x's are kept in 4 bits.
 """
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -160,7 +162,10 @@ def _weights(w, dims, what):
 
 def _type_of(x, w_type, out_dtype, *others):
     """The call's 16-bit type: x's, or for an Mx4 that of w or the other operands, else out_dtype if that is one, else bf16."""
-    types = {t.dtype for t in others if t is not None}
+    types = set()
+    for t in others:
+        if t is not None:
+            types.add(t.dtype)
     if w_type is not None:
         types.add(w_type)
     if not isinstance(x, Mx4):
@@ -184,13 +189,23 @@ def _operand(x, K, device, dims=None):
     _lib.require_device(x, "x")
     if x.dim() < 1 or x.shape[-1] != K or (dims is not None and x.dim() != dims):
         raise ValueError(f"x has shape {tuple(x.shape)}: [{'rows' if dims == 2 else '...'}, {K}] expected")
-    x2 = _lib.half_matrix(x.detach() if x.dim() == 2 else x.detach().reshape(-1, K), "x", K, device)
+    x2 = _lib.half_matrix(x if x.dim() == 2 else x.reshape(-1, K), "x", K, device)
     return x2, None, x2.shape[0]
 
 
 def _pointers(x2, q):
-    return (_lib.ptr(x2), x2.stride(0) if x2 is not None and x2.shape[0] > 1 else 0 if x2 is None else x2.shape[1],
-            None if q is None else q.codes.data_ptr(), None if q is None else q.scales.data_ptr())
+    rows = (None, 0) if x2 is None else (x2.data_ptr(), x2.stride(0) if x2.shape[0] > 1 else x2.shape[1])
+    return rows + ((None, None) if q is None else (q.codes.data_ptr(), q.scales.data_ptr()))
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, *sizes):
+    return getattr(_lib.lib(), name)(*sizes)
+
+
+def _workspace(device, name, *sizes):
+    n = _workspace_bytes(name, *sizes)
+    return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
 
 
 def _run_linear(x, w, bias, act, residual, out_dtype, keep):
@@ -209,8 +224,7 @@ def _run_linear(x, w, bias, act, residual, out_dtype, keep):
     z = torch.empty((T, N), dtype=dtype, device=device) if keep and act != NONE else None
     if keep and q is None:
         q = _new((T, K), device)
-    nws = _lib.lib().moe_mx4_linear_workspace_bytes(T, N, K)
-    ws = torch.empty(nws, dtype=torch.uint8, device=device) if nws else None
+    ws, nws = _workspace(device, "moe_mx4_linear_workspace_bytes", T, N, K)
     _lib.call("moe_mx4_linear", device, *_pointers(x2, q), w4.codes.data_ptr(), w4.scales.data_ptr(), _lib.ptr(bias),
               _lib.ptr(residual), int(act), T, N, K, _lib.DTYPE[dtype], y.data_ptr(), _lib.DTYPE[y.dtype], _lib.ptr(z), _lib.ptr(ws), nws)
     return y.view(*lead, N), z, q, w4
@@ -260,8 +274,7 @@ def _linear_dx(dz, w4):
     if T >= DECODE_ONCE:
         return _linear._dx(dz, dequantize(w4, dz.dtype))
     dx = torch.empty((T, K), dtype=dz.dtype, device=dz.device)
-    nws = _lib.lib().moe_mx4_linear_dx_workspace_bytes(T, N, K)
-    ws = torch.empty(nws, dtype=torch.uint8, device=dz.device) if nws else None
+    ws, nws = _workspace(dz.device, "moe_mx4_linear_dx_workspace_bytes", T, N, K)
     _lib.call("moe_mx4_linear_dx", dz.device, dz.data_ptr(), dz.stride(0), w4.codes.data_ptr(), w4.scales.data_ptr(), T, N, K,
               _lib.DTYPE[dz.dtype], dx.data_ptr(), _lib.ptr(ws), nws)
     return dx
@@ -309,11 +322,10 @@ def _run_grouped(x, w, offsets, bias, rows, out, out_dtype, keep):
     y = _lib.result(out, (M, N), dtype, out_dtype, device)
     if keep and q is None:
         q = _new((n, K), device)
-    nws = _lib.lib().moe_mx4_grouped_mm_workspace_bytes(M, n, K, int(rows is not None))
-    ws = torch.empty(nws, dtype=torch.uint8, device=device)
+    ws, nws = _workspace(device, "moe_mx4_grouped_mm_workspace_bytes", M, n, E, K, int(rows is not None), int(q is not None))
     _lib.call("moe_mx4_grouped_mm", device, *_pointers(x2, q), n, w4.codes.data_ptr(), w4.scales.data_ptr(), _lib.ptr(bias),
               _lib.ptr(offsets), _lib.ptr(rows), M, E, N, K, _lib.DTYPE[dtype], y.data_ptr(), _lib.DTYPE[y.dtype], int(out is None),
-              ws.data_ptr(), nws)
+              _lib.ptr(ws), nws)
     return y, q, w4
 
 

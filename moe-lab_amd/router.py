@@ -115,7 +115,8 @@ def group(idx, E):
 
 def _scored(E, k, score, bias, groups, top_groups, group_score, norm, scale, device):
     """The call's descriptor, its arguments checked, and the bias that it points to."""
-    if score not in _SCORES or group_score not in _GROUP_SCORES:
+    kind, by = _SCORES.get(score), _GROUP_SCORES.get(group_score)
+    if kind is None or by is None:
         raise ValueError(f"score {score!r}, group_score {group_score!r}: one of {list(_SCORES)}, one of {list(_GROUP_SCORES)} expected")
     if not 1 <= E <= 1024 or not 1 <= groups <= 64 or E % groups or not 1 <= top_groups <= groups:
         raise ValueError(f"{E} experts in {groups} groups, {top_groups} kept: at most 1024 in at most 64 equal groups expected")
@@ -129,8 +130,7 @@ def _scored(E, k, score, bias, groups, top_groups, group_score, norm, scale, dev
         if bias.dtype not in _lib.DTYPE or tuple(bias.shape) != (E,) or bias.device != device:
             raise ValueError(f"bias {bias.dtype} {tuple(bias.shape)} on {bias.device}: floating [{E}] on {device} expected")
         bias = _lib.dense(bias.detach(), torch.float32)
-    return _lib.Scored(E, k, _SCORES[score], groups, top_groups, _GROUP_SCORES[group_score], int(bool(norm)), float(scale),
-                       _lib.ptr(bias)), bias
+    return _lib.Scored(E, k, kind, groups, top_groups, by, 1 if norm else 0, scale, _lib.ptr(bias)), bias
 
 
 def _topk_scored(lg, desc):
