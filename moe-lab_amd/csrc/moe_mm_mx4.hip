@@ -72,10 +72,10 @@ struct MxKernel {
     static constexpr int CODES = (BI + BJ) * 128, STAGE = CODES + (SCA + SCB) * 1024;
     static constexpr int L = PA + PB + 1;
 
-    // XOR of the 16-byte pieces of a row: eight lanes that read at once have eight different ones. Rows of x go by lane; of w by
-    // column(): rows 0 .. 3 and 16 FB .. 16 FB + 3.
-    static __device__ __forceinline__ int swz_a(int r) { return r & 7; }
-    static __device__ __forceinline__ int swz_b(int r) { return (r & 3) | ((r >> 2 ^ r / (16 * FB)) & 1) << 2; }
+    // XOR of the 16-byte pieces of a row. Half a wave's reads take two cycles if none of the 16 places that 16 bytes can have in the
+    // banks occurs more than twice among them: two rows share a line of all banks, so 32 rows have each piece in four places of
+    // 8 with a XOR by the row, in all by its half (column()'s rows too): 588 of a step's 1180 cycles went to conflicts.
+    static __device__ __forceinline__ int swz(int r) { return r >> 1 & 7; }
     static __device__ __forceinline__ int column(int h, int m) { return (m >> 2 & 1) * 16 * FB + h * 16 + (m >> 3) * 4 + (m & 3); }
 
     static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* p, int64_t row0, int rows, int J, int es) {
@@ -223,7 +223,7 @@ struct MxKernel {
                 pb = (const char*)g.b + ((int64_t)(g.part ? 0 : lt.e) * g.J + lt.j0) * ld2 + (int64_t)first * 2;
 #pragma unroll
                 for (int i = 0; i < PA; ++i) {
-                    const int r = row + 8 * NL * i, c = (piece ^ swz_a(r)) * 16;
+                    const int r = row + 8 * NL * i, c = (piece ^ swz(r)) * 16;
                     int src = r;
                     if constexpr (GATHER) src = r < lt.rows ? g.arows[lt.lo + r] : -1;
                     offa[i] = !GATHER || (uint32_t)src < (uint32_t)g.a_n ? (uint32_t)src * (uint32_t)ld2 + c : MM_OOB;
@@ -231,7 +231,7 @@ struct MxKernel {
 #pragma unroll
                 for (int i = 0; i < PB; ++i) {
                     const int r = row + 8 * NL * i;
-                    offb[i] = (uint32_t)r * (uint32_t)ld2 + (piece ^ swz_b(r)) * 16;
+                    offb[i] = (uint32_t)r * (uint32_t)ld2 + (piece ^ swz(r)) * 16;
                 }
             };
             auto load = [&](uint32_t buf) {   // step ls
@@ -239,10 +239,10 @@ struct MxKernel {
                 if (left < 128 && lrows) {             // the last step ends inside a row: its pieces past the end
 #pragma unroll
                     for (int i = 0; i < PA; ++i)
-                        if ((piece ^ swz_a(row + 8 * NL * i)) * 16 >= left) offa[i] = MM_OOB;
+                        if ((piece ^ swz(row + 8 * NL * i)) * 16 >= left) offa[i] = MM_OOB;
 #pragma unroll
                     for (int i = 0; i < PB; ++i)
-                        if ((piece ^ swz_b(row + 8 * NL * i)) * 16 >= left) offb[i] = MM_OOB;
+                        if ((piece ^ swz(row + 8 * NL * i)) * 16 >= left) offb[i] = MM_OOB;
                 }
                 const uint32_t na = lrows ? (uint32_t)((GATHER ? g.a_n : lrows) - 1) * (uint32_t)ld2 + (uint32_t)left : 0,
                                nb = lrows ? (uint32_t)(min(BJ, g.J - lt.j0) - 1) * (uint32_t)ld2 + (uint32_t)left : 0;
@@ -295,13 +295,13 @@ struct MxKernel {
 #pragma unroll
         for (int f = 0; f < FA; ++f) {
             const int i = 32 * (NWI * f + wi) + r;
-            fa[f] = i * 128 + (hb ^ swz_a(i)) * 16;
+            fa[f] = i * 128 + (hb ^ swz(i)) * 16;
             xa[f] = CODES + i * 8 + hb * 4;
         }
 #pragma unroll
         for (int h = 0; h < FB; ++h) {
             const int j = 32 * FB * wj + column(h, r);
-            fb[h] = BI * 128 + j * 128 + (hb ^ swz_b(j)) * 16;
+            fb[h] = BI * 128 + j * 128 + (hb ^ swz(j)) * 16;
             xb[h] = CODES + SCA * 1024 + j * 8 + hb * 4;
         }
         f32x16 acc[FA][FB];

@@ -88,78 +88,88 @@ struct Mx4Dx {
             uint32_t offa[PA], offb[PC];
             const int KB = g.J / 2, ksteps = (g.J + 255) / 256;
             uint32_t wa = 0, wraw = 0, rraw = 0, wdec = 0;   // slots of the next loads, and of the codes and numbers of the next step
+            // where the streams are; a step adds to the pointers and takes from the counts
+            const char *pa = nullptr, *pc = nullptr, *ps = nullptr;
+            int lefta = 0, leftb = 0;      // of r, from the stream's step on
+            uint32_t basea = 0, cols = 0;   // bytes of dy's rows but the last, of a row of codes in this tile
             auto load_a = [&]() {
                 if (la.s >= la.steps) {
                     next_tile(la);
+                    const int first = la.t.e * g.part;
+                    pa = (const char*)g.a + (int64_t)la.t.lo * lda2 + (int64_t)first * 2;
+                    lefta = la.live ? la.r : 0;
+                    basea = la.live ? (uint32_t)(la.t.rows - 1) * (uint32_t)lda2 : 0u;
 #pragma unroll
                     for (int i = 0; i < PA; ++i) offa[i] = (uint32_t)((row + A::ROWS * i) * lda2 + col * 2);
                 }
-                const int first = la.t.e * g.part + 64 * la.s, left = la.r - 64 * la.s;
-                if (left < 64 && la.live && col >= left)   // the last step ends inside a row
+                if (lefta < 64 && col >= lefta)   // the last step ends inside a row
 #pragma unroll
                     for (int i = 0; i < PA; ++i) offa[i] = MM_OOB;
-                const srd_t d = srd_of((const char*)g.a + (int64_t)la.t.lo * lda2 + (int64_t)first * 2,
-                                       la.live ? (uint32_t)(la.t.rows - 1) * (uint32_t)lda2 + (uint32_t)left * 2 : 0u);
-                dma16<PA, NL * 1024>(d, offa, lds0 + wa + (uint32_t)(lw * 1024));
+                dma16<PA, NL * 1024>(srd_of(pa, basea + (uint32_t)lefta * 2), offa, lds0 + wa + (uint32_t)(lw * 1024));
                 ++la.s;
+                pa += 128;
+                lefta = max(lefta - 64, 0);
                 wa = after<RING>(wa, A::BYTES);
             };
             auto load_codes = [&]() {
                 if (lb.s >= lb.steps) {
                     next_tile(lb);
+                    const int first = lb.t.e * g.part, e = g.part ? 0 : lb.t.e;
+                    pc = (const char*)g.b + ((int64_t)e * g.R + first) * KB + lb.t.j0 / 2;
+                    ps = (const char*)g.sb + (((int64_t)e * ksteps + lb.t.j0 / 256) * g.R + first) * 8;
+                    leftb = lb.live ? lb.r : 0;
+                    cols = min(128, KB - lb.t.j0 / 2);
 #pragma unroll
                     for (int i = 0; i < PC; ++i)   // 8 rows a piece, 16 bytes a lane
                         offb[i] = lb.t.j0 + 32 * (lane & 7) < g.J ? (uint32_t)((i * NL + lw) * 8 + (lane >> 3)) * (uint32_t)KB + (lane & 7) * 16
                                                                   : MM_OOB;
                 }
-                const int first = lb.t.e * g.part + 64 * lb.s, n = min(64, lb.r - 64 * lb.s), e = g.part ? 0 : lb.t.e;
-                const srd_t dc = srd_of((const char*)g.b + ((int64_t)e * g.R + first) * KB + lb.t.j0 / 2,
-                                        lb.live ? (uint32_t)(n - 1) * (uint32_t)KB + min(128, KB - lb.t.j0 / 2) : 0u);
-                const srd_t ds = srd_of((const char*)g.sb + (((int64_t)e * ksteps + lb.t.j0 / 256) * g.R + first) * 8,
-                                        lb.live ? (uint32_t)n * 8 : 0u);
-                dma16<PC, NL * 1024>(dc, offb, lds0 + RAW + wraw + (uint32_t)(lw * 1024));
+                const int n = min(64, leftb);
+                dma16<PC, NL * 1024>(srd_of(pc, n ? (uint32_t)(n - 1) * (uint32_t)KB + cols : 0u), offb,
+                                     lds0 + RAW + wraw + (uint32_t)(lw * 1024));
                 const uint32_t off = lane * 16;
-                dma16<1, 0>(ds, &off, lds0 + RAW + wraw + CODES);   // by every wave: each loads as much as the others
+                dma16<1, 0>(srd_of(ps, (uint32_t)n * 8), &off, lds0 + RAW + wraw + CODES);   // by every wave: each loads as much
                 ++lb.s;
+                pc += (int64_t)64 * KB;
+                ps += 512;
+                leftb = max(leftb - 64, 0);
                 wraw = after<RING>(wraw, RAW_STEP);
             };
-            // A lane decodes rows 32 i + r of a step, columns 32 b ... Eight lanes that write at once have four rows and two blocks,
-            // whose granules lie in different banks.
+            // A lane decodes rows 32 i + r of a step, columns 32 b ... (16-byte writes take 13 cycles a wave at best, 8-byte ones 6.)
             const int r = 8 * lw + ((lane & 3) | (lane >> 5) << 2), b = (lane >> 2 & 1) << 1 | (lane >> 3 & 1) | (lane >> 4 & 1) << 2;
+            const uint32_t from = r * 128 + b * 16, fexp = CODES + r * 8 + mx4_byte(b);
+            uint32_t to[2];   // the block's two granules (row r + 32 has the same)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) to[h] = r * 2 * BJ + (((2 * b + h) ^ gran_swz<BJ>(r)) & (BJ / 16 - 1)) * 32;
             auto decode = [&]() {
                 u32x4 c[2];
                 uint32_t e[2];
                 const char* raw = sm + RAW + rraw;
-                char* to = sm + DEC + wdec;
+                char* dec = sm + DEC + wdec;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    c[i] = *(const u32x4*)(raw + (32 * i + r) * 128 + b * 16);
-                    e[i] = *(const uint8_t*)(raw + CODES + (32 * i + r) * 8 + mx4_byte(b));
+                    c[i] = *(const u32x4*)(raw + from + i * 32 * 128);
+                    e[i] = *(const uint8_t*)(raw + fexp + i * 32 * 8);
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const int n = 32 * i + r;
                     const float s = __uint_as_float(e[i] << 23);
 #pragma unroll
-                    for (int p = 0; p < 4; ++p)
-                        *(u32x4*)(to + n * 2 * BJ + (((2 * b + (p >> 1)) ^ gran_swz<BJ>(n)) & (BJ / 16 - 1)) * 32 + (p & 1) * 16) =
-                            decode8<F16>(c[i][p], s);
+                    for (int p = 0; p < 4; ++p) *(u32x4*)(dec + to[p >> 1] + i * 64 * BJ + (p & 1) * 16) = decode8<F16>(c[i][p], s);
                 }
                 if (__ballot(e[0] == 255 || e[1] == 255)) {   // blocks of NaN, whose codes are 0
                     for (int i = 0; i < 2; ++i)
-                        if (e[i] == 255) {
-                            const int n = 32 * i + r;
+                        if (e[i] == 255)
                             for (int p = 0; p < 4; ++p)
-                                *(u32x4*)(to + n * 2 * BJ + (((2 * b + (p >> 1)) ^ gran_swz<BJ>(n)) & (BJ / 16 - 1)) * 32 + (p & 1) * 16) =
+                                *(u32x4*)(dec + to[p >> 1] + i * 64 * BJ + (p & 1) * 16) =
                                     (u32x4){0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
-                        }
                 }
                 rraw = after<RING>(rraw, RAW_STEP);
                 wdec = after<2>(wdec, B::BYTES);
             };
             // Behind the barrier of step s the products read step s + 1. Step s + 2 is decoded (its codes have landed, and step s has
             // been read), dy of step s + 3 is loaded into the slot of step s, and the codes of step s + 4 into that of step s + 1.
-            // Before the next barrier, what was loaded behind the last one has to be here.
+            // Before the next barrier, what was loaded behind the last one has to be here. (A ring of four for the codes: no faster.)
             load_codes(), load_codes(), load_codes();
             load_a(), load_a(), load_a();
             wait_vm<0>();

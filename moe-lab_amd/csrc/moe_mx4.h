@@ -29,7 +29,9 @@ int launch_mx4_take_scales(const uint8_t* scales, int64_t n, int64_t K, const in
 // Products of few rows per group. x16 not null: a.a's rows are 16-bit numbers of the result's type there (ldx elements between
 // them), quantised by every workgroup for itself; else a.a, a.sa (not gathered: row arows[p]).
 int launch_mx4_rows(const MmArgs& a, const void* x16, int64_t ldx, hipStream_t st);
-constexpr int MX4_ROWS = 16;      // rows of a group that one pass multiplies
+// Dense products that the few-rows kernel takes: it reads x once per 16 rows of the weights, the tiles once per 64 or more (16 rows,
+// w [4096, 4096]: 4.9 us, in tiles 8.7; 32 rows 6.4 and 8.7, w [14336, 4096] 17.1 and 13.7).
+inline bool mx4_few_rows(int64_t T, int64_t N) { return T <= 16 || (T <= 32 && N <= 8192); }
 int mx4_dx_parts(int64_t rows, int64_t N, int64_t K);   // parts of a dense product of dx (moe_mm_mx4_dx.hip)
 constexpr int MX4_FUSE = 4;       // rows that are quantised inside the product
 constexpr int64_t MX4_FUSE_K = 1 << 16;   // and their elements in all, at most (LDS)

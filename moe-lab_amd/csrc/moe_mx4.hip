@@ -193,29 +193,36 @@ __device__ __forceinline__ f32x4 mma16(s16x8 a, uint32_t sa, s16x8 b, uint32_t s
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a), wide(b), c, 4, 4, B, (int)sa, B, (int)sb);
 }
 
-// Few rows: a wave multiplies 16 rows of the weights by up to 16 rows of x, with the weights' codes straight from memory as the
+// Few rows: a wave multiplies 16 rows of the weights by up to 16 NT rows of x, with the weights' codes straight from memory as the
 // matrix instruction's first operand. ks waves of a workgroup share the steps of K, and their sums meet in LDS, in the waves'
-// order. FUSE: x's rows are quantised here first, while the first weights are on their way.
+// order. FUSE: x's rows are quantised here first, while the first weights are on their way; else their codes come from memory too.
+// Bound by the weights' bytes and the latency of the first ones: AHEAD steps of a wave are loaded together.
 // Workgroups go by slot, not by group (as k_mm_rows): the one at a group's first slot does the group.
 constexpr int MXR_WAVES = 8;
-template <bool F16, bool FUSE>
+template <bool F16, bool FUSE, int NT>
 __global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, const uint16_t* x16, int64_t ldx, int ks) {
+    static_assert(!FUSE || NT == 1, "");
+    constexpr int ROWS = FUSE ? MX4_FUSE : 16 * NT, AHEAD = 4;
     extern __shared__ __attribute__((aligned(16))) uint8_t sx[];   // FUSE: codes [MX4_FUSE, K / 2], exponents [MX4_FUSE, steps, 8]
-    __shared__ f32x4 sums[MXR_WAVES][64];
+    __shared__ f32x4 sums[MXR_WAVES][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % ks;
     const int l = lane & 15, q = lane >> 4;
     const int wg0 = blockIdx.x * 16 * (MXR_WAVES / ks), n0 = wg0 + wave / ks * 16, p = blockIdx.y;
     int e = 0, lo = 0, hi = g.M;
     if (g.offsets) {
-        e = -1;   // the group whose first slot is p
-        for (int base = 0; base < g.E && e < 0; base += 64) {
-            int a = -1, b = -1;
-            if (base + lane < g.E) group_of<MM_FWD>(g, base + lane, a, b);
-            const uint64_t hit = __ballot(a == p && b > a);
-            if (hit) {
-                e = base + __builtin_ctzll(hit);
-                lo = p;
-                hi = __builtin_amdgcn_readlane(b, __builtin_ctzll(hit));
+        e = -1;   // the group whose first slot is p; 256 groups' offsets at once
+        for (int base = 0; base < g.E && e < 0; base += 256) {
+            int a[4], b[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) group_of<MM_FWD>(g, min(base + 64 * u + lane, g.E - 1), a[u], b[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const uint64_t hit = __ballot(base + 64 * u + lane < g.E && a[u] == p && b[u] > a[u]);
+                if (hit && e < 0) {
+                    e = base + 64 * u + __builtin_ctzll(hit);
+                    lo = p;
+                    hi = __builtin_amdgcn_readlane(b[u], __builtin_ctzll(hit));
+                }
             }
         }
         if (e < 0) {
@@ -237,14 +244,14 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, con
     const uint8_t* wc = (const uint8_t*)g.b + ((int64_t)e * g.J + n) * KB + q * 16;
     const uint8_t* ws = g.sb + ((int64_t)e * steps * g.J + n) * 8 + (q & 1) * 4;
     const int sh = (q >> 1) * 8;   // the first half step's exponent in byte 0, the second's in byte 2
-    constexpr int AHEAD = 4;       // steps of a wave whose weights are loaded together
     s16x8 w[AHEAD][2];
     uint32_t we[AHEAD];
     const s16x8 zero = {};
     auto load_w = [&](int s0) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            const int s = min(s0 + u * ks, steps - 1);
+            const int s = s0 + u * ks;
+            if (s >= steps) break;
 #pragma unroll
             for (int c = 0; c < 2; ++c)
                 w[u][c] = s * 256 + c * 128 + q * 32 < K ? *(const s16x8*)(wc + (int64_t)s * 128 + c * 64) : zero;
@@ -252,12 +259,16 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, con
         }
     };
     if (n0 < g.J) load_w(part);
-    for (int m0 = lo; m0 < hi; m0 += FUSE ? MX4_FUSE : MX4_ROWS) {
-        const int rows = min(hi - m0, FUSE ? MX4_FUSE : MX4_ROWS);
-        int src = -1;   // this lane's row of x
-        if (l < rows) {
-            src = g.arows ? g.arows[m0 + l] : m0 + l;
-            if ((uint32_t)src >= (uint32_t)g.a_n) src = -1;
+    for (int m0 = lo; m0 < hi; m0 += ROWS) {
+        const int rows = min(hi - m0, ROWS);
+        int src[NT];   // this lane's rows of x
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            src[i] = -1;
+            if (16 * i + l < rows) {
+                src[i] = g.arows ? g.arows[m0 + 16 * i + l] : m0 + 16 * i + l;
+                if ((uint32_t)src[i] >= (uint32_t)g.a_n) src[i] = -1;
+            }
         }
         if constexpr (FUSE) {
             if (m0 > lo) __syncthreads();   // the last rows are multiplied
@@ -275,45 +286,62 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, con
             }
             __syncthreads();
         }
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        f32x4 acc[NT] = {};
         if (n0 < g.J)
             for (int s0 = part; s0 < steps; s0 += AHEAD * ks) {
                 if (s0 != part || m0 > lo) load_w(s0);
+                s16x8 x[AHEAD][NT][2];
+                uint32_t xe[AHEAD][NT];
 #pragma unroll
                 for (int u = 0; u < AHEAD; ++u) {
                     const int s = s0 + u * ks;
                     if (s >= steps) break;
-                    s16x8 x[2] = {zero, zero};
-                    uint32_t xe = 0x7f7f7f7f;
-                    if (src >= 0) {
-                        const uint8_t* xc = FUSE ? sx + l * KB : (const uint8_t*)g.a + (int64_t)src * KB;
-                        const uint8_t* xs = FUSE ? sx + MX4_FUSE * KB + (l * steps + s) * 8 : g.sa + ((int64_t)s * g.a_n + src) * 8;
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        x[u][i][0] = x[u][i][1] = zero;
+                        xe[u][i] = 0x7f7f7f7f;
+                        if (src[i] < 0) continue;
+                        const uint8_t* xc = FUSE ? sx + l * KB : (const uint8_t*)g.a + (int64_t)src[i] * KB;
+                        const uint8_t* xs = FUSE ? sx + MX4_FUSE * KB + (l * steps + s) * 8 : g.sa + ((int64_t)s * g.a_n + src[i]) * 8;
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
-                            if (s * 256 + c * 128 + q * 32 < K) x[c] = *(const s16x8*)(xc + s * 128 + c * 64 + q * 16);
-                        xe = *(const uint32_t*)(xs + (q & 1) * 4) >> sh;
+                            if (s * 256 + c * 128 + q * 32 < K) x[u][i][c] = *(const s16x8*)(xc + s * 128 + c * 64 + q * 16);
+                        xe[u][i] = *(const uint32_t*)(xs + (q & 1) * 4) >> sh;
                     }
-                    acc = mma16<0>(w[u][0], we[u], x[0], xe, acc);
-                    acc = mma16<2>(w[u][1], we[u], x[1], xe, acc);
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    if (s0 + u * ks >= steps) break;
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        acc[i] = mma16<0>(w[u][0], we[u], x[u][i][0], xe[u][i], acc[i]);
+                        acc[i] = mma16<2>(w[u][1], we[u], x[u][i][1], xe[u][i], acc[i]);
+                    }
                 }
             }
         if (ks > 1) {
-            sums[wave][lane] = acc;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) sums[wave][i][lane] = acc[i];
             __syncthreads();
         }
         const int j = n0 + 4 * q;   // four neighbours of J (a multiple of 8)
-        if (part == 0 && l < rows && j < g.J) {
-            for (int i = 1; i < ks; ++i) acc += sums[wave + i][lane];
-            const int64_t at = (int64_t)(m0 + l) * g.J + j;
-            if (g.epi.bias) acc += load4<F16>(g.epi.bias, (int64_t)e * g.J + j);
-            if (g.epi.z) *(u32x2*)((uint16_t*)g.epi.z + at) = (u32x2){pack16<F16>(acc[0], acc[1]), pack16<F16>(acc[2], acc[3])};
+        if (part == 0 && j < g.J) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = lin_act(g.epi.act, acc[i]);
-            if (g.epi.residual) acc += load4<F16>(g.epi.residual, at);
-            if (g.ydt == MOE_DTYPE_F32) *(f32x4*)((float*)g.y + at) = acc;
-            else *(u32x2*)((uint16_t*)g.y + at) = (u32x2){pack16<F16>(acc[0], acc[1]), pack16<F16>(acc[2], acc[3])};
+            for (int i = 0; i < NT; ++i) {
+                if (16 * i + l >= rows) continue;
+                f32x4 v = acc[i];
+                for (int k = 1; k < ks; ++k) v += sums[wave + k][i][lane];
+                const int64_t at = (int64_t)(m0 + 16 * i + l) * g.J + j;
+                if (g.epi.bias) v += load4<F16>(g.epi.bias, (int64_t)e * g.J + j);
+                if (g.epi.z) *(u32x2*)((uint16_t*)g.epi.z + at) = (u32x2){pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3])};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[c] = lin_act(g.epi.act, v[c]);
+                if (g.epi.residual) v += load4<F16>(g.epi.residual, at);
+                if (g.ydt == MOE_DTYPE_F32) *(f32x4*)((float*)g.y + at) = v;
+                else *(u32x2*)((uint16_t*)g.y + at) = (u32x2){pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3])};
+            }
         }
-        if (ks > 1 && m0 + (FUSE ? MX4_FUSE : MX4_ROWS) < hi) __syncthreads();   // the sums are read
+        if (ks > 1 && m0 + ROWS < hi) __syncthreads();   // the sums are read
     }
 }
 
@@ -324,14 +352,15 @@ int launch_mx4_rows(const MmArgs& a, const void* x16, int64_t ldx, hipStream_t s
     const int rows = 16 * (MXR_WAVES / ks);
     const dim3 grid((unsigned)((a.J + rows - 1) / rows), a.offsets ? (unsigned)a.M : 1);
     const size_t lds = x16 ? (size_t)MX4_FUSE * (K / 2 + steps * 8) : 0;
-    auto go = [&](auto kernel) { kernel<<<grid, 64 * MXR_WAVES, lds, st>>>(a, (const uint16_t*)x16, ldx, ks); };
-    if (x16) {
-        if (a.f16) go(k_mx4_rows<true, true>);
-        else go(k_mx4_rows<false, true>);
-    } else {
-        if (a.f16) go(k_mx4_rows<true, false>);
-        else go(k_mx4_rows<false, false>);
-    }
+    auto go = [&](auto f16) {
+        constexpr bool F16 = decltype(f16)::value;
+        auto run = [&](auto kernel) { kernel<<<grid, 64 * MXR_WAVES, lds, st>>>(a, (const uint16_t*)x16, ldx, ks); };
+        if (x16) run(k_mx4_rows<F16, true, 1>);
+        else if (a.offsets || a.M <= 16) run(k_mx4_rows<F16, false, 1>);
+        else run(k_mx4_rows<F16, false, 2>);
+    };
+    if (a.f16) go(std::true_type{});
+    else go(std::false_type{});
     return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;
 }
 

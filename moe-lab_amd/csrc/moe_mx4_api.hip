@@ -81,7 +81,7 @@ moe::MmArgs gradient(const void* dy, int64_t ld, const void* wc, const void* ws,
     return a;
 }
 size_t linear_parts(int64_t T, int N, int K) {
-    if (T <= moe::MX4_ROWS) return 0;
+    if (moe::mx4_few_rows(T, N)) return 0;
     const int parts = moe::mm_plan(moe::MM_FWD, T, N, K / 4, true).parts;
     return parts > 1 ? up256((size_t)parts * T * N * 4) : 0;
 }
@@ -142,7 +142,7 @@ int moe_mx4_linear(const void* x, int64_t ldx, void* xc, void* xs, const void* w
     char* w = (char*)workspace;
     rc = operand(p, dtype, w, a, st);
     if (rc) return rc;
-    if (T <= moe::MX4_ROWS) return moe::launch_mx4_rows(a, nullptr, 0, st);
+    if (moe::mx4_few_rows(T, N)) return moe::launch_mx4_rows(a, nullptr, 0, st);
     const int parts = moe::mm_plan(moe::MM_FWD, T, N, K / 4, true).parts;
     if (parts > 1) return moe::launch_mm_parts(moe::MM_FWD, a, parts, (float*)w, st);
     return moe::launch_mm_fwd(a, st);

@@ -103,7 +103,7 @@ def test_layouts_and_packed_form():
 
 
 # ------------------------------------------------------------------------------------------------------ products
-SIZES = [(1, 8, 32), (1, 200, 1056), (2, 1024, 4096), (4, 264, 96), (5, 1024, 544), (16, 136, 2880), (17, 136, 288), (33, 2056, 160),
+SIZES = [(1, 8, 32), (1, 200, 1056), (2, 1024, 4096), (4, 264, 96), (5, 1024, 544), (16, 136, 2880), (17, 136, 288), (32, 264, 1056), (24, 8200, 96), (33, 2056, 160),
          (65, 520, 352), (130, 264, 1440), (237, 2048, 2816), (700, 136, 96), (1000, 1032, 224), (2048, 2048, 64), (513, 4104, 160),
          (300, 512, 8192), (3, 64, 20480)]
 
