@@ -13,7 +13,9 @@ Two levels, as in the reference:
       (reference e2e.py:66-68);
     - "deepseek": DeepSeek-V2 ``DeepseekV2Moe``: greedy gate = full-softmax probabilities of the top-k times
       ``routed_scaling_factor`` (reference e2e.py:129-150: the fused router for greedy gates, the stock gate for
-      group-limited ones), plus the shared experts added (e2e.py:146-147);
+      group-limited ones), plus the shared experts added (e2e.py:146-147). Group-limited softmax gates, and sigmoid gates
+      with a bias that ranks, run on router.route_scored if the gate's own forward does what that computes (and it is in
+      bf16, without hooks); any other gate stays stock;
     - "gpt-oss": ``GptOssMLP``: router with bias, top-k of the logits, softmax over them; MXFP4 experts stored
       transposed with gate and up interleaved, per-expert biases, clamped SwiGLU (reference e2e.py:153-175); the
       forward returns (y, routing weights) as the stock one does.
@@ -39,7 +41,7 @@ import math
 
 import torch
 
-from . import _lib, dense
+from . import _lib, dense, router
 from .experts import merge_shared, run_experts, run_layer, run_routed
 from .variants import hip_mxfp4_moe, hip_q4_moe
 
@@ -129,11 +131,12 @@ def _mlp_as_experts(mlp, F):
 @torch.no_grad()
 def block_state(block, fmt=None):
     """The block's packed state and call settings: {"kind", "state", "k", "norm", "scale", "act", "bias",
-    "stock_gate"} (stock_gate: route with the block's own gate, for gates the fused router does not implement)."""
+    "stock_gate", "scored"} (stock_gate: route by itself, not inside the layer call; scored: router.route_scored's settings,
+    or None: with the block's own gate)."""
     kind = block_kind(block)
     if kind is None:
         raise ValueError(f"{type(block).__name__}: not a sparse MoE block this patch knows")
-    cfg = {"kind": kind, "scale": 1.0, "bias": None, "stock_gate": False}
+    cfg = {"kind": kind, "scale": 1.0, "bias": None, "stock_gate": False, "scored": None}
     if kind == "gpt-oss":
         e, r = block.experts, block.router
         gu = e.gate_up_proj                       # [E, d, 2F], columns gate, up, gate, up, ...
@@ -156,7 +159,9 @@ def block_state(block, fmt=None):
     if kind == "deepseek":
         cfg["norm"] = False   # greedy: the full softmax's probabilities of the top-k
         cfg["scale"] = float(gate.routed_scaling_factor)
-        cfg["stock_gate"] = getattr(gate, "topk_method", "greedy") != "greedy"
+        cfg["stock_gate"] = getattr(gate, "topk_method", "greedy") != "greedy" or _choice_bias(gate) is not None
+        if cfg["stock_gate"]:
+            cfg["scored"] = _scored_settings(gate, cfg["k"])
         shared = block.shared_experts
     elif kind == "qwen2-shared":
         shared = block.shared_expert
@@ -173,8 +178,55 @@ def block_state(block, fmt=None):
     return cfg
 
 
+def _choice_bias(gate):
+    """The bias [E] that a sigmoid gate adds to its scores to choose by, or None."""
+    b = getattr(gate, "e_score_correction_bias", None)
+    return b if isinstance(b, torch.Tensor) else None
+
+
+def _scored_weights(x, weight, k, score, bias, groups, top_groups, group_score, norm, scale):
+    """router.topk_scored in plain 64-bit form, as weights [T, E] (0 for experts that are not chosen)."""
+    logits = x.double() @ weight.double().T
+    T, E = logits.shape
+    p = torch.softmax(logits, 1) if score == "softmax" else torch.sigmoid(logits)
+    c = p if bias is None else p + bias.double()
+    top = c.reshape(T, groups, -1).topk(1 if group_score == "max" else 2, dim=2).values.sum(2)
+    kept = torch.zeros_like(top).scatter(1, top.topk(top_groups, dim=1).indices, 1).bool().repeat_interleave(E // groups, 1)
+    idx = torch.where(kept, c, -math.inf).topk(k, dim=1).indices
+    w = p.gather(1, idx)
+    w = scale * (w / w.sum(1, keepdim=True) if norm else w)
+    return torch.zeros_like(p).scatter(1, idx, w)
+
+
+@torch.no_grad()
+def _scored_settings(gate, k):
+    """topk_scored's settings for a gate that it computes, without the bias, else None: checked on the gate's own forward, on
+    random tokens on the CPU. Gates that mask the other groups with 0 choose an expert there over a kept one whose score and
+    bias are negative together; with such a bias the gate stays stock."""
+    bias = _choice_bias(gate)
+    groups, top = int(getattr(gate, "num_group", 1) or 1), int(getattr(gate, "topk_group", 1) or 1)
+    if bias is None:
+        kw = dict(score="softmax", group_score="max", norm=False)
+    else:
+        kw = dict(score="sigmoid", group_score="top2", norm=bool(getattr(gate, "norm_topk_prob", True)))
+    kw |= dict(groups=groups, top_groups=top, scale=float(gate.routed_scaling_factor))
+    try:
+        router._scored(gate.weight.shape[0], k, kw["score"], None, groups, top, kw["group_score"], kw["norm"], kw["scale"], None)
+        if bias is not None and top < groups and float(bias.min()) < 0:
+            return None
+        g = _bare(gate).float()
+        x = torch.randn((64, g.weight.shape[1]), generator=torch.Generator("cpu").manual_seed(0), device="cpu")
+        x *= 2 / float((x @ g.weight.T).std())   # logits as far apart as a trained router's
+        out = g(x)
+        got = torch.zeros((64, g.weight.shape[0]), dtype=torch.float64, device="cpu").scatter(1, out[2].long(), out[1].double())
+        want = _scored_weights(x, g.weight, k, bias=_choice_bias(g), **kw)
+    except Exception:   # whatever a gate of another kind makes of these tokens
+        return None
+    return kw if float((got - want).abs().max()) <= 1e-4 * float(want.max()) else None
+
+
 def _route_stock(block, hidden):
-    """The block's own gate on the tokens (DeepSeek group-limited gates): (idx int32 [T, k], wts fp32 [T, k])."""
+    """The block's own gate on the tokens: (idx int32 [T, k], wts fp32 [T, k])."""
     out = block.gate(hidden)
     wts, idx = out[1], out[2]
     return idx.to(torch.int32).contiguous(), wts.float().contiguous()
@@ -198,7 +250,12 @@ def patch_block(block, fmt=None):
     def forward(hidden_states):
         shape = hidden_states.shape
         x = hidden_states.reshape(-1, shape[-1]).to(torch.bfloat16).contiguous()
-        if cfg["stock_gate"]:
+        gate = getattr(block, "gate", None)
+        if cfg["scored"] is not None and hidden_states.dtype == gate.weight.dtype == torch.bfloat16 and not _hooked(gate):
+            # the gate's own weight and bias, as they are now; in other types it computes with more digits than bf16 has
+            idx, wts = router.route_scored(x, gate.weight.detach(), cfg["k"], bias=_choice_bias(gate), **cfg["scored"])
+            y = run_layer(s, x, idx, wts, act=cfg["act"])
+        elif cfg["stock_gate"]:
             idx, wts = _route_stock(block, hidden_states.reshape(-1, shape[-1]))
             y = run_layer(s, x, idx, wts, act=cfg["act"])
         else:
