@@ -17,33 +17,24 @@ __device__ __forceinline__ f32x16 mma32(s16x8 a, uint32_t sa, s16x8 b, uint32_t 
     };
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, KS, (int)sa, KS, (int)sb);
 }
-// A lane's four 32-bit words from lane ^ X of its quad.
-template <int X>
-__device__ __forceinline__ u32x4 quad_xor(u32x4 v) {
-    constexpr int P = X == 1 ? 0xB1 : 0x4E;
-    u32x4 o;
+// Two pieces of a lane and of the one 16 further on: afterwards the first lane (of 0 .. 15, 32 .. 47) holds its own first piece in a
+// and the other's in b, the second one (16 .. 31, 48 .. 63) the first's second piece in a and its own in b. Its own inverse.
+__device__ __forceinline__ void swap16(u32x4& a, u32x4& b) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[i], P, 0xF, 0xF, false);
-    return o;
-}
-// W x W transposition (W 2 or 4) over W neighbouring lanes: afterwards lane q holds in c[j] what lane j held in c[q].
-template <int W>
-__device__ __forceinline__ void transpose(u32x4* c, int lane) {
-#pragma unroll
-    for (int i = 0; i < W; i += 2) {
-        const bool odd = lane & 1;
-        const u32x4 got = quad_xor<1>(odd ? c[i] : c[i + 1]);
-        if (odd) c[i] = got;
-        else c[i + 1] = got;
+    for (int i = 0; i < 4; ++i) {
+        const auto s = __builtin_amdgcn_permlane16_swap(a[i], b[i], false, false);
+        a[i] = s[0];
+        b[i] = s[1];
     }
-    if constexpr (W == 4) {
+}
+
+// The same with the lane 4 further on: the first one is of 0 .. 3 or 8 .. 11 of 16.
+__device__ __forceinline__ void swap4(u32x4& a, u32x4& b) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const bool high = lane & 2;
-            const u32x4 got = quad_xor<2>(high ? c[i] : c[i + 2]);
-            if (high) c[i] = got;
-            else c[i + 2] = got;
-        }
+    for (int i = 0; i < 4; ++i) {
+        const int x = a[i], y = b[i];
+        a[i] = __builtin_amdgcn_update_dpp(x, y, 0x114, 0xf, 0xa, false);   // from 4 lanes before, where bit 2 is set
+        b[i] = __builtin_amdgcn_update_dpp(y, x, 0x104, 0xf, 0x5, false);   // from 4 lanes after, where it is not
     }
 }
 
@@ -58,9 +49,10 @@ enum MxEpi { MX_PLAIN = 0, MX_LIN = 1, MX_ACT = 2 };
 // A stage is the operands' codes, 128 bytes a row, its 16-byte pieces XORed so that a fragment's rows spread over the banks, and
 // their exponents, 8 bytes a row. These lie in memory by steps (moe_mx4.h), so that a tile's are 1 KiB pieces, one to a loading
 // wave; their bytes are ordered so that a lane's four of a step are one word, which the instruction picks from.
-// The matrix instruction takes w's rows as its first operand, and row m of it is w's row column(m) of the wave's 32 FB, so that
-// a lane's sums of one row of x are 16 FB neighbours; a transposition over four lanes then makes every store instruction write
-// whole lines.
+// The matrix instruction takes w's rows as its first operand, and row m of it is w's row column(m) of a block's 32, so that a lane's
+// 16 sums of one row of x are neighbours. Exchanges with the lane of the row 16 further on and with that of the row 4 further on then
+// make every store instruction write whole lines, and loads of the residual read them. (Without the second exchange, half lines: 4096
+// x 8 rows of 128 experts, [1536, 2048], 97 us, with it 92; 32 experts, [5760, 2880], 4444 rows 118 and 112.)
 template <bool F16, int FA, int FB, int NWI, int NWJ, int ST, int GATHER, int EPI, int NL>
 struct MxKernel {
     static constexpr bool LIN = EPI != MX_PLAIN;
@@ -76,7 +68,7 @@ struct MxKernel {
     // banks occurs more than twice among them: two rows share a line of all banks, so 32 rows have each piece in four places of
     // 8 with a XOR by the row, in all by its half (column()'s rows too): 588 of a step's 1180 cycles went to conflicts.
     static __device__ __forceinline__ int swz(int r) { return r >> 1 & 7; }
-    static __device__ __forceinline__ int column(int h, int m) { return (m >> 2 & 1) * 16 * FB + h * 16 + (m >> 3) * 4 + (m & 3); }
+    static __device__ __forceinline__ int column(int m) { return (m >> 2 & 1) * 16 + (m >> 3) * 4 + (m & 3); }
 
     static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const void* p, int64_t row0, int rows, int J, int es) {
         return __builtin_amdgcn_make_buffer_rsrc((char*)const_cast<void*>(p) + row0 * J * es, 0,
@@ -86,91 +78,108 @@ struct MxKernel {
     // operands an empty descriptor. Residual rows are loaded as lines, like the stores, all before the first is needed.
     static __device__ __forceinline__ void store(const MmArgs& g, const MmTile& t, f32x16 (&acc)[FA][FB], int lane, int wi, int wj) {
         const bool f32 = g.ydt == MOE_DTYPE_F32;
-        const int ES = f32 ? 4 : 2, hb = lane >> 5;
-        const int jw = t.j0 + wj * 32 * FB + hb * 16 * FB;   // this lane's columns
+        const int ES = f32 ? 4 : 2, l = lane & 15, q = lane >> 4;
+        const int jw = t.j0 + wj * 32 * FB;   // the wave's columns; a lane's of block h: 32 h + 16 (lane >> 5) ..
         const int64_t row0 = (g.part ? (int64_t)t.e * g.M : 0) + t.lo;
         const auto yb = rows_of(g.y, row0, t.rows, g.J, ES), zb = rows_of(g.epi.z, row0, t.rows, g.J, 2),
                    rb = rows_of(g.epi.residual, row0, t.rows, g.J, 2);
-        constexpr int NC = 2 * FB, W = NC < 4 ? NC : 4;   // 16-bit: pieces of 8 columns of a lane; lanes that exchange
-        const int q = lane & (W - 1), first = lane & 31 & ~(W - 1);
-        // of piece u, W at a time: row j of the W, columns 8 (u & ~(W - 1)) + 8 q
-        const auto at = [&](int f, int u, int j) -> uint32_t {
-            const int i = 32 * (NWI * f + wi) + first + j, c = jw + 8 * ((u & ~(W - 1)) + q);
+        // 16-bit pieces of 8 columns after both exchanges: the x-th one of rows 16 s .. of row block f (one exchange where a wave has
+        // half a line of each row)
+        const auto at = [&](int f, int x, int s) -> uint32_t {
+            const int i = 32 * (NWI * f + wi) + 16 * s + (FB == 1 ? l : (l & 11) + 4 * x);
+            const int c = jw + (FB == 1 ? 0 : 32 * (l >> 2 & 1)) + 8 * q;
             return i < t.rows && c < g.J ? ((uint32_t)i * (uint32_t)g.J + c) * 2 : MM_OOB;
         };
-        u32x4 res[LIN ? FA : 1][NC];
+        const auto lines = [&](u32x4 (&v)[FB][2]) {   // between [column block][half of its 16] of a row and [x][s]
+            if constexpr (FB == 2) swap4(v[0][0], v[1][0]), swap4(v[0][1], v[1][1]);
+        };
+        const auto rows = [&](u32x4 (&v)[FB][2]) {
+#pragma unroll
+            for (int h = 0; h < FB; ++h) swap16(v[h][0], v[h][1]);
+        };
+        u32x4 res[LIN ? FA : 1][FB][2];
         if constexpr (LIN) {
 #pragma unroll
             for (int f = 0; f < FA; ++f)
 #pragma unroll
-                for (int u = 0; u < NC; ++u) res[f][u] = __builtin_amdgcn_raw_buffer_load_b128(rb, at(f, u, u & (W - 1)), 0, 0);
+                for (int x = 0; x < FB; ++x)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) res[f][x][s] = __builtin_amdgcn_raw_buffer_load_b128(rb, at(f, x, s), 0, 0);
         }
         const bool gelu = g.epi.act == MOE_LIN_GELU;
         const float c1 = gelu ? 1.5957691216057308f : 1.f, c3 = gelu ? 1.5957691216057308f * 0.044715f : 0.f;
 #pragma unroll
         for (int f = 0; f < FA; ++f) {
             if (32 * (NWI * f + wi) >= t.rows) break;
+            const auto store16 = [&](u32x4 (&v)[FB][2], __amdgpu_buffer_rsrc_t to) {
+                rows(v);
+                lines(v);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int x = 0; x < FB; ++x) __builtin_amdgcn_raw_buffer_store_b128(v[x][s], to, at(f, x, s), 0, 2);
+            };
             if constexpr (LIN) {
-                u32x4 zz[NC], bias[NC];   // loaded for each row block: its 32 values kept in fp32 would spill others
                 const auto bb = rows_of(g.epi.bias, t.e, 1, g.J, 2);
+                u32x4 zz[FB][2];
+                lines(res[f]);
+                rows(res[f]);
 #pragma unroll
-                for (int u = 0; u < NC; ++u)
-                    bias[u] = __builtin_amdgcn_raw_buffer_load_b128(bb, jw + 8 * u < g.J ? (jw + 8 * u) * 2 : MM_OOB, 0, 0);
+                for (int h = 0; h < FB; ++h) {
+                    u32x4 bias[2];   // loaded for each row block: kept in fp32 they would spill others
+                    const int c0 = jw + 32 * h + 16 * (lane >> 5);
 #pragma unroll
-                for (int u = 0; u < NC; u += W) transpose<W>(res[f] + u, lane);
+                    for (int u = 0; u < 2; ++u)
+                        bias[u] = __builtin_amdgcn_raw_buffer_load_b128(bb, c0 + 8 * u < g.J ? (c0 + 8 * u) * 2 : MM_OOB, 0, 0);
 #pragma unroll
-                for (int u = 0; u < NC; ++u) {
+                    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {   // two neighbours
-                        const int i = (u & 1) * 8 + 2 * c;
-                        float v[2];
+                        for (int c = 0; c < 4; ++c) {   // two neighbours
+                            const int i = u * 8 + 2 * c;
+                            float v[2];
 #pragma unroll
-                        for (int p = 0; p < 2; ++p) v[p] = acc[f][u >> 1][i + p] + un16<F16>(bias[u][c] >> (16 * p));
-                        zz[u][c] = pack16<F16>(v[0], v[1]);
+                            for (int p = 0; p < 2; ++p) v[p] = acc[f][h][i + p] + un16<F16>(bias[u][c] >> (16 * p));
+                            zz[h][u][c] = pack16<F16>(v[0], v[1]);
 #pragma unroll
-                        for (int p = 0; p < 2; ++p) {
-                            if constexpr (EPI == MX_ACT) v[p] *= sigmoid_fast(v[p] * (c1 + c3 * (v[p] * v[p])));
-                            acc[f][u >> 1][i + p] = v[p] + un16<F16>(res[f][u][c] >> (16 * p));
+                            for (int p = 0; p < 2; ++p) {
+                                if constexpr (EPI == MX_ACT) v[p] *= sigmoid_fast(v[p] * (c1 + c3 * (v[p] * v[p])));
+                                acc[f][h][i + p] = v[p] + un16<F16>(res[f][h][u][c] >> (16 * p));
+                            }
                         }
+                        __builtin_amdgcn_sched_barrier(0);   // not all pieces at once: they would spill
                     }
-                    __builtin_amdgcn_sched_barrier(0);   // not all pieces at once: they would spill
                 }
-                if (g.epi.z) {
-#pragma unroll
-                    for (int u = 0; u < NC; u += W) transpose<W>(zz + u, lane);
-#pragma unroll
-                    for (int u = 0; u < NC; ++u) __builtin_amdgcn_raw_buffer_store_b128(zz[u], zb, at(f, u, u & (W - 1)), 0, 2);
-                }
+                if (g.epi.z) store16(zz, zb);
             }
-            if (f32) {   // pieces of 4 columns
-                constexpr int NF = 4 * FB;
-                const int qf = lane & 3, rf = 32 * (NWI * f + wi) + (lane & 28);
+            if (f32) {   // pieces of 4 columns, a line to a block
 #pragma unroll
-                for (int u = 0; u < NF; u += 4) {
+                for (int h = 0; h < FB; ++h) {
                     u32x4 o[4];
 #pragma unroll
-                    for (int v = 0; v < 4; ++v)
+                    for (int u = 0; u < 4; ++u)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) o[v][c] = __float_as_uint(acc[f][(u + v) >> 2][((u + v) & 3) * 4 + c]);
-                    transpose<4>(o, lane);
+                        for (int c = 0; c < 4; ++c) o[u][c] = __float_as_uint(acc[f][h][u * 4 + c]);
+                    swap16(o[0], o[1]), swap16(o[2], o[3]);
+                    swap4(o[0], o[2]), swap4(o[1], o[3]);
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        const int i = rf + v, c = jw + 4 * (u + qf);
-                        __builtin_amdgcn_raw_buffer_store_b128(
-                            o[v], yb, i < t.rows && c < g.J ? ((uint32_t)i * (uint32_t)g.J + c) * 4 : MM_OOB, 0, 0);
-                    }
+                    for (int s = 0; s < 2; ++s)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int i = 32 * (NWI * f + wi) + 16 * s + (l & 11) + 4 * x;
+                            const int c = jw + 32 * h + 16 * (q >> 1) + 8 * (l >> 2 & 1) + 4 * (q & 1);
+                            __builtin_amdgcn_raw_buffer_store_b128(
+                                o[2 * x + s], yb, i < t.rows && c < g.J ? ((uint32_t)i * (uint32_t)g.J + c) * 4 : MM_OOB, 0, 0);
+                        }
                 }
             } else {
-                u32x4 o[NC];
+                u32x4 o[FB][2];
 #pragma unroll
-                for (int u = 0; u < NC; ++u)
+                for (int h = 0; h < FB; ++h)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        o[u][c] = pack16<F16>(acc[f][u >> 1][(u & 1) * 8 + 2 * c], acc[f][u >> 1][(u & 1) * 8 + 2 * c + 1]);
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int u = 0; u < NC; u += W) transpose<W>(o + u, lane);
-#pragma unroll
-                for (int u = 0; u < NC; ++u) __builtin_amdgcn_raw_buffer_store_b128(o[u], yb, at(f, u, u & (W - 1)), 0, 2);
+                        for (int c = 0; c < 4; ++c) o[h][u][c] = pack16<F16>(acc[f][h][u * 8 + 2 * c], acc[f][h][u * 8 + 2 * c + 1]);
+                store16(o, yb);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -300,7 +309,7 @@ struct MxKernel {
         }
 #pragma unroll
         for (int h = 0; h < FB; ++h) {
-            const int j = 32 * FB * wj + column(h, r);
+            const int j = 32 * (FB * wj + h) + column(r);
             fb[h] = BI * 128 + j * 128 + (hb ^ swz(j)) * 16;
             xb[h] = CODES + SCA * 1024 + j * 8 + hb * 4;
         }
