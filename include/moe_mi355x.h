@@ -466,6 +466,8 @@ int moe_router_scored(const moe_scored_t* r, const void* x, const void* wr, cons
  *       workspace: indexed, an index list is given; has_form, xc and xs are.
  *   moe_mx4_linear_dx, moe_mx4_grouped_mm_dx: dx = dz w with w's values as `dtype` numbers (fp16: rounded to it), dz [T, N] (dy
  *       [M, N]) of `dtype`, as moe_linear_dx and moe_grouped_mm_dx without an index list.
+ *   moe_mx4_bias_grad: db [E, N] of `dtype` = the sums of dy's rows by group (moe_grouped_mm's groups; offsets NULL with E = 1):
+ *       the gradient of a bias beside frozen weights. A group without rows: zeros.
  * Products of codes and powers of two are exact, their sums fp32; bias, activation and residual fp32, rounded once.
  * Requirements: K % 32 == 0, N % 8 == 0, K, N <= 2^20, rows <= 0x7fffff00, ldx % 8 == 0 and <= 2^21, E <= 1024; pointers 16-byte
  * aligned; x_rows K / 2 <= 0xB0000000 with an index list.
@@ -484,6 +486,9 @@ int moe_mx4_linear_dx(const void* dz, int64_t lddz, const void* wc, const void* 
                       void* workspace, size_t workspace_bytes, void* stream);
 int moe_mx4_grouped_mm_dx(const void* dy, int64_t lddy, const void* wc, const void* ws, const int32_t* offsets, int64_t M, int E,
                           int N, int K, int dtype, void* dx, int dx_dtype, int fill, void* stream);
+size_t moe_mx4_bias_grad_workspace_bytes(int64_t M, int E, int N);
+int moe_mx4_bias_grad(const void* dy, int64_t lddy, const int32_t* offsets, int64_t M, int E, int N, int dtype, void* db,
+                      void* workspace, size_t workspace_bytes, void* stream);
 size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int E, int K, int indexed, int has_form);
 int moe_mx4_grouped_mm(const void* x, int64_t ldx, void* xc, void* xs, int64_t x_rows, const void* wc, const void* ws,
                        const void* bias, const int32_t* offsets, const int32_t* rows, int64_t M, int E, int N, int K, int dtype,

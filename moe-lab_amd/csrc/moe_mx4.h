@@ -32,6 +32,10 @@ int launch_mx4_rows(const MmArgs& a, const void* x16, int64_t ldx, hipStream_t s
 // Dense products that the few-rows kernel takes: it reads x once per 16 rows of the weights, the tiles once per 64 or more (16 rows,
 // w [4096, 4096]: 4.9 us, in tiles 8.7; 32 rows 6.4 and 8.7, w [14336, 4096] 17.1 and 13.7).
 inline bool mx4_few_rows(int64_t T, int64_t N) { return T <= 16 || (T <= 32 && N <= 8192); }
+// Sums of dy's rows by group (gradients of biases beside frozen weights): groups of a.M slots, dy = a.a (a.lda), N = a.J, into y
+// of dy's type. parts: pieces of a group that workgroups share, > 1: joined from `sums`, fp32 [parts, E, N].
+int mx4_sum_parts(int64_t M, int64_t E, int64_t N);
+int launch_mx4_sums(const MmArgs& a, int parts, float* sums, hipStream_t st);
 int mx4_dx_parts(int64_t rows, int64_t N, int64_t K);   // parts of a dense product of dx (moe_mm_mx4_dx.hip)
 constexpr int MX4_FUSE = 4;       // rows that are quantised inside the product
 constexpr int64_t MX4_FUSE_K = 1 << 16;   // and their elements in all, at most (LDS)

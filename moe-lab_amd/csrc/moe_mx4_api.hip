@@ -182,6 +182,32 @@ int moe_mx4_grouped_mm_dx(const void* dy, int64_t lddy, const void* wc, const vo
     return moe::launch_mm_dx(a, (hipStream_t)stream);
 }
 
+size_t moe_mx4_bias_grad_workspace_bytes(int64_t M, int E, int N) {
+    if (bad_rows(M) || E < 1 || E > MM_MAX_E || bad_n(N)) return 0;
+    const int parts = moe::mx4_sum_parts(M, E, N);
+    return parts > 1 ? (size_t)parts * E * N * 4 : 0;
+}
+
+int moe_mx4_bias_grad(const void* dy, int64_t lddy, const int32_t* offsets, int64_t M, int E, int N, int dtype, void* db,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+    if (!two_byte(dtype)) return MOE_ERR_DTYPE;
+    if (E < 1 || E > MM_MAX_E || (!offsets && E != 1) || bad_rows(M) || bad_n(N) || bad_ld(lddy, N)) return MOE_ERR_ARG;
+    if (!db || (M && !dy)) return MOE_ERR_ARG;
+    if (misaligned(dy) || misaligned(db) || misaligned(workspace)) return MOE_ERR_ALIGN;
+    const size_t need = moe_mx4_bias_grad_workspace_bytes(M, E, N);
+    if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE;
+    moe::MmArgs a{};
+    a.a = dy;
+    a.y = db;
+    a.offsets = offsets;
+    a.M = (int)M;
+    a.lda = (int)lddy;
+    a.E = E;
+    a.J = N;
+    a.f16 = dtype == MOE_DTYPE_F16;
+    return moe::launch_mx4_sums(a, moe::mx4_sum_parts(M, E, N), (float*)workspace, (hipStream_t)stream);
+}
+
 size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int E, int K, int indexed, int has_form) {
     if (bad_rows(M) || bad_rows(x_rows) || M == 0 || E < 1 || bad_k(K)) return 0;
     if (few_slots(M, E) && !has_form && fused(1, K)) return 0;

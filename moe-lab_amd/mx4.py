@@ -255,13 +255,18 @@ class _Linear(torch.autograd.Function):
             if need_w:
                 dw, db = _linear._dw(dz, dequantize(Mx4(xc, xs), ctx.dtype), need_b)
             elif need_b:
-                db = _linear._dw(dz, _no_columns(dz), True)[1]
+                db = _bias_grad(dz, None, 1).view(-1)
         return dx, dw, None, db, None, dy if ctx.needs_input_grad[5] else None, None
 
 
-def _no_columns(dz):
-    """What the weight gradient's calls multiply where only the bias's is wanted: eight columns of zeros."""
-    return torch.zeros((dz.shape[0], 8), dtype=dz.dtype, device=dz.device)
+def _bias_grad(dy, offsets, E):
+    """Sums of dy's rows by group [E, N]."""
+    M, N = dy.shape
+    db = torch.empty((E, N), dtype=dy.dtype, device=dy.device)
+    ws, nws = _workspace(dy.device, "moe_mx4_bias_grad_workspace_bytes", M, E, N)
+    _lib.call("moe_mx4_bias_grad", dy.device, dy.data_ptr(), dy.stride(0), _lib.ptr(offsets), M, E, N, _lib.DTYPE[dy.dtype],
+              db.data_ptr(), _lib.ptr(ws), nws)
+    return db
 
 
 # Rows from which a dense dx multiplies by the weights' values, written out once, and not by the codes, which each tile of 128 rows
@@ -350,7 +355,7 @@ class _GroupedMm(torch.autograd.Function):
         if need_w:
             dw, db = _grouped.mm_dw(dy, dequantize(Mx4(xc, xs), ctx.dtype), offsets, wc.shape[0], x_rows=rows, bias=True)
         elif need_b:
-            db = _grouped.mm_dw(dy, _no_columns(dy), offsets, wc.shape[0], bias=True)[1]
+            db = _bias_grad(dy, offsets, wc.shape[0])
         return dx, dw, None, None, db if need_b else None, None, None
 
 

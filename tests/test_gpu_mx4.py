@@ -282,6 +282,36 @@ def test_grouped_gradients(counts, dtype, frozen):
             H.check(grads[2][e], ref, H.product_tol(ref, m, n, dtype) + d[r].abs().sum(0)[:, None] * sub)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("counts,tail,N", [([0], 5, 8), ([1, 0, 7], 2, 264), ([8, 9, 63, 64, 65, 129], 0, 520), ([0, 5000, 0], 3, 136),
+                                           ([1500] * 3, 0, 1024), ([3] * 1024, 1, 8)],
+                         ids=["empty", "few", "pieces of 8 rows", "one group has all", "shared by workgroups", "1024 groups"])
+def test_bias_gradients_beside_frozen_weights(counts, tail, N, dtype):
+    """Rows behind the last group (of NaN here) count for no bias, groups without rows get zeros."""
+    E, n, K = len(counts), sum(counts) + tail, 32
+    w, _ = M.random_mx4(E, N, K)
+    b = H.randn(E, N, dtype=dtype).requires_grad_()
+    dy = H.randn(n, N, dtype=dtype, seed=4)
+    dy[sum(counts):] = math.nan
+    y = mx4.grouped_mm(activations(n, K, dtype), w, H.offsets_of(counts), bias=b)
+    (db,) = torch.autograd.grad(y, b, dy)
+    ref = torch.zeros((E, N), dtype=torch.float64, device=DEV)
+    mags = torch.zeros_like(ref)
+    for e, r in H.ranges(counts):
+        ref[e], mags[e] = dy[r].double().sum(0), dy[r].double().abs().sum(0)
+    H.check(db, ref, H.product_tol(ref, mags, n, dtype))
+
+
+@pytest.mark.parametrize("T,N", [(0, 64), (1, 8), (100, 2056), (4097, 512)])
+def test_linear_bias_gradient_beside_frozen_weights(T, N):
+    w = M.first(M.random_mx4(1, N, 64)[0])
+    b = H.randn(N, dtype=torch.bfloat16).requires_grad_()
+    wide = H.randn(T, N + 24, dtype=torch.bfloat16, seed=4)
+    (db,) = torch.autograd.grad(mx4.linear(activations(T, 64, torch.bfloat16), w, bias=b), b, wide[:, 8:8 + N])
+    d = wide[:, 8:8 + N].double()
+    H.check(db, d.sum(0), H.product_tol(d.sum(0), d.abs().sum(0), T, torch.bfloat16))
+
+
 def test_grouped_weight_gradient_through_rows():
     T, N, K, E = 30, 64, 96, 4
     x, w = activations(T, K, torch.bfloat16), H.randn(E, N, K, dtype=torch.bfloat16, scale=0.1, seed=1).requires_grad_()
