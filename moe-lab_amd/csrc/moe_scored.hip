@@ -4,7 +4,11 @@
 //   k largest c, of equals the lowest id; w = scale s, divided by the chosen ones' sum with norm.
 // Two experts' scores can differ by less than fp32 keeps, and which one is chosen is the result, so scores and their sums are
 // fp64; ranking works on 64-bit integers that order as the numbers do, 32-bit ones without a bias.
-// One wave per token, expert 64 j + lane in a lane's slot j.
+// One wave per token, expert 64 j + lane in a lane's slot j. Bound by the latency of its chain, not by bytes or operations: the logits,
+// for a softmax its maximum and total, the groups' values, then k rounds of a maximum over the wave and one over its lanes' slots
+// (256 experts in 8 groups, k 8: 6.5 us for one token, 12.2 for 4096, whose logits are read in 1; 8191 tokens of 64 experts, k 6,
+// softmax without norm: forward 10.9 us, backward 8.0). With more tokens than the CUs hold waves the fp64 exponentials add up: they
+// are taken only where they rank or scale.
 #include "moe_common.h"
 #include "moe_scored.h"
 
@@ -34,7 +38,7 @@ __device__ __forceinline__ uint32_t key_of(float v) {
     return b >> 31 ? ~b : b | 1u << 31;
 }
 // Sums and maxima over lanes by DPP moves: a move through LDS (ds_bpermute) takes about ten times as long, and a token is a chain
-// of them (256 experts, k 8, one token: 10.0 us with those, 5.1 so; 4096 tokens 17.6 and 9.8).
+// of them (256 experts, k 8, one token: 10.0 us with those, 6.5 so; 4096 tokens 17.6 and 12.2).
 template <int CTRL, int ROWS = 0xF>
 __device__ __forceinline__ double moved64(double v) {   // lanes without a source: 0
     const u32x2 w = __builtin_bit_cast(u32x2, v);
@@ -226,9 +230,11 @@ __global__ void __launch_bounds__(64 * SC_WAVES) k_topk_scored_bwd(const LT* log
     double dw = 0.0;
     if (lane < a.k) {
         id = idx[(int64_t)t * a.k + lane];
-        l = clean(as_f32<LT>(row[id]));
-        if (a.bias && ranked(l, 0.0, a.bias, id) == -INFINITY) l = -INFINITY;
-        dw = (double)dwts[(int64_t)t * a.k + lane] * (double)a.scale;
+        if ((uint32_t)id < (uint32_t)E) {   // (no expert: no gradient)
+            l = clean(as_f32<LT>(row[id]));
+            if (a.bias && ranked(l, 0.0, a.bias, id) == -INFINITY) l = -INFINITY;
+        }
+        if (l != -INFINITY) dw = (double)dwts[(int64_t)t * a.k + lane] * (double)a.scale;
     }
     float v[JM], m = -INFINITY;
     double total = 1.0;

@@ -162,6 +162,8 @@ def block_state(block, fmt=None):
         cfg["stock_gate"] = getattr(gate, "topk_method", "greedy") != "greedy" or _choice_bias(gate) is not None
         if cfg["stock_gate"]:
             cfg["scored"] = _scored_settings(gate, cfg["k"])
+            if cfg["scored"] is not None:
+                _bias_fits(cfg, gate)
         shared = block.shared_experts
     elif kind == "qwen2-shared":
         shared = block.shared_expert
@@ -225,6 +227,20 @@ def _scored_settings(gate, k):
     return kw if float((got - want).abs().max()) <= 1e-4 * float(want.max()) else None
 
 
+def _bias_fits(cfg, gate):
+    """Whether the gate's bias, as it is now, lets route_scored choose as the gate does (_scored_settings). Looked at again only
+    after it changed; while a graph is captured, or where changes leave no trace, a bias that has changed means the stock gate."""
+    bias, kw = _choice_bias(gate), cfg["scored"]
+    if bias is None or kw["top_groups"] == kw["groups"]:
+        return True
+    seen = None if bias.is_inference() else (bias.data_ptr(), bias._version)
+    if cfg.get("bias_seen", 0) != seen or seen is None:
+        if seen is None or (bias.is_cuda and torch.cuda.is_current_stream_capturing()):
+            return False
+        cfg["bias_fits"], cfg["bias_seen"] = float(bias.detach().min()) >= 0, seen
+    return cfg["bias_fits"]
+
+
 def _route_stock(block, hidden):
     """The block's own gate on the tokens: (idx int32 [T, k], wts fp32 [T, k])."""
     out = block.gate(hidden)
@@ -251,9 +267,10 @@ def patch_block(block, fmt=None):
         shape = hidden_states.shape
         x = hidden_states.reshape(-1, shape[-1]).to(torch.bfloat16).contiguous()
         gate = getattr(block, "gate", None)
-        if cfg["scored"] is not None and hidden_states.dtype == gate.weight.dtype == torch.bfloat16 and not _hooked(gate):
+        if (cfg["scored"] is not None and hidden_states.dtype == gate.weight.dtype == torch.bfloat16 and not _hooked(gate)
+                and _bias_fits(cfg, gate)):
             # the gate's own weight and bias, as they are now; in other types it computes with more digits than bf16 has
-            idx, wts = router.route_scored(x, gate.weight.detach(), cfg["k"], bias=_choice_bias(gate), **cfg["scored"])
+            idx, wts = router.route_scored(x.detach(), gate.weight.detach(), cfg["k"], bias=_choice_bias(gate), **cfg["scored"])
             y = run_layer(s, x, idx, wts, act=cfg["act"])
         elif cfg["stock_gate"]:
             idx, wts = _route_stock(block, hidden_states.reshape(-1, shape[-1]))

@@ -413,6 +413,44 @@ def test_other_stream_and_repeat():
         assert torch.equal(first, again)
 
 
+def test_two_streams_at_once():
+    """Calls of every path on two streams, each with its own operands, equal the ones made one after the other."""
+    w, _ = M.random_mx4(6, 520, 288)
+    dense = [M.first(mx4.Mx4(w.codes[e:e + 1], M.random_mx4(1, 520, 288, seed=e)[0].scales)) for e in (0, 1)]
+    counts = ([3, 0, 40, 1, 9, 47], [0, 100, 0, 0, 0, 0])
+    xs = [activations(100, 288, torch.bfloat16, seed=s) for s in (0, 1)]
+    dy = [H.randn(100, 520, dtype=torch.bfloat16, seed=s) for s in (2, 3)]
+    offs = [H.offsets_of(c) for c in counts]
+
+    def calls(i):
+        x = xs[i]
+        return [mx4.linear(x[:1], dense[i]), mx4.linear(x[:20], dense[i], act=GELU), mx4.linear(x, dense[i]),
+                mx4.grouped_mm(x, w, offs[i]), mx4._linear_dx(dy[i], dense[i]), mx4._grouped_dx(dy[i], w, offs[i]),
+                mx4._bias_grad(dy[i], offs[i], 6)]
+    want = [calls(0), calls(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(calls(i))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
+
+
+def test_training_calls_without_rows():
+    x = torch.zeros(0, 96, dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    w, b = H.randn(64, 96, dtype=torch.bfloat16).requires_grad_(), H.randn(64, dtype=torch.bfloat16).requires_grad_()
+    for g, t in zip(torch.autograd.grad(mx4.linear(x, w, bias=b, act=SILU).sum(), (x, w, b)), (x, w, b)):
+        assert g.shape == t.shape and not g.any()
+    w, b = H.randn(3, 64, 96, dtype=torch.bfloat16).requires_grad_(), H.randn(3, 64, dtype=torch.bfloat16).requires_grad_()
+    for g, t in zip(torch.autograd.grad(mx4.grouped_mm(x, w, H.offsets_of([0, 0, 0]), bias=b).sum(), (x, w, b)), (x, w, b)):
+        assert g.shape == t.shape and not g.any()
+
+
 def test_routed_layer_of_the_operators():
     """Router, grouping, both products of an expert layer and its GLU, as a program would run them, against 64 bits with the
     intermediate rows rounded where the calls round them."""

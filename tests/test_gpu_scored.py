@@ -163,6 +163,20 @@ def test_masked_experts_have_no_gradient():
                 assert (dl[1, [5, 9]] != 0).any() and (dl[1, 10:] == 0).all()
 
 
+def test_gradients_of_masked_experts_weights_count_for_nothing():
+    """Whatever reaches the weight of an expert that was chosen at -inf, an infinity or NaN too."""
+    logits = torch.tensor([[1.0, 2.0, -math.inf, -math.inf], [0.5, -math.inf, -math.inf, -math.inf]], device=DEV)
+    for score, norm in itertools.product(("softmax", "sigmoid"), (True, False)):
+        grads = []
+        for bad in (0.0, math.inf, math.nan):
+            lg = logits.clone().requires_grad_()
+            idx, wts = router.topk_scored(lg, 3, score=score, norm=norm)
+            dw = torch.tensor([[0.3, -0.7, bad], [0.2, bad, bad]], device=DEV)
+            grads.append(torch.autograd.grad(wts, lg, dw)[0])
+        assert torch.isfinite(grads[0]).all()
+        assert torch.equal(grads[0], grads[1]) and torch.equal(grads[0], grads[2])
+
+
 def test_layouts_batches_empty():
     logits, bias = make(12, 64, torch.float32)
     idx, wts = router.topk_scored(logits, 4)

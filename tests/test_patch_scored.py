@@ -100,3 +100,47 @@ def test_the_gates_bias_is_read_when_it_is_used():
         first = block(x)
         block.gate.e_score_correction_bias.copy_(block.gate.e_score_correction_bias.flip(0) * 5)
         assert not torch.equal(first, block(x))
+
+
+@pytest.mark.gpu
+def test_a_bias_that_becomes_negative_brings_the_gate_back():
+    """Also in a graph that is captured after the change, where the bias cannot be looked at."""
+    block = sigmoid_block("cuda")
+    patch.patch_block(block)
+    x = torch.randn(1, 8, D, generator=torch.Generator().manual_seed(3)).to("cuda", torch.bfloat16)
+    calls = []
+    stock = type(block.gate).forward
+
+    class Counted(type(block.gate)):
+        def forward(self, x):
+            calls.append(1)
+            return stock(self, x)
+    block.gate.__class__ = Counted
+    bias = block.gate.e_score_correction_bias
+    with torch.no_grad():
+        for shift, own in ((0.0, True), (-1.0, False), (1.0, True), (0.5, True)):
+            bias += shift
+            calls.clear()
+            block(x)
+            assert len(calls) == (0 if own else 1), shift
+        calls.clear()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = block(x)
+        assert not calls
+        eager = block(x)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, eager)
+
+
+@pytest.mark.gpu
+def test_hidden_states_that_require_grad():
+    """A patched block has no backward pass; with gradients enabled it still runs."""
+    block = sigmoid_block("cuda")
+    patch.patch_block(block)
+    x = torch.randn(1, 8, D, generator=torch.Generator().manual_seed(3)).to("cuda", torch.bfloat16)
+    with torch.no_grad():
+        want = block(x)
+    assert torch.equal(block(x.requires_grad_()), want)
