@@ -463,7 +463,7 @@ int moe_router_scored(const moe_scored_t* r, const void* x, const void* wr, cons
  *       and xs receive its form, or are NULL) or, x NULL, its form xc, xs. bias [N], residual and z [T, N] of `dtype`, bf16 or
  *       fp16 (x's type); y of dtype or MOE_DTYPE_F32; act, z, workspace as moe_linear.
  *   moe_mx4_grouped_mm: moe_grouped_mm on w [E, N, K] and x [x_rows, K] in that form (x alike: 16-bit rows, or its form). For the
- *       workspace: indexed, an index list is given; has_form, xc and xs are.
+ *       workspace: has_form, xc and xs are given.
  *   moe_mx4_linear_dx, moe_mx4_grouped_mm_dx: dx = dz w with w's values as `dtype` numbers (fp16: rounded to it), dz [T, N] (dy
  *       [M, N]) of `dtype`, as moe_linear_dx and moe_grouped_mm_dx without an index list.
  *   moe_mx4_bias_grad: db [E, N] of `dtype` = the sums of dy's rows by group (moe_grouped_mm's groups; offsets NULL with E = 1):
@@ -489,7 +489,7 @@ int moe_mx4_grouped_mm_dx(const void* dy, int64_t lddy, const void* wc, const vo
 size_t moe_mx4_bias_grad_workspace_bytes(int64_t M, int E, int N);
 int moe_mx4_bias_grad(const void* dy, int64_t lddy, const int32_t* offsets, int64_t M, int E, int N, int dtype, void* db,
                       void* workspace, size_t workspace_bytes, void* stream);
-size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int E, int K, int indexed, int has_form);
+size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int E, int K, int has_form);
 int moe_mx4_grouped_mm(const void* x, int64_t ldx, void* xc, void* xs, int64_t x_rows, const void* wc, const void* ws,
                        const void* bias, const int32_t* offsets, const int32_t* rows, int64_t M, int E, int N, int K, int dtype,
                        void* y, int y_dtype, int fill, void* workspace, size_t workspace_bytes, void* stream);

@@ -133,7 +133,7 @@ def lib():
         L.moe_mx4_dequantize.argtypes = [vp, vp, i64, i64, i, vp, i, vp]
         L.moe_mx4_linear_workspace_bytes.argtypes = [i64, i, i]
         L.moe_mx4_linear.argtypes = [vp, i64, vp, vp, vp, vp, vp, vp, i, i64, i, i, i, vp, i, vp, vp, sz, vp]
-        L.moe_mx4_grouped_mm_workspace_bytes.argtypes = [i64, i64, i, i, i, i]
+        L.moe_mx4_grouped_mm_workspace_bytes.argtypes = [i64, i64, i, i, i]
         L.moe_mx4_grouped_mm.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, vp, vp, i64, i, i, i, i, vp, i, i, vp, sz, vp]
         L.moe_mx4_linear_dx_workspace_bytes.argtypes = [i64, i, i]
         L.moe_mx4_linear_dx.argtypes = [vp, i64, vp, vp, i64, i, i, i, vp, vp, sz, vp]

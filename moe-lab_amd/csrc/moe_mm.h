@@ -179,7 +179,7 @@ struct MmArgs {
     int f16, ydt, fill;      // ydt: MOE_DTYPE_*; fill: rows behind the last group are set to zero
     MmEpi epi;
     // MXFP4 operands (moe_mx4.h), else null. Forward: a and b are codes, their sizes along r counted in 16-bit words of four, and
-    // these the exponents, a's in slot order, b's of E matrices. dx: sb alone, b is codes.
+    // these the exponents of a's rows and of b's E matrices. dx: sb alone, b is codes.
     const uint8_t* sa;
     const uint8_t* sb;
 };

@@ -48,7 +48,8 @@ enum MxEpi { MX_PLAIN = 0, MX_LIN = 1, MX_ACT = 2 };
 // counted in 16-bit words, four codes each, so that a step is 64 words.
 // A stage is the operands' codes, 128 bytes a row, its 16-byte pieces XORed so that a fragment's rows spread over the banks, and
 // their exponents, 8 bytes a row. These lie in memory by steps (moe_mx4.h), so that a tile's are 1 KiB pieces, one to a loading
-// wave; their bytes are ordered so that a lane's four of a step are one word, which the instruction picks from.
+// wave; their bytes are ordered so that a lane's four of a step are one word, which the instruction picks from. GATHER: x's rows, and
+// their exponents in words, through the index list.
 // The matrix instruction takes w's rows as its first operand, and row m of it is w's row column(m) of a block's 32, so that a lane's
 // 16 sums of one row of x are neighbours. Exchanges with the lane of the row 16 further on and with that of the row 4 further on then
 // make every store instruction write whole lines, and loads of the residual read them. (Without the second exchange, half lines: 4096
@@ -62,7 +63,8 @@ struct MxKernel {
     static constexpr int SCA = (BI * 8 + 1023) / 1024, SCB = (BJ * 8 + 1023) / 1024;   // pieces of exponents
     static_assert(SCA + SCB <= NL, "one to a wave");
     static constexpr int CODES = (BI + BJ) * 128, STAGE = CODES + (SCA + SCB) * 1024;
-    static constexpr int L = PA + PB + 1;
+    static constexpr int SG = BI * 8 / 256;   // GATHER: pieces of x's exponents, 64 words each
+    static constexpr int L = PA + PB + 1 + GATHER;
 
     // XOR of the 16-byte pieces of a row. Half a wave's reads take two cycles if none of the 16 places that 16 bytes can have in the
     // banks occurs more than twice among them: two rows share a line of all banks, so 32 rows have each piece in four places of
@@ -212,7 +214,7 @@ struct MxKernel {
             int lid = -1, ls = 0, lsteps = 0, lrows = 0, lr = 0;
             MmTile lt{};
             const char *pa = nullptr, *pb = nullptr;
-            uint32_t offa[PA], offb[PB];
+            uint32_t offa[PA], offb[PB], offs = 0;   // offs: GATHER, of x's exponents
             auto next_tile = [&]() {
                 ls = 0;
                 do {
@@ -236,6 +238,10 @@ struct MxKernel {
                     int src = r;
                     if constexpr (GATHER) src = r < lt.rows ? g.arows[lt.lo + r] : -1;
                     offa[i] = !GATHER || (uint32_t)src < (uint32_t)g.a_n ? (uint32_t)src * (uint32_t)ld2 + c : MM_OOB;
+                }
+                if constexpr (GATHER) {
+                    const int r = lw % SG * 32 + (lane >> 1), src = r < lt.rows ? g.arows[lt.lo + r] : -1;
+                    offs = (uint32_t)src < (uint32_t)g.a_n ? (uint32_t)src * 8 + (lane & 1) * 4 : MM_OOB;
                 }
 #pragma unroll
                 for (int i = 0; i < PB; ++i) {
@@ -261,8 +267,11 @@ struct MxKernel {
                 for (int i = 0; i < PB; i += NB) dma16<NB, NL * 1024>(db, offb + i, lds0 + buf + (uint32_t)(BI * 128 + (i * NL + lw) * 1024));
 #pragma unroll
                 for (int i = 0; i < PA; i += NA) dma16<NA, NL * 1024>(da, offa + i, lds0 + buf + (uint32_t)((i * NL + lw) * 1024));
-                // this wave's piece of a's or b's exponents (waves past the last piece load one again)
-                const int p = lw % (SCA + SCB), step = ls + (g.part ? lt.e * (g.part / 64) : 0), e = g.part ? 0 : lt.e;
+                // this wave's piece of a's or b's exponents, GATHER: of each (waves past the last piece load one again)
+                const int p = GATHER ? SCA + lw % SCB : lw % (SCA + SCB), step = ls + (g.part ? lt.e * (g.part / 64) : 0), e = g.part ? 0 : lt.e;
+                if constexpr (GATHER)
+                    dma4(srd_of((const char*)g.sa + (int64_t)step * g.a_n * 8, lrows ? (uint32_t)g.a_n * 8 : 0u), offs,
+                         lds0 + buf + CODES + lw % SG * 256);
                 const uint8_t* s = g.sa + ((int64_t)step * g.M + lt.lo) * 8 + p * 1024;
                 int n = (lrows * 8 + 15) / 16 * 16 - p * 1024;
                 if (p >= SCA) {

@@ -24,8 +24,6 @@ inline size_t mx4_scale_bytes(int64_t rows, int64_t K) { return (size_t)(mx4_ste
 int launch_mx4_quantize(const void* x, int64_t ld, int64_t G, int64_t rows, int64_t K, int dtype, Mx4 out, hipStream_t st);
 int launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t G, int64_t rows, int64_t K, int dtype, void* out,
                           hipStream_t st);
-// scales of the rows idx[0 .. M) of a matrix with n rows, in their order (an index outside it: any finite scale)
-int launch_mx4_take_scales(const uint8_t* scales, int64_t n, int64_t K, const int32_t* idx, int64_t M, uint8_t* out, hipStream_t st);
 // Products of few rows per group. x16 not null: a.a's rows are 16-bit numbers of the result's type there (ldx elements between
 // them), quantised by every workgroup for itself; else a.a, a.sa (not gathered: row arows[p]).
 int launch_mx4_rows(const MmArgs& a, const void* x16, int64_t ldx, hipStream_t st);

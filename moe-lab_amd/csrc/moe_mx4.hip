@@ -126,15 +126,6 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* codes, co
     }
 }
 
-__global__ void __launch_bounds__(256) k_mx4_take_scales(const uint8_t* scales, uint32_t n, const int32_t* idx, uint32_t M,
-                                                         uint8_t* out) {
-    const uint32_t p = blockIdx.x * 256 + threadIdx.x, s = blockIdx.y;
-    if (p >= M) return;
-    const int32_t r = idx[p];
-    const uint64_t ones = 0x7f7f7f7f7f7f7f7full;
-    ((uint64_t*)out)[(int64_t)s * M + p] = (uint32_t)r < n ? ((const uint64_t*)scales)[(int64_t)s * n + r] : ones;
-}
-
 // Rows that a launch takes: its items are counted in 32 bits.
 static int64_t rows_at_once(int64_t rows, int64_t per_row) {
     const int64_t fit = ((int64_t)1 << 31) / per_row;
@@ -172,13 +163,6 @@ int launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t G
         if (hipGetLastError() != hipSuccess) return MOE_ERR_LAUNCH;
     }
     return MOE_OK;
-}
-
-int launch_mx4_take_scales(const uint8_t* scales, int64_t n, int64_t K, const int32_t* idx, int64_t M, uint8_t* out,
-                           hipStream_t st) {
-    const dim3 grid((unsigned)((M + 255) / 256), (unsigned)mx4_steps(K));
-    k_mx4_take_scales<<<grid, 256, 0, st>>>(scales, (uint32_t)n, idx, (uint32_t)M, out);
-    return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;
 }
 
 // Sums of 16-bit rows by group: a workgroup 256 columns (8 to a lane, 32 lanes a row) of a piece of a group's rows, 8 of them at a

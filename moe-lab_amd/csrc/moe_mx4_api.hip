@@ -208,10 +208,10 @@ int moe_mx4_bias_grad(const void* dy, int64_t lddy, const int32_t* offsets, int6
     return moe::launch_mx4_sums(a, moe::mx4_sum_parts(M, E, N), (float*)workspace, (hipStream_t)stream);
 }
 
-size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int E, int K, int indexed, int has_form) {
+size_t moe_mx4_grouped_mm_workspace_bytes(int64_t M, int64_t x_rows, int E, int K, int has_form) {
     if (bad_rows(M) || bad_rows(x_rows) || M == 0 || E < 1 || bad_k(K)) return 0;
     if (few_slots(M, E) && !has_form && fused(1, K)) return 0;
-    return (has_form ? 0 : x_bytes(x_rows, K)) + (indexed && !few_slots(M, E) ? up256(moe::mx4_scale_bytes(M, K)) : 0);
+    return has_form ? 0 : x_bytes(x_rows, K);
 }
 
 int moe_mx4_grouped_mm(const void* x, int64_t ldx, void* xc, void* xs, int64_t x_rows, const void* wc, const void* ws,
@@ -227,7 +227,7 @@ int moe_mx4_grouped_mm(const void* x, int64_t ldx, void* xc, void* xs, int64_t x
     if (x_rows < (rows ? 1 : M)) return MOE_ERR_ARG;
     if (rows && x_rows * (K / 2) > 0xB0000000ll) return MOE_ERR_ARG;   // addressed with 32 bits from its start
     if (misaligned(bias) || misaligned(workspace)) return MOE_ERR_ALIGN;
-    const size_t need = moe_mx4_grouped_mm_workspace_bytes(M, x_rows, E, K, rows != nullptr, xc != nullptr);
+    const size_t need = moe_mx4_grouped_mm_workspace_bytes(M, x_rows, E, K, xc != nullptr);
     if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE;
     const hipStream_t st = (hipStream_t)stream;
     moe::MmArgs a = product(p, M, E, N, dtype, y, y_dtype);
@@ -242,11 +242,6 @@ int moe_mx4_grouped_mm(const void* x, int64_t ldx, void* xc, void* xs, int64_t x
     rc = operand(p, dtype, w, a, st);
     if (rc) return rc;
     if (few) return moe::launch_mx4_rows(a, nullptr, 0, st);
-    if (rows) {   // the tiles take x's scales in slot order
-        rc = moe::launch_mx4_take_scales(a.sa, x_rows, K, rows, M, (uint8_t*)w, st);
-        if (rc) return rc;
-        a.sa = (const uint8_t*)w;
-    }
     return moe::launch_mm_fwd(a, st);
 }
 

@@ -327,7 +327,7 @@ def _run_grouped(x, w, offsets, bias, rows, out, out_dtype, keep):
     y = _lib.result(out, (M, N), dtype, out_dtype, device)
     if keep and q is None:
         q = _new((n, K), device)
-    ws, nws = _workspace(device, "moe_mx4_grouped_mm_workspace_bytes", M, n, E, K, int(rows is not None), int(q is not None))
+    ws, nws = _workspace(device, "moe_mx4_grouped_mm_workspace_bytes", M, n, E, K, int(q is not None))
     _lib.call("moe_mx4_grouped_mm", device, *_pointers(x2, q), n, w4.codes.data_ptr(), w4.scales.data_ptr(), _lib.ptr(bias),
               _lib.ptr(offsets), _lib.ptr(rows), M, E, N, K, _lib.DTYPE[dtype], y.data_ptr(), _lib.DTYPE[y.dtype], int(out is None),
               _lib.ptr(ws), nws)

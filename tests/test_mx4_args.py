@@ -98,9 +98,9 @@ def test_sizes():
     assert L.moe_mx4_scale_bytes(3, 10, 288) == 3 * 2 * 10 * 8 + 16
     assert L.moe_mx4_linear_workspace_bytes(0, 64, 64) == L.moe_mx4_linear_workspace_bytes(1, 64, 64) == 0
     assert L.moe_mx4_linear_workspace_bytes(100, 64, 64) >= 100 * 32 + 100 * 8
-    assert L.moe_mx4_grouped_mm_workspace_bytes(8, 1, 128, 2048, 1, 0) == 0
-    assert L.moe_mx4_grouped_mm_workspace_bytes(800, 100, 8, 2048, 0, 1) == 0
-    assert L.moe_mx4_grouped_mm_workspace_bytes(800, 100, 8, 2048, 1, 1) >= 800 * 64
+    assert L.moe_mx4_grouped_mm_workspace_bytes(8, 1, 128, 2048, 0) == 0
+    assert L.moe_mx4_grouped_mm_workspace_bytes(800, 100, 8, 2048, 1) == 0
+    assert L.moe_mx4_grouped_mm_workspace_bytes(800, 100, 8, 2048, 0) >= 100 * (1024 + 64)
 
 
 def test_packed_form_on_the_cpu():
