@@ -422,10 +422,16 @@ static int launch_cfg(const MmArgs& a, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;
 }
 
+// A group has about M / 128 + 1/2 row tiles of 128, one at least. Where that makes a tile of 128 x 256 for every CU, it reads the
+// weights fastest, however few rows use them (us in 64 x 64, 128 x 128, 128 x 256 tiles: 128 experts x 4 rows, [1536, 2048], 42.8,
+// 43.4, 37.1; 64 x 8, [2048, 2048], 29.6, 30.9, 27.4; x 256 rows of 128 experts 156, 87, 78). With fewer, up to 32 rows in
+// smaller tiles (8 experts x 32, [4096, 4096]: 16.2, 17.4, 18.4), and more rows in 128 x 128 while those are one round of the CUs
+// (4 x 256, [2048, 2048]: 11.1, 9.9, 11.7).
 static int grouped(const MmArgs& a) {
-    const int64_t live = a.E < a.M ? a.E : a.M;
+    const int64_t live = a.E < a.M ? a.E : a.M, half = live / 2 + a.M / 128, tiles = live > half ? live : half;
+    if (tiles * ((a.J + 255) / 256) >= 256) return MM_128x256;
     if (a.M / live <= 32) return MM_64;
-    return (live / 2 + a.M / 128) * ((a.J + 127) / 128) <= 256 ? MM_128_DEEP : MM_128x256;
+    return half * ((a.J + 127) / 128) <= 256 ? MM_128_DEEP : MM_128x256;
 }
 
 template <bool F16>

@@ -76,7 +76,9 @@ __device__ __forceinline__ void write_exponent(uint8_t* s, int b, uint32_t e, bo
         for (int p = b + 1; p < 8; ++p) s[mx4_byte(p)] = 127;
 }
 
-// One item: 8 columns of a row, its 4-lane neighbours the rest of its block.
+// One item: 8 columns of a row, its 4-lane neighbours the rest of its block: a block's largest magnitude is two DPP steps away, loads
+// are 16 bytes a lane (fp32: two of them), and nothing is read twice. Bound by memory: [14336, 4096] bf16 29 us (149 MB, 5.1 TB/s, the
+// rate of a large copy), [5760, 2880] fp32 13 us (75 MB); 5 rows 2.5 us, the launch.
 template <int DT>
 __global__ void __launch_bounds__(256) k_mx4_quantize(const char* x, int64_t ld, uint32_t items, uint32_t per_row, uint32_t row0,
                                                       uint32_t rows, int64_t scale_stride, uint8_t* codes, uint8_t* scales) {
@@ -96,6 +98,7 @@ __global__ void __launch_bounds__(256) k_mx4_quantize(const char* x, int64_t ld,
     }
 }
 
+// The same items. Bound by memory too: [14336, 4096] to bf16 23.5 us (149 MB; its writes go past 5.1 TB/s), [5760, 2880] to fp32 14.
 template <int DT>
 __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, uint32_t items,
                                                         uint32_t per_row, uint32_t row0, uint32_t rows, int64_t scale_stride,
@@ -166,8 +169,8 @@ int launch_mx4_dequantize(const uint8_t* codes, const uint8_t* scales, int64_t G
 }
 
 // Sums of 16-bit rows by group: a workgroup 256 columns (8 to a lane, 32 lanes a row) of a piece of a group's rows, 8 of them at a
-// time, the 8 partial sums joined in LDS in order. Bound by the one read of dy: 4444 x 5760 of 32 groups 12.3 us (4.1 TB/s), 32768 x
-// 1536 of 128 19.8 us (5.1), 4096 x 4096 of one 8.9 us. (Before, the weight gradient's product with columns of zeros: 27, 37, 50.)
+// time, the 8 partial sums joined in LDS in order. Bound by the one read of dy: 4444 x 5760 of 32 groups 10.5 us (4.8 TB/s), 32768 x
+// 1536 of 128 17 us (5.9), 4096 x 4096 of one 7.2 us. (The weight gradient's product with columns of zeros: 27, 37, 50.)
 constexpr int SUM_COLS = 256, SUM_ROWS = 8;
 template <bool F16>
 __global__ void __launch_bounds__(256) k_mx4_sums(const MmArgs g, int parts, float* out) {
@@ -218,11 +221,12 @@ __global__ void __launch_bounds__(256) k_mx4_join_sums(const float* sums, int pa
     y[i] = (uint16_t)pack16<F16>(s, 0.f);
 }
 
-// Pieces so that about 1024 workgroups have 64 rows or more each: one group of 4096 rows would have 16 workgroups of its columns.
+// Pieces so that about 512 workgroups have 64 rows or more each: one group of 4096 rows would have 16 workgroups of its columns.
+// (About 1024: a join where 736 workgroups do without, 4444 x 5760 of 32 groups 12.3 us.)
 int mx4_sum_parts(int64_t M, int64_t E, int64_t N) {
     const int64_t wgs = E * ((N + SUM_COLS - 1) / SUM_COLS), rows = M / E;
     int parts = 1;
-    while (wgs * parts < 1024 && rows >= 128 * parts) parts *= 2;
+    while (wgs * parts < 512 && rows >= 128 * parts) parts *= 2;
     return parts;
 }
 
@@ -256,7 +260,10 @@ __device__ __forceinline__ f32x4 mma16(s16x8 a, uint32_t sa, s16x8 b, uint32_t s
 // Few rows: a wave multiplies 16 rows of the weights by up to 16 NT rows of x, with the weights' codes straight from memory as the
 // matrix instruction's first operand. ks waves of a workgroup share the steps of K, and their sums meet in LDS, in the waves'
 // order. FUSE: x's rows are quantised here first, while the first weights are on their way; else their codes come from memory too.
-// Bound by the weights' bytes and the latency of the first ones: AHEAD steps of a wave are loaded together.
+// Bound by the weights' bytes and the latency of the first ones: AHEAD steps of a wave are loaded together. One row, [14336, 4096]
+// 8.3 us (31 MB, 3.8 TB/s), [4096, 4096] 4.5; 8 of 128 experts, [1536, 2048], 7.6 (13 MB: a chain of index list, row, weights).
+// FUSE: to quantise one row needs a launch of 2.5 us in front and its codes back from memory; with 4 rows every workgroup quantises
+// 4 K numbers for itself while its weights come, with more that takes longer than the launch. Their codes have to fit LDS.
 // Workgroups go by slot, not by group (as k_mm_rows): the one at a group's first slot does the group.
 constexpr int MXR_WAVES = 8;
 template <bool F16, bool FUSE, int NT>
@@ -407,7 +414,9 @@ __global__ void __launch_bounds__(64 * MXR_WAVES) k_mx4_rows(const MmArgs g, con
 
 int launch_mx4_rows(const MmArgs& a, const void* x16, int64_t ldx, hipStream_t st) {
     const int64_t K = (int64_t)a.R * 4, steps = mx4_steps(K), blocks = (int64_t)((a.J + 15) / 16) * (a.offsets ? a.M : 1);
-    int ks = 1;   // waves that share K
+    // Waves that share K, until 2048 of them have work (us with 1024, 2048, 4096: one row, [4096, 4096], 6.3, 5.6, 5.6, [4096, 14336]
+    // 13.4, 10.9, 11.0, [14336, 4096] 10.0, 9.4, 12.0; 8 of 128 experts, [1536, 2048], 6.0, 6.1, 7.6).
+    int ks = 1;
     while (ks < MXR_WAVES && ks < steps && blocks * ks < 2048) ks *= 2;
     const int rows = 16 * (MXR_WAVES / ks);
     const dim3 grid((unsigned)((a.J + rows - 1) / rows), a.offsets ? (unsigned)a.M : 1);
