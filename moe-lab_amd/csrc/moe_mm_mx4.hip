@@ -434,9 +434,17 @@ static int grouped(const MmArgs& a) {
     return half * ((a.J + 127) / 128) <= 256 ? MM_128_DEEP : MM_128x256;
 }
 
+// The 16-bit products' plan (E: parts), but 64 x 64 only while a CU has one of them at most: codes arrive so fast that a second round
+// costs more than larger tiles do (us in 64 x 64 and 128 x 128 tiles: 512 rows, [4096, 4096], 14.4 and 12.7, 256 rows 10.4 and 12.2;
+// 128 rows, [14336, 4096], 14.6 and 13.1).
+static int dense(const MmArgs& a) {
+    const int shape = mm_plan(MM_FWD, a.M, a.J, a.R, a.part != 0).shape;
+    return shape == MM_64 && ((int64_t)a.M + 63) / 64 * ((a.J + 63) / 64) * a.E > 256 ? MM_128_DEEP : shape;
+}
+
 template <bool F16>
 static int launch(const MmArgs& a, hipStream_t st) {
-    switch (a.offsets ? grouped(a) : mm_plan(MM_FWD, a.M, a.J, a.R, a.part != 0).shape) {
+    switch (a.offsets ? grouped(a) : dense(a)) {
         case MM_128x256: return launch_cfg<F16, 2, 2, 2, 4, 3, 1, 4>(a, st);
         case MM_128_DEEP: return launch_cfg<F16, 2, 2, 2, 2, 4, 1, 4>(a, st);
         default: return launch_cfg<F16, 1, 1, 2, 2, 4, 2, 4>(a, st);

@@ -105,7 +105,7 @@ def test_layouts_and_packed_form():
 # ------------------------------------------------------------------------------------------------------ products
 SIZES = [(1, 8, 32), (1, 200, 1056), (2, 1024, 4096), (4, 264, 96), (5, 1024, 544), (16, 136, 2880), (17, 136, 288), (32, 264, 1056), (24, 8200, 96), (33, 2056, 160),
          (65, 520, 352), (130, 264, 1440), (237, 2048, 2816), (700, 136, 96), (1000, 1032, 224), (2048, 2048, 64), (513, 4104, 160),
-         (300, 512, 8192), (3, 64, 20480)]
+         (300, 512, 8192), (3, 64, 20480), (2049, 4104, 288)]
 
 
 def linear_reference(xv, wv, b, r, act):
@@ -202,7 +202,7 @@ def test_gradient_against_differences():
 
 
 GROUPS = [[1], [5], [0, 3, 0], [1] * 8, [40, 0, 1, 17, 0], [0, 0, 0], [130, 64, 1, 65, 2], [33] * 20, [700, 0, 300], [256] * 9,
-          [3, 1, 0, 0, 200, 0, 5, 31] * 4]
+          [3, 1, 0, 0, 200, 0, 5, 31] * 4, [3, 0, 40, 1] * 20]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
