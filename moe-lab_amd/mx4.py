@@ -56,6 +56,13 @@ def _set(q, codes, scales, shape):
         object.__setattr__(q, name, value)
 
 
+def _of(codes, scales):
+    """The Mx4 of tensors that came from one."""
+    q = Mx4.__new__(Mx4)
+    _set(q, codes, scales, (*codes.shape[:-1], 2 * codes.shape[-1]))
+    return q
+
+
 def _scale_bytes(shape):
     E = shape[0] if len(shape) == 3 else 1
     return 8 * E * shape[-2] * (-(-shape[-1] // STEP)) + 16
@@ -251,9 +258,9 @@ class _Linear(torch.autograd.Function):
             if ctx.act != NONE:
                 dz = _linear._act_backward(dz, z, ctx.act, None, None)
             if need_x:
-                dx = _linear_dx(dz, Mx4(wc, ws)).view(ctx.x_shape)
+                dx = _linear_dx(dz, _of(wc, ws)).view(ctx.x_shape)
             if need_w:
-                dw, db = _linear._dw(dz, dequantize(Mx4(xc, xs), ctx.dtype), need_b)
+                dw, db = _linear._dw(dz, dequantize(_of(xc, xs), ctx.dtype), need_b)
             elif need_b:
                 db = _bias_grad(dz, None, 1).view(-1)
         return dx, dw, None, db, None, dy if ctx.needs_input_grad[5] else None, None
@@ -351,9 +358,9 @@ class _GroupedMm(torch.autograd.Function):
         dy = _lib.half_matrix(dy.to(ctx.dtype), "dy")
         dx = dw = db = None
         if need_x:
-            dx = _grouped_dx(dy, Mx4(wc, ws), offsets)
+            dx = _grouped_dx(dy, _of(wc, ws), offsets)
         if need_w:
-            dw, db = _grouped.mm_dw(dy, dequantize(Mx4(xc, xs), ctx.dtype), offsets, wc.shape[0], x_rows=rows, bias=True)
+            dw, db = _grouped.mm_dw(dy, dequantize(_of(xc, xs), ctx.dtype), offsets, wc.shape[0], x_rows=rows, bias=True)
         elif need_b:
             db = _bias_grad(dy, offsets, wc.shape[0])
         return dx, dw, None, None, db if need_b else None, None, None

@@ -12,7 +12,9 @@ softmax or sigmoid scores, a bias that only ranks, groups of experts of which th
 x . Wr^T (+ bias) are computed in the same kernel, in fp32, in one fixed reduction order, so a CPU
 restatement reproduces them bit for bit and the chosen ids are exact.
 """
+import functools
 import math
+import operator
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -113,8 +115,9 @@ def group(idx, E):
     return counts, offsets, srt[:n], active, meta
 
 
-def _scored(E, k, score, bias, groups, top_groups, group_score, norm, scale, device):
-    """The call's descriptor, its arguments checked, and the bias that it points to."""
+@functools.lru_cache(maxsize=1024)
+def _settings(E, k, score, groups, top_groups, group_score, norm, scale):
+    """The descriptor of these settings, checked, without a bias."""
     kind, by = _SCORES.get(score), _GROUP_SCORES.get(group_score)
     if kind is None or by is None:
         raise ValueError(f"score {score!r}, group_score {group_score!r}: one of {list(_SCORES)}, one of {list(_GROUP_SCORES)} expected")
@@ -126,11 +129,25 @@ def _scored(E, k, score, bias, groups, top_groups, group_score, norm, scale, dev
         raise ValueError(f"k = {k}: 1 to {min(32, top_groups * (E // groups))} expected (32, or the experts in the kept groups)")
     if not math.isfinite(scale):
         raise ValueError(f"scale {scale}: a finite number expected")
-    if bias is not None:
-        if bias.dtype not in _lib.DTYPE or tuple(bias.shape) != (E,) or bias.device != device:
-            raise ValueError(f"bias {bias.dtype} {tuple(bias.shape)} on {bias.device}: floating [{E}] on {device} expected")
-        bias = _lib.dense(bias.detach(), torch.float32)
-    return _lib.Scored(E, k, kind, groups, top_groups, by, 1 if norm else 0, scale, _lib.ptr(bias)), bias
+    return _lib.Scored(E, k, kind, groups, top_groups, by, norm, scale, None)
+
+
+def _scored(E, k, score, bias, groups, top_groups, group_score, norm, scale, device):
+    """The call's descriptor, its arguments checked, and the bias that it points to."""
+    desc = _settings(E, operator.index(k), score, operator.index(groups), operator.index(top_groups), group_score,
+                     1 if norm else 0, float(scale))
+    if bias is None:
+        return desc, None
+    if bias.dtype not in _lib.DTYPE or tuple(bias.shape) != (E,) or bias.device != device:
+        raise ValueError(f"bias {bias.dtype} {tuple(bias.shape)} on {bias.device}: floating [{E}] on {device} expected")
+    bias = _lib.dense(bias.detach(), torch.float32)
+    return _with_bias(desc, bias), bias
+
+
+def _with_bias(desc, bias):
+    desc = _lib.Scored.from_buffer_copy(desc)
+    desc.bias = bias.data_ptr()
+    return desc
 
 
 def _topk_scored(lg, desc):
@@ -143,12 +160,11 @@ def _topk_scored(lg, desc):
 
 class _TopkScored(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, bias, settings):
-        desc, bias = _scored(logits.shape[1], *settings[:2], bias, *settings[2:], logits.device)
+    def forward(ctx, logits, desc, bias):
         lg = _lib.dense(logits)
         idx, wts = _topk_scored(lg, desc)
-        ctx.save_for_backward(logits if lg is logits else lg, bias, idx)
-        ctx.settings = settings
+        ctx.save_for_backward(lg, bias, idx)
+        ctx.desc = desc
         ctx.mark_non_differentiable(idx)
         ctx.set_materialize_grads(False)
         return idx, wts
@@ -158,11 +174,11 @@ class _TopkScored(torch.autograd.Function):
     def backward(ctx, _, dwts):
         if dwts is None:
             return None, None, None
-        logits, bias, idx = ctx.saved_tensors
-        lg = _lib.dense(logits)
-        desc, bias = _scored(lg.shape[1], *ctx.settings[:2], bias, *ctx.settings[2:], lg.device)
-        dw = _lib.dense(dwts, torch.float32)
-        dl = torch.empty_like(lg)
+        lg, bias, idx = ctx.saved_tensors
+        desc = ctx.desc
+        if bias is not None and bias.data_ptr() != desc.bias:   # kept elsewhere in between
+            desc = _with_bias(desc, bias)
+        dw, dl = _lib.dense(dwts, torch.float32), torch.empty_like(lg)
         _lib.call("moe_topk_scored_bwd", lg.device, desc, lg.data_ptr(), _lib.DTYPE[lg.dtype], lg.shape[0], idx.data_ptr(),
                   dw.data_ptr(), dl.data_ptr())
         return dl, None, None
@@ -182,10 +198,9 @@ def topk_scored(logits, k, score="softmax", bias=None, groups=1, top_groups=1, g
     if logits.dtype not in _lib.DTYPE:
         raise TypeError(f"logits are {logits.dtype}: fp32, bf16 or fp16 expected")
     lg = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
-    settings = (k, score, groups, top_groups, group_score, norm, scale)
-    if _lib.wants_grad(logits):
-        return _TopkScored.apply(lg, bias, settings)
     desc, bias = _scored(lg.shape[1], k, score, bias, groups, top_groups, group_score, norm, scale, lg.device)
+    if _lib.wants_grad(logits):
+        return _TopkScored.apply(lg, desc, bias)
     return _topk_scored(_lib.dense(lg), desc)
 
 

@@ -269,3 +269,21 @@ def test_captured_calls():
         torch.cuda.synchronize()
         for a, b in zip([t.clone() for t in got], step()):
             assert torch.equal(a, b)
+
+
+def test_saved_elsewhere_in_between():
+    """What the backward pass needs goes to the host and back, the bias to another address."""
+    logits, bias = make(20, 64, torch.float32)
+    kw = dict(score="sigmoid", groups=4, top_groups=2, group_score="top2")
+    dw = torch.ones(20, 6, device=DEV) * torch.arange(6, device=DEV)
+    bias[7] = -math.inf
+    grads = []
+    for away in (False, True):
+        lg = logits.clone().requires_grad_()
+        b = bias.clone()
+        with torch.autograd.graph.save_on_cpu() if away else torch.enable_grad():
+            idx, wts = router.topk_scored(lg, 6, bias=b.bfloat16(), **kw)
+        del b
+        waste = torch.full((64,), -math.inf, device=DEV)
+        grads.append(torch.autograd.grad(wts, lg, dw)[0])
+    assert torch.equal(*grads) and grads[0].any()
