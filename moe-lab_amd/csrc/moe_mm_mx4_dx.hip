@@ -21,6 +21,11 @@ __device__ __forceinline__ u32x4 decode8(uint32_t w, float s) {
 // KiB a step, into another; the loading waves then decode a step's codes to the 32 KiB that the products read, of which there are
 // two. All of it is a step or more ahead, so that a step has one barrier, as the 16-bit products' have. (Codes on their way in
 // registers instead: the compiler waits for a load as soon as its count is not certain, 4096^3 190 us.)
+// What bounds it: LDS, which takes in dy and the codes, gives the codes to be decoded, takes them in again as numbers and gives the
+// fragments: 4096^3 148 us, without decoding 124 (the weights as 16-bit numbers in memory: 124, and 12 to write them), without any
+// loads 123. 4444 rows of 32 experts, [5760, 2880], 270-290: half of the row tiles hold 11 rows, and cost 0.75 us a step where full
+// ones take 1.1. Tiles of 256 x 128 halve the decoding and that (257), but few rows then take twice the steps (64 experts x 16,
+// [2048, 2048]: 59 and 115).
 template <bool F16>
 struct Mx4Dx {
     static constexpr int FA = 4, FB = 4, NWJ = 4, NWC = 2 * NWJ, NL = 4;
