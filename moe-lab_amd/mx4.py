@@ -215,8 +215,8 @@ def _workspace(device, name, *sizes):
     return (torch.empty(n, dtype=torch.uint8, device=device), n) if n else (None, 0)
 
 
-def _run_linear(x, w, bias, act, residual, out_dtype, keep):
-    """y, z, x's Mx4 and w's (keep: x's form and z are kept for the backward pass)."""
+def _run_linear(x, w, bias, act, residual, out_dtype, keep_z, keep_x):
+    """y, z (None unless keep_z), x's Mx4 (keep_x: made for a 16-bit x too) and w's."""
     if act not in (NONE, SILU, GELU):
         raise ValueError(f"act {act}: NONE, SILU or GELU expected")
     w4, w_type = _weights(w, 2, "[N, K]")
@@ -228,8 +228,8 @@ def _run_linear(x, w, bias, act, residual, out_dtype, keep):
     bias = _lib.plain(bias, "bias", (N,), device, dtype)
     residual = _lib.plain(residual, "residual", (*lead, N), device, dtype)
     y = _lib.result(None, (T, N), dtype, out_dtype, device)
-    z = torch.empty((T, N), dtype=dtype, device=device) if keep and act != NONE else None
-    if keep and q is None:
+    z = torch.empty((T, N), dtype=dtype, device=device) if keep_z else None
+    if keep_x and q is None:
         q = _new((T, K), device)
     ws, nws = _workspace(device, "moe_mx4_linear_workspace_bytes", T, N, K)
     _lib.call("moe_mx4_linear", device, *_pointers(x2, q), w4.codes.data_ptr(), w4.scales.data_ptr(), _lib.ptr(bias),
@@ -240,9 +240,12 @@ def _run_linear(x, w, bias, act, residual, out_dtype, keep):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w4, bias, act, residual, out_dtype):
-        y, z, q, w4 = _run_linear(x, w if w4 is None else w4, bias, act, residual, out_dtype, True)
+        need_x, need_w, _, need_b = ctx.needs_input_grad[:4]
+        y, z, q, w4 = _run_linear(x, w if w4 is None else w4, bias, act, residual, out_dtype,
+                                  act != NONE and (need_x or need_w or need_b), need_w)
         # the weights' 4-bit form stands for w from here on, also where w changes before the backward pass
-        ctx.save_for_backward(q.codes, q.scales, w4.codes, w4.scales, z)
+        ctx.save_for_backward(*((q.codes, q.scales) if need_w else (None, None)),
+                              *((w4.codes, w4.scales) if need_x else (None, None)), z)
         ctx.act, ctx.x_shape, ctx.dtype = act, x.shape, x.dtype
         return y
 
@@ -309,7 +312,7 @@ def linear(x, w, bias=None, act=NONE, residual=None, out_dtype=None):
     operands' type first."""
     x_grad, w_grad = (None if isinstance(t, Mx4) else t for t in (x, w))
     if not _lib.wants_grad(x_grad, w_grad, bias, residual):
-        return _run_linear(x, w, bias, act, residual, out_dtype, False)[0]
+        return _run_linear(x, w, bias, act, residual, out_dtype, False, False)[0]
     if x_grad is None:
         raise ValueError("an Mx4 x takes no part in a backward pass: give its 16-bit form")
     return _Linear.apply(x, w_grad, w if w_grad is None else None, bias, act, residual, out_dtype)
@@ -344,10 +347,11 @@ def _run_grouped(x, w, offsets, bias, rows, out, out_dtype, keep):
 class _GroupedMm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w4, offsets, bias, rows, out_dtype):
-        need_w = ctx.needs_input_grad[1]
+        need_x, need_w = ctx.needs_input_grad[:2]
         y, q, w4 = _run_grouped(x, w if w4 is None else w4, offsets, bias, rows, None, out_dtype, need_w)
-        ctx.save_for_backward(*((q.codes, q.scales) if need_w else (None, None)), w4.codes, w4.scales, offsets, rows)
-        ctx.dtype = x.dtype
+        ctx.save_for_backward(*((q.codes, q.scales) if need_w else (None, None)), *((w4.codes, w4.scales) if need_x else (None, None)),
+                              offsets, rows)
+        ctx.dtype, ctx.experts = x.dtype, w4.shape[0]
         return y
 
     @staticmethod
@@ -360,9 +364,9 @@ class _GroupedMm(torch.autograd.Function):
         if need_x:
             dx = _grouped_dx(dy, _of(wc, ws), offsets)
         if need_w:
-            dw, db = _grouped.mm_dw(dy, dequantize(_of(xc, xs), ctx.dtype), offsets, wc.shape[0], x_rows=rows, bias=True)
+            dw, db = _grouped.mm_dw(dy, dequantize(_of(xc, xs), ctx.dtype), offsets, ctx.experts, x_rows=rows, bias=True)
         elif need_b:
-            db = _bias_grad(dy, offsets, wc.shape[0])
+            db = _bias_grad(dy, offsets, ctx.experts)
         return dx, dw, None, None, db if need_b else None, None, None
 
 

@@ -441,6 +441,43 @@ def test_two_streams_at_once():
             assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
 
 
+@pytest.mark.parametrize("act", [NONE, SILU])
+def test_each_gradient_alone(act):
+    """Any one of the operands that can have a gradient, the others without: equal to it among all of them, and no more kept."""
+    T, N, K = 70, 136, 96
+    x, w, b = activations(T, K, torch.bfloat16), H.randn(N, K, dtype=torch.bfloat16, scale=0.1, seed=1), H.randn(N, dtype=torch.bfloat16)
+    r, dy = H.randn(T, N, dtype=torch.bfloat16, seed=2), H.randn(T, N, dtype=torch.bfloat16, seed=3)
+    kept = []
+
+    def pack(t):
+        kept.append(t.numel() * t.element_size())
+        return t
+
+    def grads(needs):
+        kept.clear()
+        leaves = [t.clone().requires_grad_(i in needs) for i, t in enumerate((x, w, b, r))]
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            y = mx4.linear(*leaves[:2], bias=leaves[2], act=act, residual=leaves[3])
+        return torch.autograd.grad(y, [leaves[i] for i in needs], dy), sum(kept)
+    every, _ = grads([0, 1, 2, 3])
+    z = T * N * 2 if act != NONE else 0
+    form = lambda rows: rows * K // 2 + rows * 8 + 16
+    for i, keeps in enumerate((z + form(N), z + form(T), z, 0)):
+        (g,), n = grads([i])
+        assert torch.equal(g, every[i]) or i == 2   # (the bias's sums have another order beside the weights' gradient)
+        assert n == keeps, (i, n, keeps)
+    E, off = 2, H.offsets_of([30, 40])
+    w, b = H.randn(E, N, K, dtype=torch.bfloat16, scale=0.1, seed=1), H.randn(E, N, dtype=torch.bfloat16)
+
+    def grouped_grads(needs):
+        leaves = [t.clone().requires_grad_(i in needs) for i, t in enumerate((x, w, b))]
+        y = mx4.grouped_mm(*leaves[:2], off, bias=leaves[2])
+        return torch.autograd.grad(y, [leaves[i] for i in needs], dy)
+    every = grouped_grads([0, 1, 2])
+    for i in range(3):
+        assert torch.equal(grouped_grads([i])[0], every[i]) or i == 2
+
+
 def test_training_calls_without_rows():
     x = torch.zeros(0, 96, dtype=torch.bfloat16, device=DEV, requires_grad=True)
     w, b = H.randn(64, 96, dtype=torch.bfloat16).requires_grad_(), H.randn(64, dtype=torch.bfloat16).requires_grad_()
