@@ -466,6 +466,9 @@ int moe_router_scored(const moe_scored_t* r, const void* x, const void* wr, cons
  *       workspace: has_form, xc and xs are given.
  *   moe_mx4_linear_dx, moe_mx4_grouped_mm_dx: dx = dz w with w's values as `dtype` numbers (fp16: rounded to it), dz [T, N] (dy
  *       [M, N]) of `dtype`, as moe_linear_dx and moe_grouped_mm_dx without an index list.
+ *   moe_mx4_linear_bwd: the gradients of moe_mx4_linear that are wanted (dx [T, K], dw [N, K], db [N]; any NULL): dz = dy act'(z) in
+ *       `dtype` (act MOE_LIN_NONE: dy itself, z not read), dx = dz w, dw = dz^T x at the values of xc, xs (needed for dw) and
+ *       wc, ws (for dx).
  *   moe_mx4_bias_grad: db [E, N] of `dtype` = the sums of dy's rows by group (moe_grouped_mm's groups; offsets NULL with E = 1):
  *       the gradient of a bias beside frozen weights. A group without rows: zeros.
  * Products of codes and powers of two are exact, their sums fp32; bias, activation and residual fp32, rounded once.
@@ -486,6 +489,10 @@ int moe_mx4_linear_dx(const void* dz, int64_t lddz, const void* wc, const void* 
                       void* workspace, size_t workspace_bytes, void* stream);
 int moe_mx4_grouped_mm_dx(const void* dy, int64_t lddy, const void* wc, const void* ws, const int32_t* offsets, int64_t M, int E,
                           int N, int K, int dtype, void* dx, int dx_dtype, int fill, void* stream);
+size_t moe_mx4_linear_bwd_workspace_bytes(int64_t T, int N, int K, int act, int dx, int dw, int db);
+int moe_mx4_linear_bwd(const void* dy, int64_t lddy, const void* z, int act, const void* xc, const void* xs, const void* wc,
+                       const void* ws, int64_t T, int N, int K, int dtype, void* dx, void* dw, void* db, void* workspace,
+                       size_t workspace_bytes, void* stream);
 size_t moe_mx4_bias_grad_workspace_bytes(int64_t M, int E, int N);
 int moe_mx4_bias_grad(const void* dy, int64_t lddy, const int32_t* offsets, int64_t M, int E, int N, int dtype, void* db,
                       void* workspace, size_t workspace_bytes, void* stream);

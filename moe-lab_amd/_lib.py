@@ -33,7 +33,8 @@ EXPORTS = ("moe_router", "moe_router_counter_count", "moe_topk", "moe_group", "m
            "moe_mlp_fwd_workspace_bytes", "moe_mlp_bwd_workspace_bytes", "moe_topk_scored", "moe_topk_scored_bwd",
            "moe_router_scored", "moe_mx4_scale_bytes", "moe_mx4_quantize", "moe_mx4_dequantize", "moe_mx4_linear_workspace_bytes",
            "moe_mx4_linear", "moe_mx4_grouped_mm_workspace_bytes", "moe_mx4_grouped_mm", "moe_mx4_linear_dx_workspace_bytes",
-           "moe_mx4_linear_dx", "moe_mx4_grouped_mm_dx", "moe_mx4_bias_grad_workspace_bytes", "moe_mx4_bias_grad")
+           "moe_mx4_linear_dx", "moe_mx4_grouped_mm_dx", "moe_mx4_bias_grad_workspace_bytes", "moe_mx4_bias_grad",
+           "moe_mx4_linear_bwd_workspace_bytes", "moe_mx4_linear_bwd")
 PROBE_SINK = 1024   # MOE_PROBE_SINK
 STATIC_SCRATCH_BYTES = 32 << 20   # MOE_STATIC_SCRATCH_BYTES: the workspace array of moe_experts_run_static
 STAGE_GATE_UP, STAGE_DOWN, STAGE_ALL = 1, 2, 3
@@ -138,10 +139,12 @@ def lib():
         L.moe_mx4_linear_dx_workspace_bytes.argtypes = [i64, i, i]
         L.moe_mx4_linear_dx.argtypes = [vp, i64, vp, vp, i64, i, i, i, vp, vp, sz, vp]
         L.moe_mx4_grouped_mm_dx.argtypes = [vp, i64, vp, vp, vp, i64, i, i, i, i, vp, i, i, vp]
+        L.moe_mx4_linear_bwd_workspace_bytes.argtypes = [i64, i, i, i, i, i, i]
+        L.moe_mx4_linear_bwd.argtypes = [vp, i64, vp, i, vp, vp, vp, vp, i64, i, i, i, vp, vp, vp, vp, sz, vp]
         L.moe_mx4_bias_grad_workspace_bytes.argtypes = [i64, i, i]
         L.moe_mx4_bias_grad.argtypes = [vp, i64, vp, i64, i, i, i, vp, vp, sz, vp]
         for n in ("moe_mx4_linear_dx_workspace_bytes", "moe_mx4_scale_bytes", "moe_mx4_linear_workspace_bytes",
-                  "moe_mx4_grouped_mm_workspace_bytes", "moe_mx4_bias_grad_workspace_bytes"):
+                  "moe_mx4_grouped_mm_workspace_bytes", "moe_mx4_bias_grad_workspace_bytes", "moe_mx4_linear_bwd_workspace_bytes"):
             getattr(L, n).restype = sz
         L.moe_row_bytes.argtypes = [i, i]
         L.moe_row_bytes.restype = sz
@@ -162,7 +165,7 @@ def lib():
                   "moe_linear_dx", "moe_linear_dw", "moe_linear_act_bwd", "moe_act8_pack", "moe_act8_unpack", "moe_glu_fwd",
                   "moe_glu_bwd", "moe_mlp_fwd", "moe_mlp_bwd", "moe_topk_scored", "moe_topk_scored_bwd", "moe_router_scored",
                   "moe_mx4_quantize", "moe_mx4_dequantize", "moe_mx4_linear", "moe_mx4_grouped_mm", "moe_mx4_linear_dx",
-                  "moe_mx4_grouped_mm_dx", "moe_mx4_bias_grad"):
+                  "moe_mx4_grouped_mm_dx", "moe_mx4_bias_grad", "moe_mx4_linear_bwd"):
             getattr(L, n).restype = ctypes.c_int
         _lib = L
     return _lib

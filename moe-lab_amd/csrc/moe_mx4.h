@@ -35,6 +35,9 @@ inline bool mx4_few_rows(int64_t T, int64_t N) { return T <= 16 || (T <= 32 && N
 int mx4_sum_parts(int64_t M, int64_t E, int64_t N);
 int launch_mx4_sums(const MmArgs& a, int parts, float* sums, hipStream_t st);
 int mx4_dx_parts(int64_t rows, int64_t N, int64_t K);   // parts of a dense product of dx (moe_mm_mx4_dx.hip)
+// Rows from which a dense dx multiplies by the weights' values, written out once, and not by the codes, which each tile of 128 rows
+// decodes anew (us from codes and values, w [4096, 4096]: 2048 rows 72 and 73, 4096 rows 148 and 128, 8192 rows 250 and 231).
+constexpr int64_t MX4_DECODE_ONCE = 4096;
 constexpr int MX4_FUSE = 4;       // rows that are quantised inside the product (k_mx4_rows)
 constexpr int64_t MX4_FUSE_K = 1 << 16;   // and their elements in all, at most (LDS)
 

@@ -150,6 +150,7 @@ int moe_mx4_linear(const void* x, int64_t ldx, void* xc, void* xs, const void* w
 
 size_t moe_mx4_linear_dx_workspace_bytes(int64_t T, int N, int K) {
     if (bad_rows(T) || T == 0 || bad_n(N) || bad_k(K)) return 0;
+    if (T >= moe::MX4_DECODE_ONCE) return up256((size_t)N * K * 2) + moe_linear_dx_workspace_bytes(T, N, K);
     const int parts = moe::mx4_dx_parts(T, N, K);
     return parts > 1 ? (size_t)parts * T * K * 4 : 0;
 }
@@ -163,10 +164,63 @@ int moe_mx4_linear_dx(const void* dz, int64_t lddz, const void* wc, const void* 
     if (misaligned(dz) || misaligned(wc) || misaligned(ws) || misaligned(dx) || misaligned(workspace)) return MOE_ERR_ALIGN;
     const size_t need = moe_mx4_linear_dx_workspace_bytes(T, N, K);
     if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE;
+    if (T >= moe::MX4_DECODE_ONCE) {
+        const int rc = moe::launch_mx4_dequantize((const uint8_t*)wc, (const uint8_t*)ws, 1, N, K, dtype, workspace, (hipStream_t)stream);
+        if (rc) return rc;
+        const size_t used = up256((size_t)N * K * 2);
+        return moe_linear_dx(dz, workspace, T, lddz, N, K, dtype, dx, (char*)workspace + used, workspace_bytes - used, stream);
+    }
     const moe::MmArgs a = gradient(dz, lddz, wc, ws, T, 1, N, K, dtype, dx, dtype);
     const int parts = moe::mx4_dx_parts(T, N, K);
     if (parts > 1) return moe::launch_mm_parts(moe::MM_DX, a, parts, (float*)workspace, (hipStream_t)stream);
     return moe::launch_mm_dx(a, (hipStream_t)stream);
+}
+
+size_t moe_mx4_linear_bwd_workspace_bytes(int64_t T, int N, int K, int act, int dx, int dw, int db) {
+    if (bad_rows(T) || bad_n(N) || bad_k(K)) return 0;
+    size_t n = 0, m = 0;   // dz and x's values; the gradients' own, one after the other
+    if (act != MOE_LIN_NONE) n += up256((size_t)T * N * 2);
+    if (dw) n += up256((size_t)T * K * 2);
+    if (dx) m = moe_mx4_linear_dx_workspace_bytes(T, N, K);
+    const size_t w = dw ? moe_linear_dw_workspace_bytes(T, N, K) : db ? moe_mx4_bias_grad_workspace_bytes(T, 1, N) : 0;
+    return n + (w > m ? w : m);
+}
+
+int moe_mx4_linear_bwd(const void* dy, int64_t lddy, const void* z, int act, const void* xc, const void* xs, const void* wc,
+                       const void* ws, int64_t T, int N, int K, int dtype, void* dx, void* dw, void* db, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+    if (!two_byte(dtype)) return MOE_ERR_DTYPE;
+    if (act < MOE_LIN_NONE || act > MOE_LIN_GELU) return MOE_ERR_ARG;
+    if (bad_rows(T) || bad_n(N) || bad_k(K) || bad_ld(lddy, N)) return MOE_ERR_ARG;
+    if (T && (!dy || (act != MOE_LIN_NONE && !z) || (dx && (!wc || !ws)) || (dw && (!xc || !xs)))) return MOE_ERR_ARG;
+    if (misaligned(dy) || misaligned(z) || misaligned(xc) || misaligned(xs) || misaligned(wc) || misaligned(ws) || misaligned(dx) ||
+        misaligned(dw) || misaligned(db) || misaligned(workspace))
+        return MOE_ERR_ALIGN;
+    const size_t need = moe_mx4_linear_bwd_workspace_bytes(T, N, K, act, dx != nullptr, dw != nullptr, db != nullptr);
+    if (workspace_bytes < need || (need && !workspace)) return MOE_ERR_WORKSPACE;
+    char* w = (char*)workspace;
+    const auto take = [&](size_t n) {
+        char* p = w;
+        w += up256(n);
+        workspace_bytes -= up256(n);
+        return p;
+    };
+    int rc = MOE_OK;
+    if (act != MOE_LIN_NONE) {
+        void* dz = take((size_t)T * N * 2);
+        rc = moe_linear_act_bwd(dy, lddy, z, nullptr, nullptr, act, T, N, dtype, dz, stream);
+        dy = dz;
+        lddy = N;
+    }
+    void* x = dw ? take((size_t)T * K * 2) : nullptr;
+    if (!rc && dx) rc = moe_mx4_linear_dx(dy, lddy, wc, ws, T, N, K, dtype, dx, w, workspace_bytes, stream);
+    if (!rc && dw) {
+        rc = moe_mx4_dequantize(xc, xs, 1, T, K, x, dtype, stream);
+        if (!rc) rc = moe_linear_dw(dy, x, T, lddy, K, N, K, dtype, dw, db, w, workspace_bytes, stream);
+    } else if (!rc && db) {
+        rc = moe_mx4_bias_grad(dy, lddy, nullptr, T, 1, N, dtype, db, w, workspace_bytes, stream);
+    }
+    return rc;
 }
 
 int moe_mx4_grouped_mm_dx(const void* dy, int64_t lddy, const void* wc, const void* ws, const int32_t* offsets, int64_t M, int E,

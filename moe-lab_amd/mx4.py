@@ -18,7 +18,7 @@ import functools
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib, formats, grouped as _grouped, linear as _linear
+from . import _lib, formats, grouped as _grouped
 from .linear import GELU, NONE, SILU   # noqa: F401
 
 BLOCK = formats.GS_MXFP4   # elements that share an exponent
@@ -246,7 +246,7 @@ class _Linear(torch.autograd.Function):
         # the weights' 4-bit form stands for w from here on, also where w changes before the backward pass
         ctx.save_for_backward(*((q.codes, q.scales) if need_w else (None, None)),
                               *((w4.codes, w4.scales) if need_x else (None, None)), z)
-        ctx.act, ctx.x_shape, ctx.dtype = act, x.shape, x.dtype
+        ctx.act, ctx.x_shape, ctx.dtype = int(act), x.shape, x.dtype
         return y
 
     @staticmethod
@@ -257,15 +257,18 @@ class _Linear(torch.autograd.Function):
         dy = dy.to(ctx.dtype)
         dx = dw = db = None
         if need_x or need_w or need_b:
-            dz = _lib.half_matrix(dy.reshape(-1, dy.shape[-1]), "dy")
-            if ctx.act != NONE:
-                dz = _linear._act_backward(dz, z, ctx.act, None, None)
+            d, K = _lib.half_matrix(dy.reshape(-1, dy.shape[-1]), "dy"), ctx.x_shape[-1]
+            T, N = d.shape
             if need_x:
-                dx = _linear_dx(dz, _of(wc, ws)).view(ctx.x_shape)
+                dx = torch.empty(ctx.x_shape, dtype=d.dtype, device=d.device)
             if need_w:
-                dw, db = _linear._dw(dz, dequantize(_of(xc, xs), ctx.dtype), need_b)
-            elif need_b:
-                db = _bias_grad(dz, None, 1).view(-1)
+                dw = torch.empty((N, K), dtype=d.dtype, device=d.device)
+            if need_b:
+                db = torch.empty(N, dtype=d.dtype, device=d.device)
+            work, n = _workspace(d.device, "moe_mx4_linear_bwd_workspace_bytes", T, N, K, ctx.act, int(need_x), int(need_w), int(need_b))
+            _lib.call("moe_mx4_linear_bwd", d.device, d.data_ptr(), d.stride(0), _lib.ptr(z), ctx.act, _lib.ptr(xc), _lib.ptr(xs),
+                      _lib.ptr(wc), _lib.ptr(ws), T, N, K, _lib.DTYPE[d.dtype], _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
+                      _lib.ptr(work), n)
         return dx, dw, None, db, None, dy if ctx.needs_input_grad[5] else None, None
 
 
@@ -277,22 +280,6 @@ def _bias_grad(dy, offsets, E):
     _lib.call("moe_mx4_bias_grad", dy.device, dy.data_ptr(), dy.stride(0), _lib.ptr(offsets), M, E, N, _lib.DTYPE[dy.dtype],
               db.data_ptr(), _lib.ptr(ws), nws)
     return db
-
-
-# Rows from which a dense dx multiplies by the weights' values, written out once, and not by the codes, which each tile of 128 rows
-# decodes anew (us from codes and values, w [4096, 4096]: 2048 rows 68 and 73, 4096 rows 130 and 124, 8192 rows 250 and 231).
-DECODE_ONCE = 4096
-
-
-def _linear_dx(dz, w4):
-    (T, N), K = dz.shape, w4.shape[1]
-    if T >= DECODE_ONCE:
-        return _linear._dx(dz, dequantize(w4, dz.dtype))
-    dx = torch.empty((T, K), dtype=dz.dtype, device=dz.device)
-    ws, nws = _workspace(dz.device, "moe_mx4_linear_dx_workspace_bytes", T, N, K)
-    _lib.call("moe_mx4_linear_dx", dz.device, dz.data_ptr(), dz.stride(0), w4.codes.data_ptr(), w4.scales.data_ptr(), T, N, K,
-              _lib.DTYPE[dz.dtype], dx.data_ptr(), _lib.ptr(ws), nws)
-    return dx
 
 
 def _grouped_dx(dy, w4, offsets):

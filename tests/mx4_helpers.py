@@ -4,7 +4,7 @@ import math
 import torch
 
 import dense_helpers as H
-from moelab_amd import mx4
+from moelab_amd import _lib, mx4
 
 MAGS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
@@ -93,3 +93,13 @@ def route(logits, k, score="softmax", bias=None, groups=1, top_groups=1, group_s
         ids.append(torch.tensor(order))
         wts.append(s * scale)
     return torch.stack(ids).to(logits.device), torch.stack(wts).to(logits.device)
+
+
+def linear_dx(dz, w4):
+    """The library's call by itself."""
+    (T, N), K = dz.shape, w4.shape[1]
+    dx = torch.empty((T, K), dtype=dz.dtype, device=dz.device)
+    ws, nws = mx4._workspace(dz.device, "moe_mx4_linear_dx_workspace_bytes", T, N, K)
+    _lib.call("moe_mx4_linear_dx", dz.device, dz.data_ptr(), dz.stride(0), w4.codes.data_ptr(), w4.scales.data_ptr(), T, N, K,
+              _lib.DTYPE[dz.dtype], dx.data_ptr(), _lib.ptr(ws), nws)
+    return dx

@@ -425,7 +425,7 @@ def test_two_streams_at_once():
     def calls(i):
         x = xs[i]
         return [mx4.linear(x[:1], dense[i]), mx4.linear(x[:20], dense[i], act=GELU), mx4.linear(x, dense[i]),
-                mx4.grouped_mm(x, w, offs[i]), mx4._linear_dx(dy[i], dense[i]), mx4._grouped_dx(dy[i], w, offs[i]),
+                mx4.grouped_mm(x, w, offs[i]), M.linear_dx(dy[i], dense[i]), mx4._grouped_dx(dy[i], w, offs[i]),
                 mx4._bias_grad(dy[i], offs[i], 6)]
     want = [calls(0), calls(1)]
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]

@@ -64,7 +64,7 @@ def test_last_rows_of_many():
     assert not y[:5000].any() and not y[T // 2:T // 2 + 5000].any()
     y[-n:] = H.randn(n, N, dtype=BF, seed=5)   # zeros but for the last rows: dy
     d = y[-n:].double()
-    for dx in (mx4._linear_dx(y, w), mx4._grouped_dx(y, mx4.Mx4(w.codes[None], w.scales), H.offsets_of([T]))):
+    for dx in (M.linear_dx(y, w), mx4._grouped_dx(y, mx4.Mx4(w.codes[None], w.scales), H.offsets_of([T]))):
         H.check(dx[-n:], d @ wv, H.product_tol(d @ wv, d.abs() @ wv.abs(), N, BF))
         assert not dx[:-n].any()
     H.check(mx4._bias_grad(y, None, 1)[0], d.sum(0), H.product_tol(d.sum(0), d.abs().sum(0), T, BF))

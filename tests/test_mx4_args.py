@@ -30,6 +30,11 @@ def lindx(**k):
     return _lib.lib().moe_mx4_linear_dx(*a.values(), None)
 
 
+def linbwd(**k):
+    a = dict(dy=P, ld=64, z=P, act=1, xc=P, xs=P, wc=P, ws=P, T=4, N=64, K=64, dt=0, dx=P, dw=P, db=P, w=P, n=1 << 40) | k
+    return _lib.lib().moe_mx4_linear_bwd(*a.values(), None)
+
+
 def grp(**k):
     a = dict(x=P, ldx=64, xc=None, xs=None, xr=4, wc=P, ws=P, b=None, off=P, rows=None, M=4, E=2, N=64, K=64, dt=0, y=P, ydt=0, fill=0, w=P,
              n=1 << 40) | k
@@ -101,6 +106,19 @@ def test_sizes():
     assert L.moe_mx4_grouped_mm_workspace_bytes(8, 1, 128, 2048, 0) == 0
     assert L.moe_mx4_grouped_mm_workspace_bytes(800, 100, 8, 2048, 1) == 0
     assert L.moe_mx4_grouped_mm_workspace_bytes(800, 100, 8, 2048, 0) >= 100 * (1024 + 64)
+
+
+NOTHING = dict(dx=None, dw=None, db=None, act=0)
+
+
+@pytest.mark.parametrize("case,rc", [
+    (dict(dt=2), DT), (dict(act=3), ARG), (dict(act=-1), ARG), (dict(T=-1), ARG), (dict(T=ROWS + 1), ARG), (dict(N=4), ARG), (dict(K=48), ARG),
+    (dict(ld=56), ARG), (dict(ld=2 ** 22), ARG), (dict(dy=None), ARG), (dict(z=None), ARG), (dict(xc=None), ARG), (dict(xs=None), ARG),
+    (dict(wc=None), ARG), (dict(ws=None), ARG), (dict(w=None), WS), (dict(n=0), WS), (dict(act=0, dx=None, db=None, n=0), WS),
+    (NOTHING, 0), (NOTHING | dict(T=0, dy=None, xc=None, wc=None, w=None, n=0), 0)]
+    + [({n: BAD}, AL) for n in ("dy", "z", "xc", "xs", "wc", "ws", "dx", "dw", "db", "w")])
+def test_linear_bwd(case, rc):
+    assert linbwd(**case) == rc
 
 
 def test_packed_form_on_the_cpu():
