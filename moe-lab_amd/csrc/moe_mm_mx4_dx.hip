@@ -16,22 +16,22 @@ __device__ __forceinline__ u32x4 decode8(uint32_t w, float s) {
     return (u32x4){decode2<F16, 0>(w, s), decode2<F16, 1>(w, s), decode2<F16, 2>(w, s), decode2<F16, 3>(w, s)};
 }
 
-// The 16-bit products' tile of 128 x 256 outputs (moe_mm.h: fragments, order of the tiles and stores), 8 waves that multiply and 4
+// The 16-bit products' tile of 32 FA x 256 outputs (moe_mm.h: fragments, order of the tiles and stores), 8 waves that multiply and 4
 // that load. Loads go straight into LDS, dy's rows into a ring of three steps, and of the weights their codes and exponents, 8.5
 // KiB a step, into another; the loading waves then decode a step's codes to the 32 KiB that the products read, of which there are
 // two. All of it is a step or more ahead, so that a step has one barrier, as the 16-bit products' have. (Codes on their way in
 // registers instead: the compiler waits for a load as soon as its count is not certain, 4096^3 190 us.)
 // What bounds it: LDS, which takes in dy and the codes, gives the codes to be decoded, takes them in again as numbers and gives the
 // fragments: 4096^3 148 us, without decoding 124 (the weights as 16-bit numbers in memory: 124, and 12 to write them), without any
-// loads 123. 4444 rows of 32 experts, [5760, 2880], 270-290: half of the row tiles hold 11 rows, and cost 0.75 us a step where full
-// ones take 1.1. Tiles of 256 x 128 halve the decoding and that (257), but few rows then take twice the steps (64 experts x 16,
-// [2048, 2048]: 59 and 115).
-template <bool F16>
+// loads 123. A step takes 0.75 us with 11 rows of the tile and 1.1 with 128. Tiles of 256 x 128 halve the decoding of full ones, but
+// few rows then take twice the steps (64 experts x 16, [2048, 2048]: 59 and 115 us).
+template <bool F16, int FA>
 struct Mx4Dx {
-    static constexpr int FA = 4, FB = 4, NWJ = 4, NWC = 2 * NWJ, NL = 4;
+    static constexpr int FB = 4, NWJ = 4, NWC = 2 * NWJ, NL = 4;
     using Tile = MmKernel<MM_DX, F16, FA, FB, NWJ, 3, 0, EPI_PLAIN, false, NL>;
     static constexpr int BI = Tile::BI, BJ = Tile::BJ;
     static_assert(BJ == 256, "a row's exponents of one step");
+    static_assert(FA == 4 || FA == 5, "load_a");
     using A = Operand<false, BI, NL>;
     using B = Operand<true, BJ, NL>;
     static constexpr int PA = A::PIECES, PC = 64 * 128 / 1024 / NL, L = PA + PC + 1;   // loads of a wave and step
@@ -110,7 +110,9 @@ struct Mx4Dx {
                 if (lefta < 64 && col >= lefta)   // the last step ends inside a row
 #pragma unroll
                     for (int i = 0; i < PA; ++i) offa[i] = MM_OOB;
-                dma16<PA, NL * 1024>(srd_of(pa, basea + (uint32_t)lefta * 2), offa, lds0 + wa + (uint32_t)(lw * 1024));
+                const srd_t da = srd_of(pa, basea + (uint32_t)lefta * 2);
+                dma16<4, NL * 1024>(da, offa, lds0 + wa + (uint32_t)(lw * 1024));
+                if constexpr (PA == 5) dma16<1, 0>(da, offa + 4, lds0 + wa + (uint32_t)((4 * NL + lw) * 1024));
                 ++la.s;
                 pa += 128;
                 lefta = max(lefta - 64, 0);
@@ -232,7 +234,7 @@ struct Mx4Dx {
             for (int s = 0; s < steps; ++s) {
 #pragma unroll
                 for (int f = 0; f < FA; ++f) {
-                    rb[1][f] = B::read(sm + bbuf, frb, f, 1, 1);
+                    if (f < FB) rb[1][f] = B::read(sm + bbuf, frb, f, 1, 1);
                     if (f < nf) {
                         ra[1][f] = A::read(sm + abuf, fra, f, 2, 1);
                         mul(0, f);
@@ -245,7 +247,7 @@ struct Mx4Dx {
                 bbuf = DEC + after<2>(bbuf - DEC, B::BYTES);
 #pragma unroll
                 for (int f = 0; f < FA; ++f) {
-                    rb[0][f] = B::read(sm + bbuf, frb, f, 1, 0);
+                    if (f < FB) rb[0][f] = B::read(sm + bbuf, frb, f, 1, 0);
                     ra[0][f] = A::read(sm + abuf, fra, f, 2, 0);
                     if (f < nf) mul(1, f);
                     __builtin_amdgcn_sched_barrier(0);
@@ -256,25 +258,35 @@ struct Mx4Dx {
     }
 };
 
-template <bool F16>
-__global__ void __launch_bounds__(64 * (Mx4Dx<F16>::NWC + Mx4Dx<F16>::NL), (Mx4Dx<F16>::NWC + Mx4Dx<F16>::NL) / 4)
+template <bool F16, int FA>
+__global__ void __launch_bounds__(64 * (Mx4Dx<F16, FA>::NWC + Mx4Dx<F16, FA>::NL), (Mx4Dx<F16, FA>::NWC + Mx4Dx<F16, FA>::NL) / 4)
 k_mm_mx4_dx(const MmArgs g) {
-    using K = Mx4Dx<F16>;
+    using K = Mx4Dx<F16, FA>;
     __shared__ __attribute__((aligned(1024))) char sm[K::BYTES];
     __shared__ int pre[MM_MAX_E + 1];
+    static_assert(sizeof(sm) + sizeof(pre) <= 160 * 1024, "");
     K::block(g, sm, pre);
 }
 
-int launch_mm_mx4_dx(const MmArgs& a, hipStream_t st) {
-    constexpr int BI = Mx4Dx<true>::BI, BJ = Mx4Dx<true>::BJ, CUT = 4;   // pieces that a tile can be cut into
+template <int FA>
+static int launch_dx(const MmArgs& a, hipStream_t st) {
+    constexpr int BI = Mx4Dx<true, FA>::BI, BJ = Mx4Dx<true, FA>::BJ, CUT = 4;   // pieces that a tile can be cut into
     const int64_t ni = mm_row_tiles(a, BI), nj = (a.J + BJ - 1) / BJ;
     if (ni * nj == 0) return MOE_OK;
     if (ni * nj > 0x70000000) return MOE_ERR_ARG;
     const int64_t grid = round8(CUT * ni * nj) < 256 ? round8(CUT * ni * nj) : 256;   // 256 CUs
-    constexpr int threads = 64 * (Mx4Dx<true>::NWC + Mx4Dx<true>::NL);
-    if (a.f16) k_mm_mx4_dx<true><<<(unsigned)grid, threads, 0, st>>>(a);
-    else k_mm_mx4_dx<false><<<(unsigned)grid, threads, 0, st>>>(a);
+    constexpr int threads = 64 * (Mx4Dx<true, FA>::NWC + Mx4Dx<true, FA>::NL);
+    if (a.f16) k_mm_mx4_dx<true, FA><<<(unsigned)grid, threads, 0, st>>>(a);
+    else k_mm_mx4_dx<false, FA><<<(unsigned)grid, threads, 0, st>>>(a);
     return hipGetLastError() == hipSuccess ? MOE_OK : MOE_ERR_LAUNCH;
+}
+// Tiles of 160 rows for groups of about 112 and more (of those that can have rows): a step of a full one takes 10% longer, of a short
+// one 8%, but there are fewer, and groups that differ a little do not end in a short one each (us in tiles of 128 and 160 rows,
+// random routing: 32 experts x 128, [5760, 2880], 237 and 192, x 139 254 and 190, x 256 342 and 308, x 62 152 and 160; 8 x 256,
+// [4096, 4096], 119 and 78, x 2048 555 and 503; 64 x 16, [2048, 2048], 59 and 63).
+int launch_mm_mx4_dx(const MmArgs& a, hipStream_t st) {
+    const int live = a.E < a.M ? a.E : a.M;
+    return a.offsets && a.M / live >= 112 ? launch_dx<5>(a, st) : launch_dx<4>(a, st);
 }
 
 // Parts of a dense product, by the estimate of mm_plan: rounds of tiles over the CUs, a step at its measured time, a tile's start and

@@ -256,7 +256,7 @@ def test_grouped_rows(T, k, E, N, K, form):
 
 @pytest.mark.parametrize("frozen", [True, False], ids=["frozen", "master"])
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
-@pytest.mark.parametrize("counts", [[1], [0, 3, 0, 70], [130, 64, 0, 65, 2]])
+@pytest.mark.parametrize("counts", [[1], [0, 3, 0, 70], [130, 64, 0, 65, 2], [160, 161, 500, 0, 33, 1]])
 def test_grouped_gradients(counts, dtype, frozen):
     N, K, E, n = 136, 224, len(counts), sum(counts)
     x, b, dy = activations(n, K, dtype), H.randn(E, N, dtype=dtype, seed=2), H.randn(n, N, dtype=dtype, seed=4)
