@@ -325,6 +325,22 @@ def test_grouped_weight_gradient_through_rows():
         H.check(dw[e], ref, H.product_tol(ref, m, 2 * T, torch.bfloat16))
 
 
+def test_x_that_an_index_list_cannot_address(monkeypatch):
+    """Past the bytes that a list's rows can be addressed with, x is indexed first: the same results and weight gradients."""
+    T, N, K, E = 30, 64, 96, 4
+    x, w = activations(T, K, torch.bfloat16), H.randn(E, N, K, dtype=torch.bfloat16, scale=0.1, seed=1).requires_grad_()
+    rows = (torch.arange(2 * T, device=DEV).flip(0) // 2).to(torch.int32)
+    rows[3], rows[50] = -1, T
+    off, dy = H.offsets_of([20, 0, 25, 15]), H.randn(2 * T, N, dtype=torch.bfloat16, seed=4)
+    results = []
+    for limit in (grouped.MAX_INDEXED_BYTES, T * K // 2 - 1):
+        monkeypatch.setattr(grouped, "MAX_INDEXED_BYTES", limit)
+        y = mx4.grouped_mm(x, w, off, rows=rows)
+        results.append((y.detach(), torch.autograd.grad(y, w, dy)[0]))
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and a.any()
+
+
 # ------------------------------------------------------------------------------------------------ values and use
 def test_bad_values_stay_in_their_rows():
     """An infinity or NaN in x makes its row NaN, one in the weights its column; the others are untouched."""
