@@ -70,7 +70,7 @@ def _scale_bytes(shape):
 
 def _new(shape, device):
     q = Mx4.__new__(Mx4)
-    _set(q, torch.empty((*shape[:-1], shape[-1] // 2), dtype=torch.uint8, device=device),
+    _set(q, torch.empty(*shape[:-1], shape[-1] // 2, dtype=torch.uint8, device=device),
          torch.empty(_scale_bytes(shape), dtype=torch.uint8, device=device), tuple(shape))
     return q
 
@@ -111,7 +111,7 @@ def dequantize(q, dtype=torch.bfloat16):
     _lib.require_device(q.codes, "q")
     if dtype not in _lib.DTYPE:
         raise TypeError(f"dtype {dtype}: bf16, fp16 or fp32 expected")
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    out = torch.empty(*q.shape, dtype=dtype, device=q.device)
     E = q.shape[0] if len(q.shape) == 3 else 1
     _lib.call("moe_mx4_dequantize", q.device, q.codes.data_ptr(), q.scales.data_ptr(), E, q.shape[-2], q.shape[-1], out.data_ptr(),
               _lib.DTYPE[dtype])
@@ -234,7 +234,7 @@ def _run_linear(x, w, bias, act, residual, out_dtype, keep_z, keep_x):
     ws, nws = _workspace(device, "moe_mx4_linear_workspace_bytes", T, N, K)
     _lib.call("moe_mx4_linear", device, *_pointers(x2, q), w4.codes.data_ptr(), w4.scales.data_ptr(), _lib.ptr(bias),
               _lib.ptr(residual), int(act), T, N, K, _lib.DTYPE[dtype], y.data_ptr(), _lib.DTYPE[y.dtype], _lib.ptr(z), _lib.ptr(ws), nws)
-    return y.view(*lead, N), z, q, w4
+    return y if len(lead) == 1 else y.view(*lead, N), z, q, w4
 
 
 class _Linear(torch.autograd.Function):

@@ -152,9 +152,10 @@ def _with_bias(desc, bias):
 
 def _topk_scored(lg, desc):
     T = lg.shape[0]
-    idx = torch.empty((T, desc.k), dtype=torch.int32, device=lg.device)
-    wts = torch.empty((T, desc.k), dtype=torch.float32, device=lg.device)
-    _lib.call("moe_topk_scored", lg.device, desc, lg.data_ptr(), _lib.DTYPE[lg.dtype], T, idx.data_ptr(), wts.data_ptr())
+    k, device = desc.k, lg.device
+    idx = torch.empty(T, k, dtype=torch.int32, device=device)
+    wts = torch.empty(T, k, dtype=torch.float32, device=device)
+    _lib.call("moe_topk_scored", device, desc, lg.data_ptr(), _lib.DTYPE[lg.dtype], T, idx.data_ptr(), wts.data_ptr())
     return idx, wts
 
 
