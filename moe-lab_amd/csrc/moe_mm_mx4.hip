@@ -278,7 +278,7 @@ struct MxKernel {
                 if constexpr (GATHER)
                     dma4(srd_of((const char*)g.sa + (int64_t)step * g.a_n * 8, lrows ? (uint32_t)g.a_n * 8 : 0u), offs,
                          lds0 + buf + CODES + lw % SG * 256);
-                const uint8_t* s = g.sa + ((int64_t)step * g.M + lt.lo) * 8 + p * 1024;
+                const uint8_t* s = g.sa + ((int64_t)step * g.a_n + lt.lo) * 8 + p * 1024;
                 int n = (lrows * 8 + 15) / 16 * 16 - p * 1024;
                 if (p >= SCA) {
                     s = g.sb + (((int64_t)e * ksteps + step) * g.J + lt.j0) * 8 + (p - SCA) * 1024;

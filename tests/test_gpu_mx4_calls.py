@@ -1,0 +1,42 @@
+"""Calls of the MXFP4 products that their documentation allows beside the plain ones: more rows of x than slots, offsets as a view, sums whose
+square is past fp32, slots behind the last group in the gradients, values outside fp16's range."""
+import math
+
+import pytest
+import torch
+
+import dense_helpers as H
+import mx4_helpers as M
+from dense_helpers import DEV, TYPES
+from moelab_amd import _lib, mx4
+from moelab_amd.linear import GELU, SILU
+from test_gpu_mx4 import IDS, activations, linear_reference
+
+pytestmark = pytest.mark.gpu
+
+
+def grouped_call(x, q, w, off, M_, rows=None):
+    """moe_mx4_grouped_mm with as many rows of x as it has and M_ slots."""
+    E, N, K = w.shape
+    n = (x if q is None else q.codes).shape[0]
+    y = torch.full((M_, N), 7.0, dtype=torch.bfloat16, device=DEV)
+    ws, nws = mx4._workspace(y.device, "moe_mx4_grouped_mm_workspace_bytes", M_, n, E, K, int(q is not None))
+    _lib.call("moe_mx4_grouped_mm", y.device, *mx4._pointers(x, q), n, w.codes.data_ptr(), w.scales.data_ptr(), None, _lib.ptr(off),
+              _lib.ptr(rows), M_, E, N, K, 0, y.data_ptr(), 0, 1, _lib.ptr(ws), nws)
+    return y
+
+
+@pytest.mark.parametrize("form", ["16-bit", "mx4"])
+@pytest.mark.parametrize("counts,N", [([1] * 8, 264), ([20, 0, 31] * 4, 136), ([300, 0, 90], 264), ([256] * 9, 1032)],
+                         ids=["few rows", "64 x 64", "128 x 128", "128 x 256"])
+@pytest.mark.parametrize("K", [160, 288, 1056])
+def test_more_rows_than_slots(counts, N, K, form):
+    """Without an index list slot p reads x's row p, however many rows follow; K past one step of exponents among them."""
+    n = sum(counts)
+    w, wv = M.random_mx4(len(counts), N, K)
+    x = activations(n + 57, K, torch.bfloat16)
+    y = grouped_call(*((x, None) if form == "16-bit" else (None, mx4.quantize(x))), w, H.offsets_of(counts), n)
+    xv = M.values(x)
+    for e, r in H.ranges(counts):
+        ref, mags = xv[r] @ wv[e].T, xv[r].abs() @ wv[e].abs().T
+        H.check(y[r], ref, H.product_tol(ref, mags, K, torch.bfloat16), (e, r))
