@@ -150,7 +150,8 @@ struct MxKernel {
                             zz[h][u][c] = pack16<F16>(v[0], v[1]);
 #pragma unroll
                             for (int p = 0; p < 2; ++p) {
-                                if constexpr (EPI == MX_ACT) v[p] *= sigmoid_fast(v[p] * (c1 + c3 * (v[p] * v[p])));
+                                // (the square bounded: SiLU's c3 is 0, and 0 times an infinity NaN)
+                                if constexpr (EPI == MX_ACT) v[p] *= sigmoid_fast(v[p] * (c1 + c3 * fminf(v[p] * v[p], 1e30f)));
                                 acc[f][h][i + p] = v[p] + un16<F16>(res[f][h][u][c] >> (16 * p));
                             }
                         }

@@ -40,3 +40,18 @@ def test_more_rows_than_slots(counts, N, K, form):
     for e, r in H.ranges(counts):
         ref, mags = xv[r] @ wv[e].T, xv[r].abs() @ wv[e].abs().T
         H.check(y[r], ref, H.product_tol(ref, mags, K, torch.bfloat16), (e, r))
+
+
+@pytest.mark.parametrize("act", [SILU, GELU])
+@pytest.mark.parametrize("T", [3, 17, 40, 300, 2048])
+def test_sums_whose_square_overflows(T, act):
+    """Activations of sums past 2^64, on every path: themselves, or zero on the negative side."""
+    N, K = 264, 64
+    x = (activations(T, K, torch.float32) * 2.0 ** 40).to(torch.bfloat16)
+    w = (H.randn(N, K, dtype=torch.float32, seed=1) * 2.0 ** 40).to(torch.bfloat16)
+    b, r = H.randn(N, dtype=torch.bfloat16, seed=2), H.randn(T, N, dtype=torch.bfloat16, seed=3)
+    z, _, y, tol = linear_reference(M.values(x), M.values(w), b, r, act)
+    assert float(z.abs().max()) > 2.0 ** 64
+    for dtype in (torch.bfloat16, torch.float32):
+        step = H.half_step(torch.bfloat16) if dtype == torch.bfloat16 else 2.0 ** -23
+        H.check(mx4.linear(x, w, bias=b, act=act, residual=r, out_dtype=dtype), y, tol + step * y.abs())
