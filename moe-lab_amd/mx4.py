@@ -306,7 +306,8 @@ def linear(x, w, bias=None, act=NONE, residual=None, out_dtype=None):
 
 
 def _run_grouped(x, w, offsets, bias, rows, out, out_dtype, keep):
-    """y, x's Mx4 (keep: made for a 16-bit x too), w's, and the list of its rows (None also where x was indexed first)."""
+    """y, x's Mx4 (keep: made for a 16-bit x too), w's, the offsets as the library reads them, and the list of x's rows (None also
+    where x was indexed first)."""
     w4, w_type = _weights(w, 3, "[experts, N, K]")
     E, N, K = w4.shape
     device = w4.device
@@ -329,14 +330,14 @@ def _run_grouped(x, w, offsets, bias, rows, out, out_dtype, keep):
     _lib.call("moe_mx4_grouped_mm", device, *_pointers(x2, q), n, w4.codes.data_ptr(), w4.scales.data_ptr(), _lib.ptr(bias),
               _lib.ptr(offsets), _lib.ptr(rows), M, E, N, K, _lib.DTYPE[dtype], y.data_ptr(), _lib.DTYPE[y.dtype], int(out is None),
               _lib.ptr(ws), nws)
-    return y, q, w4, rows
+    return y, q, w4, offsets, rows
 
 
 class _GroupedMm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, w4, offsets, bias, rows, out_dtype):
         need_x, need_w = ctx.needs_input_grad[:2]
-        y, q, w4, rows = _run_grouped(x, w if w4 is None else w4, offsets, bias, rows, None, out_dtype, need_w)
+        y, q, w4, offsets, rows = _run_grouped(x, w if w4 is None else w4, offsets, bias, rows, None, out_dtype, need_w)
         ctx.save_for_backward(*((q.codes, q.scales) if need_w else (None, None)), *((w4.codes, w4.scales) if need_x else (None, None)),
                               offsets, rows)
         ctx.dtype, ctx.experts = x.dtype, w4.shape[0]

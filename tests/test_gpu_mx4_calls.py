@@ -55,3 +55,23 @@ def test_sums_whose_square_overflows(T, act):
     for dtype in (torch.bfloat16, torch.float32):
         step = H.half_step(torch.bfloat16) if dtype == torch.bfloat16 else 2.0 ** -23
         H.check(mx4.linear(x, w, bias=b, act=act, residual=r, out_dtype=dtype), y, tol + step * y.abs())
+
+
+@pytest.mark.parametrize("counts", [[9, 0, 30, 1], [200, 130, 0, 161]])
+def test_offsets_with_a_stride(counts):
+    """Offsets as a column of a table of counts: the forward pass and every gradient read the view, not what lies behind its first."""
+    E, N, K, n = len(counts), 136, 224, sum(counts)
+    plain = H.offsets_of(counts)
+    view = torch.stack([plain, torch.full_like(plain, n)], 1)[:, 0]
+    assert not view.is_contiguous()
+    x, dy = activations(n, K, torch.bfloat16), H.randn(n, N, dtype=torch.bfloat16, seed=4)
+    b = H.randn(E, N, dtype=torch.bfloat16, seed=2)
+    frozen, _ = M.random_mx4(E, N, K)
+    for w in (frozen, H.randn(E, N, K, dtype=torch.bfloat16, scale=K ** -0.5, seed=1)):
+        got = []
+        for off in (plain, view):
+            leaves = [t.clone().requires_grad_() for t in ((x, b) if w is frozen else (x, b, w))]
+            y = mx4.grouped_mm(leaves[0], w if w is frozen else leaves[2], off, bias=leaves[1])
+            got.append((y.detach(), *torch.autograd.grad(y, leaves, dy)))
+        for i, (p, q) in enumerate(zip(*got)):
+            assert torch.equal(p, q), i
