@@ -164,7 +164,8 @@ class _TopkScored(torch.autograd.Function):
     def forward(ctx, logits, desc, bias):
         lg = _lib.dense(logits)
         idx, wts = _topk_scored(lg, desc)
-        ctx.save_for_backward(lg, bias, idx)
+        # the backward pass reads in the bias which experts it took out: as it was here, also where its owner moves it in between
+        ctx.save_for_backward(lg, None if bias is None else bias.clone(), idx)
         ctx.desc = desc
         ctx.mark_non_differentiable(idx)
         ctx.set_materialize_grads(False)
@@ -177,7 +178,7 @@ class _TopkScored(torch.autograd.Function):
             return None, None, None
         lg, bias, idx = ctx.saved_tensors
         desc = ctx.desc
-        if bias is not None and bias.data_ptr() != desc.bias:   # kept elsewhere in between
+        if bias is not None:
             desc = _with_bias(desc, bias)
         dw, dl = _lib.dense(dwts, torch.float32), torch.empty_like(lg)
         _lib.call("moe_topk_scored_bwd", lg.device, desc, lg.data_ptr(), _lib.DTYPE[lg.dtype], lg.shape[0], idx.data_ptr(),
@@ -192,7 +193,7 @@ def topk_scored(logits, k, score="softmax", bias=None, groups=1, top_groups=1, g
     largest ranking value (group_score "max") or the sum of its two largest ("top2"). idx: the k experts that rank highest, best
     first, of equals the lowest id. wts: scale * score, with norm divided by the k scores' sum (0 where that is 0).
     NaN logits count as -inf; experts at -inf are chosen last, with weight 0 and no gradient. E <= 1024, groups <= 64, k <= 32.
-    Scores are ranked in fp64. The bias and the choice have no gradient."""
+    Scores are ranked in fp64. The bias and the choice have no gradient; the bias may change before the backward pass."""
     _lib.require_device(logits, "logits")
     if logits.dim() < 1:
         raise ValueError("logits [..., E] expected")
