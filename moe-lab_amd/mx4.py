@@ -135,7 +135,7 @@ def from_packed(codes, scales):
         c = torch.where((scales == 0).repeat_interleave(16, -1), torch.zeros_like(c), c)
     E, N, S = shape[0] if len(shape) == 3 else 1, shape[-2], _steps_of(shape)
     s = torch.full((E, N, 8 * S), 127, dtype=torch.uint8, device=codes.device)
-    s[..., :shape[-1] // BLOCK] = scales.reshape(E, N, -1)
+    s[..., :shape[-1] // BLOCK] = scales.reshape(E, N, shape[-1] // BLOCK)
     flat = torch.zeros(_scale_bytes(shape), dtype=torch.uint8, device=codes.device)
     flat[:-16] = s.reshape(E, N, S, 4, 2).permute(0, 2, 1, 4, 3).reshape(-1)
     return Mx4(c.clone() if c.data_ptr() == codes.data_ptr() else c, flat)
@@ -145,7 +145,7 @@ def to_packed(q):
     """(codes int32 [..., K / 8], scales uint8 [..., K / 32]) of an Mx4."""
     E, N, S = q.shape[0] if len(q.shape) == 3 else 1, q.shape[-2], _steps_of(q.shape)
     s = q.scales[:-16].reshape(E, S, N, 2, 4).permute(0, 2, 1, 4, 3).reshape(E, N, 8 * S)[..., :q.shape[-1] // BLOCK]
-    return q.codes.clone().view(torch.int32), s.reshape(*q.shape[:-1], -1).contiguous()
+    return q.codes.clone().view(torch.int32), s.reshape(*q.shape[:-1], q.shape[-1] // BLOCK).contiguous()
 
 
 # ------------------------------------------------------------------------------------------------------ products
