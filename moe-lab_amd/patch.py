@@ -19,6 +19,9 @@ Two levels, as in the reference:
     - "gpt-oss": ``GptOssMLP``: router with bias, top-k of the logits, softmax over them; MXFP4 experts stored
       transposed with gate and up interleaved, per-expert biases, clamped SwiGLU (reference e2e.py:153-175); the
       forward returns (y, routing weights) as the stock one does.
+  A block of the first three is taken for its family by what its own forward does with random tokens, experts aside (on the CPU): the
+  weights that it gives its experts, and what it adds to their result. One that does something else (sigmoid scores, shared experts
+  of another form, a norm in between) keeps its own forward, and only its experts run on the kernels.
   Shared experts whose width is S times the routed experts' are split into S experts of that width and merged into
   the routed set (one expert call per layer, experts.merge_shared); other widths run as a second call.
 * ``patch_experts`` (the reference's SwitchGLU-level universal patch) replaces only an experts module's per-slot
@@ -94,6 +97,19 @@ def _bare(module):
     return c
 
 
+def _shell(module, without):
+    """A module's class and another module of it, on the CPU: its settings, buffers and children, without hooks, without the children
+    `without` and without its own parameters. Its forward is the class's own."""
+    cls = torch.nn.utils.parametrize.type_before_parametrizations(module)
+    m = cls.__new__(cls)
+    torch.nn.Module.__init__(m)
+    kept = {n: _bare(c) for n, c in module._modules.items() if n not in (*without, "parametrizations")}
+    own = {n: v for n, v in module.__dict__.items() if n not in m.__dict__}
+    m.__dict__.update({n: v for n, v in own.items() if n not in ("forward", "_moelab_stock_forward")})
+    m._buffers, m._modules = dict(module._buffers), kept
+    return cls, m
+
+
 def _act_of(module, tol=1e-3):
     """The GLU of a module with this act_fn, which may differ from the kernels' function by tol: by default as far as the exact
     GELU does from the tanh form (4.7e-4, below what 4-bit weights do to a layer), but not as far as a function of another kind
@@ -132,7 +148,8 @@ def _mlp_as_experts(mlp, F):
 def block_state(block, fmt=None):
     """The block's packed state and call settings: {"kind", "state", "k", "norm", "scale", "act", "bias",
     "stock_gate", "scored"} (stock_gate: route by itself, not inside the layer call; scored: router.route_scored's settings,
-    or None: with the block's own gate)."""
+    or None: with the block's own gate). kind: block_kind's, or "own" for a block whose own forward does not route and add up as its
+    kind does: it runs, and only its experts are packed."""
     kind = block_kind(block)
     if kind is None:
         raise ValueError(f"{type(block).__name__}: not a sparse MoE block this patch knows")
@@ -151,21 +168,13 @@ def block_state(block, fmt=None):
     e, gate = block.experts, block.gate
     F = e.gate_up_proj.shape[1] // 2
     fmt = fmt or "int4"
+    cfg.update(act=_act_of(e), **_routing(block, kind))
     s = _quantise(fmt, e.gate_up_proj[:, :F], e.gate_up_proj[:, F:], e.down_proj)
     s["wr"] = gate.weight.detach().to(torch.bfloat16).contiguous()
-    cfg.update(k=int(getattr(gate, "top_k", getattr(block, "top_k", 0))), norm=bool(getattr(gate, "norm_topk_prob", True)),
-               act=_act_of(e))
     shared = None
-    if kind == "deepseek":
-        cfg["norm"] = False   # greedy: the full softmax's probabilities of the top-k
-        cfg["scale"] = float(gate.routed_scaling_factor)
-        cfg["stock_gate"] = getattr(gate, "topk_method", "greedy") != "greedy" or _choice_bias(gate) is not None
-        if cfg["stock_gate"]:
-            cfg["scored"] = _scored_settings(gate, cfg["k"])
-            if cfg["scored"] is not None:
-                _bias_fits(cfg, gate)
+    if cfg["kind"] == "deepseek":
         shared = block.shared_experts
-    elif kind == "qwen2-shared":
+    elif cfg["kind"] == "qwen2-shared":
         shared = block.shared_expert
         s["shared_gate"] = block.shared_expert_gate.weight.detach().reshape(-1).to(torch.bfloat16).contiguous()
     if shared is not None:
@@ -178,6 +187,105 @@ def block_state(block, fmt=None):
                                                                    shared.down_proj.weight)))
     cfg["state"] = s
     return cfg
+
+
+class _Heard(torch.nn.Module):
+    """Stands for a block's experts or shared experts: returns the numbers y and keeps what it is called with."""
+
+    def __init__(self, y):
+        super().__init__()
+        self.y, self.calls = y, []
+
+    def forward(self, *args, **kw):
+        self.calls.append((*args, *kw.values()))
+        return self.y.reshape(args[0].shape)
+
+
+@torch.no_grad()
+def _listen(block, kind, seed):
+    """What a block's own forward does with random tokens, on the CPU in fp32: the tokens x [T, d], its router's weight [E, d], the
+    weights [T, E] that it gives its experts and their number k, and whether it returns the experts' result and what its kind adds,
+    of these tokens, and nothing else. Raises where it does not call its experts with tokens, ids and weights once."""
+    E, d = block.experts.gate_up_proj.shape[0], block.experts.gate_up_proj.shape[2]
+    g, T = torch.Generator("cpu").manual_seed(seed), 32
+
+    def rand(*shape):
+        return torch.randn(shape, generator=g, device="cpu")
+    names = [n for n in ("experts", "shared_experts", "shared_expert") if getattr(block, n, None) is not None]
+    cls, m = _shell(block, names)
+    for n, b in m._buffers.items():
+        m._buffers[n] = b if b is None else b.detach().cpu()
+    m._parameters = {n: None if p is None else torch.nn.Parameter(p.detach().cpu(), requires_grad=False) for n, p in block._parameters.items()}
+    heard = {n: _Heard(rand(T, d)) for n in names}
+    m._modules.update(heard)
+    m.float().eval()
+    weight, x = m.gate.weight.detach(), rand(T, d)
+    spread = float((x @ weight.T).std())
+    x *= 2 / spread if 0 < spread < math.inf else 1.0   # logits as far apart as a trained router's
+    out = cls.forward(m, x[None].clone())
+    ((tokens, idx, wts),) = heard["experts"].calls
+    k = idx.shape[1]
+    if tokens.shape != x.shape or idx.shape != (T, k) or wts.shape != (T, k) or idx.is_floating_point() or not 0 <= int(idx.min()) <= int(idx.max()) < E:
+        raise ValueError(f"experts called with {tuple(tokens.shape)}, {tuple(idx.shape)}, {tuple(wts.shape)}")
+    want = heard["experts"].y
+    same = torch.equal(tokens.float(), x)
+    shared = {"deepseek": "shared_experts", "qwen2-shared": "shared_expert"}.get(kind)
+    if shared:
+        y, (call,) = heard[shared].y, heard[shared].calls
+        same = same and len(call) == 1 and torch.equal(call[0].reshape(x.shape).float(), x)
+        want = want + (y if kind == "deepseek" else torch.sigmoid(x @ m.shared_expert_gate.weight.T) * y)
+    same = same and isinstance(out, torch.Tensor) and out.shape == (1, T, d) and bool(((out[0] - want).abs() <= 1e-4).all())
+    return x, weight, torch.zeros((T, E), dtype=torch.float64, device="cpu").scatter_add(1, idx.long(), wts.double()), k, same
+
+
+@torch.no_grad()
+def _routing(block, kind):
+    """The settings with which a block of this kind routes, by its own forward: the fused router's softmax top-k, route_scored's, the
+    block's gate by itself, or (kind "own") all of the block."""
+    gate = block.gate
+    cfg = dict(kind=kind, norm=kind != "deepseek" and bool(getattr(gate, "norm_topk_prob", True)),
+               scale=float(gate.routed_scaling_factor) if kind == "deepseek" else 1.0)
+    with torch.device("cpu"):   # whatever the program's default device is
+        try:
+            heard = [_listen(block, kind, seed) for seed in (0, 1)]
+        except Exception as e:
+            raise NotImplementedError(f"{type(block).__name__} does not call its experts as the kernels take it ({type(e).__name__}: {e}); "
+                                      f"patch_experts leaves all of the block but the experts as it is") from e
+        cfg["k"] = heard[0][3]
+
+        def is_it(weights):
+            """Whether the block gave its experts these weights, for one set of tokens at least (two experts' scores can be equal in fp32)."""
+            for x, w, got, _, same in heard:
+                try:
+                    want = weights(x, w)
+                    if same and got.shape == want.shape and float((got - want).abs().max()) <= 1e-4 * float(want.max()):
+                        return True
+                except Exception:   # another gate's result: no such experts, no such tuple
+                    pass
+            return False
+
+        def softmax(norm):
+            return is_it(lambda x, w: _scored_weights(x, w, cfg["k"], "softmax", None, 1, 1, "max", norm, cfg["scale"]))
+
+        def own_gate(x, w):
+            out = _bare(gate).float()(x)
+            return torch.zeros((len(x), w.shape[0]), dtype=torch.float64).scatter_add(1, out[2].long(), out[1].double())
+        for norm in (cfg["norm"], not cfg["norm"]):   # (kinds of one name are not all alike in it)
+            if softmax(norm):
+                return cfg | dict(norm=norm)
+        if kind == "deepseek":
+            cfg["stock_gate"], cfg["scored"] = True, _scored_settings(gate, cfg["k"])
+            if cfg["scored"] is not None and is_it(lambda x, w: _scored_weights(x, w, cfg["k"], bias=_cpu(_choice_bias(gate)), **cfg["scored"])):
+                _bias_fits(cfg, gate)
+                return cfg
+            cfg["scored"] = None
+            if is_it(own_gate):
+                return cfg
+    return cfg | dict(kind="own", stock_gate=False)
+
+
+def _cpu(t):
+    return None if t is None else t.detach().cpu()
 
 
 def _choice_bias(gate):
@@ -262,6 +370,15 @@ def patch_block(block, fmt=None):
     the stacked families) or "mxfp4" (default for gpt-oss)."""
     cfg = block_state(block, fmt)
     s = cfg["state"]
+    if cfg["kind"] == "own":
+        def experts(hidden_states, top_k_index, top_k_weights):
+            x = hidden_states.to(torch.bfloat16).contiguous()
+            y = run_experts(s, x, top_k_index.to(torch.int32).contiguous(), top_k_weights.float().contiguous(), act=cfg["act"],
+                            out_dtype=None if hidden_states.dtype == torch.bfloat16 else torch.float32)
+            return y.to(hidden_states.dtype)
+        block._moelab_cfg = cfg
+        _install(block.experts, experts, s)
+        return _install(block, getattr(block, "_moelab_stock_forward", block.forward), s)
 
     def forward(hidden_states):
         shape = hidden_states.shape
@@ -288,6 +405,8 @@ def patch_block(block, fmt=None):
 
 
 def unpatch_block(block):
+    if block._moelab_cfg["kind"] == "own":
+        unpatch_experts(block.experts)
     block.forward = block._moelab_stock_forward
     del block._moelab_stock_forward, block._moelab_state, block._moelab_cfg
     return block
@@ -360,14 +479,8 @@ def _probe(module, d, F, E, dtype, act):
         return torch.randn(shape, generator=g, dtype=torch.float64, device="cpu").to(dtype)
     scales = torch.tensor([0.25, 2.0, 8.0] if dtype.itemsize == 2 else [0.25, 2.0, 16.0, 128.0], device="cpu")
     x = rand(4 * len(scales), d) * scales.repeat(4)[:, None].to(dtype)
-    cls = torch.nn.utils.parametrize.type_before_parametrizations(module)
-    m = cls.__new__(cls)   # the module with other parameters, without its hooks
-    torch.nn.Module.__init__(m)
     names = ("gate_up_proj", "down_proj") if E else ("gate_proj", "up_proj", "down_proj")
-    kept = {n: _bare(c) for n, c in module._modules.items() if n not in names + ("parametrizations",)}
-    own = {n: v for n, v in module.__dict__.items() if n not in m.__dict__}
-    m.__dict__.update({n: v for n, v in own.items() if n not in ("forward", "_moelab_stock_forward")})
-    m._buffers, m._modules = dict(module._buffers), kept
+    cls, m = _shell(module, names)
     if E:
         n = E if F <= 32 else 1   # at the module's own sizes its experts are one and the same
         gu, dn = rand(n, 2 * F, d).expand(E, 2 * F, d), rand(n, d, F).expand(E, d, F)
