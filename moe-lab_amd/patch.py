@@ -155,6 +155,7 @@ def block_state(block, fmt=None):
         raise ValueError(f"{type(block).__name__}: not a sparse MoE block this patch knows")
     cfg = {"kind": kind, "scale": 1.0, "bias": None, "stock_gate": False, "scored": None}
     if kind == "gpt-oss":
+        _check_gptoss(block)
         e, r = block.experts, block.router
         gu = e.gate_up_proj                       # [E, d, 2F], columns gate, up, gate, up, ...
         s = _quantise(fmt or "mxfp4", gu[..., ::2].transpose(1, 2), gu[..., 1::2].transpose(1, 2),
@@ -168,7 +169,7 @@ def block_state(block, fmt=None):
     e, gate = block.experts, block.gate
     F = e.gate_up_proj.shape[1] // 2
     fmt = fmt or "int4"
-    cfg.update(act=_act_of(e), **_routing(block, kind))
+    cfg.update(act=_glu_of(e), **_routing(block, kind))
     s = _quantise(fmt, e.gate_up_proj[:, :F], e.gate_up_proj[:, F:], e.down_proj)
     s["wr"] = gate.weight.detach().to(torch.bfloat16).contiguous()
     shared = None
@@ -187,6 +188,53 @@ def block_state(block, fmt=None):
                                                                    shared.down_proj.weight)))
     cfg["state"] = s
     return cfg
+
+
+def _glu_of(experts):
+    """The activation of a stacked experts module that computes the plain GLU layer: as near as _act_of takes its function for it."""
+    act = _act_of(experts)
+    E, d, F = experts.down_proj.shape
+    _check_glu(experts, act, True, d, F, E, least=1e-2, train=False)
+    return act
+
+
+@torch.no_grad()
+def _check_gptoss(block):
+    """Raises where the block's own forward, run with experts of 32 x 32 random numbers, is not the clamped layer of the kernels with
+    gate and up interleaved. (Modules that cannot be run at another size than their own are taken by their parameters.)"""
+    e, T = block.experts, 8
+    E, d, F = e.gate_up_proj.shape[0], e.gate_up_proj.shape[1], e.gate_up_proj.shape[2] // 2
+    g = torch.Generator("cpu").manual_seed(0)
+
+    def rand(*shape, scale=1.0):
+        return torch.randn(shape, generator=g, device="cpu") * scale
+
+    def small(module, names, params):
+        cls, m = _shell(module, names)
+        m.__dict__.update({n: 64 if v == 2 * F and v != d else 32 for n, v in m.__dict__.items()
+                           if type(v) is int and v in (d, F, 2 * F) and n != "num_experts"})
+        m._parameters = {n: torch.nn.Parameter(v, requires_grad=False) for n, v in params.items()}
+        return cls, m.eval()
+    w, b, k = rand(E, 32, scale=0.5), rand(E), int(block.router.top_k)
+    gu, gb, dn, db = rand(E, 32, 64), rand(E, 64), rand(E, 32, 32), rand(E, 32)
+    try:
+        with torch.device("cpu"):   # whatever the program's default device is
+            cls, m = small(block, ("router", "experts"), {})
+            m._modules["router"] = small(block.router, (), dict(weight=w, bias=b))[1]
+            m._modules["experts"] = small(e, (), dict(gate_up_proj=gu, gate_up_proj_bias=gb, down_proj=dn, down_proj_bias=db))[1]
+            x = rand(T, 32)
+            got = cls.forward(m, x[None].clone())[0].reshape(T, 32)
+    except Exception:
+        return
+    top, ids = (x @ w.T + b).topk(k, 1)
+    z = torch.einsum("td,tkdf->tkf", x, gu[ids]) + gb[ids]
+    gate, up = z[..., ::2].clamp(max=7.0), z[..., 1::2].clamp(-7.0, 7.0)
+    h = gate * torch.sigmoid(1.702 * gate) * (up + 1)
+    y = ((torch.einsum("tkf,tkfd->tkd", h, dn[ids]) + db[ids]) * torch.softmax(top, 1)[..., None]).sum(1)
+    gap = float((got - y).abs().max() / y.abs().max())
+    if not gap <= 1e-3:
+        raise ValueError(f"{type(block).__name__} computes something else than the kernels' clamped layer with its gate and up interleaved "
+                         f"(off by {gap:.1e} on random weights)")
 
 
 class _Heard(torch.nn.Module):
@@ -421,9 +469,9 @@ def patch_experts(experts, fmt="int4"):
     if not _stacked(experts):
         raise ValueError(f"{type(experts).__name__}: not a stacked experts module")
     F = experts.gate_up_proj.shape[1] // 2
+    act = _glu_of(experts)
     with torch.no_grad():
         s = _quantise(fmt, experts.gate_up_proj[:, :F], experts.gate_up_proj[:, F:], experts.down_proj)
-    act = _act_of(experts)
 
     def forward(hidden_states, top_k_index, top_k_weights):
         T, d = hidden_states.shape
@@ -469,7 +517,7 @@ def _hooked(x):
     return any(getattr(x, n, None) for n in _HOOKS)
 
 
-def _probe(module, d, F, E, dtype, act):
+def _probe(module, d, F, E, dtype, act, train=True):
     """The largest error of a module's own forward against the plain GLU layer, relative to the magnitudes that its sums add,
     on small random weights in its parameters' place (E None: a dense GLU MLP). Gates reach the hundreds, so that a clamp shows;
     routing weights are not 1, so that a weight at another place does."""
@@ -497,7 +545,7 @@ def _probe(module, d, F, E, dtype, act):
         dn = m.down_proj.weight[None]
         idx, wts = torch.zeros(len(x), 1, dtype=torch.int64, device="cpu"), torch.ones(len(x), 1, device="cpu")
         args = (x,)
-    got = cls.forward(m.train(), *args)   # as in training: a dropout shows too
+    got = cls.forward(m.train(train), *args)   # in training a dropout shows too
     if E:
         # ids past the experts: most forwards raise, some skip them as the kernels do, some take the last expert instead; but
         # some have experts without weights there
@@ -518,19 +566,20 @@ def _probe(module, d, F, E, dtype, act):
     return float(((got.double() - ref).abs() / mags).max())   # a NaN or another shape fails too
 
 
-def _check_glu(module, act, stacked, d, F, E):
-    """Raises unless the module's own forward is the plain GLU layer that the kernels compute."""
+def _check_glu(module, act, stacked, d, F, E, least=0.0, train=True):
+    """Raises unless the module's own forward, in training or not, is the plain GLU layer that the kernels compute (least: a difference
+    that passes in every type)."""
     tried = []
     own = (module.down_proj if stacked else module.down_proj.weight).dtype
     for size in ((16, 32), (d, F)):   # some forwards know their sizes
         for dtype, tol in ((torch.float64, 1e-6), (torch.float32, 1e-4), (own, 0.05)):
             try:
                 with torch.no_grad(), torch.device("cpu"):   # whatever the program's default device is
-                    gap = _probe(module, *size, E if stacked else None, dtype, act)
+                    gap = _probe(module, *size, E if stacked else None, dtype, act, train)
             except Exception as e:   # a type or a size that this forward does not take
                 tried.append(f"{type(e).__name__}: {e}")
                 continue
-            if gap <= tol:
+            if gap <= max(tol, least):
                 return
             raise ValueError(f"{type(module).__name__} computes something else than the plain GLU layer of the kernels (off by "
                              f"{gap:.1e} of its sums on random weights): a clamp, another gate or other routing weights")
