@@ -359,8 +359,9 @@ def _scored_weights(x, weight, k, score, bias, groups, top_groups, group_score, 
 @torch.no_grad()
 def _scored_settings(gate, k):
     """topk_scored's settings for a gate that it computes, without the bias, else None: checked on the gate's own forward, on
-    random tokens on the CPU. Gates that mask the other groups with 0 choose an expert there over a kept one whose score and
-    bias are negative together; with such a bias the gate stays stock."""
+    random tokens on the CPU. Where groups are masked, with all scores and biases negative together as well: a gate that masks the
+    other groups with 0, not with -inf, then chooses an expert there, and stays stock. So a gate that is taken chooses alike whatever
+    becomes of its bias; one whose bias has a negative element now stays stock as well (_bias_fits)."""
     bias = _choice_bias(gate)
     groups, top = int(getattr(gate, "num_group", 1) or 1), int(getattr(gate, "topk_group", 1) or 1)
     if bias is None:
@@ -373,19 +374,29 @@ def _scored_settings(gate, k):
         if bias is not None and top < groups and float(bias.min()) < 0:
             return None
         g = _bare(gate).float()
-        x = torch.randn((64, g.weight.shape[1]), generator=torch.Generator("cpu").manual_seed(0), device="cpu")
-        x *= 2 / float((x @ g.weight.T).std())   # logits as far apart as a trained router's
-        out = g(x)
-        got = torch.zeros((64, g.weight.shape[0]), dtype=torch.float64, device="cpu").scatter(1, out[2].long(), out[1].double())
-        want = _scored_weights(x, g.weight, k, bias=_choice_bias(g), **kw)
+
+        def alike(seed):
+            x = torch.randn((64, g.weight.shape[1]), generator=torch.Generator("cpu").manual_seed(seed), device="cpu")
+            x *= 2 / float((x @ g.weight.T).std())   # logits as far apart as a trained router's
+            out = g(x)
+            got = torch.zeros((64, g.weight.shape[0]), dtype=torch.float64, device="cpu").scatter(1, out[2].long(), out[1].double())
+            want = _scored_weights(x, g.weight, k, bias=_choice_bias(g), **kw)
+            return float((got - want).abs().max()) <= 1e-4 * float(want.max())
+        if not (alike(0) or alike(1)):   # (two experts' scores can be equal in fp32)
+            return None
+        if bias is not None and top < groups:
+            _choice_bias(g).sub_(float(bias.max()) + 1.5)
+            if not (alike(0) or alike(1)):
+                return None
     except Exception:   # whatever a gate of another kind makes of these tokens
         return None
-    return kw if float((got - want).abs().max()) <= 1e-4 * float(want.max()) else None
+    return kw
 
 
 def _bias_fits(cfg, gate):
-    """Whether the gate's bias, as it is now, lets route_scored choose as the gate does (_scored_settings). Looked at again only
-    after it changed; while a graph is captured, or where changes leave no trace, a bias that has changed means the stock gate."""
+    """Whether route_scored takes the gate's place with the bias as it is: not with a negative element while groups are masked. Looked
+    at again only after the bias changed; while a graph is captured, or where changes leave no trace, a bias that has changed means
+    the stock gate. (A change that goes unseen, through .data or between a graph's replays, does no harm: _scored_settings.)"""
     bias, kw = _choice_bias(gate), cfg["scored"]
     if bias is None or kw["top_groups"] == kw["groups"]:
         return True
