@@ -15,7 +15,7 @@ Two levels, as in the reference:
       ``routed_scaling_factor`` (reference e2e.py:129-150: the fused router for greedy gates, the stock gate for
       group-limited ones), plus the shared experts added (e2e.py:146-147). Group-limited softmax gates, and sigmoid gates
       with a bias that ranks, run on router.route_scored if the gate's own forward does what that computes (and it is in
-      bf16, without hooks); any other gate stays stock;
+      bf16, without hooks or a forward put in its place); any other gate stays stock;
     - "gpt-oss": ``GptOssMLP``: router with bias, top-k of the logits, softmax over them; MXFP4 experts stored
       transposed with gate and up interleaved, per-expert biases, clamped SwiGLU (reference e2e.py:153-175); the
       forward returns (y, routing weights) as the stock one does.
@@ -95,6 +95,13 @@ def _bare(module):
         for n in _HOOKS:
             getattr(m, n).clear()
     return c
+
+
+def _own_forwards(module):
+    """The module, its parts' own forwards in place of those put there (which can compute with the modules that this one is a copy of)."""
+    for m in module.modules():
+        m.__dict__.pop("forward", None)
+    return module
 
 
 def _shell(module, without):
@@ -266,7 +273,7 @@ def _listen(block, kind, seed):
     m._parameters = {n: None if p is None else torch.nn.Parameter(p.detach().cpu(), requires_grad=False) for n, p in block._parameters.items()}
     heard = {n: _Heard(rand(T, d)) for n in names}
     m._modules.update(heard)
-    m.float().eval()
+    _own_forwards(m).float().eval()
     weight, x = m.gate.weight.detach(), rand(T, d)
     spread = float((x @ weight.T).std())
     x *= 2 / spread if 0 < spread < math.inf else 1.0   # logits as far apart as a trained router's
@@ -316,7 +323,7 @@ def _routing(block, kind):
             return is_it(lambda x, w: _scored_weights(x, w, cfg["k"], "softmax", None, 1, 1, "max", norm, cfg["scale"]))
 
         def own_gate(x, w):
-            out = _bare(gate).float()(x)
+            out = _own_forwards(_bare(gate)).float()(x)
             return torch.zeros((len(x), w.shape[0]), dtype=torch.float64).scatter_add(1, out[2].long(), out[1].double())
         for norm in (cfg["norm"], not cfg["norm"]):   # (kinds of one name are not all alike in it)
             if softmax(norm):
@@ -373,7 +380,7 @@ def _scored_settings(gate, k):
         router._scored(gate.weight.shape[0], k, kw["score"], None, groups, top, kw["group_score"], kw["norm"], kw["scale"], None)
         if bias is not None and top < groups and float(bias.min()) < 0:
             return None
-        g = _bare(gate).float()
+        g = _own_forwards(_bare(gate)).float()
 
         def alike(seed):
             x = torch.randn((64, g.weight.shape[1]), generator=torch.Generator("cpu").manual_seed(seed), device="cpu")
@@ -444,7 +451,7 @@ def patch_block(block, fmt=None):
         x = hidden_states.reshape(-1, shape[-1]).to(torch.bfloat16).contiguous()
         gate = getattr(block, "gate", None)
         if (cfg["scored"] is not None and hidden_states.dtype == gate.weight.dtype == torch.bfloat16 and not _hooked(gate)
-                and _bias_fits(cfg, gate)):
+                and "forward" not in gate.__dict__ and _bias_fits(cfg, gate)):
             # the gate's own weight and bias, as they are now; in other types it computes with more digits than bf16 has
             idx, wts = router.route_scored(x.detach(), gate.weight.detach(), cfg["k"], bias=_choice_bias(gate), **cfg["scored"])
             y = run_layer(s, x, idx, wts, act=cfg["act"])
