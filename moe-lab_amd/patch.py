@@ -332,6 +332,7 @@ def _routing(block, kind):
             cfg["stock_gate"], cfg["scored"] = True, _scored_settings(gate, cfg["k"])
             if cfg["scored"] is not None and is_it(lambda x, w: _scored_weights(x, w, cfg["k"], bias=_cpu(_choice_bias(gate)), **cfg["scored"])):
                 _bias_fits(cfg, gate)
+                cfg["scored_for"] = _gate_settings(gate)
                 return cfg
             cfg["scored"] = None
             if is_it(own_gate):
@@ -400,6 +401,10 @@ def _scored_settings(gate, k):
     return kw
 
 
+def _gate_settings(gate):
+    return tuple(getattr(gate, n, None) for n in ("top_k", "num_group", "topk_group", "norm_topk_prob", "routed_scaling_factor"))
+
+
 def _bias_fits(cfg, gate):
     """Whether route_scored takes the gate's place with the bias as it is: not with a negative element while groups are masked. Looked
     at again only after the bias changed; while a graph is captured, or where changes leave no trace, a bias that has changed means
@@ -451,8 +456,8 @@ def patch_block(block, fmt=None):
         x = hidden_states.reshape(-1, shape[-1]).to(torch.bfloat16).contiguous()
         gate = getattr(block, "gate", None)
         if (cfg["scored"] is not None and hidden_states.dtype == gate.weight.dtype == torch.bfloat16 and not _hooked(gate)
-                and "forward" not in gate.__dict__ and _bias_fits(cfg, gate)):
-            # the gate's own weight and bias, as they are now; in other types it computes with more digits than bf16 has
+                and "forward" not in gate.__dict__ and _gate_settings(gate) == cfg["scored_for"] and _bias_fits(cfg, gate)):
+            # the gate's own weight and bias, as they are now, in the settings it was checked with; in other types it computes with more digits than bf16 has
             idx, wts = router.route_scored(x.detach(), gate.weight.detach(), cfg["k"], bias=_choice_bias(gate), **cfg["scored"])
             y = run_layer(s, x, idx, wts, act=cfg["act"])
         elif cfg["stock_gate"]:

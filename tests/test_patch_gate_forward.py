@@ -28,3 +28,17 @@ def test_a_wrapped_gate_runs(kind, when):
         assert len(calls) == 1
         del block.gate.forward
         assert len(calls) == 1 and block(x).shape == y.shape and len(calls) == 1
+
+
+@pytest.mark.gpu
+def test_a_gate_whose_settings_change_runs():
+    block = sigmoid_block("cuda")
+    patch.patch_block(block)
+    x = torch.randn(1, 8, D, generator=torch.Generator().manual_seed(3)).to("cuda", torch.bfloat16)
+    with torch.no_grad():
+        first = block(x)
+        gate = block.gate
+        scale, gate.routed_scaling_factor = gate.routed_scaling_factor, 25.0
+        assert not torch.allclose(first, block(x), rtol=0.1, atol=0.0)
+        gate.routed_scaling_factor = scale
+        assert torch.equal(first, block(x))
