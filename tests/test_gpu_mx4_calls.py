@@ -75,3 +75,64 @@ def test_offsets_with_a_stride(counts):
             got.append((y.detach(), *torch.autograd.grad(y, leaves, dy)))
         for i, (p, q) in enumerate(zip(*got)):
             assert torch.equal(p, q), i
+
+
+def wide_weights(E, N, K):
+    """Weights of positive values in blocks of three kinds: some past fp16's largest number, fp16's own, and some below its smallest."""
+    q, _ = M.random_mx4(E, N, K)
+    codes, _ = mx4.to_packed(q)
+    codes &= 0x77777777
+    kinds = torch.tensor([127 + 15, 127, 127 - 25], device=DEV).repeat(K // 96)
+    q = mx4.from_packed(codes, kinds.to(torch.uint8).expand(E, N, -1).contiguous())
+    v = mx4.dequantize(q, torch.float32).double()
+    assert float(v.max()) > 65520 and 0 < float(v[v > 0].min()) < 2.0 ** -24
+    return q, v
+
+
+@pytest.mark.parametrize("T", [3, 130, 4100])
+def test_gradients_in_fp16_through_weights_outside_its_range(T):
+    """The weights' values are rounded to fp16 there: infinity past its largest, what fp16 has below its smallest. The forward
+    product takes them as they are."""
+    N, K = 72, 288
+    w, v = wide_weights(1, N, K)
+    x, dy = activations(T, K, torch.float16), H.randn(T, N, dtype=torch.float16, seed=4).abs() + 0.25
+    v16 = v[0].half().double()
+    with torch.no_grad():
+        x[:, (torch.arange(K, device=DEV) // 32) % 3 == 0] *= 2.0 ** -14
+    x = x.requires_grad_()
+    y = mx4.linear(x, M.first(w))
+    xv = M.values(x.detach())
+    ref = xv @ v[0].T
+    assert torch.isfinite(y).all()
+    H.check(y.detach(), ref, H.product_tol(ref, xv.abs() @ v[0].T, K, torch.float16))
+    (dx,) = torch.autograd.grad(y, x, dy)
+    ref = dy.double() @ v16
+    assert torch.isinf(ref).any() and torch.isfinite(ref).any()
+    H.check(dx, ref, H.product_tol(ref, ref, N, torch.float16))
+
+
+@pytest.mark.parametrize("counts", [[9, 0, 30], [200, 130, 0, 161]])
+def test_grouped_gradients_in_fp16_through_weights_outside_its_range(counts):
+    E, N, K, n = len(counts), 72, 288, sum(counts)
+    w, v = wide_weights(E, N, K)
+    v16 = v.half().double()
+    x, dy = activations(n, K, torch.float16).requires_grad_(), H.randn(n, N, dtype=torch.float16, seed=4).abs() + 0.25
+    (dx,) = torch.autograd.grad(mx4.grouped_mm(x, w, H.offsets_of(counts), out_dtype=torch.float32), x, dy.float())
+    for e, r in H.ranges(counts):
+        ref = dy[r].double() @ v16[e]
+        H.check(dx[r], ref, H.product_tol(ref, ref, N, torch.float16))
+
+
+def test_gradients_through_weights_with_bad_blocks():
+    """Blocks with an infinity or NaN read as NaN: their columns of dx are NaN, no others."""
+    for T, N, K in ((3, 72, 288), (300, 72, 288), (4100, 64, 96)):
+        w = H.randn(N, K, dtype=torch.bfloat16, scale=0.1, seed=1)
+        w[5, K - 1], w[N - 1, 3] = math.nan, -math.inf
+        x, dy = activations(T, K, torch.bfloat16).requires_grad_(), H.randn(T, N, dtype=torch.bfloat16, seed=4)
+        (dx,) = torch.autograd.grad(mx4.linear(x, mx4.quantize(w)), x, dy)
+        v = M.values(w)
+        bad = torch.isnan(v).any(0)
+        assert torch.isnan(dx[:, bad]).all() and int(bad.sum()) == 64
+        v = torch.where(torch.isnan(v), 0, v)
+        ref = dy.double() @ v
+        H.check(dx[:, ~bad], ref[:, ~bad], H.product_tol(ref, dy.double().abs() @ v.abs(), N, torch.bfloat16)[:, ~bad])
