@@ -136,3 +136,27 @@ def test_gradients_through_weights_with_bad_blocks():
         v = torch.where(torch.isnan(v), 0, v)
         ref = dy.double() @ v
         H.check(dx[:, ~bad], ref[:, ~bad], H.product_tol(ref, dy.double().abs() @ v.abs(), N, torch.bfloat16)[:, ~bad])
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("counts", [[0, 0], [9, 0, 30, 1], [200, 130, 0, 161], [40, 0, 1000]])
+def test_gradients_of_slots_behind_the_last_group(counts, out):
+    """Their rows of dy (NaN here) are not read. dx is zero there in the backward pass; the library call leaves them as they were
+    with fill = 0. Tiles of both heights."""
+    E, N, K, n, tail = len(counts), 136, 288, sum(counts), 7
+    w, wv = M.random_mx4(E, N, K)
+    off, dy = H.offsets_of(counts), H.randn(n + tail, N, dtype=torch.bfloat16, seed=4)
+    dy[n:] = math.nan
+    x = activations(n + tail, K, torch.bfloat16).requires_grad_()
+    (g,) = torch.autograd.grad(mx4.grouped_mm(x, w, off), x, dy)
+    ref, mags = torch.zeros(2, n + tail, K, dtype=torch.float64, device=DEV)
+    for e, r in H.ranges(counts):
+        ref[r], mags[r] = dy[r].double() @ wv[e], dy[r].double().abs() @ wv[e].abs()
+    H.check(g, ref, H.product_tol(ref, mags, N, torch.bfloat16))
+    for fill in (0, 1):
+        dx = torch.full((n + tail, K), 7.0, dtype=out, device=DEV)
+        _lib.call("moe_mx4_grouped_mm_dx", dx.device, dy.data_ptr(), dy.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), off.data_ptr(),
+                  n + tail, E, N, K, 0, dx.data_ptr(), _lib.DTYPE[out], fill)
+        assert (dx[n:] == (0 if fill else 7)).all()
+        step = H.half_step(torch.bfloat16) if out == torch.bfloat16 else 2.0 ** -23
+        H.check(dx[:n], ref[:n], step * ref[:n].abs() + (N + 8) * 2.0 ** -23 * mags[:n])
