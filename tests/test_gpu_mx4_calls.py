@@ -160,3 +160,59 @@ def test_gradients_of_slots_behind_the_last_group(counts, out):
         assert (dx[n:] == (0 if fill else 7)).all()
         step = H.half_step(torch.bfloat16) if out == torch.bfloat16 else 2.0 ** -23
         H.check(dx[:n], ref[:n], step * ref[:n].abs() + (N + 8) * 2.0 ** -23 * mags[:n])
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("form", ["16-bit", "mx4"])
+@pytest.mark.parametrize("counts,tail", [([0] * 40 + [90] + [0] * 40, 5), ([1] * 30 + [47] + [0, 2] * 20 + [17, 5], 0), ([130] + [0] * 127, 3)])
+def test_few_slots_a_group_but_one_busy(counts, tail, form, bias):
+    """About one slot a group on average, most of them in one: the kernel of few rows goes through it piece by piece."""
+    E, n, N, K = len(counts), sum(counts), 200, 544
+    assert (n + tail) // min(E, n + tail) <= 1
+    w, wv = M.random_mx4(E, N, K)
+    x, b = activations(n + tail, K, torch.bfloat16), H.randn(E, N, dtype=torch.bfloat16, seed=2) if bias else None
+    xv = M.values(x)
+    ref, mags = torch.zeros(2, n + tail, N, dtype=torch.float64, device=DEV)
+    for e, r in H.ranges(counts):
+        c = b[e].double() if bias else torch.zeros(N, dtype=torch.float64, device=DEV)
+        ref[r], mags[r] = xv[r] @ wv[e].T + c, xv[r].abs() @ wv[e].abs().T + c.abs()
+    off, operand = H.offsets_of(counts), x if form == "16-bit" else mx4.quantize(x)
+    H.check(mx4.grouped_mm(operand, w, off, bias=b), ref, H.product_tol(ref, mags, K, torch.bfloat16))
+    back = torch.arange(n + tail, device=DEV).flip(0).to(torch.int32)
+    flipped = x.flip(0) if form == "16-bit" else mx4.quantize(x.flip(0))
+    H.check(mx4.grouped_mm(flipped, w, off, bias=b, rows=back), ref, H.product_tol(ref, mags, K, torch.bfloat16))
+
+
+@pytest.mark.parametrize("M_", [6, 200, 900])
+def test_captured_grouped_calls(M_):
+    """A captured product and its gradients, replayed on other offsets and rows between eager calls, equal the eager ones each time."""
+    E, N, K = 6, 264, 288
+    w, _ = M.random_mx4(E, N, K)
+    b = H.randn(E, N, dtype=torch.bfloat16, seed=2).requires_grad_()
+    x = activations(M_, K, torch.bfloat16).requires_grad_()
+    dy, off = H.randn(M_, N, dtype=torch.bfloat16, seed=4), torch.zeros(E + 1, dtype=torch.int32, device=DEV)
+
+    def step():
+        y = mx4.grouped_mm(x, w, off, bias=b)
+        return (y.detach(), *torch.autograd.grad(y, (x, b), dy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    g = torch.Generator().manual_seed(M_)
+    for case in range(5):
+        cuts = torch.randint(0, M_ + 1, (E,), generator=g).sort().values
+        cuts = [torch.full((E,), M_), torch.cat([torch.zeros(E - 1), torch.tensor([M_])]), torch.zeros(E)][case] if case < 3 else cuts
+        with torch.no_grad():
+            off[1:] = cuts.to(DEV, torch.int32)
+            x.copy_(activations(M_, K, torch.bfloat16, seed=case))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in got]
+        for p, q in zip(kept, step()):
+            assert torch.equal(p, q), case
