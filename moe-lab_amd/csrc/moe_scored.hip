@@ -6,8 +6,8 @@
 // fp64; ranking works on 64-bit integers that order as the numbers do, 32-bit ones without a bias.
 // One wave per token, expert 64 j + lane in a lane's slot j. Bound by the latency of its chain, not by bytes or operations: the logits,
 // for a softmax its maximum and total, the groups' values, then k rounds of a maximum over the wave and one over its lanes' slots
-// (256 experts in 8 groups, k 8: 6.5 us for one token, 12.2 for 4096, whose logits are read in 1; 8191 tokens of 64 experts, k 6,
-// softmax without norm: forward 10.9 us, backward 8.0). With more tokens than the CUs hold waves the fp64 exponentials add up: they
+// (traced: 256 experts in 8 groups, k 8: 6.5 us for one token, 12 for 4096, whose logits are read in 1, in a captured graph 7.0 and 11.5;
+// 8191 tokens of 64 experts, k 6, softmax without norm: forward 11 us, backward 8). With more tokens than the CUs hold waves the fp64 exponentials add up: they
 // are taken only where they rank or scale.
 #include "moe_common.h"
 #include "moe_scored.h"
@@ -38,7 +38,8 @@ __device__ __forceinline__ uint32_t key_of(float v) {
     return b >> 31 ? ~b : b | 1u << 31;
 }
 // Sums and maxima over lanes by DPP moves: a move through LDS (ds_bpermute) takes about ten times as long, and a token is a chain
-// of them (256 experts, k 8, one token: 10.0 us with those, 6.5 so; 4096 tokens 17.6 and 12.2).
+// of them (256 experts, k 8, one token: 10.0 us with those, 5.1 so; 4096 tokens 17.6 and 9.8: both measured together,
+// on an earlier form of the kernel than the figures above).
 template <int CTRL, int ROWS = 0xF>
 __device__ __forceinline__ double moved64(double v) {   // lanes without a source: 0
     const u32x2 w = __builtin_bit_cast(u32x2, v);

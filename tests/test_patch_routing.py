@@ -31,16 +31,19 @@ def changed(block, after=lambda self, x, y: y, before=lambda self, x: x):
     return block
 
 
-def minimax_m2(device):
-    """Sigmoid scores and a bias that ranks, which lies beside the gate."""
-    from transformers.models.minimax_m2.configuration_minimax_m2 import MiniMaxM2Config
-    from transformers.models.minimax_m2.modeling_minimax_m2 import MiniMaxM2SparseMoeBlock
-    cfg = MiniMaxM2Config(hidden_size=D, intermediate_size=192, num_local_experts=8, num_experts_per_tok=3)
-    block = _init(MiniMaxM2SparseMoeBlock(cfg), device)
-    with torch.no_grad():
-        for n, b in block.named_buffers():
-            if "bias" in n:
-                b.copy_(0.3 * torch.rand(b.shape, generator=torch.Generator().manual_seed(5)))
+def bias_beside(device):
+    """Sigmoid scores and a bias that ranks, which the block holds and not its gate."""
+    block = make_block("mixtral", device)
+
+    class Block(type(block)):
+        def forward(self, x):
+            flat = x.reshape(-1, x.shape[-1])
+            s = torch.sigmoid(torch.nn.functional.linear(flat, self.gate.weight)).float()
+            idx = (s + self.choice_bias).topk(2, dim=-1).indices
+            w = s.gather(1, idx)
+            return self.experts(flat, idx, w / w.sum(-1, keepdim=True)).reshape(x.shape)
+    block.__class__ = Block
+    block.register_buffer("choice_bias", torch.tensor([0.3, 0.0, 0.1, 0.2], device=device))
     return block
 
 
@@ -52,7 +55,7 @@ def shared_beside(device):
     return changed(block, after=lambda self, x, y: y + self.shared_experts(x))
 
 
-OWN = {"sigmoid gate": lambda d: sigmoid_gate(make_block("mixtral", d)), "minimax-m2": minimax_m2, "shared beside": shared_beside,
+OWN = {"sigmoid gate": lambda d: sigmoid_gate(make_block("mixtral", d)), "bias beside": bias_beside, "shared beside": shared_beside,
        "scaled result": lambda d: changed(make_block("olmoe", d), after=lambda self, x, y: 2.5 * y),
        "residual": lambda d: changed(make_block("qwen3", d), after=lambda self, x, y: x + y),
        "scaled tokens": lambda d: changed(make_block("qwen3", d), before=lambda self, x: 0.5 * x),
