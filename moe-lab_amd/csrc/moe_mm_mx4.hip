@@ -58,8 +58,8 @@ enum MxEpi { MX_PLAIN = 0, MX_LIN = 1, MX_ACT = 2 };
 // What bounds it: in large tiles a step's fragment reads take LDS as long as the matrix cores take for its products, loads into LDS 40%
 // more on top, and beside them the clock falls with the power: [4096, 16384] by [16384, 4096] 155 us, 3.5 PFLOP/s of the 6.3 that the
 // instruction reaches by itself, 4096^3 41-46 us (3.0-3.3, by the card; bf16 110), 4096 x 8 rows of 128 experts, [1536, 2048], 88-93 (8
-// steps a tile: stores and the first loads are a fifth). A wave to 64 x 128 outputs, which reads a quarter less, has nothing to cover its own
-// latency: 4096^3 47 us. In 64 x 64 tiles, L2: 237 rows, [4096, 4096], 10.4 us for 75 MB of loads; 8 stages of one workgroup instead of 4
+// steps a tile: stores and the first loads are a fifth). A wave to 64 x 128 outputs, which reads a quarter less, has nothing to cover
+// its own latency: 4096^3 47 us. In 64 x 64 tiles, L2: 237 rows, [4096, 4096], 10.4 us for 75 MB of loads; 8 stages of one workgroup instead of 4
 // of two: 12.3.
 template <bool F16, int FA, int FB, int NWI, int NWJ, int ST, int GATHER, int EPI, int NL>
 struct MxKernel {

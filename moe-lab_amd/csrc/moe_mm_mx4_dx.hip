@@ -1,7 +1,7 @@
 // Gradients in x of products with MXFP4 weights: dx[p][k] = sum_n dy[p][n] w[e][n][k], dy in 16 bits, w codes with an exponent per
 // 32 of k. The sums go over n, along which the exponents change, so the block-scaled instruction does not apply: the codes become
-// 16-bit numbers on their way into LDS: in bf16 exactly, in fp16 rounded, past its largest number to infinity (blocks whose exponent byte
-// is 141 or more can hold such values, below 104 such that fp16 has no bits for).
+// 16-bit numbers on their way into LDS: in bf16 exactly, in fp16 rounded, past its largest number to infinity (blocks whose exponent
+// byte is 141 or more can hold such values, below 104 such that fp16 has no bits for).
 #include "moe_mx4.h"
 
 namespace moe {

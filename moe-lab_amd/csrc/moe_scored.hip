@@ -6,9 +6,9 @@
 // fp64; ranking works on 64-bit integers that order as the numbers do, 32-bit ones without a bias.
 // One wave per token, expert 64 j + lane in a lane's slot j. Bound by the latency of its chain, not by bytes or operations: the logits,
 // for a softmax its maximum and total, the groups' values, then k rounds of a maximum over the wave and one over its lanes' slots
-// (traced: 256 experts in 8 groups, k 8: 6.5 us for one token, 12 for 4096, whose logits are read in 1, in a captured graph 7.0 and 11.5;
-// 8191 tokens of 64 experts, k 6, softmax without norm: forward 11 us, backward 8). With more tokens than the CUs hold waves the fp64 exponentials add up: they
-// are taken only where they rank or scale.
+// (traced: 256 experts in 8 groups, k 8: 6.5 us for one token, 12 for 4096, whose logits are read in 1, in a captured graph 7.0 and
+// 11.5; 8191 tokens of 64 experts, k 6, softmax without norm: forward 11 us, backward 8). With more tokens than the CUs hold waves the
+// fp64 exponentials add up: they are taken only where they rank or scale.
 #include "moe_common.h"
 #include "moe_scored.h"
 

@@ -240,8 +240,8 @@ def _check_gptoss(block):
     y = ((torch.einsum("tkf,tkfd->tkd", h, dn[ids]) + db[ids]) * torch.softmax(top, 1)[..., None]).sum(1)
     gap = float((got - y).abs().max() / y.abs().max())
     if not gap <= 1e-3:
-        raise ValueError(f"{type(block).__name__} computes something else than the kernels' clamped layer with its gate and up interleaved "
-                         f"(off by {gap:.1e} on random weights)")
+        raise ValueError(f"{type(block).__name__} computes something else than the kernels' clamped layer with its gate and up "
+                         f"interleaved (off by {gap:.1e} on random weights)")
 
 
 class _Heard(torch.nn.Module):
@@ -270,7 +270,8 @@ def _listen(block, kind, seed):
     cls, m = _shell(block, names)
     for n, b in m._buffers.items():
         m._buffers[n] = b if b is None else b.detach().cpu()
-    m._parameters = {n: None if p is None else torch.nn.Parameter(p.detach().cpu(), requires_grad=False) for n, p in block._parameters.items()}
+    m._parameters = {n: None if p is None else torch.nn.Parameter(p.detach().cpu(), requires_grad=False)
+                     for n, p in block._parameters.items()}
     heard = {n: _Heard(rand(T, d)) for n in names}
     m._modules.update(heard)
     _own_forwards(m).float().eval()
@@ -280,7 +281,8 @@ def _listen(block, kind, seed):
     out = cls.forward(m, x[None].clone())
     ((tokens, idx, wts),) = heard["experts"].calls
     k = idx.shape[1]
-    if tokens.shape != x.shape or idx.shape != (T, k) or wts.shape != (T, k) or idx.is_floating_point() or not 0 <= int(idx.min()) <= int(idx.max()) < E:
+    if (tokens.shape != x.shape or idx.shape != (T, k) or wts.shape != (T, k) or idx.is_floating_point()
+            or not 0 <= int(idx.min()) <= int(idx.max()) < E):
         raise ValueError(f"experts called with {tuple(tokens.shape)}, {tuple(idx.shape)}, {tuple(wts.shape)}")
     want = heard["experts"].y
     same = torch.equal(tokens.float(), x)
@@ -304,12 +306,13 @@ def _routing(block, kind):
         try:
             heard = [_listen(block, kind, seed) for seed in (0, 1)]
         except Exception as e:
-            raise NotImplementedError(f"{type(block).__name__} does not call its experts as the kernels take it ({type(e).__name__}: {e}); "
-                                      f"patch_experts leaves all of the block but the experts as it is") from e
+            raise NotImplementedError(f"{type(block).__name__} does not call its experts as the kernels take it ({type(e).__name__}: "
+                                      f"{e}); patch_experts leaves all of the block but the experts as it is") from e
         cfg["k"] = heard[0][3]
 
         def is_it(weights):
-            """Whether the block gave its experts these weights, for one set of tokens at least (two experts' scores can be equal in fp32)."""
+            """Whether the block gave its experts these weights, for one set of tokens at least: two experts' scores can be equal in
+            fp32."""
             for x, w, got, _, same in heard:
                 try:
                     want = weights(x, w)
@@ -330,7 +333,9 @@ def _routing(block, kind):
                 return cfg | dict(norm=norm)
         if kind == "deepseek":
             cfg["stock_gate"], cfg["scored"] = True, _scored_settings(gate, cfg["k"])
-            if cfg["scored"] is not None and is_it(lambda x, w: _scored_weights(x, w, cfg["k"], bias=_cpu(_choice_bias(gate)), **cfg["scored"])):
+            bias = _choice_bias(gate)
+            if cfg["scored"] is not None and is_it(
+                    lambda x, w: _scored_weights(x, w, cfg["k"], bias=None if bias is None else bias.cpu(), **cfg["scored"])):
                 _bias_fits(cfg, gate)
                 cfg["scored_for"] = _gate_settings(gate)
                 return cfg
@@ -338,10 +343,6 @@ def _routing(block, kind):
             if is_it(own_gate):
                 return cfg
     return cfg | dict(kind="own", stock_gate=False)
-
-
-def _cpu(t):
-    return None if t is None else t.detach().cpu()
 
 
 def _choice_bias(gate):
@@ -457,7 +458,8 @@ def patch_block(block, fmt=None):
         gate = getattr(block, "gate", None)
         if (cfg["scored"] is not None and hidden_states.dtype == gate.weight.dtype == torch.bfloat16 and not _hooked(gate)
                 and "forward" not in gate.__dict__ and _gate_settings(gate) == cfg["scored_for"] and _bias_fits(cfg, gate)):
-            # the gate's own weight and bias, as they are now, in the settings it was checked with; in other types it computes with more digits than bf16 has
+            # the gate's own weight and bias, as they are now, in the settings it was checked with; in other types it computes with
+            # more digits than bf16 has
             idx, wts = router.route_scored(x.detach(), gate.weight.detach(), cfg["k"], bias=_choice_bias(gate), **cfg["scored"])
             y = run_layer(s, x, idx, wts, act=cfg["act"])
         elif cfg["stock_gate"]:

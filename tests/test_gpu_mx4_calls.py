@@ -1,5 +1,6 @@
-"""Calls of the MXFP4 products that their documentation allows beside the plain ones: more rows of x than slots, offsets as a view, sums whose
-square is past fp32, slots behind the last group in the gradients, values outside fp16's range."""
+"""Calls of the MXFP4 products that their documentation allows beside the plain ones: more rows of x than slots, offsets as a view, sums
+whose square is past fp32, slots behind the last group in the gradients, values outside fp16's range, one busy group among many of few
+slots, captured calls."""
 import math
 
 import pytest
