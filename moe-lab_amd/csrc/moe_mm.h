@@ -411,7 +411,8 @@ struct MmKernel {
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
                             const float z = v[u][c], r = un16<F16>(rw[c >> 1] >> (16 * (c & 1)));
-                            v[u][c] = (lin ? z : z * sigmoid_fast(z * (c1 + c3 * (z * z)))) + r;
+                            // (the square bounded: SiLU's c3 is 0, and 0 times an infinity NaN)
+                            v[u][c] = (lin ? z : z * sigmoid_fast(z * (c1 + c3 * fminf(z * z, 1e30f)))) + r;
                         }
                     }
                 }
